@@ -234,6 +234,21 @@ int kv800_hip_step_tables(const int32_t* qbt, int64_t qbt_stride, int64_t bsq, i
 int kv800_hip_step_meta(const int32_t* bt, int64_t bt_stride, int64_t npages, const int64_t* lens, int64_t R,
                         int64_t ebs, int64_t* slot, int64_t* pos, int32_t* lens32, void* stream);
 
+/* Metadata of a step whose rows bring any number of new tokens, and the growth of the rows' block tables, from lengths on
+ * the device (step_meta is its one-token form; a mixed step's lengths on the host are vllm_attn.py:255-270). Row r: n = lens[r]
+ * positions, the step's tokens included (int64), c = qlens[r] of them new (int32, clamped to [0, n]); ebs tokens a page.
+ * qsl (R + 1) int64: exclusive prefix sum of c. For token qsl[r] + i, i < c: pos = n - c + i, slot = page * ebs + pos % ebs
+ * with page = bt[r, pos / ebs] (-1 where the table has no such page), row = r; the padding behind, up to `tokens`, gets slot
+ * and pos -1 and row 0. lens32[r] = n. tokens >= the sum of c: a smaller one cuts the last rows (qsl is cut too).
+ * held != NULL: row r holds held[r] pages (int32) and takes max(0, ceil(n / ebs) - held[r]) more, at most up to npages, from
+ * free_pages (nfree int32 page numbers) in row order, behind the taken[0] that are gone already: written to bt in place from
+ * entry held[r] on; held_out[r] and taken_out[0] are the counts behind the step (not in place). A list that runs out leaves
+ * entries as they are and their tokens without a slot. bt: (R, bt_stride) int32, npages of a row in use. R >= 1. */
+int kv800_hip_chunk_meta(int32_t* bt, int64_t bt_stride, int64_t npages, const int64_t* lens, const int32_t* qlens,
+                         int64_t R, int64_t ebs, int64_t tokens, const int32_t* held, const int32_t* free_pages,
+                         int64_t nfree, const int64_t* taken, int32_t* held_out, int64_t* taken_out, int64_t* qsl,
+                         int64_t* slot, int64_t* pos, int64_t* row, int32_t* lens32, void* stream);
+
 /* off[r, p] = bt[r, p] * scale + add for p < npages (off row stride npages): an exact group's (R, bt_stride) int32
  * block table as element offsets of its pages, the eoff table the decode and flush read (the reference forms it with
  * torch ops per step, vllm_attn.py:320-323). */
@@ -268,6 +283,26 @@ int kv800_hip_decode_sized(const kv800_paged_t* P, const uint16_t* q, int64_t B,
 int kv800_hip_decode_noalloc(const kv800_paged_t* P, const uint16_t* q, int64_t B, const uint16_t* cos_t,
                              const uint16_t* sin_t, int64_t rope_rows, const uint32_t* cs2, int64_t qpool_bytes,
                              int64_t epool_elems, int64_t sink_elems, uint16_t* out, int64_t spb, void* stream);
+
+/* Attention of a step's new tokens over the paged cache as it is (drafted tokens to verify, short prompt chunks): row r's
+ * queries q[qsl[r], qsl[r + 1]) ((T, 16, 128) bf16, post-RoPE; qsl (R + 1) int64 on the device, as kv800_hip_chunk_meta makes
+ * it) stand at the positions P->N[r] - c + i, c = qsl[r + 1] - qsl[r], and their rows are in the exact pages already.
+ * Replaces, for such rows, the assembly of the whole history as bf16 keys (vllm_attn.py:351-402). A query sees the positions
+ * up to its own:
+ *   P->win = 0: sub-blocks [0, P->NQ[r]), then the exact pages from position 256 NQ[r] on. NQ: the sub-blocks flushed before
+ *     the step's tokens (a larger one is masked by position). nqmax >= every NQ; 0: exact pages alone.
+ *   P->win > 0: the exact pages, positions > position - win; with P->sk also the sinks: positions < 4 from sk / sv as far
+ *     as they lie below the first query's window, else from the exact pages.
+ * Keys rotated with the (rope_rows, 32) bf16 tables and rounded to bf16, or as stored (cos_t = sin_t = NULL: sliding layers).
+ * cs2: kv800_hip_rope_table of the same rows (needed with sub-blocks). V of sub-blocks is not rounded to bf16. Offsets outside
+ * the pools and positions past the tables are skipped. out (T, 16, 128) bf16; a query without keys and the padding
+ * [qsl[R], T) get zeros. ws: kv800_hip_decode_chunk_workspace(R, T, nqmax) bytes (0 for nqmax = 0 or window layers), 16-byte
+ * aligned, of this call alone. The result does not depend on the other rows of the call, but on their number by rounding. */
+int64_t kv800_hip_decode_chunk_workspace(int64_t R, int64_t T, int64_t nqmax);
+int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int64_t* qsl, int64_t R, int64_t T,
+                           const uint16_t* cos_t, const uint16_t* sin_t, int64_t rope_rows, const uint32_t* cs2,
+                           int64_t qpool_bytes, int64_t epool_elems, int64_t sink_elems, uint16_t* out, void* ws,
+                           int64_t ws_bytes, void* stream);
 
 /* Streaming read of bytes (a positive multiple of 16) from buf with `groups` workgroups (8 plain 16-byte loads in
  * flight per lane), writing one xor word per workgroup to out[0 .. groups). No counterpart in the reference: a

@@ -9,6 +9,8 @@
 //                        the step's nnew tokens (the flush range's start, vllm_attn.py:297-317), the block table as
 //                        int64 and the offsets of the sink aux areas (vllm_attn.py:276-291).
 //   step_meta_kernel     per row of a decode step: the new token's slot, its position and the int32 length
+//   chunk_meta_kernel    per new token of a step whose rows bring any number of them: slot, position and row, their prefix
+//                        sums over the rows, and the pages that rows outgrow their block table by, from a list of free ones.
 //   page_offsets_kernel  off[r, p] = bt[r, p] * scale + add: an exact group's block table as element offsets of its
 //                        pages (the eoff table of the decode and flush kernels).
 // All are plain data movement: one thread per 16-byte piece or per table entry, coalesced along the row.
@@ -85,6 +87,124 @@ step_meta_kernel(const int32_t* __restrict__ bt, int64_t bt_stride, int64_t npag
   slot[r] = (pg >= 0 && pg < npages) ? (int64_t)bt[r * bt_stride + pg] * ebs + p % ebs : -1;
   pos[r] = p >= 0 ? p : -1;
   lens32[r] = (int32_t)n;
+}
+
+// Slots, positions and rows of a step's new tokens, and the growth of the block tables, from the rows' lengths on the
+// device. Row r has n = lens[r] positions of which c = min(max(qlens[r], 0), n) are new: its tokens are
+// qsl[r] .. qsl[r] + c - 1 (qsl the exclusive prefix sum of c), token qsl[r] + i at position n - c + i. With `held` it
+// takes max(0, ceil(n / ebs) - held[r]) further pages (as many as its table has room for), consecutive entries of the free
+// list behind the earlier rows' ones.
+// No workgroup waits for another: workgroup (x, y) takes the rows [256 x, 256 x + 256) and, of their tokens, every
+// gridDim.y-th piece of 256. It sums the earlier rows' counts itself (12 bytes a row, from the L2) and scans its own in
+// LDS; a token finds its row by 8 steps of a binary search there. Fresh table entries are read from the free list, not
+// from the table, so the order in which workgroups write the table does not matter.
+// Bound: launch and two dependent rounds of loads. 398 rows x 8 tokens: CHUNK_META_TIME.
+struct MetaArgs {
+  int32_t* bt;
+  int64_t bt_stride, npages;
+  const int64_t* lens;
+  const int32_t* qlens;
+  int64_t R, ebs, tokens;
+  const int32_t* held;      // null: no growth
+  const int32_t* freep;
+  int64_t nfree;
+  const int64_t* taken;
+  int32_t* held_out;
+  int64_t* taken_out;
+  int64_t *qsl, *slot, *pos, *row;
+  int32_t* lens32;
+};
+constexpr int MROWS = 256;   // rows and threads per workgroup
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// a row's length, new tokens and (with held) pages before the step and to add; everything is clamped to what is possible
+struct MetaRow { int64_t n, c, have, add; };
+__device__ __forceinline__ MetaRow meta_row(const MetaArgs& A, int64_t r) {
+  MetaRow m;
+  m.n = min(max(A.lens[r], (int64_t)0), (int64_t)0x7FFFFFFF);
+  m.c = min(max((int64_t)A.qlens[r], (int64_t)0), m.n);
+  m.have = A.npages;
+  m.add = 0;
+  if (A.held) {
+    m.have = min(max((int64_t)A.held[r], (int64_t)0), A.npages);
+    m.add = max(min((m.n + A.ebs - 1) / A.ebs, A.npages) - m.have, (int64_t)0);
+  }
+  return m;
+}
+__global__ void __launch_bounds__(MROWS) chunk_meta_kernel(MetaArgs A) {
+  __shared__ int64_t first[MROWS + 1];                 // first token of each of the rows, and the next workgroup's
+  __shared__ int64_t pos0[MROWS], page0[MROWS];        // position of a row's first token; its first fresh free-list entry
+  __shared__ int32_t have[MROWS], all[MROWS];          // pages held before the step, and after it
+  __shared__ int64_t wc[4], wa[4], bc[4], ba[4];
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int64_t r0 = (int64_t)blockIdx.x * MROWS, r = r0 + tid;
+  const bool last = blockIdx.x == gridDim.x - 1;
+  int64_t ec = 0, ea = 0;                              // the earlier rows' tokens and fresh pages
+  for (int64_t i = tid; i < r0; i += MROWS) {
+    const MetaRow m = meta_row(A, i);
+    ec += m.c;
+    ea += m.add;
+  }
+  MetaRow m = {0, 0, 0, 0};
+  if (r < A.R) m = meta_row(A, r);
+  int64_t sc = m.c, sa = m.add;                        // inclusive scan over the wave
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t pc = __shfl_up(sc, o, 64), pa = __shfl_up(sa, o, 64);
+    if (lane >= o) { sc += pc; sa += pa; }
+  }
+  ec = wave_sum64(ec);
+  ea = wave_sum64(ea);
+  if (lane == 63) { wc[w] = sc; wa[w] = sa; }
+  if (lane == 0) { bc[w] = ec; ba[w] = ea; }
+  __syncthreads();
+  int64_t basec = bc[0] + bc[1] + bc[2] + bc[3], basea = ba[0] + ba[1] + ba[2] + ba[3];
+  for (int k = 0; k < w; ++k) { basec += wc[k]; basea += wa[k]; }
+  const int64_t f = basec + sc - m.c;                  // the row's first token
+  const int64_t tk = A.held ? min(max(A.taken[0], (int64_t)0), A.nfree) : 0;
+  const int64_t at = tk + basea + sa - m.add;          // its first fresh page in the free list
+  const int64_t got = m.have + max(min(m.add, A.nfree - at), (int64_t)0);
+  first[tid] = f;
+  if (tid == MROWS - 1) first[MROWS] = f + m.c;
+  pos0[tid] = m.n - m.c;
+  page0[tid] = at - m.have;
+  have[tid] = (int32_t)m.have;
+  all[tid] = (int32_t)(A.held ? got : A.npages);
+  if (blockIdx.y == 0 && r < A.R) {
+    A.qsl[r] = min(f, A.tokens);
+    A.lens32[r] = (int32_t)m.n;
+    if (r == A.R - 1) A.qsl[A.R] = min(f + m.c, A.tokens);
+    if (A.held) {
+      A.held_out[r] = (int32_t)got;
+      if (r == A.R - 1) A.taken_out[0] = min(at + m.add, A.nfree);
+      for (int64_t p = m.have; p < got; ++p) A.bt[r * A.bt_stride + p] = A.freep[at + p - m.have];
+    }
+  }
+  __syncthreads();
+  // ---- the tokens of these rows; behind the last row's, the padding
+  const int64_t end = min(first[MROWS], A.tokens), stop = last ? A.tokens : end;
+  for (int64_t t = first[0] + (int64_t)blockIdx.y * MROWS + tid; t < stop; t += (int64_t)gridDim.y * MROWS) {
+    int64_t sl = -1, ps = -1, rw = 0;
+    if (t < end) {
+      int lo = 0;                                      // the last row with first[row] <= t: it holds t
+#pragma unroll
+      for (int s = MROWS / 2; s > 0; s >>= 1)
+        if (first[lo + s] <= t) lo += s;
+      rw = r0 + lo;
+      ps = pos0[lo] + (t - first[lo]);
+      const int64_t pg = ps / A.ebs;
+      int64_t page = -1;
+      if (pg < have[lo]) page = A.bt[rw * A.bt_stride + pg];
+      else if (pg < all[lo]) page = A.freep[page0[lo] + pg];
+      if (page >= 0) sl = page * A.ebs + ps % A.ebs;
+    }
+    A.slot[t] = sl;
+    A.pos[t] = ps;
+    A.row[t] = rw;
+  }
 }
 
 // Streaming-read probe (a measurement aid of bench.py, not part of the cache path): workgroup g reads the 16-byte
@@ -188,6 +308,27 @@ int kv800_hip_step_meta(const int32_t* bt, int64_t bt_stride, int64_t npages, co
   hipLaunchKernelGGL(step_meta_kernel, dim3((unsigned)((R + 255) / 256)), dim3(256), 0, (hipStream_t)stream, bt,
                      bt_stride, npages, lens, R, ebs, slot, pos, lens32);
   return check_launch("step_meta");
+}
+
+int kv800_hip_chunk_meta(int32_t* bt, int64_t bt_stride, int64_t npages, const int64_t* lens, const int32_t* qlens,
+                         int64_t R, int64_t ebs, int64_t tokens, const int32_t* held, const int32_t* free_pages,
+                         int64_t nfree, const int64_t* taken, int32_t* held_out, int64_t* taken_out, int64_t* qsl,
+                         int64_t* slot, int64_t* pos, int64_t* row, int32_t* lens32, void* stream) {
+  KV800_REQUIRE(R >= 1 && ebs > 0 && npages >= 0 && npages <= 0x7FFFFFFF && bt_stride >= npages && tokens >= 0,
+                "chunk_meta: need R >= 1, ebs > 0, bt_stride >= npages >= 0 and tokens >= 0");
+  KV800_REQUIRE((bt || npages == 0) && lens && qlens && qsl && lens32 && (tokens == 0 || (slot && pos && row)),
+                "chunk_meta: null pointer");
+  KV800_REQUIRE(!held || (taken && held_out && taken_out && nfree >= 0 && (free_pages || nfree == 0)),
+                "chunk_meta: a growing table needs the free list, taken, held_out and taken_out");
+  KV800_REQUIRE(!held || (held != held_out && taken != taken_out), "chunk_meta: held and taken are not updated in place");
+  const int64_t nb = (R + MROWS - 1) / MROWS;
+  KV800_REQUIRE(nb <= 0x7FFFFFFF, "chunk_meta: R too large");
+  const int64_t ny = (tokens + nb * 4 * MROWS - 1) / (nb * 4 * MROWS);   // about four tokens a thread
+  const MetaArgs A = {bt, bt_stride, npages, lens, qlens, R, ebs, tokens, held, free_pages, held ? nfree : 0, taken,
+                      held_out, taken_out, qsl, slot, pos, row, lens32};
+  hipLaunchKernelGGL(chunk_meta_kernel, dim3((unsigned)nb, (unsigned)(ny < 1 ? 1 : ny > 256 ? 256 : ny)), dim3(MROWS), 0,
+                     (hipStream_t)stream, A);
+  return check_launch("chunk_meta");
 }
 
 int kv800_hip_read_probe(const void* buf, int64_t bytes, uint32_t* out, int64_t groups, void* stream) {

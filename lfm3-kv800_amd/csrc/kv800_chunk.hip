@@ -1,0 +1,838 @@
+// kv800_chunk.hip -- attention of a few new tokens per row over the paged 800h cache for gfx950 (decode_chunk): the rows of a
+// step that verifies drafted tokens, or brings a short prompt chunk. The reference attends such rows by assembling
+// their whole history as bf16 keys first (vllm_attn.py:351-402); here the compressed blocks and pages are read as they are.
+//
+// Row r has c = qsl[r + 1] - qsl[r] queries at positions N[r] - c + i, 16 query heads over 4 KV heads (head 4 h + e reads KV
+// head h), head_dim 128. Its keys: positions below 256 NQ[r] from the quantized sub-blocks (K = bf16(code ksc + klo),
+// V = (bit vsc + vlo) H), the others from the exact pages, or its sinks; K rotated in fp32 and rounded to bf16 as the model
+// does; scores q . K / sqrt(128), softmax over the positions that the query may see, in fp32.
+//
+// A tile is QT = 4 CT queries of one row; for one KV head they are 16 CT columns (query, query head) of a matrix product,
+// so that the 16 columns of an MFMA, of which a single token fills 4, are all of use: the keys of a chunk are
+// unpacked and rotated once for all of a tile's queries. Tile k of row r has the number r + qsl[r] / QT + k (ascending over
+// the rows without a scan; at most R + T / QT numbers, of which some stay without a tile).
+//
+//   chunk_quant_kernel   the sub-blocks, one workgroup of 4 waves per equal share of the (tile, sub-block) list, wave = KV
+//                        head; writes a partial (m, l, acc) per tile that it enters
+//   chunk_exact_kernel   exact rows and sinks, one workgroup per (tile, KV head); writes a partial, or for layers without
+//                        sub-blocks the output
+//   chunk_merge_kernel   partials of a (tile, KV head) joined, Hadamard transform of the quantized part, bf16 output
+#include <mutex>
+
+#include "kv800_attn.h"
+#include "../../include/kv800_hip.h"
+
+namespace kv800 {
+namespace {
+
+// v_maximum3_f32, which needs no operand quieted first (fmaxf does, for operands straight from an MFMA); NaN wins
+__device__ __forceinline__ float maxn(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+struct ChunkArgs {
+  kv800_paged_t P;
+  const uint16_t* q;
+  const int64_t* qsl;
+  int64_t R, T;
+  const uint16_t *cos_t, *sin_t;   // null: keys as stored
+  const uint32_t* cs2;
+  int64_t rope_rows, qpool_bytes, epool_elems, sink_elems;
+  int64_t G, I;                    // workgroups of the quantized list; tile numbers
+  int64_t* pre;                    // R + 1: the quantized list's entries before each row; then entries per workgroup
+  float *mo, *lo, *ao;             // partial slots: [slot][4 heads][16 CT columns] and, for ao, [128]
+  uint16_t* out;
+  float scale;                     // log2(e) / sqrt(128)
+  int nsink;
+};
+
+// A tile: its row, the row's first token and queries, the tile's first query and queries
+struct Tile { int64_t row, t0; int c, q0, nq; };
+template <int QT>
+__device__ __forceinline__ int64_t tile_number(const int64_t* qsl, int64_t T, int64_t r) { return r + min(qsl[r], T) / QT; }
+// Tile `it`: 64-way search for the last row whose first tile number is <= it, by a whole wave; false if the number has none.
+template <int QT>
+__device__ __forceinline__ bool find_tile(const ChunkArgs& A, int64_t it, Tile& t) {
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = A.R;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 63) / 64, i = lo + lane * step;
+    const int c = __popcll(__ballot(i < hi && tile_number<QT>(A.qsl, A.T, i < hi ? i : lo) <= it));
+    lo += (c > 0 ? c - 1 : 0) * step;
+    hi = min(hi, lo + step);
+  }
+  t.row = lo;
+  t.t0 = min(A.qsl[lo], A.T);
+  t.c = (int)(min(A.qsl[lo + 1], A.T) - t.t0);
+  t.q0 = (int)min((it - (lo + t.t0 / QT)) * QT, (int64_t)0x7FFFFFFF);
+  t.nq = min(QT, t.c - t.q0);
+  return t.nq > 0;
+}
+
+// ---------------------------------------------------------------- quantized sub-blocks
+struct ChunkQ {                // one 32-token chunk's data in registers; lane (g, n) = (lane / 16, lane % 16)
+  uint2 kc[2];                 // tile u: kc bytes of token 16 u + n, channels 8 g .. 8 g + 7
+  u4v cs[2][2];                // [u][d]: (cos, sin) pairs of channels 8 g + 4 d .. + 3 at the token's position
+  uint2 vb;                    // vb bytes 8 (lane % 2) .. + 7 of token lane / 2
+};
+struct QLutWords { uint32_t la, lb, sa, sb; };   // klo / ksc bytes of the table that the lane builds
+struct alignas(16) ChunkQLds {
+  uint32_t lut[4][1024];       // each wave's code tables of the sub-block it is in
+  u4v vb[4][32];               // each wave's copy of its chunk's vb rows, row vb_slot(t) of token t
+  float vs[4][64], vl[4][64];  // decoded vsc / vlo of 64 tokens
+  int64_t ws[4];
+  int64_t row, pre, total;
+};
+
+// 16 tables of 4 groups: block (kind, d, e) of 256 bytes holds the tables of channels 8 g + 4 d + e, g = 0..3, entry (ca, cb)
+// of group g at byte 64 cb + 16 g + 4 ca. Lane l builds the table of g = l % 4, block l / 4.
+__device__ __forceinline__ QLutWords lut_words(rsrc_t rs, int h, int lane) {
+  const int kind = lane >> 5, j = 8 * (lane & 3) + 4 * ((lane >> 4) & 1) + ((lane >> 2) & 3);
+  const int o = 128 * h + 32 * kind + j;
+  return QLutWords{__builtin_amdgcn_raw_buffer_load_b8(rs, o, KLO_O, 0), __builtin_amdgcn_raw_buffer_load_b8(rs, o + 64, KLO_O, 0),
+                   __builtin_amdgcn_raw_buffer_load_b8(rs, o, KSC_O, 0), __builtin_amdgcn_raw_buffer_load_b8(rs, o + 64, KSC_O, 0)};
+}
+__device__ __forceinline__ void lut_build(uint32_t* lut, int lane, const QLutWords& b) {
+  float v[4];
+  f8x4(b.la | (b.lb << 8) | (b.sa << 16) | (b.sb << 24), v);   // klo_a, klo_b, ksc_a, ksc_b
+  uint32_t pa[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) pa[c] = bfpk(fmaf((float)c, v[2], v[0]), fmaf((float)c, v[3], v[1]));
+  uint32_t* tab = lut + 64 * (lane >> 2) + 4 * (lane & 3);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {                                // lanes 4 i .. 4 i + 3 start at row i % 4: all banks at once
+    const int cb = (k + (lane >> 2)) & 3;
+    const uint32_t hi = (cb & 2 ? (cb & 1 ? pa[3] : pa[2]) : (cb & 1 ? pa[1] : pa[0])) & 0xFFFF0000u;
+    *reinterpret_cast<u4v*>(tab + 16 * cb) =
+        u4v{(pa[0] & 0xFFFFu) | hi, (pa[1] & 0xFFFFu) | hi, (pa[2] & 0xFFFFu) | hi, (pa[3] & 0xFFFFu) | hi};
+  }
+}
+__device__ __forceinline__ void chunk_load(ChunkQ& C, rsrc_t rs, rsrc_t rc, int cpos, int t0, int h, int lane) {
+  const int g = lane >> 4, n = lane & 15;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    C.kc[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, n * 128 + 8 * g + 32 * h + 2048 * u,
+                                                                             KC_O + t0 * 128, 0));
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+      C.cs[u][d] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rc, n * 128 + 32 * g + 16 * d + 2048 * u,
+                                                                                 (cpos + t0) * 128, 0));
+  }
+  C.vb = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 64 * (lane >> 1) + 8 * (lane & 1) + 16 * h,
+                                                                        VB_O + t0 * 64, 0));
+}
+__device__ __forceinline__ uint32_t chunk_scales(rsrc_t rs, int t0, int h, int lane) {   // vlo | vsc << 8 of token t0 + lane
+  const int o = 2 * lane + (h >> 1);
+  return (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rs, o, VLO_O + 2 * t0, 0) |
+         ((uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rs, o, VSC_O + 2 * t0, 0) << 8);
+}
+
+// The list of (tile, sub-block) pairs, tile by tile: row r has tiles x sub-blocks of them.
+// Sub-blocks past the host's bound, the offset table or the rope table are not read.
+__device__ __forceinline__ int row_nq(const ChunkArgs& A, int64_t r) { return min(max(A.P.NQ[r], 0), 1 << 22); }
+__device__ __forceinline__ int row_blocks(const ChunkArgs& A, int64_t r) {
+  return (int)min(min((int64_t)row_nq(A, r), A.P.nqmax), min(A.P.boff_stride, A.rope_rows / BLK));
+}
+template <int QT>
+__device__ __forceinline__ int64_t row_pairs(const ChunkArgs& A, int64_t r) {
+  const int64_t c = min(A.qsl[r + 1], A.T) - min(A.qsl[r], A.T);
+  return (max(c, (int64_t)0) + QT - 1) / QT * row_blocks(A, r);
+}
+
+// Attention of one tile's columns of KV head h (the wave's) over sub-blocks [j0, j1) of its row, into partial slot `slot`.
+// As in decode_quant_kernel, with the wave's one head: K pairs by table lookup, RoPE by v_dot2_f32_bf16, Q K^T on bf16 MFMA
+// with exact products; fp32 online softmax with the exact running max (the largest weight is exactly its vsc);
+// P V on fp16 MFMA over the bit planes, weights fp16(p vsc): 11 bits, an eighth of the output's own rounding.
+template <int CT>
+__device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, const Tile& t, int j0, int j1, int64_t slot) {
+  constexpr int NC = 16 * CT;
+  const int h = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, n = lane & 15;
+  const char* lutc = reinterpret_cast<const char*>(&L.lut[0][0]);
+  const int pbase = A.P.N[t.row] - t.c + t.q0;       // position of the tile's first query
+  int pcol[CT];
+  b8 bq[CT][4];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int qi = 4 * ct + (n >> 2);
+    pcol[ct] = pbase + qi;
+    const uint16_t* qr = A.q + ((t.t0 + t.q0 + min(qi, t.nq - 1)) * 16 + 4 * h + (n & 3)) * 128 + 8 * g;
+    const u4v Q0 = *reinterpret_cast<const u4v*>(qr), Q1 = *reinterpret_cast<const u4v*>(qr + 32);
+    const u4v Q2 = *reinterpret_cast<const u4v*>(qr + 64), Q3 = *reinterpret_cast<const u4v*>(qr + 96);
+    auto el = [](const u4v& Q, int i) -> uint32_t { return (Q[i >> 1] >> (16 * (i & 1))) & 0xFFFFu; };
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      uint32_t r[4], p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        r[e] = el(Q0, 4 * d + e) | (el(Q2, 4 * d + e) << 16);
+        p[e] = el(Q1, 4 * d + e) | (el(Q3, 4 * d + e) << 16);
+      }
+      bq[ct][d] = pack8b(r);
+      bq[ct][2 + d] = pack8b(p);
+    }
+  }
+  float m[CT], lsum[CT], lvs[CT];
+  f4 acc[CT][8];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = NEG_BIG; lsum[ct] = 0.f; lvs[ct] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[ct][i] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale = A.scale;
+  auto stage_scales = [&](uint32_t x) {
+    float v[4];
+    f8x4(x, v);
+    L.vl[h][lane] = v[0];
+    L.vs[h][lane] = v[1];
+  };
+  const uint32_t kg = (uint32_t)h * 4096u + 16u * (uint32_t)g;
+  // one 32-token chunk, tokens 32 cc .. of the staged 64; kpos: position of its first token
+  auto chunk = [&](const ChunkQ& C, int cc, int kpos) {
+    {
+      const int tk = lane >> 1;
+      asm volatile("" ::: "memory");
+      reinterpret_cast<uint2*>(&L.vb[h][vb_slot(tk)])[lane & 1] = C.vb;
+      asm volatile("" ::: "memory");
+    }
+    f4 sc[2][CT];
+    __builtin_amdgcn_s_setprio(3);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t kk[2][4], an[2][4];
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const uint32_t x = d ? C.kc[u].y : C.kc[u].x;
+        const uint32_t xr = (x << 2) & 0xCCCCCCCCu, xn = x & 0xCCCCCCCCu;
+        const char *br = lutc + 256 * (4 * d), *bn = lutc + 256 * (8 + 4 * d);
+        kk[d][0] = *reinterpret_cast<const uint32_t*>(br + byte_or<0>(xr, kg));
+        an[d][0] = *reinterpret_cast<const uint32_t*>(bn + byte_or<0>(xn, kg));
+        kk[d][1] = *reinterpret_cast<const uint32_t*>(br + 256 + byte_or<1>(xr, kg));
+        an[d][1] = *reinterpret_cast<const uint32_t*>(bn + 256 + byte_or<1>(xn, kg));
+        kk[d][2] = *reinterpret_cast<const uint32_t*>(br + 512 + byte_or<2>(xr, kg));
+        an[d][2] = *reinterpret_cast<const uint32_t*>(bn + 512 + byte_or<2>(xn, kg));
+        kk[d][3] = *reinterpret_cast<const uint32_t*>(br + 768 + byte_or<3>(xr, kg));
+        an[d][3] = *reinterpret_cast<const uint32_t*>(bn + 768 + byte_or<3>(xn, kg));
+      }
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        uint32_t c4[4], s4[4], ar[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          c4[e] = C.cs[u][d][e];
+          s4[e] = __builtin_amdgcn_alignbit(C.cs[u][d][e], C.cs[u][d][e], 16);
+        }
+        rope4(kk[d], c4, s4, ar);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          sc[u][ct] = mfma_bf(pack8b(ar), bq[ct][d], d == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sc[u][ct]);
+          sc[u][ct] = mfma_bf(pack8b(an[d]), bq[ct][2 + d], sc[u][ct]);
+        }
+      }
+    }
+    __builtin_amdgcn_s_setprio(2);
+    if (kpos + 31 > pbase) {                           // a caller's NQ that reaches into the new tokens: mask by position
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (kpos + 16 * u + 4 * g + i > pcol[ct]) sc[u][ct][i] = -INFINITY;
+    }
+    h8 Bw[CT];
+    float4 vs4[2], vl4[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int tk = 32 * cc + 16 * u + 4 * g;
+      vs4[u] = *reinterpret_cast<const float4*>(&L.vs[h][tk]);
+      vl4[u] = *reinterpret_cast<const float4*>(&L.vl[h][tk]);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const f4 s0 = sc[0][ct], s1 = sc[1][ct];
+      float tmax = maxn(maxn(maxn(s0[0], s0[1]), maxn(s0[2], s0[3])), maxn(maxn(s1[0], s1[1]), maxn(s1[2], s1[3])));
+      tmax = max4rows(tmax) * scale;
+      if (__any(tmax > m[ct])) {
+        const float mn = fmaxf(m[ct], tmax);
+        const float al = __builtin_amdgcn_exp2f(m[ct] - mn);
+        m[ct] = mn; lsum[ct] *= al; lvs[ct] *= al;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[ct][i] *= al;
+      }
+      float wt[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][0], scale, -m[ct]));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][1], scale, -m[ct]));
+        const float p2 = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][2], scale, -m[ct]));
+        const float p3 = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][3], scale, -m[ct]));
+        lsum[ct] += (p0 + p1) + (p2 + p3);
+        lvs[ct] += (p0 * vl4[u].x + p1 * vl4[u].y) + (p2 * vl4[u].z + p3 * vl4[u].w);
+        wt[u][0] = p0 * vs4[u].x; wt[u][1] = p1 * vs4[u].y; wt[u][2] = p2 * vs4[u].z; wt[u][3] = p3 * vs4[u].w;
+      }
+      Bw[ct] = pack8(pk2(wt[0][0], wt[0][2]), pk2(wt[0][1], wt[0][3]), pk2(wt[1][0], wt[1][2]), pk2(wt[1][1], wt[1][3]));
+    }
+    __builtin_amdgcn_s_setprio(0);
+    typedef __attribute__((address_space(3))) i2v lds_i2;
+    const i2v X = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(reinterpret_cast<char*>(L.vb[h]) + 128 * g + 8 * n));
+    const uint32_t x0 = (uint32_t)X.x, x1 = (uint32_t)X.x >> 8, x2 = (uint32_t)X.y, x3 = (uint32_t)X.y >> 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t msk = (1u << i) | (1u << (16 + i));
+      const h8 a = pack8(x0 & msk, x1 & msk, x2 & msk, x3 & msk);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) acc[ct][i] = mfma16(a, Bw[ct], acc[ct][i]);
+    }
+    asm volatile("" ::: "memory");
+  };
+
+  // the span's 4 (j1 - j0) pairs of chunks, one after the other; loads one chunk ahead, tables and scales one pair ahead
+  const int64_t* brow = A.P.boff + t.row * A.P.boff_stride;
+  auto sanitize = [&](int64_t raw, int jb) -> int64_t {
+    return (raw < 0 || raw > A.qpool_bytes - SUB || (int64_t)(jb + 1) * BLK > A.rope_rows) ? -1 : raw;
+  };
+  const rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(A.cs2), (short)0,
+                                                      (int)min(A.rope_rows * 128, (int64_t)INT32_MAX), RSRC_WORD3);
+  int jb = j0, pin = 0;
+  int64_t base = sanitize(brow[jb], jb), nraw = brow[min(jb + 1, j1 - 1)];
+  rsrc_t rs = sub_rsrc(A.P.qpool + (base < 0 ? 0 : base));
+  int cpos = base < 0 ? 0 : jb * BLK;
+  ChunkQ C0, C1;
+  chunk_load(C0, rs, rc, cpos, 0, h, lane);
+  lut_build(L.lut[h], lane, lut_words(rs, h, lane));
+  stage_scales(chunk_scales(rs, 0, h, lane));
+  const int np = 4 * (j1 - j0);
+  for (int p = 0; p < np; ++p) {
+    const bool more = p + 1 < np, cross = more && pin == 3;
+    const int njb = cross ? jb + 1 : jb, npin = cross ? 0 : (pin + 1) & 3;
+    int64_t nbase = base;
+    rsrc_t nrs = rs;
+    int ncpos = cpos;
+    if (cross) {
+      nbase = sanitize(nraw, njb);
+      nrs = sub_rsrc(A.P.qpool + (nbase < 0 ? 0 : nbase));
+      ncpos = nbase < 0 ? 0 : njb * BLK;
+      nraw = brow[min(njb + 1, j1 - 1)];
+    }
+    const QLutWords nlw = lut_words(nrs, h, lane);
+    const uint32_t nsc = chunk_scales(nrs, 64 * npin, h, lane);
+    chunk_load(C1, rs, rc, cpos, 64 * pin + 32, h, lane);
+    if (base >= 0) chunk(C0, 0, cpos + 64 * pin);
+    chunk_load(C0, nrs, rc, ncpos, 64 * npin, h, lane);
+    if (base >= 0) chunk(C1, 1, cpos + 64 * pin + 32);
+    if (more) {
+      if (cross) lut_build(L.lut[h], lane, nlw);
+      stage_scales(nsc);
+    }
+    jb = njb; pin = npin; base = nbase; rs = nrs; cpos = ncpos;
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float ls = sum4rows(lsum[ct]), lv = sum4rows(lvs[ct]);
+    if (4 * ct + (n >> 2) < t.nq) {
+      const int64_t col = (slot * 4 + h) * NC + 16 * ct + n;
+      if (g == 0) { A.mo[col] = m[ct]; A.lo[col] = ls; }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {                    // plane i: dims 16 i + 4 g + r, bits worth 2^(i - 24)
+        const float ps = __uint_as_float((uint32_t)(127 + 24 - i) << 23);
+        const f4 o = acc[ct][i];
+        *reinterpret_cast<float4*>(A.ao + col * 128 + 16 * i + 4 * g) =
+            make_float4(o[0] * ps + lv, o[1] * ps + lv, o[2] * ps + lv, o[3] * ps + lv);
+      }
+    }
+  }
+}
+
+// Workgroup w takes entries [w C, (w + 1) C) of the list, C = ceil(total / G). The part of a tile that it begins with goes
+// to slot w; a tile that starts inside its range goes to slot G + the tile's number (nobody else enters that tile from an
+// earlier entry).
+template <int CT>
+__global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
+  constexpr int QT = 4 * CT;
+  __shared__ ChunkQLds L;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  // every workgroup sums the rows' entries itself: thread i takes the rows [i k, i k + k)
+  const int64_t k = (A.R + 255) / 256, ra = min((int64_t)tid * k, A.R), rb = min(ra + k, A.R);
+  int64_t mine = 0;
+  for (int64_t r = ra; r < rb; ++r) mine += row_pairs<QT>(A, r);
+  int64_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t x = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += x;
+  }
+  if (lane == 63) L.ws[w] = inc;
+  __syncthreads();
+  int64_t pre = inc - mine;
+  for (int i = 0; i < w; ++i) pre += L.ws[i];
+  const int64_t total = L.ws[0] + L.ws[1] + L.ws[2] + L.ws[3], C = (total + A.G - 1) / A.G;
+  if (blockIdx.x == 0) {                               // for the merge
+    int64_t x = pre;
+    for (int64_t r = ra; r < rb; ++r) { A.pre[r] = x; x += row_pairs<QT>(A, r); }
+    if (tid == 0) A.pre[A.R] = C;
+  }
+  int64_t v = (int64_t)blockIdx.x * C;
+  const int64_t v1 = min(v + C, total);
+  if (v >= v1) return;                                 // uniform
+  if (v >= pre && v < pre + mine) {                    // one thread
+    int64_t x = pre;
+    for (int64_t r = ra; r < rb; ++r) {
+      const int64_t y = row_pairs<QT>(A, r);
+      if (v < x + y) { L.row = r; L.pre = x; break; }
+      x += y;
+    }
+  }
+  __syncthreads();
+  int64_t r = L.row, x = L.pre;
+  bool first = true;
+  while (v < v1) {
+    const int64_t y = row_pairs<QT>(A, r);
+    if (v >= x + y) { x += y; ++r; continue; }
+    const int nb = row_blocks(A, r);
+    const int64_t tile = (v - x) / nb;
+    const int j0 = (int)((v - x) - tile * nb), j1 = (int)min((int64_t)nb, j0 + (v1 - v));
+    Tile t;
+    t.row = r;
+    t.t0 = min(A.qsl[r], A.T);
+    t.c = (int)(min(A.qsl[r + 1], A.T) - t.t0);
+    t.q0 = (int)(tile * QT);
+    t.nq = min(QT, t.c - t.q0);
+    chunk_span<CT>(L, A, t, j0, j1, first ? (int64_t)blockIdx.x : A.G + tile_number<QT>(A.qsl, A.T, r) + tile);
+    first = false;
+    v += j1 - j0;
+  }
+}
+
+// ---------------------------------------------------------------- exact rows and sinks
+// NW waves per (tile, KV head) take the 32-token chunks of the tile's keys in turn and join their states at the end. The keys
+// in order: the row's sinks, exact positions below the sink count (kept out of the window too), exact positions from the
+// first one in a query's window up to the last query. As decode_exact_kernel otherwise: Q K^T and P V on bf16 MFMA, weights
+// as hi + lo bf16 pairs (16 bits), V^T by transposed reads from an LDS copy.
+constexpr int XCH = 32, XVROW = 144;
+template <int CT, int NW>
+struct alignas(16) ChunkXLds {
+  union {
+    uint16_t v[NW][XCH][XVROW];
+    float o[NW > 1 ? NW - 1 : 1][16 * CT][132];   // the end: the other waves' accumulators, scaled to the common max
+  };
+  float m[NW][16 * CT], l[NW][16 * CT];
+};
+struct ChunkX {                        // one chunk in registers; lane (g, n): token 16 u + n of tile u
+  u4v k[2][4], v[2][4], c[2], s[2];    // K, V dims 32 s + 8 g .. + 7; cos / sin of channels 8 g .. + 7
+  uint32_t ok;                         // chunk tokens with a key
+};
+
+template <int CT, int NW, bool DIRECT>
+__global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
+  constexpr int QT = 4 * CT, NC = 16 * CT;
+  __shared__ ChunkXLds<CT, NW> L;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, g = lane >> 4, n = lane & 15;
+  if (DIRECT && (int64_t)blockIdx.x == 4 * A.I) {      // the padding's output rows
+    const int64_t e0 = min(A.qsl[A.R], A.T) * 256;
+    for (int64_t i = e0 + tid; i < A.T * 256; i += 64 * NW) reinterpret_cast<u4v*>(A.out)[i] = u4v{0u, 0u, 0u, 0u};
+    return;
+  }
+  const int64_t it = blockIdx.x >> 2;
+  const int h = blockIdx.x & 3;
+  Tile t;
+  if (!find_tile<QT>(A, it, t)) return;
+  const int N = A.P.N[t.row], win = (int)A.P.win;
+  const int pbase = N - t.c + t.q0, plast = pbase + t.nq - 1;
+  // key list: sinks [0, cnt), exact positions lo_row .. + cnt2, then lo_tile ..
+  int lo_row, lo_tile;
+  if (win > 0) {
+    lo_row = max(0, N - t.c - (win - 1));
+    lo_tile = max(lo_row, pbase - (win - 1));
+  } else {
+    lo_row = lo_tile = A.P.NQ ? row_nq(A, t.row) * BLK : 0;
+  }
+  const int hi = min(N, plast + 1);
+  const int cnt = max(0, min(min(A.nsink, lo_row), hi));
+  const int cnt2 = win > 0 ? max(0, min(min(A.nsink, hi) - lo_row, lo_tile - lo_row)) : 0;
+  const int rest = lo_tile - cnt - cnt2;               // list index i >= cnt + cnt2 is position rest + i
+  const int nk = cnt + cnt2 + max(0, hi - lo_tile);
+  const int64_t* et = A.P.eoff + t.row * A.P.eoff_stride;
+  const int64_t sko = cnt ? A.P.skoff[t.row] : 0, svo = cnt ? A.P.svoff[t.row] : 0;
+  const bool rot = A.cos_t != nullptr;
+  auto posof = [&](int i) { return i < cnt ? i : i < cnt + cnt2 ? lo_row + i - cnt : rest + i; };
+  const uint16_t* qf = A.q + t.t0 * 2048 + 8 * g;      // what lanes without a key read (finite or not, their weight is zero)
+  auto load = [&](int c0, ChunkX& C) {
+    uint32_t okm = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = c0 + 16 * u + n;
+      const uint16_t *kr = qf, *vr = qf, *cr = qf, *sr = qf;
+      bool ok = false;
+      if (i < nk) {
+        const int pos = posof(i);
+        int64_t ko, vo;
+        if (i < cnt) {
+          ko = sko + ((int64_t)i * 4 + h) * 128;
+          vo = svo + ((int64_t)i * 4 + h) * 128;
+          ok = ko >= 0 && vo >= 0 && ko + 128 <= A.sink_elems && vo + 128 <= A.sink_elems;
+          kr = A.P.sk; vr = A.P.sv;
+        } else {
+          const int64_t pg = pos / A.P.ebs;
+          const int64_t b = pg < A.P.eoff_stride ? et[pg] : -1;
+          ko = b + h * A.P.e_hs + (pos - pg * A.P.ebs) * A.P.e_ts;
+          vo = ko + A.P.e_v;
+          ok = b >= 0 && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
+          kr = vr = A.P.epool;
+        }
+        ok = ok && (!rot || pos < A.rope_rows);
+        if (ok) {
+          kr += ko + 8 * g;
+          vr += vo + 8 * g;
+          if (rot) { cr = A.cos_t + (int64_t)pos * 32 + 8 * g; sr = A.sin_t + (int64_t)pos * 32 + 8 * g; }
+        } else {
+          kr = vr = qf;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) C.k[u][s] = *reinterpret_cast<const u4v*>(kr + 32 * s);
+      C.c[u] = *reinterpret_cast<const u4v*>(cr);
+      C.s[u] = *reinterpret_cast<const u4v*>(sr);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) C.v[u][s] = *reinterpret_cast<const u4v*>(vr + 32 * s);
+      if (!ok) {                                       // a zero weight times a NaN would be one
+#pragma unroll
+        for (int s = 0; s < 4; ++s) C.v[u][s] = u4v{0u, 0u, 0u, 0u};
+      }
+      okm |= ((uint32_t)__ballot(ok) & 0xFFFFu) << (16 * u);
+    }
+    C.ok = okm;
+  };
+  b8 bq[CT][4];
+  int pcol[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int qi = 4 * ct + (n >> 2);
+    pcol[ct] = pbase + qi;
+    const uint16_t* qr = A.q + ((t.t0 + t.q0 + min(qi, t.nq - 1)) * 16 + 4 * h + (n & 3)) * 128 + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) bq[ct][s] = as_b8(*reinterpret_cast<const u4v*>(qr + 32 * s));
+  }
+  float m[CT], lsum[CT];
+  f4 acc[CT][8];                                       // dims 16 j + 4 g + i of column n
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = NEG_BIG; lsum[ct] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[ct][j] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  uint16_t (*Vs)[XVROW] = L.v[w];
+  auto body = [&](const ChunkX& C, int c0) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) *reinterpret_cast<u4v*>(&Vs[16 * u + n][32 * s + 8 * g]) = C.v[u][s];
+    f4 sc[2][CT];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      u4v a0 = C.k[u][0], a2 = C.k[u][2];
+      if (rot) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          float r0[2], r2[2];
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+#pragma clang fp contract(off)   // products rounded before the sum, as torch_decode.py:22-23 evaluates them
+            const float k0 = bf_elem(C.k[u][0], e + d), k2 = bf_elem(C.k[u][2], e + d);
+            const float cs = bf_elem(C.c[u], e + d), sn = bf_elem(C.s[u], e + d);
+            r0[d] = k0 * cs - k2 * sn;
+            r2[d] = k2 * cs + k0 * sn;
+          }
+          a0[e >> 1] = bfpk(r0[0], r0[1]);
+          a2[e >> 1] = bfpk(r2[0], r2[1]);
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        f4 x = {0.f, 0.f, 0.f, 0.f};
+        x = mfma_bf(as_b8(a0), bq[ct][0], x);
+        x = mfma_bf(as_b8(C.k[u][1]), bq[ct][1], x);
+        x = mfma_bf(as_b8(a2), bq[ct][2], x);
+        sc[u][ct] = mfma_bf(as_b8(C.k[u][3]), bq[ct][3], x);
+      }
+    }
+    const uint32_t tb = C.ok >> (4 * g);               // bit 16 u + i: token 16 u + 4 g + i
+    int kp[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kp[u][i] = ((tb >> (16 * u + i)) & 1u) ? posof(c0 + 16 * u + 4 * g + i) : 0x7FFFFFFF;
+    u4v bh[CT], bl[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float xs[2][4], cm = -INFINITY;
+      const int wlo = win > 0 ? pcol[ct] - win : -1;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool keep = kp[u][i] <= pcol[ct] && (kp[u][i] > wlo || kp[u][i] < A.nsink);
+          xs[u][i] = keep ? sc[u][ct][i] * A.scale : -INFINITY;
+          cm = fmaxf(cm, xs[u][i]);
+        }
+      cm = max4rows(cm);
+      if (__any(cm > m[ct])) {
+        const float mn = fmaxf(m[ct], cm), al = __builtin_amdgcn_exp2f(m[ct] - mn);
+        m[ct] = mn;
+        lsum[ct] *= al;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[ct][j] *= al;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int u = k >> 1, i = 2 * (k & 1);
+        const float pa = __builtin_amdgcn_exp2f(xs[u][i] - m[ct]), pb = __builtin_amdgcn_exp2f(xs[u][i + 1] - m[ct]);
+        lsum[ct] += pa + pb;
+        bh[ct][k] = bfpk(pa, pb);
+        bl[ct][k] = bfpk(pa - __uint_as_float(bh[ct][k] << 16), pb - __uint_as_float(bh[ct][k] & 0xFFFF0000u));
+      }
+    }
+    asm volatile("" ::: "memory");   // the staged V rows are written before the transposed reads
+    const int vrow = 4 * g + (n >> 2), vcol = 4 * (n & 3);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const s4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&Vs[vrow][16 * j + vcol]);
+      const s4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&Vs[vrow + 16][16 * j + vcol]);
+      const u4v av = {__builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 0, 1)),
+                      __builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 2, 3)),
+                      __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 0, 1)),
+                      __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 2, 3))};
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        acc[ct][j] = mfma_bf(as_b8(av), as_b8(bh[ct]), acc[ct][j]);
+        acc[ct][j] = mfma_bf(as_b8(av), as_b8(bl[ct]), acc[ct][j]);
+      }
+    }
+    asm volatile("" ::: "memory");   // and read before the next chunk's rows overwrite them
+  };
+  constexpr int STEP = NW * XCH;
+  if (w * XCH < nk) {
+    ChunkX C0, C1;
+    load(w * XCH, C0);
+    for (int c0 = w * XCH;;) {
+      load(c0 + STEP, C1);
+      body(C0, c0);
+      c0 += STEP;
+      if (c0 >= nk) break;
+      load(c0 + STEP, C0);
+      body(C1, c0);
+      c0 += STEP;
+      if (c0 >= nk) break;
+    }
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) lsum[ct] = sum4rows(lsum[ct]);
+  if (NW > 1) {
+    __syncthreads();                                   // every wave is done with its V rows
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+      if (g == 0) { L.m[w][16 * ct + n] = m[ct]; L.l[w][16 * ct + n] = lsum[ct]; }
+    __syncthreads();
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float M = NEG_BIG, l = 0.f;
+      for (int k = 0; k < NW; ++k) M = fmaxf(M, L.m[k][16 * ct + n]);
+      for (int k = 0; k < NW; ++k) l += L.l[k][16 * ct + n] * __builtin_amdgcn_exp2f(L.m[k][16 * ct + n] - M);
+      const float f = __builtin_amdgcn_exp2f(m[ct] - M);
+      m[ct] = M;
+      lsum[ct] = l;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[ct][j] *= f;
+        if (w > 0) *reinterpret_cast<f4*>(&L.o[w - 1][16 * ct + n][16 * j + 4 * g]) = acc[ct][j];
+      }
+    }
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        for (int k = 0; k < NW - 1; ++k) acc[ct][j] += *reinterpret_cast<const f4*>(&L.o[k][16 * ct + n][16 * j + 4 * g]);
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int qi = 4 * ct + (n >> 2);
+    if (qi >= t.nq) continue;
+    if (DIRECT) {
+      const float inv = lsum[ct] > 0.f ? 1.0f / lsum[ct] : 0.f;
+      uint16_t* o = A.out + ((t.t0 + t.q0 + qi) * 16 + 4 * h + (n & 3)) * 128 + 4 * g;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const f4 a = acc[ct][j];
+        *reinterpret_cast<uint2*>(o + 16 * j) = make_uint2(bfpk(a[0] * inv, a[1] * inv), bfpk(a[2] * inv, a[3] * inv));
+      }
+    } else {
+      const int64_t col = ((A.G + A.I + it) * 4 + h) * NC + 16 * ct + n;
+      if (g == 0) { A.mo[col] = m[ct]; A.lo[col] = lsum[ct]; }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) *reinterpret_cast<f4*>(A.ao + col * 128 + 16 * j + 4 * g) = acc[ct][j];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- merge
+// One workgroup per (tile, KV head), a wave per column in turn; lane = dims 2 lane, 2 lane + 1.
+template <int CT>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
+  constexpr int QT = 4 * CT, NC = 16 * CT;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  if ((int64_t)blockIdx.x == 4 * A.I) {                // the padding's output rows
+    const int64_t e0 = min(A.qsl[A.R], A.T) * 256;
+    for (int64_t i = e0 + tid; i < A.T * 256; i += 256) reinterpret_cast<u4v*>(A.out)[i] = u4v{0u, 0u, 0u, 0u};
+    return;
+  }
+  const int64_t it = blockIdx.x >> 2;
+  const int h = blockIdx.x & 3;
+  Tile t;
+  if (!find_tile<QT>(A, it, t)) return;
+  const int64_t C = A.pre[A.R], nb = row_blocks(A, t.row);
+  const int64_t s = A.pre[t.row] + t.q0 / QT * nb, e = s + nb;   // the tile's entries of the list
+  const int64_t w0 = nb ? s / C : 0, w1 = nb ? (e - 1) / C : -1;
+  const int dd = 2 * lane;
+  for (int c = w; c < 4 * t.nq; c += 4) {
+    const int64_t cx = ((A.G + A.I + it) * 4 + h) * NC + c;
+    auto slot = [&](int64_t k) { return ((k * C >= s ? k : A.G + it) * 4 + h) * NC + c; };
+    const float mx = A.mo[cx];
+    float M = mx;
+    for (int64_t k = w0; k <= w1; ++k) M = fmaxf(M, A.mo[slot(k)]);
+    const float fx = __builtin_amdgcn_exp2f(mx - M);
+    float l = fx * A.lo[cx], x0 = 0.f, x1 = 0.f;
+    for (int64_t k = w0; k <= w1; ++k) {
+      const int64_t p = slot(k);
+      const float f = __builtin_amdgcn_exp2f(A.mo[p] - M);
+      const float2 a = *reinterpret_cast<const float2*>(A.ao + p * 128 + dd);
+      l += f * A.lo[p];
+      x0 += f * a.x;
+      x1 += f * a.y;
+    }
+    {                                                  // H x: bit 0 of the dim in the lane, bits 1..6 across the lanes
+      const float a = x0, b = x1;
+      x0 = a + b;
+      x1 = a - b;
+    }
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      const int msk = 1 << k;
+      const float p0 = __shfl_xor(x0, msk), p1 = __shfl_xor(x1, msk);
+      x0 = (lane & msk) ? p0 - x0 : x0 + p0;
+      x1 = (lane & msk) ? p1 - x1 : x1 + p1;
+    }
+    const float hn = __uint_as_float(0x3DB504F3u);     // 1 / sqrt(128)
+    const float2 a = *reinterpret_cast<const float2*>(A.ao + cx * 128 + dd);
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const int64_t tok = t.t0 + t.q0 + (c >> 2);
+    *reinterpret_cast<uint32_t*>(A.out + (tok * 16 + 4 * h + (c & 3)) * 128 + dd) =
+        bfpk((x0 * hn + fx * a.x) * inv, (x1 * hn + fx * a.y) * inv);
+  }
+}
+
+// queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8
+int chunk_ct(int64_t R, int64_t T) { return T <= 4 * R ? 1 : 2; }
+
+int64_t chunk_groups() {
+  static std::mutex mu;
+  static int64_t cache[64] = {0};
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) { (void)hipGetLastError(); return 512; }
+  std::lock_guard<std::mutex> lock(mu);
+  if (cache[dev] == 0) {
+    int cu = 0;
+    if (hipDeviceGetAttribute(&cu, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cu <= 0) {
+      (void)hipGetLastError();
+      cu = 256;
+    }
+    cache[dev] = 2 * (int64_t)cu;
+  }
+  return cache[dev];
+}
+
+struct ChunkPlan { int ct; int64_t G, I, cols, pre; };   // cols: partial columns; pre: int64 entries
+ChunkPlan chunk_plan(int64_t R, int64_t T, int64_t nqmax) {
+  ChunkPlan p;
+  p.ct = chunk_ct(R, T);
+  p.I = R + T / (4 * p.ct);
+  p.G = nqmax > 0 ? chunk_groups() : 0;
+  p.cols = nqmax > 0 ? (p.G + 2 * p.I) * 64 * p.ct : 0;
+  p.pre = nqmax > 0 ? (R + 2) / 2 * 2 : 0;
+  return p;
+}
+
+template <int CT>
+int chunk_launch(const ChunkArgs& A, bool quant, hipStream_t s) {
+  const unsigned nx = (unsigned)(4 * A.I);
+  if (quant) {
+    hipLaunchKernelGGL(chunk_quant_kernel<CT>, dim3((unsigned)A.G), dim3(256), 0, s, A);
+    int rc = check_launch("chunk_quant");
+    if (rc != KV800_OK) return rc;
+    hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, false>), dim3(nx), dim3(256), 0, s, A);
+    rc = check_launch("chunk_exact");
+    if (rc != KV800_OK) return rc;
+    hipLaunchKernelGGL(chunk_merge_kernel<CT>, dim3(nx + 1), dim3(256), 0, s, A);
+    return check_launch("chunk_merge");
+  }
+  hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, true>), dim3(nx + 1), dim3(256), 0, s, A);
+  return check_launch("chunk_exact");
+}
+
+}  // namespace
+}  // namespace kv800
+
+using namespace kv800;
+
+extern "C" {
+
+int64_t kv800_hip_decode_chunk_workspace(int64_t R, int64_t T, int64_t nqmax) {
+  if (R <= 0 || T <= 0 || nqmax <= 0) return 0;
+  const ChunkPlan p = chunk_plan(R, T, nqmax);
+  return p.pre * 8 + p.cols * 130 * 4;
+}
+
+int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int64_t* qsl, int64_t R, int64_t T,
+                           const uint16_t* cos_t, const uint16_t* sin_t, int64_t rope_rows, const uint32_t* cs2,
+                           int64_t qpool_bytes, int64_t epool_elems, int64_t sink_elems, uint16_t* out, void* ws,
+                           int64_t ws_bytes, void* stream) {
+  KV800_REQUIRE(P && R >= 0 && T >= 0 && (R > 0 || T == 0), "decode_chunk: bad row or token count");
+  if (T == 0) return KV800_OK;
+  KV800_REQUIRE(q && qsl && out && P->epool && P->eoff && P->N, "decode_chunk: null pointer");
+  KV800_REQUIRE(P->ebs > 0 && P->eoff_stride > 0 && P->win >= 0 && P->win < (1LL << 31) && P->nqmax >= 0,
+                "decode_chunk: bad page geometry, window or nqmax");
+  KV800_REQUIRE(P->e_hs % 8 == 0 && P->e_ts % 8 == 0 && P->e_v % 8 == 0, "decode_chunk: strides must be multiples of 8 elements");
+  KV800_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)P->epool) % 16 == 0, "decode_chunk: q, out and epool must be 16-byte aligned");
+  KV800_REQUIRE((cos_t == nullptr) == (sin_t == nullptr), "decode_chunk: cos and sin tables go together");
+  KV800_REQUIRE(!cos_t || ((((uintptr_t)cos_t | (uintptr_t)sin_t) % 16) == 0 && rope_rows > 0),
+                "decode_chunk: rope tables must be 16-byte aligned and not empty");
+  const bool quant = P->win == 0 && P->nqmax > 0;
+  if (quant)
+    KV800_REQUIRE(P->qpool && P->boff && P->boff_stride > 0 && P->NQ && cos_t && cs2 && qpool_bytes >= SUB && (uintptr_t)cs2 % 16 == 0 &&
+                      (uintptr_t)P->qpool % 16 == 0,
+                  "decode_chunk: quantized layers need NQ, the quant pool (16-byte aligned, one sub-block at least), its offsets and the rope tables");
+  const bool sinks = P->win > 0 && P->sk;
+  KV800_REQUIRE(!sinks || (P->sv && P->skoff && P->svoff && (((uintptr_t)P->sk | (uintptr_t)P->sv) % 16) == 0),
+                "decode_chunk: sinks need sv, skoff, svoff and 16-byte aligned buffers");
+  const ChunkPlan p = chunk_plan(R, T, quant ? P->nqmax : 0);
+  KV800_REQUIRE(p.I <= (1LL << 28), "decode_chunk: too many rows and tokens");
+  KV800_REQUIRE(!quant || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= kv800_hip_decode_chunk_workspace(R, T, P->nqmax)),
+                "decode_chunk: the workspace is too small or not 16-byte aligned");
+  ChunkArgs A;
+  A.P = *P;
+  A.q = q; A.qsl = qsl; A.R = R; A.T = T;
+  A.cos_t = cos_t; A.sin_t = sin_t; A.cs2 = cs2;
+  A.rope_rows = rope_rows; A.qpool_bytes = qpool_bytes; A.epool_elems = epool_elems; A.sink_elems = sink_elems;
+  A.G = p.G; A.I = p.I;
+  A.pre = reinterpret_cast<int64_t*>(ws);
+  A.ao = quant ? reinterpret_cast<float*>(A.pre + p.pre) : nullptr;
+  A.mo = quant ? A.ao + p.cols * 128 : nullptr;
+  A.lo = quant ? A.mo + p.cols : nullptr;
+  A.out = out;
+  A.scale = 1.4426950408889634f * 0.08838834764831845f;
+  A.nsink = sinks ? NSINK : 0;
+  const hipStream_t s = (hipStream_t)stream;
+  return p.ct == 1 ? chunk_launch<1>(A, quant, s) : chunk_launch<2>(A, quant, s);
+}
+
+}  // extern "C"

@@ -12,6 +12,7 @@ import ctypes
 import math
 import os
 from collections import OrderedDict
+from dataclasses import dataclass
 
 import numpy as np
 
@@ -83,6 +84,11 @@ SIGNATURES = {
     "kv800_hip_fake_quant_v": (_I32, [_VP, _I64, _VP, _VP]),
     "kv800_hip_decode_noalloc": (_I32, [ctypes.POINTER(Paged), _VP, _I64, _VP, _VP, _I64, _VP, _I64, _I64, _I64, _VP,
                                         _I64, _VP]),
+    "kv800_hip_chunk_meta": (_I32, [_VP, _I64, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _VP, _VP, _VP, _VP,
+                                    _VP, _VP, _VP, _VP]),
+    "kv800_hip_decode_chunk_workspace": (_I64, [_I64, _I64, _I64]),
+    "kv800_hip_decode_chunk": (_I32, [ctypes.POINTER(Paged), _VP, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _I64, _I64,
+                                      _VP, _VP, _I64, _VP]),
 }
 
 
@@ -133,6 +139,23 @@ def _ptr(t):
 
 def _stream(dev):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+class _Here:
+    """The current device already: nothing to switch."""
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(dev):
+    """Context in which dev is the current device: a launch goes to the current device's queue, whatever its stream."""
+    return _HERE if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _extent(t):
@@ -290,6 +313,60 @@ def step_meta(bt, lens, ebs):
     _check(L.kv800_hip_step_meta(_ptr(bt), bt.stride(0), bt.shape[1], _ptr(lens.contiguous()), R, int(ebs), _ptr(slot),
                                  _ptr(pos), _ptr(l32), _stream(dev)))
     return slot, pos, l32
+
+
+@dataclass
+class ChunkMeta:
+    """A step's new tokens, made on the device by chunk_meta: qsl (R + 1,) int64 row starts; slot, pos, row (tokens,) int64
+    per token (padding: -1, -1, 0); lens32 (R,) int32; held (R,) int32 and taken (1,) int64 page counts behind the step, or
+    None."""
+    qsl: torch.Tensor
+    slot: torch.Tensor
+    pos: torch.Tensor
+    row: torch.Tensor
+    lens32: torch.Tensor
+    held: torch.Tensor = None
+    taken: torch.Tensor = None
+
+
+def chunk_meta(bt, lens, qlens, ebs, tokens, held=None, free=None, taken=None):
+    """ChunkMeta of a step whose rows bring qlens[r] new tokens each (kv800_hip_chunk_meta): bt (R, pages) int32 block table,
+    lens (R,) int64 lengths with the new tokens, qlens (R,) int32, all on the device; tokens: room for the step's tokens (at
+    least their number; the rest is padding). With held (R,) int32, free (F,) int32 page numbers and taken (1,) int64 the rows'
+    tables grow in place: row r takes the pages that lens[r] needs beyond its held[r], in row order, behind the free list's
+    first taken[0] entries; the counts behind the step come back in the result."""
+    L = ops()
+    dev = bt.device
+    _need(bt, "bt", torch.int32, dev); _need(lens, "lens", torch.int64, dev); _need(qlens, "qlens", torch.int32, dev)
+    R, tokens, ebs = bt.shape[0], int(tokens), int(ebs)
+    if bt.dim() != 2 or (R and bt.shape[1] and bt.stride(-1) != 1) or lens.shape != (R,) or qlens.shape != (R,):
+        raise ValueError("bt must be (R, pages) with contiguous rows, lens and qlens (R,)")
+    if tokens < 0 or ebs < 1:
+        raise ValueError("tokens must be >= 0 and ebs >= 1")
+    grow = held is not None
+    if grow != (free is not None) or grow != (taken is not None):
+        raise ValueError("held, free and taken go together")
+    if grow:
+        _need(held, "held", torch.int32, dev); _need(free, "free", torch.int32, dev); _need(taken, "taken", torch.int64, dev)
+        if held.shape != (R,) or free.dim() != 1 or taken.shape != (1,):
+            raise ValueError("held must be (R,), free (F,) and taken (1,)")
+        if R > 1 and bt.stride(0) < bt.shape[1]:
+            raise ValueError("the rows of a growing block table must not overlap")
+        held, free, taken = held.contiguous(), free.contiguous(), taken.contiguous()
+    if R == 0:
+        pad = torch.full((tokens,), -1, dtype=torch.int64, device=dev)
+        return ChunkMeta(torch.zeros(1, dtype=torch.int64, device=dev), pad, pad.clone(), torch.zeros_like(pad),
+                         torch.empty(0, dtype=torch.int32, device=dev), held, taken)
+    lens, qlens = lens.contiguous(), qlens.contiguous()
+    m = torch.empty(R + 1 + 3 * tokens + 1, dtype=torch.int64, device=dev)   # one allocation: qsl, slot, pos, row, taken
+    qsl, slot, pos, row, tk = m.split((R + 1, tokens, tokens, tokens, 1))
+    i32 = torch.empty((2 if grow else 1) * R, dtype=torch.int32, device=dev)
+    with _on(dev):
+        _check(L.kv800_hip_chunk_meta(_ptr(bt), bt.stride(0) if R > 1 else max(bt.shape[1], 1), bt.shape[1], _ptr(lens),
+                                      _ptr(qlens), R, ebs, tokens, _ptr(held), _ptr(free), free.shape[0] if grow else 0,
+                                      _ptr(taken), _ptr(i32[R:]) if grow else None, _ptr(tk) if grow else None, _ptr(qsl),
+                                      _ptr(slot), _ptr(pos), _ptr(row), _ptr(i32), _stream(dev)))
+    return ChunkMeta(qsl, slot, pos, row, i32[:R], i32[R:] if grow else None, tk if grow else None)
 
 
 def page_offsets(bt, scale, add=0):
@@ -660,24 +737,35 @@ def combine(MO, LO, AO, ns):
 
 
 # ---------------------------------------------------------------- decode
-_PAIRS = OrderedDict()     # (device, cos ptr, sin ptr, rows) -> (cos_t, sin_t, versions, pair table)
+_PAIRS = OrderedDict()     # (device, cos ptr, sin ptr, rows) -> (cos_t, sin_t, versions, pair table, stream, event)
 
 
 def rope_pairs(cos_t, sin_t):
     """Packed bf16 (cos, sin) pair table of every row of the bf16 tables (kv800_hip_rope_table), cached per table
     tensors. The entry holds the two tables themselves, so their storage cannot be freed and reused by other tensors
-    while it is cached; it is rebuilt when either tensor is modified in place (version counter) or replaced."""
+    while it is cached; it is rebuilt when either tensor is modified in place (version counter) or replaced. A call on
+    another stream than the one that built it waits for it; a table built while a graph is captured belongs to that graph
+    alone, whose replays fill it."""
     key = (str(cos_t.device), cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0])
     ent = _PAIRS.get(key)
     ver = (cos_t._version, sin_t._version)
+    now = torch.cuda.current_stream(cos_t.device)
+    capturing = torch.cuda.is_current_stream_capturing()
     if ent is not None and ent[0] is cos_t and ent[1] is sin_t and ent[2] == ver:
         _PAIRS.move_to_end(key)
+        if ent[4] != now and not capturing:   # a capture begins by waiting for the device
+            now.wait_event(ent[5])
+            ent[3].record_stream(now)
         return ent[3]
     L = ops()
     P = cos_t.shape[0]
     t = torch.empty(P, 32, dtype=torch.int32, device=cos_t.device)
     _check(L.kv800_hip_rope_table(_ptr(cos_t), _ptr(sin_t), P, _ptr(t), _stream(cos_t.device)))
-    _PAIRS[key] = (cos_t, sin_t, ver, t)
+    if capturing:
+        return t
+    done = torch.cuda.Event()
+    done.record(now)
+    _PAIRS[key] = (cos_t, sin_t, ver, t, now, done)
     _PAIRS.move_to_end(key)
     while len(_PAIRS) > 8:
         _PAIRS.popitem(last=False)
@@ -769,6 +857,46 @@ def decode(P, q, cos_t, sin_t, spb=None, target=None, groups=None):
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     _check(L.kv800_hip_decode_sized(ctypes.byref(s), _ptr(q), B, _ptr(cos_t), _ptr(sin_t), cos_t.shape[0], _ptr(cs2),
                                     qbytes, eelems, selems, _ptr(out), _ptr(ws), wsb, arg, _stream(dev)))
+    return out
+
+
+def decode_chunk(P, q, qsl, cos_t, sin_t):
+    """Attention of a step's new tokens over the paged cache of one layer (kv800_hip_decode_chunk): q (T, 16, 128) bf16
+    post-RoPE, row r's queries q[qsl[r]:qsl[r + 1]] with qsl (R + 1,) int64 on the device (chunk_meta), at the row's last
+    positions, P.N[r] of them in all; their K / V rows are in the exact pages already. P.NQ: the sub-blocks flushed before
+    these tokens, P.nqmax the host's bound of it; window layers (P.win > 0) read the exact pages and, with P.sk, the
+    sinks. cos_t / sin_t (P, 32) bf16, or None: keys as stored. Returns (T, 16, 128) bf16, zeros for the tokens behind the
+    last row's. For chunks of many tokens the assembled prefill (prefill_keys, prefill) takes less time."""
+    L = ops()
+    dev = q.device
+    _need(q, "q", torch.bfloat16, dev); _need(qsl, "qsl", torch.int64, dev)
+    if q.dim() != 3 or tuple(q.shape[1:]) != (16, 128):
+        raise ValueError(f"q must be (T, 16, 128), got {tuple(q.shape)}")
+    if qsl.dim() != 1 or qsl.shape[0] < 1:
+        raise ValueError("qsl must be (R + 1,)")
+    T, R = q.shape[0], qsl.shape[0] - 1
+    if (cos_t is None) != (sin_t is None):
+        raise ValueError("cos_t and sin_t go together")
+    _need(P.epool, "epool", torch.bfloat16, dev)
+    if T == 0 or R == 0:
+        return torch.zeros(T, 16, 128, dtype=torch.bfloat16, device=dev)
+    rot = cos_t is not None
+    if rot:
+        cos_t, sin_t = _rope32(cos_t, sin_t, dev)
+    s, qbytes, eelems, selems = paged_struct(P, R)
+    if P.eoff.shape[0] < R or (s.nqmax and P.boff.shape[0] < R) or (s.sk and min(P.skoff.shape[0], P.svoff.shape[0]) < R):
+        raise ValueError("eoff, boff, skoff and svoff must cover the rows")
+    if s.nqmax and not rot:
+        raise ValueError("quantized layers need the rope tables")
+    q, qsl = q.contiguous(), qsl.contiguous()
+    out = torch.empty(T, 16, 128, dtype=torch.bfloat16, device=dev)
+    with _on(dev):
+        cs2 = rope_pairs(cos_t, sin_t) if s.nqmax else None
+        wsb = int(L.kv800_hip_decode_chunk_workspace(R, T, s.nqmax))
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+        _check(L.kv800_hip_decode_chunk(ctypes.byref(s), _ptr(q), _ptr(qsl), R, T, _ptr(cos_t), _ptr(sin_t),
+                                        cos_t.shape[0] if rot else 0, _ptr(cs2), qbytes, eelems, selems, _ptr(out), _ptr(ws),
+                                        wsb, _stream(dev)))
     return out
 
 

@@ -1,0 +1,133 @@
+"""ctypes binding of the model-side operators of a step whose rows bring several new tokens each (include/lfm3_spec.h, in
+libkv800_hip.so): the short conv over a row's new tokens, its state moved on over the kept ones, the verification of drafts.
+
+A step's tokens lie row after row; qsl (R + 1,) int64 on the device holds the rows' starts (kv800_hip.chunk_meta). Like
+kv800_hip, there is no fallback: without the library or a GPU the first call raises ImportError. Launches go on the current
+stream of the tensors' device; workspaces are torch allocations of the call."""
+import ctypes
+
+import torch
+
+from . import kv800_hip
+from .kv800_hip import _need, _on, _ptr, _stream
+
+_VP, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+SIGNATURES = {
+    "lfm3_hip_conv_chunk": (_I32, [_VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _VP, _VP, _VP]),
+    "lfm3_hip_conv_commit": (_I32, [_VP, _VP, _VP, _VP, _I64, _I64, _I64, _VP]),
+    "lfm3_hip_verify_workspace": (_I64, [_I64, _I64]),
+    "lfm3_hip_verify_drafts": (_I32, [_VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _I64,
+                                      _VP]),
+}
+_BOUND = {}
+
+
+def _lib():
+    L = kv800_hip.ops()
+    if id(L) not in _BOUND:
+        for name, (res, args) in SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = res, args
+        _BOUND.clear()
+        _BOUND[id(L)] = True
+    return L
+
+
+def _rows(qsl, dev):
+    _need(qsl, "qsl", torch.int64, dev)
+    if qsl.dim() != 1 or qsl.shape[0] < 1:
+        raise ValueError("qsl must be (R + 1,)")
+    return qsl.contiguous(), qsl.shape[0] - 1
+
+
+def _state(state, R, dev):
+    _need(state, "state", torch.bfloat16, dev)
+    if state.dim() != 3 or state.shape[0] != R or state.shape[2] != 6 or state.shape[1] % 8 or not state.is_contiguous():
+        raise ValueError(f"state must be a contiguous ({R}, H, 6) with H a multiple of 8, got {tuple(state.shape)}")
+
+
+def conv_chunk(bcx, conv_w, state, qsl):
+    """Short conv over each row's new tokens (lfm3_hip_conv_chunk): bcx (T, >= 3H) bf16 rows [B | C | x], conv_w (H, 7),
+    state (R, H, 6), read only. Returns (out (T, H), taps (T, H)) bf16: the conv outputs, and bf16(B x) of every token, from
+    which conv_commit moves the state on."""
+    L = _lib()
+    dev = bcx.device
+    qsl, R = _rows(qsl, dev)
+    _need(bcx, "bcx", torch.bfloat16, dev); _need(conv_w, "conv_w", torch.bfloat16, dev)
+    _state(state, R, dev)
+    H = state.shape[1]
+    if bcx.dim() != 2 or bcx.shape[1] < 3 * H or tuple(conv_w.shape) != (H, 7):
+        raise ValueError(f"bcx must be (T, >= {3 * H}) and conv_w ({H}, 7), got {tuple(bcx.shape)}, {tuple(conv_w.shape)}")
+    T = bcx.shape[0]
+    if bcx.stride(-1) != 1 or bcx.stride(0) % 8 or bcx.stride(0) < 3 * H or bcx.data_ptr() % 16:
+        bcx = bcx.contiguous()
+        if bcx.stride(0) % 8:      # an odd width: the three parts alone
+            bcx = bcx[:, :3 * H].contiguous()
+    out = torch.empty(2, T, H, dtype=torch.bfloat16, device=dev)
+    if T == 0 or R == 0 or H == 0:
+        return out.zero_().unbind(0)
+    with _on(dev):
+        kv800_hip._check(L.lfm3_hip_conv_chunk(_ptr(bcx), bcx.stride(0), _ptr(conv_w.contiguous()), _ptr(state), _ptr(qsl), R, T,
+                                               H, _ptr(out[0]), _ptr(out[1]), _stream(dev)))
+    return out.unbind(0)
+
+
+def conv_commit(state, taps, qsl, kept):
+    """state (R, H, 6) moved on, in place, over the first kept[r] ((R,) int32) of each row's new tokens, whose taps
+    conv_chunk returned (lfm3_hip_conv_commit)."""
+    L = _lib()
+    dev = state.device
+    qsl, R = _rows(qsl, dev)
+    _state(state, R, dev)
+    _need(taps, "taps", torch.bfloat16, dev); _need(kept, "kept", torch.int32, dev)
+    H = state.shape[1]
+    if taps.dim() != 2 or taps.shape[1] != H or kept.shape != (R,):
+        raise ValueError(f"taps must be (T, {H}) and kept ({R},), got {tuple(taps.shape)}, {tuple(kept.shape)}")
+    if R == 0 or H == 0 or taps.shape[0] == 0:
+        return
+    taps, kept = taps.contiguous(), kept.contiguous()
+    with _on(dev):
+        kv800_hip._check(L.lfm3_hip_conv_commit(_ptr(state), _ptr(taps), _ptr(qsl), _ptr(kept), R, taps.shape[0], H, _stream(dev)))
+
+
+def verify_drafts(logits, tokens, qsl, temperature, u, u_next, draft_probs=None):
+    """Which drafts of a step are kept, and the token behind them (lfm3_hip_verify_drafts). logits (T, V) bf16: the target's
+    behind every token; tokens (T,) int64: the step's tokens, each row's drafts behind its first one; temperature (R,) fp32 (0:
+    greedy); u (T,) and u_next (R,) fp32 in [0, 1): u[t] decides on the draft that logits row t judges, u_next[r] picks
+    the token behind; draft_probs (T, V) fp32: row t the distribution that token t + 1 was drawn from (None: drafts without
+    one, all of it on the draft). Returns (tokens (T,) int64, count (R,) int32): row r's kept drafts and the token
+    behind them at qsl[r] .., count[r] of them, -1 elsewhere."""
+    L = _lib()
+    dev = logits.device
+    qsl, R = _rows(qsl, dev)
+    _need(logits, "logits", torch.bfloat16, dev); _need(tokens, "tokens", torch.int64, dev)
+    for t, name in ((temperature, "temperature"), (u, "u"), (u_next, "u_next")):
+        _need(t, name, torch.float32, dev)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be (T, V), got {tuple(logits.shape)}")
+    T, V = logits.shape
+    if tokens.shape != (T,) or u.shape != (T,) or temperature.shape != (R,) or u_next.shape != (R,):
+        raise ValueError(f"tokens and u must be ({T},), temperature and u_next ({R},)")
+    if draft_probs is not None:
+        _need(draft_probs, "draft_probs", torch.float32, dev)
+        if draft_probs.shape != (T, V):
+            raise ValueError(f"draft_probs must be ({T}, {V}), got {tuple(draft_probs.shape)}")
+        draft_probs = _row_major(draft_probs)
+    logits = _row_major(logits)
+    out = torch.empty(T, dtype=torch.int64, device=dev)
+    count = torch.empty(R, dtype=torch.int32, device=dev)
+    if R == 0 or T == 0:
+        return out.fill_(-1), count.zero_()
+    wsb = int(L.lfm3_hip_verify_workspace(T, V))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        kv800_hip._check(L.lfm3_hip_verify_drafts(
+            _ptr(logits), logits.stride(0), _ptr(tokens.contiguous()), _ptr(qsl), _ptr(temperature.contiguous()),
+            _ptr(u.contiguous()), _ptr(u_next.contiguous()), _ptr(draft_probs),
+            0 if draft_probs is None else draft_probs.stride(0), R, T, V, _ptr(out), _ptr(count), _ptr(ws), wsb, _stream(dev)))
+    return out, count
+
+
+def _row_major(x):
+    """x with contiguous rows that do not overlap."""
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
