@@ -28,6 +28,11 @@ namespace {
 // v_maximum3_f32, which needs no operand quieted first (fmaxf does, for operands straight from an MFMA); NaN wins
 __device__ __forceinline__ float maxn(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+__device__ __forceinline__ int64_t uniform64(int64_t x) {   // a value that all lanes share, as a scalar
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
 struct ChunkArgs {
   kv800_paged_t P;
   const uint16_t* q;
@@ -44,6 +49,24 @@ struct ChunkArgs {
   int nsink;
 };
 
+// The last i in [0, n) with below(i), for a predicate that holds up to some index, 0 among them: 64-way search by a whole
+// wave, the same result in every lane; n of a few hundred takes two dependent loads.
+template <typename F>
+__device__ __forceinline__ int64_t last_at(int64_t n, F below) {
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 63) / 64, i = lo + lane * step;
+    const int c = __popcll(__ballot(i < hi && below(i < hi ? i : lo)));
+    lo += (c > 0 ? c - 1 : 0) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+__device__ __forceinline__ int64_t row_of(const int64_t* qsl, int64_t R, int64_t t) {
+  return last_at(R, [&](int64_t i) { return qsl[i] <= t; });
+}
+
 // A tile: its row, the row's first token and queries, the tile's first query and queries
 struct Tile { int64_t row, t0; int c, q0, nq; };
 template <int QT>
@@ -51,14 +74,7 @@ __device__ __forceinline__ int64_t tile_number(const int64_t* qsl, int64_t T, in
 // Tile `it`: 64-way search for the last row whose first tile number is <= it, by a whole wave; false if the number has none.
 template <int QT>
 __device__ __forceinline__ bool find_tile(const ChunkArgs& A, int64_t it, Tile& t) {
-  const int lane = threadIdx.x & 63;
-  int64_t lo = 0, hi = A.R;
-  while (hi - lo > 1) {
-    const int64_t step = (hi - lo + 63) / 64, i = lo + lane * step;
-    const int c = __popcll(__ballot(i < hi && tile_number<QT>(A.qsl, A.T, i < hi ? i : lo) <= it));
-    lo += (c > 0 ? c - 1 : 0) * step;
-    hi = min(hi, lo + step);
-  }
+  const int64_t lo = last_at(A.R, [&](int64_t i) { return tile_number<QT>(A.qsl, A.T, i) <= it; });
   t.row = lo;
   t.t0 = min(A.qsl[lo], A.T);
   t.c = (int)(min(A.qsl[lo + 1], A.T) - t.t0);
@@ -147,7 +163,7 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
   const int h = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
   const char* lutc = reinterpret_cast<const char*>(&L.lut[0][0]);
-  const int pbase = A.P.N[t.row] - t.c + t.q0;       // position of the tile's first query
+  const int pbase = __builtin_amdgcn_readfirstlane(A.P.N[t.row] - t.c + t.q0);   // position of the tile's first query
   int pcol[CT];
   b8 bq[CT][4];
 #pragma unroll
@@ -288,7 +304,8 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
 
   // the span's 4 (j1 - j0) pairs of chunks, one after the other; loads one chunk ahead, tables and scales one pair ahead
   const int64_t* brow = A.P.boff + t.row * A.P.boff_stride;
-  auto sanitize = [&](int64_t raw, int jb) -> int64_t {
+  auto sanitize = [&](int64_t x, int jb) -> int64_t {
+    const int64_t raw = uniform64(x);
     return (raw < 0 || raw > A.qpool_bytes - SUB || (int64_t)(jb + 1) * BLK > A.rope_rows) ? -1 : raw;
   };
   const rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(A.cs2), (short)0,
@@ -365,7 +382,7 @@ __global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
   __syncthreads();
   int64_t pre = inc - mine;
   for (int i = 0; i < w; ++i) pre += L.ws[i];
-  const int64_t total = L.ws[0] + L.ws[1] + L.ws[2] + L.ws[3], C = (total + A.G - 1) / A.G;
+  const int64_t total = uniform64(L.ws[0] + L.ws[1] + L.ws[2] + L.ws[3]), C = (total + A.G - 1) / A.G;
   if (blockIdx.x == 0) {                               // for the merge
     int64_t x = pre;
     for (int64_t r = ra; r < rb; ++r) { A.pre[r] = x; x += row_pairs<QT>(A, r); }
@@ -383,18 +400,19 @@ __global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
     }
   }
   __syncthreads();
-  int64_t r = L.row, x = L.pre;
+  // the walk over the list in scalars: the sub-blocks' buffer resources, offsets and loop bounds stay in SGPRs
+  int64_t r = uniform64(L.row), x = uniform64(L.pre);
   bool first = true;
   while (v < v1) {
-    const int64_t y = row_pairs<QT>(A, r);
+    const int64_t y = uniform64(row_pairs<QT>(A, r));
     if (v >= x + y) { x += y; ++r; continue; }
-    const int nb = row_blocks(A, r);
+    const int nb = __builtin_amdgcn_readfirstlane(row_blocks(A, r));
     const int64_t tile = (v - x) / nb;
     const int j0 = (int)((v - x) - tile * nb), j1 = (int)min((int64_t)nb, j0 + (v1 - v));
     Tile t;
     t.row = r;
-    t.t0 = min(A.qsl[r], A.T);
-    t.c = (int)(min(A.qsl[r + 1], A.T) - t.t0);
+    t.t0 = uniform64(min(A.qsl[r], A.T));
+    t.c = (int)(uniform64(min(A.qsl[r + 1], A.T)) - t.t0);
     t.q0 = (int)(tile * QT);
     t.nq = min(QT, t.c - t.q0);
     chunk_span<CT>(L, A, t, j0, j1, first ? (int64_t)blockIdx.x : A.G + tile_number<QT>(A.qsl, A.T, r) + tile);
@@ -454,6 +472,8 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   const int64_t* et = A.P.eoff + t.row * A.P.eoff_stride;
   const int64_t sko = cnt ? A.P.skoff[t.row] : 0, svo = cnt ? A.P.svoff[t.row] : 0;
   const bool rot = A.cos_t != nullptr;
+  const int ebs = (int)A.P.ebs;
+  const double iebs = 1.0 / (double)ebs;
   auto posof = [&](int i) { return i < cnt ? i : i < cnt + cnt2 ? lo_row + i - cnt : rest + i; };
   const uint16_t* qf = A.q + t.t0 * 2048 + 8 * g;      // what lanes without a key read (finite or not, their weight is zero)
   auto load = [&](int c0, ChunkX& C) {
@@ -472,9 +492,11 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
           ok = ko >= 0 && vo >= 0 && ko + 128 <= A.sink_elems && vo + 128 <= A.sink_elems;
           kr = A.P.sk; vr = A.P.sv;
         } else {
-          const int64_t pg = pos / A.P.ebs;
+          int pg = (int)((double)pos * iebs), in = pos - pg * ebs;   // within one of the quotient
+          if (in < 0) { --pg; in += ebs; }
+          if (in >= ebs) { ++pg; in -= ebs; }
           const int64_t b = pg < A.P.eoff_stride ? et[pg] : -1;
-          ko = b + h * A.P.e_hs + (pos - pg * A.P.ebs) * A.P.e_ts;
+          ko = b + h * A.P.e_hs + in * A.P.e_ts;
           vo = ko + A.P.e_v;
           ok = b >= 0 && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
           kr = vr = A.P.epool;
@@ -676,59 +698,76 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
 }
 
 // ---------------------------------------------------------------- merge
-// One workgroup per (tile, KV head), a wave per column in turn; lane = dims 2 lane, 2 lane + 1.
+// One workgroup per (token, KV head), one wave per query head. Lanes take the partials' m and l side by side (64 at a time),
+// then the wave adds up the partials' accumulators, lane = dims 2 lane, 2 lane + 1, eight loads in flight.
 template <int CT>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
   constexpr int QT = 4 * CT, NC = 16 * CT;
-  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-  if ((int64_t)blockIdx.x == 4 * A.I) {                // the padding's output rows
-    const int64_t e0 = min(A.qsl[A.R], A.T) * 256;
-    for (int64_t i = e0 + tid; i < A.T * 256; i += 256) reinterpret_cast<u4v*>(A.out)[i] = u4v{0u, 0u, 0u, 0u};
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = blockIdx.x & 3, dd = 2 * lane;
+  const int64_t tok = blockIdx.x >> 2;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(A.out + (tok * 16 + 4 * h + w) * 128 + dd);
+  if (tok >= min(A.qsl[A.R], A.T)) {                   // padding
+    *dst = 0u;
     return;
   }
-  const int64_t it = blockIdx.x >> 2;
-  const int h = blockIdx.x & 3;
-  Tile t;
-  if (!find_tile<QT>(A, it, t)) return;
-  const int64_t C = A.pre[A.R], nb = row_blocks(A, t.row);
-  const int64_t s = A.pre[t.row] + t.q0 / QT * nb, e = s + nb;   // the tile's entries of the list
-  const int64_t w0 = nb ? s / C : 0, w1 = nb ? (e - 1) / C : -1;
-  const int dd = 2 * lane;
-  for (int c = w; c < 4 * t.nq; c += 4) {
-    const int64_t cx = ((A.G + A.I + it) * 4 + h) * NC + c;
-    auto slot = [&](int64_t k) { return ((k * C >= s ? k : A.G + it) * 4 + h) * NC + c; };
-    const float mx = A.mo[cx];
-    float M = mx;
-    for (int64_t k = w0; k <= w1; ++k) M = fmaxf(M, A.mo[slot(k)]);
-    const float fx = __builtin_amdgcn_exp2f(mx - M);
-    float l = fx * A.lo[cx], x0 = 0.f, x1 = 0.f;
-    for (int64_t k = w0; k <= w1; ++k) {
-      const int64_t p = slot(k);
-      const float f = __builtin_amdgcn_exp2f(A.mo[p] - M);
-      const float2 a = *reinterpret_cast<const float2*>(A.ao + p * 128 + dd);
-      l += f * A.lo[p];
-      x0 += f * a.x;
-      x1 += f * a.y;
-    }
-    {                                                  // H x: bit 0 of the dim in the lane, bits 1..6 across the lanes
-      const float a = x0, b = x1;
-      x0 = a + b;
-      x1 = a - b;
-    }
+  const int64_t row = row_of(A.qsl, A.R, tok), i = tok - A.qsl[row];
+  const int64_t it = tile_number<QT>(A.qsl, A.T, row) + i / QT;
+  const int c = 4 * (int)(i % QT) + w;
+  const int64_t C = A.pre[A.R], nb = row_blocks(A, row);
+  const int64_t s = A.pre[row] + i / QT * nb, e = s + nb;        // the tile's entries of the list
+  const int64_t w0 = nb ? s / C : 0;
+  const int n = nb ? (int)((e - 1) / C - w0) + 1 : 0;            // partials of the quantized list
+  const bool mid = nb && w0 * C < s;                             // the first of them starts inside its workgroup's range
+  auto slot = [&](int k) { return ((k == 0 && mid ? A.G + it : w0 + k) * 4 + h) * NC + c; };
+  const int64_t cx = ((A.G + A.I + it) * 4 + h) * NC + c;
+  const float mx = A.mo[cx], lx = A.lo[cx];
+  const float2 ax = *reinterpret_cast<const float2*>(A.ao + cx * 128 + dd);
+  float M = mx, l = 0.f, x0 = 0.f, x1 = 0.f;
+  for (int k0 = 0; k0 < n; k0 += 64) {
+    const bool in = k0 + lane < n;
+    const int64_t p = slot(in ? k0 + lane : 0);
+    const float mk = in ? A.mo[p] : NEG_BIG, lk = in ? A.lo[p] : 0.f;
+    float m2 = mk;
 #pragma unroll
-    for (int k = 0; k < 6; ++k) {
-      const int msk = 1 << k;
-      const float p0 = __shfl_xor(x0, msk), p1 = __shfl_xor(x1, msk);
-      x0 = (lane & msk) ? p0 - x0 : x0 + p0;
-      x1 = (lane & msk) ? p1 - x1 : x1 + p1;
+    for (int o = 32; o > 0; o >>= 1) m2 = fmaxf(m2, __shfl_xor(m2, o, 64));
+    m2 = fmaxf(m2, M);
+    const float al = __builtin_amdgcn_exp2f(M - m2), f = __builtin_amdgcn_exp2f(mk - m2);
+    M = m2;
+    l = l * al + f * lk;                               // the lane's own share; M starts at the exact part's m
+    x0 *= al;
+    x1 *= al;
+    const int kn = min(64, n - k0);
+    for (int k = 0; k < kn; k += 8) {
+      float2 a[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = *reinterpret_cast<const float2*>(A.ao + slot(k0 + min(k + j, kn - 1)) * 128 + dd);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float fk = k + j < kn ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(k + j, 63))) : 0.f;
+        x0 += fk * a[j].x;
+        x1 += fk * a[j].y;
+      }
     }
-    const float hn = __uint_as_float(0x3DB504F3u);     // 1 / sqrt(128)
-    const float2 a = *reinterpret_cast<const float2*>(A.ao + cx * 128 + dd);
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    const int64_t tok = t.t0 + t.q0 + (c >> 2);
-    *reinterpret_cast<uint32_t*>(A.out + (tok * 16 + 4 * h + (c & 3)) * 128 + dd) =
-        bfpk((x0 * hn + fx * a.x) * inv, (x1 * hn + fx * a.y) * inv);
   }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  const float fx = __builtin_amdgcn_exp2f(mx - M);
+  l += fx * lx;
+  {                                                    // H x: bit 0 of the dim in the lane, bits 1..6 across the lanes
+    const float a = x0, b = x1;
+    x0 = a + b;
+    x1 = a - b;
+  }
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    const int msk = 1 << k;
+    const float p0 = __shfl_xor(x0, msk), p1 = __shfl_xor(x1, msk);
+    x0 = (lane & msk) ? p0 - x0 : x0 + p0;
+    x1 = (lane & msk) ? p1 - x1 : x1 + p1;
+  }
+  const float hn = __uint_as_float(0x3DB504F3u);       // 1 / sqrt(128)
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  *dst = bfpk((x0 * hn + fx * ax.x) * inv, (x1 * hn + fx * ax.y) * inv);
 }
 
 // queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8
@@ -769,13 +808,19 @@ int chunk_launch(const ChunkArgs& A, bool quant, hipStream_t s) {
     hipLaunchKernelGGL(chunk_quant_kernel<CT>, dim3((unsigned)A.G), dim3(256), 0, s, A);
     int rc = check_launch("chunk_quant");
     if (rc != KV800_OK) return rc;
-    hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, false>), dim3(nx), dim3(256), 0, s, A);
+    if (A.R <= 128)
+      hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, false>), dim3(nx), dim3(256), 0, s, A);
+    else
+      hipLaunchKernelGGL((chunk_exact_kernel<CT, 1, false>), dim3(nx), dim3(64), 0, s, A);
     rc = check_launch("chunk_exact");
     if (rc != KV800_OK) return rc;
-    hipLaunchKernelGGL(chunk_merge_kernel<CT>, dim3(nx + 1), dim3(256), 0, s, A);
+    hipLaunchKernelGGL(chunk_merge_kernel<CT>, dim3((unsigned)(4 * A.T)), dim3(256), 0, s, A);
     return check_launch("chunk_merge");
   }
-  hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, true>), dim3(nx + 1), dim3(256), 0, s, A);
+  if (A.R <= 128)
+    hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, true>), dim3(nx + 1), dim3(256), 0, s, A);
+  else
+    hipLaunchKernelGGL((chunk_exact_kernel<CT, 1, true>), dim3(nx + 1), dim3(64), 0, s, A);
   return check_launch("chunk_exact");
 }
 
@@ -815,7 +860,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
   KV800_REQUIRE(!sinks || (P->sv && P->skoff && P->svoff && (((uintptr_t)P->sk | (uintptr_t)P->sv) % 16) == 0),
                 "decode_chunk: sinks need sv, skoff, svoff and 16-byte aligned buffers");
   const ChunkPlan p = chunk_plan(R, T, quant ? P->nqmax : 0);
-  KV800_REQUIRE(p.I <= (1LL << 28), "decode_chunk: too many rows and tokens");
+  KV800_REQUIRE(p.I <= (1LL << 28) && T <= (1LL << 28) && P->ebs < (1LL << 30), "decode_chunk: too many rows and tokens");
   KV800_REQUIRE(!quant || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= kv800_hip_decode_chunk_workspace(R, T, P->nqmax)),
                 "decode_chunk: the workspace is too small or not 16-byte aligned");
   ChunkArgs A;

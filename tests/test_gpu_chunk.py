@@ -292,8 +292,8 @@ def test_conv_in_pieces_and_step(hip):
         assert torch.equal(out, whole[at:at + n])
         so.conv_commit(state, taps, q, torch.tensor([n], dtype=torch.int32, device="cuda"))
         at += n
+    mag = ref.conv(bcx[:1].abs(), w.abs(), first.abs(), [0, 1])[0]   # of the state before conv_step moves it on
     one = mo.conv_step(bcx[:1], w, first)
-    mag = ref.conv(bcx[:1].abs(), w.abs(), first.abs(), [0, 1])[0]
     assert ((one.double() - whole[:1].double()).abs() <= 2 ** -6 * mag).all()
 
 
