@@ -84,18 +84,22 @@ __device__ __forceinline__ bool find_tile(const ChunkArgs& A, int64_t it, Tile& 
 }
 
 // ---------------------------------------------------------------- quantized sub-blocks
-struct ChunkQ {                // one 32-token chunk's data in registers; lane (g, n) = (lane / 16, lane % 16)
-  uint2 kc[2];                 // tile u: kc bytes of token 16 u + n, channels 8 g .. 8 g + 7
-  u4v cs[2][2];                // [u][d]: (cos, sin) pairs of channels 8 g + 4 d .. + 3 at the token's position
-  uint2 vb;                    // vb bytes 8 (lane % 2) .. + 7 of token lane / 2
+// Log2 units by which a score may exceed the running max before the state is rescaled: weights p vsc <= 2^4 448 stay within
+// fp16, whose 11 bits round alike at every size; with the exact max a quarter of the chunks rescaled (52 instructions).
+constexpr float QLAZY = 4.f;
+constexpr int QCH = 32;        // tokens per stage
+// A stage as it lies in LDS: kc, (cos, sin) and vb rows of 32 tokens, all heads, in pieces of 16 bytes. Pieces are permuted
+// within a row so that the reads of one piece of 16 rows spread over the banks: piece p of token t at p ^ (t % 8), of vb rows
+// (4 pieces) at p ^ (t / 2 % 4).
+struct alignas(16) ChunkStage {
+  uint8_t kc[QCH * 128], cs[QCH * 128], vb[QCH * 64];
 };
 struct QLutWords { uint32_t la, lb, sa, sb; };   // klo / ksc bytes of the table that the lane builds
 struct alignas(16) ChunkQLds {
   uint32_t lut[4][1024];       // each wave's code tables of the sub-block it is in
-  u4v vb[4][32];               // each wave's copy of its chunk's vb rows, row vb_slot(t) of token t
   float vs[4][64], vl[4][64];  // decoded vsc / vlo of 64 tokens
   int64_t ws[4];
-  int64_t row, pre, total;
+  int64_t row, pre;
 };
 
 // 16 tables of 4 groups: block (kind, d, e) of 256 bytes holds the tables of channels 8 g + 4 d + e, g = 0..3, entry (ca, cb)
@@ -121,19 +125,20 @@ __device__ __forceinline__ void lut_build(uint32_t* lut, int lane, const QLutWor
         u4v{(pa[0] & 0xFFFFu) | hi, (pa[1] & 0xFFFFu) | hi, (pa[2] & 0xFFFFu) | hi, (pa[3] & 0xFFFFu) | hi};
   }
 }
-__device__ __forceinline__ void chunk_load(ChunkQ& C, rsrc_t rs, rsrc_t rc, int cpos, int t0, int h, int lane) {
-  const int g = lane >> 4, n = lane & 15;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    C.kc[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, n * 128 + 8 * g + 32 * h + 2048 * u,
-                                                                             KC_O + t0 * 128, 0));
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-      C.cs[u][d] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rc, n * 128 + 32 * g + 16 * d + 2048 * u,
-                                                                                 (cpos + t0) * 128, 0));
-  }
-  C.vb = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 64 * (lane >> 1) + 8 * (lane & 1) + 16 * h,
-                                                                        VB_O + t0 * 64, 0));
+// Wave w's part of a stage, straight into LDS: tokens 8 w .. + 7 of kc and cs, and (waves 0, 1) tokens 16 w .. + 15 of vb. Lane l
+// writes bytes 16 l .. + 15 of the wave's kilobyte and fetches the piece that belongs there, so that a load reads whole
+// lines: rows fetched straight into the operand layout (lane = token, 128 bytes apart) cost the L1 one line per lane, 460
+// per chunk and head, and held it busy 86 % of the time (64 rows x 32K x 4: 242 us; staged STAGED_US us).
+__device__ __forceinline__ void stage_load(ChunkStage& S, rsrc_t rs, rsrc_t rc, int cpos, int t0, int w, int lane) {
+  typedef __attribute__((address_space(3))) void lds_v;
+  const int o = (lane >> 3) * 128 + 16 * ((lane & 7) ^ (lane >> 3));
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_v*)&S.kc[1024 * w], 16, o, KC_O + (t0 + 8 * w) * 128, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, (lds_v*)&S.cs[1024 * w], 16, o, (cpos + t0 + 8 * w) * 128, 0, 0);
+  if (w < 2)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_v*)&S.vb[1024 * w], 16,
+                                             (lane >> 2) * 64 + 16 * ((lane & 3) ^ ((lane >> 3) & 3)),
+                                             VB_O + (t0 + 16 * w) * 64, 0, 0);
+  asm volatile("" ::"s"((uint32_t)(uintptr_t)&S) : "memory");   // the loads write S behind the compiler's view
 }
 __device__ __forceinline__ uint32_t chunk_scales(rsrc_t rs, int t0, int h, int lane) {   // vlo | vsc << 8 of token t0 + lane
   const int o = 2 * lane + (h >> 1);
@@ -155,10 +160,9 @@ __device__ __forceinline__ int64_t row_pairs(const ChunkArgs& A, int64_t r) {
 
 // Attention of one tile's columns of KV head h (the wave's) over sub-blocks [j0, j1) of its row, into partial slot `slot`.
 // As in decode_quant_kernel, with the wave's one head: K pairs by table lookup, RoPE by v_dot2_f32_bf16, Q K^T on bf16 MFMA
-// with exact products; fp32 online softmax with the exact running max (the largest weight is exactly its vsc);
-// P V on fp16 MFMA over the bit planes, weights fp16(p vsc): 11 bits, an eighth of the output's own rounding.
+// with exact products; fp32 online softmax; P V on fp16 MFMA over the bit planes, weights fp16(p vsc): 11 bits, an eighth of the output's own rounding.
 template <int CT>
-__device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, const Tile& t, int j0, int j1, int64_t slot) {
+__device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkStage& SB, const ChunkArgs& A, const Tile& t, int j0, int j1, int64_t slot) {
   constexpr int NC = 16 * CT;
   const int h = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
@@ -203,21 +207,26 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
   };
   const uint32_t kg = (uint32_t)h * 4096u + 16u * (uint32_t)g;
   // one 32-token chunk, tokens 32 cc .. of the staged 64; kpos: position of its first token
-  auto chunk = [&](const ChunkQ& C, int cc, int kpos) {
-    {
-      const int tk = lane >> 1;
-      asm volatile("" ::: "memory");
-      reinterpret_cast<uint2*>(&L.vb[h][vb_slot(tk)])[lane & 1] = C.vb;
-      asm volatile("" ::: "memory");
-    }
+  const int okc = n * 128 + 16 * ((2 * h + (g >> 1)) ^ (n & 7)) + 8 * (g & 1);   // kc bytes of channels 8 g .. of token n
+  const int ocs = n * 128 + 16 * ((2 * g) ^ (n & 7));                            // its pairs of channels 8 g .. + 3; the next
+                                                                                 // four in the piece beside it (^ 16)
+  // the transposed vb read: lane n of group g gives row n / 2 of the group's 8 tokens 4 g .., 16 + 4 g .. (the tokens whose
+  // scores its lanes hold), half n % 2
+  const int tvb = 4 * g + ((n >> 1) & 3) + 16 * (n >> 3);
+  const int ovb = tvb * 64 + 16 * (h ^ ((tvb >> 1) & 3)) + 8 * (n & 1);
+  auto chunk = [&](const ChunkStage& S, int cc, int kpos) {
     f4 sc[2][CT];
     __builtin_amdgcn_s_setprio(3);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint32_t kk[2][4], an[2][4];
+      const uint2 kc = *reinterpret_cast<const uint2*>(&S.kc[okc + 2048 * u]);
+      u4v cs[2];
+#pragma unroll
+      for (int d = 0; d < 2; ++d) cs[d] = *reinterpret_cast<const u4v*>(&S.cs[(ocs ^ (16 * d)) + 2048 * u]);
 #pragma unroll
       for (int d = 0; d < 2; ++d) {
-        const uint32_t x = d ? C.kc[u].y : C.kc[u].x;
+        const uint32_t x = d ? kc.y : kc.x;
         const uint32_t xr = (x << 2) & 0xCCCCCCCCu, xn = x & 0xCCCCCCCCu;
         const char *br = lutc + 256 * (4 * d), *bn = lutc + 256 * (8 + 4 * d);
         kk[d][0] = *reinterpret_cast<const uint32_t*>(br + byte_or<0>(xr, kg));
@@ -234,8 +243,8 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
         uint32_t c4[4], s4[4], ar[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          c4[e] = C.cs[u][d][e];
-          s4[e] = __builtin_amdgcn_alignbit(C.cs[u][d][e], C.cs[u][d][e], 16);
+          c4[e] = cs[d][e];
+          s4[e] = __builtin_amdgcn_alignbit(cs[d][e], cs[d][e], 16);
         }
         rope4(kk[d], c4, s4, ar);
 #pragma unroll
@@ -268,7 +277,7 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
       const f4 s0 = sc[0][ct], s1 = sc[1][ct];
       float tmax = maxn(maxn(maxn(s0[0], s0[1]), maxn(s0[2], s0[3])), maxn(maxn(s1[0], s1[1]), maxn(s1[2], s1[3])));
       tmax = max4rows(tmax) * scale;
-      if (__any(tmax > m[ct])) {
+      if (__any(tmax > m[ct] + QLAZY)) {
         const float mn = fmaxf(m[ct], tmax);
         const float al = __builtin_amdgcn_exp2f(m[ct] - mn);
         m[ct] = mn; lsum[ct] *= al; lvs[ct] *= al;
@@ -283,14 +292,14 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
         const float p2 = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][2], scale, -m[ct]));
         const float p3 = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][3], scale, -m[ct]));
         lsum[ct] += (p0 + p1) + (p2 + p3);
-        lvs[ct] += (p0 * vl4[u].x + p1 * vl4[u].y) + (p2 * vl4[u].z + p3 * vl4[u].w);
+        lvs[ct] = fmaf(p3, vl4[u].w, fmaf(p2, vl4[u].z, fmaf(p1, vl4[u].y, fmaf(p0, vl4[u].x, lvs[ct]))));
         wt[u][0] = p0 * vs4[u].x; wt[u][1] = p1 * vs4[u].y; wt[u][2] = p2 * vs4[u].z; wt[u][3] = p3 * vs4[u].w;
       }
       Bw[ct] = pack8(pk2(wt[0][0], wt[0][2]), pk2(wt[0][1], wt[0][3]), pk2(wt[1][0], wt[1][2]), pk2(wt[1][1], wt[1][3]));
     }
     __builtin_amdgcn_s_setprio(0);
     typedef __attribute__((address_space(3))) i2v lds_i2;
-    const i2v X = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(reinterpret_cast<char*>(L.vb[h]) + 128 * g + 8 * n));
+    const i2v X = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(const_cast<uint8_t*>(S.vb) + ovb));
     const uint32_t x0 = (uint32_t)X.x, x1 = (uint32_t)X.x >> 8, x2 = (uint32_t)X.y, x3 = (uint32_t)X.y >> 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -302,7 +311,7 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
     asm volatile("" ::: "memory");
   };
 
-  // the span's 4 (j1 - j0) pairs of chunks, one after the other; loads one chunk ahead, tables and scales one pair ahead
+  // the span's 4 (j1 - j0) pairs of 32-token stages, one after the other; loads one stage ahead, tables and scales one pair
   const int64_t* brow = A.P.boff + t.row * A.P.boff_stride;
   auto sanitize = [&](int64_t x, int jb) -> int64_t {
     const int64_t raw = uniform64(x);
@@ -310,21 +319,22 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
   };
   const rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(A.cs2), (short)0,
                                                       (int)min(A.rope_rows * 128, (int64_t)INT32_MAX), RSRC_WORD3);
+  const int np = 4 * (j1 - j0);
   int jb = j0, pin = 0;
   int64_t base = sanitize(brow[jb], jb), nraw = brow[min(jb + 1, j1 - 1)];
   rsrc_t rs = sub_rsrc(A.P.qpool + (base < 0 ? 0 : base));
   int cpos = base < 0 ? 0 : jb * BLK;
-  ChunkQ C0, C1;
-  chunk_load(C0, rs, rc, cpos, 0, h, lane);
+  stage_load(SA, rs, rc, cpos, 0, h, lane);
   lut_build(L.lut[h], lane, lut_words(rs, h, lane));
   stage_scales(chunk_scales(rs, 0, h, lane));
-  const int np = 4 * (j1 - j0);
+  __syncthreads();
   for (int p = 0; p < np; ++p) {
     const bool more = p + 1 < np, cross = more && pin == 3;
     const int njb = cross ? jb + 1 : jb, npin = cross ? 0 : (pin + 1) & 3;
     int64_t nbase = base;
     rsrc_t nrs = rs;
     int ncpos = cpos;
+    stage_load(SB, rs, rc, cpos, 64 * pin + 32, h, lane);
     if (cross) {
       nbase = sanitize(nraw, njb);
       nrs = sub_rsrc(A.P.qpool + (nbase < 0 ? 0 : nbase));
@@ -333,14 +343,15 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, const ChunkArgs& A, con
     }
     const QLutWords nlw = lut_words(nrs, h, lane);
     const uint32_t nsc = chunk_scales(nrs, 64 * npin, h, lane);
-    chunk_load(C1, rs, rc, cpos, 64 * pin + 32, h, lane);
-    if (base >= 0) chunk(C0, 0, cpos + 64 * pin);
-    chunk_load(C0, nrs, rc, ncpos, 64 * npin, h, lane);
-    if (base >= 0) chunk(C1, 1, cpos + 64 * pin + 32);
+    if (base >= 0) chunk(SA, 0, cpos + 64 * pin);
+    __syncthreads();                                   // SB is whole, and everyone is done with SA
+    if (more) stage_load(SA, nrs, rc, ncpos, 64 * npin, h, lane);
+    if (base >= 0) chunk(SB, 1, cpos + 64 * pin + 32);
     if (more) {
       if (cross) lut_build(L.lut[h], lane, nlw);
       stage_scales(nsc);
     }
+    __syncthreads();
     jb = njb; pin = npin; base = nbase; rs = nrs; cpos = ncpos;
   }
 #pragma unroll
@@ -367,6 +378,7 @@ template <int CT>
 __global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
   constexpr int QT = 4 * CT;
   __shared__ ChunkQLds L;
+  __shared__ ChunkStage SA, SB;   // two objects: a read of one is not held for the other's loads
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   // every workgroup sums the rows' entries itself: thread i takes the rows [i k, i k + k)
   const int64_t k = (A.R + 255) / 256, ra = min((int64_t)tid * k, A.R), rb = min(ra + k, A.R);
@@ -415,7 +427,7 @@ __global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
     t.c = (int)(uniform64(min(A.qsl[r + 1], A.T)) - t.t0);
     t.q0 = (int)(tile * QT);
     t.nq = min(QT, t.c - t.q0);
-    chunk_span<CT>(L, A, t, j0, j1, first ? (int64_t)blockIdx.x : A.G + tile_number<QT>(A.qsl, A.T, r) + tile);
+    chunk_span<CT>(L, SA, SB, A, t, j0, j1, first ? (int64_t)blockIdx.x : A.G + tile_number<QT>(A.qsl, A.T, r) + tile);
     first = false;
     v += j1 - j0;
   }
@@ -425,26 +437,41 @@ __global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
 // NW waves per (tile, KV head) take the 32-token chunks of the tile's keys in turn and join their states at the end. The keys
 // in order: the row's sinks, exact positions below the sink count (kept out of the window too), exact positions from the
 // first one in a query's window up to the last query. As decode_exact_kernel otherwise: Q K^T and P V on bf16 MFMA, weights
-// as hi + lo bf16 pairs (16 bits), V^T by transposed reads from an LDS copy.
-constexpr int XCH = 32, XVROW = 144;
+// as hi + lo bf16 pairs (16 bits), V^T by transposed reads.
+// K and V rows of a chunk go straight into LDS, whole 256-byte rows by 16 lanes each (fetched in the operand layout, lane =
+// token, every lane is a cache line of its own: 1,280 line requests per chunk, and 398 rows of a window layer took
+// 80 us), in pieces of 16 bytes permuted within the row so that operand reads spread over the banks. One buffer for each: the
+// next chunk's K is requested when this one's scores are formed, its V when this one's V is read, so that each is
+// in flight for about half a chunk, and 17 KB a wave leave room for nine waves on a CU.
+constexpr int XCH = 32;
+template <int NW>
+struct alignas(16) ChunkXRows { uint16_t r[NW][XCH * 128]; };
 template <int CT, int NW>
 struct alignas(16) ChunkXLds {
-  union {
-    uint16_t v[NW][XCH][XVROW];
-    float o[NW > 1 ? NW - 1 : 1][16 * CT][132];   // the end: the other waves' accumulators, scaled to the common max
-  };
   float m[NW][16 * CT], l[NW][16 * CT];
 };
-struct ChunkX {                        // one chunk in registers; lane (g, n): token 16 u + n of tile u
-  u4v k[2][4], v[2][4], c[2], s[2];    // K, V dims 32 s + 8 g .. + 7; cos / sin of channels 8 g .. + 7
-  uint32_t ok;                         // chunk tokens with a key
-};
+__device__ const uint4 chunk_zeros[16] = {};           // a row for tokens without a key: a zero weight needs a finite value
+
+// 16 bytes per lane from p to LDS bytes 16 lane .. of dst (the same for all lanes). The compiler does not see the load: whoever
+// reads dst waits for it by the memory counter (vm_wait), which retires loads in order; its own waits only come out
+// longer. As a builtin, every read of LDS waited for every such load, whichever array it fills.
+__device__ __forceinline__ void load_lds(const uint16_t* p, uint16_t* dst) {
+  typedef __attribute__((address_space(3))) uint16_t lds_u16;
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               ::"v"(p), "s"(__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_u16*)dst)) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void vm_wait() {            // all but the N youngest loads are done
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 template <int CT, int NW, bool DIRECT>
 __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
-  constexpr int QT = 4 * CT, NC = 16 * CT;
+  constexpr int QT = 4 * CT, NC = 16 * CT, XROW = 132;
+  __shared__ ChunkXRows<NW> Ks, Vs;                    // two objects: a read of one is not held for the other's loads
   __shared__ ChunkXLds<CT, NW> L;
-  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, g = lane >> 4, n = lane & 15;
+  static_assert((NW - 1) * 16 * XROW * 4 <= (int)sizeof(Ks) || NW == 1, "the join must fit");
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, n = lane & 15;
   if (DIRECT && (int64_t)blockIdx.x == 4 * A.I) {      // the padding's output rows
     const int64_t e0 = min(A.qsl[A.R], A.T) * 256;
     for (int64_t i = e0 + tid; i < A.T * 256; i += 64 * NW) reinterpret_cast<u4v*>(A.out)[i] = u4v{0u, 0u, 0u, 0u};
@@ -454,7 +481,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   const int h = blockIdx.x & 3;
   Tile t;
   if (!find_tile<QT>(A, it, t)) return;
-  const int N = A.P.N[t.row], win = (int)A.P.win;
+  const int N = __builtin_amdgcn_readfirstlane(A.P.N[t.row]), win = (int)A.P.win;
   const int pbase = N - t.c + t.q0, plast = pbase + t.nq - 1;
   // key list: sinks [0, cnt), exact positions lo_row .. + cnt2, then lo_tile ..
   int lo_row, lo_tile;
@@ -462,7 +489,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
     lo_row = max(0, N - t.c - (win - 1));
     lo_tile = max(lo_row, pbase - (win - 1));
   } else {
-    lo_row = lo_tile = A.P.NQ ? row_nq(A, t.row) * BLK : 0;
+    lo_row = lo_tile = A.P.NQ ? __builtin_amdgcn_readfirstlane(row_nq(A, t.row)) * BLK : 0;
   }
   const int hi = min(N, plast + 1);
   const int cnt = max(0, min(min(A.nsink, lo_row), hi));
@@ -474,55 +501,79 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   const bool rot = A.cos_t != nullptr;
   const int ebs = (int)A.P.ebs;
   const double iebs = 1.0 / (double)ebs;
+  const uint16_t* const zeros = reinterpret_cast<const uint16_t*>(chunk_zeros);
   auto posof = [&](int i) { return i < cnt ? i : i < cnt + cnt2 ? lo_row + i - cnt : rest + i; };
-  const uint16_t* qf = A.q + t.t0 * 2048 + 8 * g;      // what lanes without a key read (finite or not, their weight is zero)
-  auto load = [&](int c0, ChunkX& C) {
-    uint32_t okm = 0;
+  // Lane l (and l ^ 32) looks after token l % 32 of a chunk. page(): its page's offset, asked for two chunks ahead, before the
+  // rows of the chunk between: loads retire in order. locate(): its K and V row of head h.
+  auto split = [&](int pos, int& pg, int& in) {        // pos = pg ebs + in
+    pg = (int)((double)pos * iebs);                    // within one of the quotient
+    in = pos - pg * ebs;
+    if (in < 0) { --pg; in += ebs; }
+    if (in >= ebs) { ++pg; in -= ebs; }
+  };
+  auto page = [&](int c0) -> int64_t {
+    const int i = c0 + (lane & 31);
+    int pg = 0, in;
+    if (i >= cnt && i < nk) split(posof(i), pg, in);
+    return et[min((int64_t)pg, A.P.eoff_stride - 1)];
+  };
+  struct Where { const uint16_t *k, *v; uint32_t ok; };   // bit t of ok: token t of the chunk has a key
+  auto locate = [&](int c0, int64_t base) {
+    const int i = c0 + (lane & 31);
+    Where r = {zeros, zeros, 0u};
+    bool ok = false;
+    if (i < nk) {
+      const int pos = posof(i);
+      int64_t ko, vo;
+      const uint16_t *kb = A.P.epool, *vb = A.P.epool;
+      if (i < cnt) {
+        ko = sko + ((int64_t)i * 4 + h) * 128;
+        vo = svo + ((int64_t)i * 4 + h) * 128;
+        ok = ko >= 0 && vo >= 0 && ko + 128 <= A.sink_elems && vo + 128 <= A.sink_elems;
+        kb = A.P.sk; vb = A.P.sv;
+      } else {
+        int pg, in;
+        split(pos, pg, in);
+        ko = base + h * A.P.e_hs + in * A.P.e_ts;
+        vo = ko + A.P.e_v;
+        ok = base >= 0 && pg < A.P.eoff_stride && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
+      }
+      ok = ok && (!rot || pos < A.rope_rows);
+      if (ok) { r.k = kb + ko; r.v = vb + vo; }
+    }
+    r.ok = (uint32_t)__ballot(ok);
+    return r;
+  };
+  const int r4 = lane >> 4, pc = lane & 15;            // an instruction fills 4 rows: row r4, piece pc
+  auto row_at = [&](const uint16_t* p, int t) {        // token t's pointer
+    const uint64_t x = (uint64_t)p;
+    const uint32_t lo = __shfl((uint32_t)x, t, 64), hi = __shfl((uint32_t)(x >> 32), t, 64);
+    return (const uint16_t*)(((uint64_t)hi << 32) | lo);
+  };
+  auto load_k = [&](const uint16_t* p) {               // piece p of token t at p ^ (t % 16)
+    const uint16_t* src[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) src[i] = row_at(p, 4 * i + r4) + 8 * (pc ^ ((4 * i + r4) & 15));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load_lds(src[i], &Ks.r[w][512 * i]);
+  };
+  auto load_v = [&](const uint16_t* p) {               // at p ^ 2 (t % 8): pairs of pieces stay together
+    const uint16_t* src[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) src[i] = row_at(p, 4 * i + r4) + 8 * (pc ^ (2 * ((4 * i + r4) & 7)));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load_lds(src[i], &Vs.r[w][512 * i]);
+  };
+  struct Rope { u4v c[2], s[2]; };                     // cos / sin of channels 8 g .. + 7 at token 16 u + n
+  auto load_rope = [&](int c0, Rope& r) {
+    if (!rot) return;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int i = c0 + 16 * u + n;
-      const uint16_t *kr = qf, *vr = qf, *cr = qf, *sr = qf;
-      bool ok = false;
-      if (i < nk) {
-        const int pos = posof(i);
-        int64_t ko, vo;
-        if (i < cnt) {
-          ko = sko + ((int64_t)i * 4 + h) * 128;
-          vo = svo + ((int64_t)i * 4 + h) * 128;
-          ok = ko >= 0 && vo >= 0 && ko + 128 <= A.sink_elems && vo + 128 <= A.sink_elems;
-          kr = A.P.sk; vr = A.P.sv;
-        } else {
-          int pg = (int)((double)pos * iebs), in = pos - pg * ebs;   // within one of the quotient
-          if (in < 0) { --pg; in += ebs; }
-          if (in >= ebs) { ++pg; in -= ebs; }
-          const int64_t b = pg < A.P.eoff_stride ? et[pg] : -1;
-          ko = b + h * A.P.e_hs + in * A.P.e_ts;
-          vo = ko + A.P.e_v;
-          ok = b >= 0 && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
-          kr = vr = A.P.epool;
-        }
-        ok = ok && (!rot || pos < A.rope_rows);
-        if (ok) {
-          kr += ko + 8 * g;
-          vr += vo + 8 * g;
-          if (rot) { cr = A.cos_t + (int64_t)pos * 32 + 8 * g; sr = A.sin_t + (int64_t)pos * 32 + 8 * g; }
-        } else {
-          kr = vr = qf;
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < 4; ++s) C.k[u][s] = *reinterpret_cast<const u4v*>(kr + 32 * s);
-      C.c[u] = *reinterpret_cast<const u4v*>(cr);
-      C.s[u] = *reinterpret_cast<const u4v*>(sr);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) C.v[u][s] = *reinterpret_cast<const u4v*>(vr + 32 * s);
-      if (!ok) {                                       // a zero weight times a NaN would be one
-#pragma unroll
-        for (int s = 0; s < 4; ++s) C.v[u][s] = u4v{0u, 0u, 0u, 0u};
-      }
-      okm |= ((uint32_t)__ballot(ok) & 0xFFFFu) << (16 * u);
+      const int64_t p = i < nk ? min((int64_t)posof(i), A.rope_rows - 1) : 0;
+      r.c[u] = *reinterpret_cast<const u4v*>(A.cos_t + p * 32 + 8 * g);
+      r.s[u] = *reinterpret_cast<const u4v*>(A.sin_t + p * 32 + 8 * g);
     }
-    C.ok = okm;
   };
   b8 bq[CT][4];
   int pcol[CT];
@@ -542,120 +593,134 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[ct][j] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  uint16_t (*Vs)[XVROW] = L.v[w];
-  auto body = [&](const ChunkX& C, int c0) {
+  constexpr int STEP = NW * XCH;
+  if (w * XCH < nk) {
+    Rope rp = {};
+    int64_t pg = page(w * XCH), pgn = page(w * XCH + STEP);
+    Where at = locate(w * XCH, pg);
+    load_rope(w * XCH, rp);
+    asm volatile("" ::"v"(rp.c[0]), "v"(rp.c[1]), "v"(rp.s[0]), "v"(rp.s[1]), "v"(pgn) : "memory");   // waited for here
+    load_k(at.k);
+    load_v(at.v);
+    vm_wait<8>();                                      // K is there, V under way
+    for (int c0 = w * XCH; c0 < nk; c0 += STEP) {
+      const bool more = c0 + STEP < nk;                // uniform
+      const Where nx = locate(c0 + STEP, pgn);
+      const uint16_t* kw = Ks.r[w];
+      f4 sc[2][CT];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        u4v k[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) *reinterpret_cast<u4v*>(&Vs[16 * u + n][32 * s + 8 * g]) = C.v[u][s];
-    f4 sc[2][CT];
+        for (int s = 0; s < 4; ++s) k[s] = *reinterpret_cast<const u4v*>(kw + (16 * u + n) * 128 + 8 * ((4 * s + g) ^ n));
+        if (rot) {
+          u4v a0, a2;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      u4v a0 = C.k[u][0], a2 = C.k[u][2];
-      if (rot) {
+          for (int e = 0; e < 8; e += 2) {
+            float r0[2], r2[2];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          float r0[2], r2[2];
-#pragma unroll
-          for (int d = 0; d < 2; ++d) {
+            for (int d = 0; d < 2; ++d) {
 #pragma clang fp contract(off)   // products rounded before the sum, as torch_decode.py:22-23 evaluates them
-            const float k0 = bf_elem(C.k[u][0], e + d), k2 = bf_elem(C.k[u][2], e + d);
-            const float cs = bf_elem(C.c[u], e + d), sn = bf_elem(C.s[u], e + d);
-            r0[d] = k0 * cs - k2 * sn;
-            r2[d] = k2 * cs + k0 * sn;
+              const float k0 = bf_elem(k[0], e + d), k2 = bf_elem(k[2], e + d);
+              const float cs = bf_elem(rp.c[u], e + d), sn = bf_elem(rp.s[u], e + d);
+              r0[d] = k0 * cs - k2 * sn;
+              r2[d] = k2 * cs + k0 * sn;
+            }
+            a0[e >> 1] = bfpk(r0[0], r0[1]);
+            a2[e >> 1] = bfpk(r2[0], r2[1]);
           }
-          a0[e >> 1] = bfpk(r0[0], r0[1]);
-          a2[e >> 1] = bfpk(r2[0], r2[1]);
+          k[0] = a0;
+          k[2] = a2;
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < 4; ++s) x = mfma_bf(as_b8(k[s]), bq[ct][s], x);
+          sc[u][ct] = x;
         }
       }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        f4 x = {0.f, 0.f, 0.f, 0.f};
-        x = mfma_bf(as_b8(a0), bq[ct][0], x);
-        x = mfma_bf(as_b8(C.k[u][1]), bq[ct][1], x);
-        x = mfma_bf(as_b8(a2), bq[ct][2], x);
-        sc[u][ct] = mfma_bf(as_b8(C.k[u][3]), bq[ct][3], x);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K is read: its rows may be overwritten
+      if (more) {
+        pgn = page(c0 + 2 * STEP);
+        load_rope(c0 + STEP, rp);
+        load_k(nx.k);
       }
-    }
-    const uint32_t tb = C.ok >> (4 * g);               // bit 16 u + i: token 16 u + 4 g + i
-    int kp[2][4];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) kp[u][i] = ((tb >> (16 * u + i)) & 1u) ? posof(c0 + 16 * u + 4 * g + i) : 0x7FFFFFFF;
-    u4v bh[CT], bl[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float xs[2][4], cm = -INFINITY;
-      const int wlo = win > 0 ? pcol[ct] - win : -1;
+      const uint32_t tb = at.ok >> (4 * g);               // bit 16 u + i: token 16 u + 4 g + i
+      int kp[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool keep = kp[u][i] <= pcol[ct] && (kp[u][i] > wlo || kp[u][i] < A.nsink);
-          xs[u][i] = keep ? sc[u][ct][i] * A.scale : -INFINITY;
-          cm = fmaxf(cm, xs[u][i]);
-        }
-      cm = max4rows(cm);
-      if (__any(cm > m[ct])) {
-        const float mn = fmaxf(m[ct], cm), al = __builtin_amdgcn_exp2f(m[ct] - mn);
-        m[ct] = mn;
-        lsum[ct] *= al;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[ct][j] *= al;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int u = k >> 1, i = 2 * (k & 1);
-        const float pa = __builtin_amdgcn_exp2f(xs[u][i] - m[ct]), pb = __builtin_amdgcn_exp2f(xs[u][i + 1] - m[ct]);
-        lsum[ct] += pa + pb;
-        bh[ct][k] = bfpk(pa, pb);
-        bl[ct][k] = bfpk(pa - __uint_as_float(bh[ct][k] << 16), pb - __uint_as_float(bh[ct][k] & 0xFFFF0000u));
-      }
-    }
-    asm volatile("" ::: "memory");   // the staged V rows are written before the transposed reads
-    const int vrow = 4 * g + (n >> 2), vcol = 4 * (n & 3);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const s4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&Vs[vrow][16 * j + vcol]);
-      const s4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&Vs[vrow + 16][16 * j + vcol]);
-      const u4v av = {__builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 0, 1)),
-                      __builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 2, 3)),
-                      __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 0, 1)),
-                      __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 2, 3))};
+        for (int i = 0; i < 4; ++i) kp[u][i] = ((tb >> (16 * u + i)) & 1u) ? posof(c0 + 16 * u + 4 * g + i) : 0x7FFFFFFF;
+      u4v bh[CT], bl[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        acc[ct][j] = mfma_bf(as_b8(av), as_b8(bh[ct]), acc[ct][j]);
-        acc[ct][j] = mfma_bf(as_b8(av), as_b8(bl[ct]), acc[ct][j]);
+        float xs[2][4], cm = -INFINITY;
+        const int wlo = win > 0 ? pcol[ct] - win : -1;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool keep = kp[u][i] <= pcol[ct] && (kp[u][i] > wlo || kp[u][i] < A.nsink);
+            xs[u][i] = keep ? sc[u][ct][i] * A.scale : -INFINITY;
+            cm = fmaxf(cm, xs[u][i]);
+          }
+        cm = max4rows(cm);
+        if (__any(cm > m[ct])) {
+          const float mn = fmaxf(m[ct], cm), al = __builtin_amdgcn_exp2f(m[ct] - mn);
+          m[ct] = mn;
+          lsum[ct] *= al;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[ct][j] *= al;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int u = k >> 1, i = 2 * (k & 1);
+          const float pa = __builtin_amdgcn_exp2f(xs[u][i] - m[ct]), pb = __builtin_amdgcn_exp2f(xs[u][i + 1] - m[ct]);
+          lsum[ct] += pa + pb;
+          bh[ct][k] = bfpk(pa, pb);
+          bl[ct][k] = bfpk(pa - __uint_as_float(bh[ct][k] << 16), pb - __uint_as_float(bh[ct][k] & 0xFFFF0000u));
+        }
       }
-    }
-    asm volatile("" ::: "memory");   // and read before the next chunk's rows overwrite them
-  };
-  constexpr int STEP = NW * XCH;
-  if (w * XCH < nk) {
-    ChunkX C0, C1;
-    load(w * XCH, C0);
-    for (int c0 = w * XCH;;) {
-      load(c0 + STEP, C1);
-      body(C0, c0);
-      c0 += STEP;
-      if (c0 >= nk) break;
-      load(c0 + STEP, C0);
-      body(C1, c0);
-      c0 += STEP;
-      if (c0 >= nk) break;
+      if (more) vm_wait<8>(); else vm_wait<0>();       // V is there, the next K under way
+      // V^T: lane (g, n) gives 4 values of row 4 g + n / 4 from dim 16 j + 4 (n % 4) on
+      uint16_t* vw = Vs.r[w];
+      const int vrow = 4 * g + (n >> 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = vrow * 128 + 8 * ((2 * j + ((n & 3) >> 1)) ^ (2 * (vrow & 7))) + 4 * (n & 1);
+        const s4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[at]);
+        const s4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[at + 16 * 128]);
+        const u4v av = {__builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 0, 1)),
+                        __builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 2, 3)),
+                        __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 0, 1)),
+                        __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 2, 3))};
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          acc[ct][j] = mfma_bf(as_b8(av), as_b8(bh[ct]), acc[ct][j]);
+          acc[ct][j] = mfma_bf(as_b8(av), as_b8(bl[ct]), acc[ct][j]);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V is read
+      // the register loads are waited for here, before loads that a later wait would include
+      asm volatile("" ::"v"(rp.c[0]), "v"(rp.c[1]), "v"(rp.s[0]), "v"(rp.s[1]), "v"(pgn) : "memory");
+      if (more) {
+        load_v(nx.v);
+        vm_wait<8>();
+      }
+      at = nx;
     }
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) lsum[ct] = sum4rows(lsum[ct]);
-  if (NW > 1) {
-    __syncthreads();                                   // every wave is done with its V rows
+  if constexpr (NW > 1) {
+    float (*O)[16][XROW] = reinterpret_cast<float (*)[16][XROW]>(&Ks);   // the other waves' accumulators, scaled alike
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
       if (g == 0) { L.m[w][16 * ct + n] = m[ct]; L.l[w][16 * ct + n] = lsum[ct]; }
-    __syncthreads();
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+      __syncthreads();                                 // the chunks, and the last column tile's join, are done
       float M = NEG_BIG, l = 0.f;
       for (int k = 0; k < NW; ++k) M = fmaxf(M, L.m[k][16 * ct + n]);
       for (int k = 0; k < NW; ++k) l += L.l[k][16 * ct + n] * __builtin_amdgcn_exp2f(L.m[k][16 * ct + n] - M);
@@ -665,16 +730,16 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         acc[ct][j] *= f;
-        if (w > 0) *reinterpret_cast<f4*>(&L.o[w - 1][16 * ct + n][16 * j + 4 * g]) = acc[ct][j];
+        if (w > 0) *reinterpret_cast<f4*>(&O[w - 1][n][16 * j + 4 * g]) = acc[ct][j];
+      }
+      __syncthreads();
+      if (w == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          for (int k = 0; k < NW - 1; ++k) acc[ct][j] += *reinterpret_cast<const f4*>(&O[k][n][16 * j + 4 * g]);
       }
     }
-    __syncthreads();
     if (w > 0) return;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        for (int k = 0; k < NW - 1; ++k) acc[ct][j] += *reinterpret_cast<const f4*>(&L.o[k][16 * ct + n][16 * j + 4 * g]);
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -773,11 +838,11 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
 // queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8
 int chunk_ct(int64_t R, int64_t T) { return T <= 4 * R ? 1 : 2; }
 
-int64_t chunk_groups() {
+int64_t chunk_cus() {
   static std::mutex mu;
   static int64_t cache[64] = {0};
   int dev = -1;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) { (void)hipGetLastError(); return 512; }
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) { (void)hipGetLastError(); return 256; }
   std::lock_guard<std::mutex> lock(mu);
   if (cache[dev] == 0) {
     int cu = 0;
@@ -785,7 +850,7 @@ int64_t chunk_groups() {
       (void)hipGetLastError();
       cu = 256;
     }
-    cache[dev] = 2 * (int64_t)cu;
+    cache[dev] = cu;
   }
   return cache[dev];
 }
@@ -795,33 +860,34 @@ ChunkPlan chunk_plan(int64_t R, int64_t T, int64_t nqmax) {
   ChunkPlan p;
   p.ct = chunk_ct(R, T);
   p.I = R + T / (4 * p.ct);
-  p.G = nqmax > 0 ? chunk_groups() : 0;
+  p.G = nqmax > 0 ? chunk_cus() * (p.ct == 1 ? 3 : 2) : 0;   // what is resident at 150 / 207 VGPRs
   p.cols = nqmax > 0 ? (p.G + 2 * p.I) * 64 * p.ct : 0;
   p.pre = nqmax > 0 ? (R + 2) / 2 * 2 : 0;
   return p;
 }
 
+template <int CT, int NW>
+int chunk_exact(const ChunkArgs& A, bool quant, hipStream_t s) {
+  const unsigned nx = (unsigned)(4 * A.I);
+  if (quant)
+    hipLaunchKernelGGL((chunk_exact_kernel<CT, NW, false>), dim3(nx), dim3(64 * NW), 0, s, A);
+  else
+    hipLaunchKernelGGL((chunk_exact_kernel<CT, NW, true>), dim3(nx + 1), dim3(64 * NW), 0, s, A);
+  return check_launch("chunk_exact");
+}
 template <int CT>
 int chunk_launch(const ChunkArgs& A, bool quant, hipStream_t s) {
-  const unsigned nx = (unsigned)(4 * A.I);
+  int rc;
   if (quant) {
     hipLaunchKernelGGL(chunk_quant_kernel<CT>, dim3((unsigned)A.G), dim3(256), 0, s, A);
-    int rc = check_launch("chunk_quant");
-    if (rc != KV800_OK) return rc;
-    if (A.R <= 128)
-      hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, false>), dim3(nx), dim3(256), 0, s, A);
-    else
-      hipLaunchKernelGGL((chunk_exact_kernel<CT, 1, false>), dim3(nx), dim3(64), 0, s, A);
-    rc = check_launch("chunk_exact");
-    if (rc != KV800_OK) return rc;
-    hipLaunchKernelGGL(chunk_merge_kernel<CT>, dim3((unsigned)(4 * A.T)), dim3(256), 0, s, A);
-    return check_launch("chunk_merge");
+    if ((rc = check_launch("chunk_quant")) != KV800_OK) return rc;
   }
-  if (A.R <= 128)
-    hipLaunchKernelGGL((chunk_exact_kernel<CT, 4, true>), dim3(nx + 1), dim3(256), 0, s, A);
-  else
-    hipLaunchKernelGGL((chunk_exact_kernel<CT, 1, true>), dim3(nx + 1), dim3(64), 0, s, A);
-  return check_launch("chunk_exact");
+  // waves per (tile, KV head): as many as are resident at once, by the rows' (tile, head) pairs (70, 35 and 17 KB of LDS)
+  const int64_t cu = chunk_cus(), pairs = 4 * max(A.R, A.T / (4 * CT));
+  rc = pairs <= 2 * cu ? chunk_exact<CT, 4>(A, quant, s) : pairs <= 4 * cu ? chunk_exact<CT, 2>(A, quant, s) : chunk_exact<CT, 1>(A, quant, s);
+  if (rc != KV800_OK || !quant) return rc;
+  hipLaunchKernelGGL(chunk_merge_kernel<CT>, dim3((unsigned)(4 * A.T)), dim3(256), 0, s, A);
+  return check_launch("chunk_merge");
 }
 
 }  // namespace
