@@ -29,8 +29,8 @@ int lfm3_hip_conv_chunk(const uint16_t* bcx, int64_t stride, const uint16_t* con
 int lfm3_hip_conv_commit(uint16_t* state, const uint16_t* taps, const int64_t* qsl, const int32_t* kept, int64_t R,
                          int64_t T, int64_t H, void* stream);
 
-/* Workspace bytes of lfm3_hip_verify_drafts for T rows of V logits. */
-int64_t lfm3_hip_verify_workspace(int64_t T, int64_t V);
+/* Workspace bytes of lfm3_hip_verify_drafts for R rows with T tokens in all and V logits each. */
+int64_t lfm3_hip_verify_workspace(int64_t R, int64_t T, int64_t V);
 
 /* Verification of drafted tokens. logits (T, V) bf16 (row stride ld): row t holds the target's logits behind token t; within a
  * row's tokens, token t + 1 is the draft that logits row t judges. p = softmax(logits / temp[r]) in 64 bits. A draft d is
@@ -41,7 +41,7 @@ int64_t lfm3_hip_verify_workspace(int64_t T, int64_t V);
  * largest logit (the first of equal ones; the first NaN ranks above every number) and the row ends with that one.
  * Drafts outside [0, V) are never kept. out (T) int64: row r's kept drafts and its last token at qsl[r] .., -1 in the rest
  * and in the padding; count (R) int32: how many (0 for a row without tokens). u (T), u_next (R) fp32 in [0, 1). Sums run in
- * a fixed order. ws: lfm3_hip_verify_workspace bytes, 16-byte aligned; 0 < V < 2^31, any strides >= V. */
+ * a fixed order. ws: lfm3_hip_verify_workspace bytes, 16-byte aligned; 0 < V < 2^31, any strides >= V; R, T <= 65,535. */
 int lfm3_hip_verify_drafts(const uint16_t* logits, int64_t ld, const int64_t* tokens, const int64_t* qsl, const float* temp,
                            const float* u, const float* u_next, const float* draft_probs, int64_t ldq, int64_t R,
                            int64_t T, int64_t V, int64_t* out, int32_t* count, void* ws, int64_t ws_bytes, void* stream);

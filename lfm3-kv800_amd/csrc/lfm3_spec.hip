@@ -2,8 +2,9 @@
 //
 //   conv_chunk_kernel     the gated short conv over each row's new tokens, from the row's 6-tap state
 //   conv_commit_kernel    that state moved on over the tokens that were kept
-//   verify_stats_kernel   per piece of a logits row: largest value, its index, sum of exponentials
-//   verify_pick_kernel    per row of the batch: which drafts are kept, and the token behind them
+//   verify_stats_kernel     per piece of a logits row: largest value, its index, sum of exponentials
+//   verify_residual_kernel  per piece of the logits row that ends a batch row: what p has over q
+//   verify_pick_kernel      per batch row: which drafts are kept, and the token behind them
 #include "kv800_common.h"
 #include "../../include/kv800_hip.h"
 #include "../../include/lfm3_spec.h"
@@ -179,11 +180,15 @@ conv_commit_kernel(uint16_t* __restrict__ state, const uint16_t* __restrict__ ta
 }
 
 // ---------------------------------------------------------------- verification of drafts
-// A logits row is cut into pieces of VP; a piece gives its largest value m, its index and s = sum exp((x - m) / temp) in
-// 64 bits. Why 64: the token behind a rejection is found by the running sum passing u W, and among 65,536 tokens the sums
-// of neighbours lie 1e-5 apart where 32-bit exponentials are 1e-7 off; and the choice has to be the same whatever
-// way the row is cut.
-constexpr int VT = 256, VE = 32, VP = VT * VE;         // threads, values a thread, values a piece
+// A logits row is cut into pieces; verify_stats gives each piece's largest value m, its index and s = sum exp((x - m) / temp).
+// verify_residual (drafts with a distribution) and verify_pick derive from these which row of logits ends a batch row, each
+// workgroup for itself; the first sums max(p - q, 0) over its piece of that row, the second picks the piece in which the
+// running sum passes u W and scans it. So every row of logits is read once, the deciding one of each batch row (and its
+// q) once more, and one piece of it again.
+// All in 64 bits: the running sums of neighbours among 65,536 tokens lie 1e-5 apart where 32-bit exponentials are
+// 1e-7 off, and the choice has to be the same whatever way a row is cut. Bound: the logits' bytes and the exponentials'
+// instructions alike (about 20 of 64 bits per value). VERIFY_TIME
+constexpr int VT = 256;                                // threads; a piece holds VT x VE values, VE = 8 or 32 a thread
 struct Stat { double s; float m; int32_t at; };        // 16 bytes
 
 // (a, ia) ranks before (b, ib): larger first, the smaller index among equals, the first NaN before every number
@@ -199,29 +204,92 @@ __device__ __forceinline__ double wave_sumd(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-__device__ __forceinline__ double expo(float x, float m, double it) { return exp(((double)x - (double)m) * it); }
+// exp(y), y <= 0, within 2^-51: y = (16 k + j) ln2 / 16 + r, |r| <= ln2 / 32; 2^(j / 16) from a table of 16 in LDS (32 banks:
+// any lanes at once), exp(r) as its series to r^6 / 720 (the next term is 5e-16). y = -inf gives 0.
+__device__ const double POW16[16] = {1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+__device__ __forceinline__ double expo(double y, const double* pow16) {
+  y = fmax(y, -800.0);
+  const double z = rint(y * 23.083120654223414);       // 16 / ln2
+  const double r = fma(z, -0.043321698784996581, y);   // ln2 / 16
+  const int k = (int)z;
+  double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+  p = fma(r, p, 1.0 / 24.0);
+  p = fma(r, p, 1.0 / 6.0);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, 1.0);
+  p = fma(r, p, 1.0);
+  return ldexp(p * pow16[k & 15], k >> 4);
+}
+__device__ __forceinline__ double expo(float x, float m, double it, const double* pow16) {
+  return expo(((double)x - (double)m) * it, pow16);
+}
 
-__global__ void __launch_bounds__(VT)
-verify_stats_kernel(const uint16_t* __restrict__ logits, int64_t ld, const int64_t* __restrict__ qsl,
-                    const float* __restrict__ temp, int64_t R, int64_t T, int64_t V, int64_t pieces, Stat* __restrict__ st) {
+// A thread's values of a piece: in group k of VE / 8, the 8 from index 8 (256 k + tid) on. 16-byte loads where a whole aligned
+// group is there, else one by one; what lies past n is `fill`.
+template <int VE>
+__device__ __forceinline__ void load_piece(const uint16_t* p, int n, float fill, float (&x)[VE / 8][8]) {
+  const bool al = ((uintptr_t)p & 15) == 0;
+#pragma unroll
+  for (int k = 0; k < VE / 8; ++k) {
+    const int i = 8 * (VT * k + (int)threadIdx.x);
+    if (al && i + 8 <= n) load8(p + i, x[k]);
+    else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] = i + e < n ? bf2f(p[i + e]) : fill;
+    }
+  }
+}
+template <int VE>
+__device__ __forceinline__ void load_piece(const float* p, int n, float fill, float (&x)[VE / 8][8]) {
+  const bool al = ((uintptr_t)p & 15) == 0;
+#pragma unroll
+  for (int k = 0; k < VE / 8; ++k) {
+    const int i = 8 * (VT * k + (int)threadIdx.x);
+    if (al && i + 8 <= n) {
+      const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
+      x[k][0] = a.x; x[k][1] = a.y; x[k][2] = a.z; x[k][3] = a.w;
+      x[k][4] = b.x; x[k][5] = b.y; x[k][6] = b.z; x[k][7] = b.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] = i + e < n ? p[i + e] : fill;
+    }
+  }
+}
+
+struct VerifyArgs {
+  const uint16_t* logits;
+  int64_t ld;
+  const int64_t *tokens, *qsl;
+  const float *temp, *u, *u_next, *q;
+  int64_t ldq, R, T, V, pieces;
+  Stat* st;            // (T, pieces)
+  double* left;        // (R, pieces): sums of max(p - q, 0) over the deciding rows' pieces
+  int64_t* out;
+  int32_t* count;
+};
+
+template <int VE>
+__global__ void __launch_bounds__(VT) verify_stats_kernel(VerifyArgs A) {
+  __shared__ double pow16[16], rs[4];
   __shared__ float rm[4];
   __shared__ int ri[4];
-  __shared__ double rs[4];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-  const int64_t t = blockIdx.y, v0 = (int64_t)blockIdx.x * VP;
-  if (t >= min(qsl[R], T)) return;                     // uniform
-  const float tp = temp[row_of(qsl, R, t)];
-  const int n = (int)min((int64_t)VP, V - v0);
-  const uint16_t* row = logits + t * ld + v0;
-  float x[VE];
+  const int64_t t = blockIdx.y, v0 = (int64_t)blockIdx.x * (VT * VE);
+  if (t >= min(A.qsl[A.R], A.T)) return;               // uniform
+  const int n = (int)min((int64_t)(VT * VE), A.V - v0);
+  float x[VE / 8][8];
+  load_piece<VE>(A.logits + t * A.ld + v0, n, -INFINITY, x);
+  if (tid < 16) pow16[tid] = POW16[tid];
+  const float tp = A.temp[row_of(A.qsl, A.R, t)];
   float bm = -INFINITY;
   int bi = 0x7FFFFFFF;
 #pragma unroll
-  for (int k = 0; k < VE; ++k) {
-    const int i = tid + VT * k;
-    x[k] = i < n ? bf2f(row[i]) : -INFINITY;
-    if (i < n && ranks_before(x[k], i, bm, bi)) { bm = x[k]; bi = i; }
-  }
+  for (int k = 0; k < VE / 8; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = 8 * (VT * k + tid) + e;
+      if (i < n && ranks_before(x[k][e], i, bm, bi)) { bm = x[k][e]; bi = i; }
+    }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float m2 = __shfl_xor(bm, o, 64);
@@ -237,46 +305,42 @@ verify_stats_kernel(const uint16_t* __restrict__ logits, int64_t ld, const int64
   if (sampled(tp, bm)) {
     const double it = 1.0 / (double)tp;
 #pragma unroll
-    for (int k = 0; k < VE; ++k)
-      if (tid + VT * k < n) s += expo(x[k], bm, it);
+    for (int k = 0; k < VE / 8; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += expo(x[k][e], bm, it, pow16);   // 0 for what lies past the row
   }
   s = wave_sumd(s);
   if (lane == 0) rs[w] = s;
   __syncthreads();
-  if (tid == 0) st[t * pieces + blockIdx.x] = Stat{(rs[0] + rs[1]) + (rs[2] + rs[3]), bm, (int32_t)(v0 + bi)};
+  if (tid == 0) A.st[t * A.pieces + blockIdx.x] = Stat{(rs[0] + rs[1]) + (rs[2] + rs[3]), bm, (int32_t)(v0 + bi)};
 }
 
-// One workgroup of 1,024 threads per row of the batch.
-constexpr int PT = 1024, PW = PT / 64;
-__global__ void __launch_bounds__(PT)
-verify_pick_kernel(const uint16_t* __restrict__ logits, int64_t ld, const int64_t* __restrict__ tokens,
-                   const int64_t* __restrict__ qsl, const float* __restrict__ temp, const float* __restrict__ u,
-                   const float* __restrict__ u_next, const float* __restrict__ q, int64_t ldq, int64_t R, int64_t T,
-                   int64_t V, int64_t pieces, const Stat* __restrict__ st, int64_t* __restrict__ out,
-                   int32_t* __restrict__ count) {
-  __shared__ long long stop;                           // the first logits row that ends the batch row
-  __shared__ double seg[PW], top_s;
-  __shared__ float top_m;
-  __shared__ int top_at, found, part;
+// What a batch row comes to, the same in every thread of the workgroup.
+struct Verdict {
+  int64_t s0, s1, t;   // the row's tokens; the logits row that ends it
+  float m;             // that row's largest logit,
+  int at;              // where it is,
+  double s;            // sum of exp((x - m) / temp)
+  double it;           // 1 / temp
+  bool sample, full;   // sampled; all drafts kept
+};
+struct VerdictLds { long long stop; double pow16[16], s; float m; int at; };
+__device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, VerdictLds& L) {
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-  const int64_t r = blockIdx.x;
-  const int64_t s0 = min(qsl[r], T), s1 = min(qsl[r + 1], T);
-  if (r == R - 1)
-    for (int64_t t = s1 + tid; t < T; t += PT) out[t] = -1;   // the padding
-  if (s1 <= s0) {
-    if (tid == 0) count[r] = 0;
-    return;
-  }
-  const float tp = temp[r];
-  const double it = 1.0 / (double)tp;
-  if (tid == 0) { stop = s1 - 1; found = -1; }
+  Verdict d;
+  d.s0 = min(A.qsl[r], A.T);
+  d.s1 = min(A.qsl[r + 1], A.T);
+  const float tp = A.temp[r];
+  d.it = 1.0 / (double)tp;
+  if (tid < 16) L.pow16[tid] = POW16[tid];
+  if (tid == 0) L.stop = d.s1 - 1;
   __syncthreads();
-  // a logits row's pieces combined: largest value, its index and the sum about it, the same in every lane
+  // a logits row's pieces combined, by a wave: the same result in every lane
   auto combine = [&](int64_t t, float& M, int& at, double& S) {
     M = -INFINITY;
     at = 0x7FFFFFFF;
-    for (int64_t p = lane; p < pieces; p += 64) {
-      const Stat a = st[t * pieces + p];
+    for (int64_t p = lane; p < A.pieces; p += 64) {
+      const Stat a = A.st[t * A.pieces + p];
       if (ranks_before(a.m, a.at, M, at)) { M = a.m; at = a.at; }
     }
 #pragma unroll
@@ -287,110 +351,251 @@ verify_pick_kernel(const uint16_t* __restrict__ logits, int64_t ld, const int64_
     }
     S = 0.0;
     if (sampled(tp, M))
-      for (int64_t p = lane; p < pieces; p += 64) {
-        const Stat a = st[t * pieces + p];
-        if (a.m > -INFINITY) S += a.s * expo(a.m, M, it);
+      for (int64_t p = lane; p < A.pieces; p += 64) {
+        const Stat a = A.st[t * A.pieces + p];
+        S += a.s * expo(a.m, M, d.it, L.pow16);
       }
     S = wave_sumd(S);
   };
-  for (int64_t t = s0 + w; t < s1 - 1; t += PW) {
+  for (int64_t t = d.s0 + w; t < d.s1 - 1; t += VT / 64) {
     float M;
     int at;
     double S;
+    const int64_t k = A.tokens[t + 1];
+    const bool in = k >= 0 && k < A.V;
+    const float xk = in ? bf2f(A.logits[t * A.ld + k]) : -INFINITY, ut = A.u[t];
+    const double qk = A.q ? (in ? (double)A.q[t * A.ldq + k] : 0.0) : 1.0;
     combine(t, M, at, S);
-    const int64_t d = tokens[t + 1];
-    bool keep;
-    if (!sampled(tp, M)) keep = d == at;
-    else {
-      keep = d >= 0 && d < V;
-      if (keep) {
-        const double pd = expo(bf2f(logits[t * ld + d]), M, it) / S;
-        keep = (double)u[t] * (q ? (double)q[t * ldq + d] : 1.0) < pd;
-      }
-    }
+    const bool keep = sampled(tp, M) ? in && (double)ut * qk < expo(xk, M, d.it, L.pow16) / S : k == at;
     if (!keep) {
-      if (lane == 0) atomicMin((long long*)&stop, (long long)t);
+      if (lane == 0) atomicMin(&L.stop, (long long)t);
       break;
     }
   }
   __syncthreads();
-  const int64_t tt = stop;
+  d.t = L.stop;
   if (w == 0) {
     float M;
     int at;
     double S;
-    combine(tt, M, at, S);
-    if (lane == 0) { top_m = M; top_at = at; top_s = S; }
+    combine(d.t, M, at, S);
+    if (lane == 0) { L.m = M; L.at = at; L.s = S; }
   }
   __syncthreads();
-  const float M = top_m;
-  int64_t pick = top_at;
-  if (sampled(tp, M)) {                                // uniform over the workgroup
-    const double S = top_s;
-    const bool full = tt == s1 - 1;
-    const int64_t d = full ? -1 : tokens[tt + 1];
-    const uint16_t* row = logits + tt * ld;
-    const float* qr = (q && !full) ? q + tt * ldq : nullptr;
-    // mode 0: the row's distribution; 1: what p has over q; either way the weight of token i
-    auto weight = [&](int64_t i, bool plain) -> double {
-      const double p = expo(bf2f(row[i]), M, it) / S;
-      if (plain || full) return p;
-      if (!qr) return i == d ? 0.0 : p;
-      const double x = p - (double)qr[i];
-      return x > 0.0 ? x : 0.0;
-    };
-    for (int plain = 0; plain < 2; ++plain) {
-      // wave w sums its 1/16 of the row
-      const int64_t per = (V + PW - 1) / PW, a = min(V, w * per), b = min(V, a + per);
-      double s = 0.0;
-      for (int64_t i = a + lane; i < b; i += 64) s += weight(i, plain);
-      s = wave_sumd(s);
-      if (lane == 0) seg[w] = s;
-      __syncthreads();
-      double W = 0.0;
-      for (int k = 0; k < PW; ++k) W += seg[k];
-      if (W > 0.0 || plain) {
-        const double goal = fmax((double)u_next[r] * W, 0.0);
-        if (tid == 0) {                                // the wave in whose part the sum passes the goal
-          double c = 0.0;
-          int k = 0, lastk = 0;
-          for (; k < PW; ++k) {
-            if (seg[k] > 0.0) lastk = k;
-            if (c + seg[k] > goal) break;
-            c += seg[k];
-          }
-          part = k < PW ? k : lastk;
-        }
-        __syncthreads();
-        if (w == part) {
-          double c = 0.0;
-          for (int k = 0; k < w; ++k) c += seg[k];
-          int64_t at = -1, some = -1;                  // the token found; the last one with any weight
-          for (int64_t i0 = a; i0 < b && at < 0; i0 += 64) {
-            const int64_t i = i0 + lane;
-            const double x = i < b ? weight(i, plain) : 0.0;
-            double y = x;
+  d.m = L.m;
+  d.at = L.at;
+  d.s = L.s;
+  d.sample = sampled(tp, d.m);
+  d.full = d.t == d.s1 - 1;
+  return d;
+}
+
+// Weights of a piece of the deciding row: MODE 0: exp((x - m) / temp); 1: the same without token `skip`; 2: max(p - q, 0).
+template <int VE>
+__device__ __forceinline__ void piece_weights(const VerifyArgs& A, const Verdict& d, const double* pow16, int64_t piece, int mode,
+                                              int64_t skip, double (&g)[VE / 8][8]) {
+  const int64_t v0 = piece * (VT * VE);
+  const int n = (int)min((int64_t)(VT * VE), A.V - v0);
+  float x[VE / 8][8], q[VE / 8][8];
+  load_piece<VE>(A.logits + d.t * A.ld + v0, n, -INFINITY, x);
+  if (mode == 2) load_piece<VE>(A.q + d.t * A.ldq + v0, n, 0.f, q);
+  const double inv = 1.0 / d.s;
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-              const double z = __shfl_up(y, o, 64);
-              if (lane >= o) y += z;
-            }
-            const uint64_t over = __ballot(i < b && c + y > goal), any = __ballot(x > 0.0);
-            if (any) some = i0 + 63 - __clzll(any);
-            if (over) at = i0 + __ffsll((unsigned long long)over) - 1;
-            c += __shfl(y, 63, 64);
+  for (int k = 0; k < VE / 8; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      double y = expo(x[k][e], d.m, d.it, pow16);
+      if (mode == 1) y = v0 + 8 * (VT * k + (int)threadIdx.x) + e == skip ? 0.0 : y;
+      if (mode == 2) {
+        y = y * inv - (double)q[k][e];
+        y = y > 0.0 ? y : 0.0;                         // and for a q that is NaN
+      }
+      g[k][e] = y;
+    }
+}
+__device__ __forceinline__ double sum8(const double (&g)[8]) {
+  return ((g[0] + g[1]) + (g[2] + g[3])) + ((g[4] + g[5]) + (g[6] + g[7]));
+}
+// the piece's sum, in the order in which pick_in_piece takes it apart; the same in every thread
+template <int VE>
+__device__ __forceinline__ double piece_sum(const double (&g)[VE / 8][8], double* seg) {
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __syncthreads();                                     // seg's last readers are done
+#pragma unroll
+  for (int k = 0; k < VE / 8; ++k) {
+    const double s = wave_sumd(sum8(g[k]));
+    if (lane == 0) seg[4 * k + w] = s;                 // 64 lanes x 8 values from index 512 (4 k + w) on
+  }
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < VE / 2; ++k) s += seg[k];
+  return s;
+}
+
+template <int VE>
+__global__ void __launch_bounds__(VT) verify_residual_kernel(VerifyArgs A) {
+  __shared__ VerdictLds L;
+  __shared__ double seg[VE / 2];
+  const int64_t r = blockIdx.y;
+  if (min(A.qsl[r + 1], A.T) - min(A.qsl[r], A.T) < 2) return;   // no drafts
+  const Verdict d = decide(A, r, L);
+  if (!d.sample || d.full) return;
+  double g[VE / 8][8];
+  piece_weights<VE>(A, d, L.pow16, blockIdx.x, 2, -1, g);
+  const double s = piece_sum<VE>(g, seg);
+  if (threadIdx.x == 0) A.left[r * A.pieces + blockIdx.x] = s;
+}
+
+template <int VE>
+__global__ void __launch_bounds__(VT) verify_pick_kernel(VerifyArgs A) {
+  __shared__ VerdictLds L;
+  __shared__ double seg[VE / 2], total;
+  __shared__ int piece, where;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int64_t r = blockIdx.x;
+  {
+    const int64_t s0 = min(A.qsl[r], A.T), s1 = min(A.qsl[r + 1], A.T);
+    if (r == A.R - 1)
+      for (int64_t t = s1 + tid; t < A.T; t += VT) A.out[t] = -1;   // the padding
+    if (s1 <= s0) {
+      if (tid == 0) A.count[r] = 0;
+      return;
+    }
+  }
+  const Verdict d = decide(A, r, L);
+  int64_t pick = d.at;
+  if (d.sample) {                                      // uniform, like all of the branches below
+    const int64_t skip = d.full || A.q ? -1 : A.tokens[d.t + 1];
+    int mode = d.full ? 0 : A.q ? 2 : 1;
+    double g[VE / 8][8];
+    // first the piece that lacks a token, whose sum is taken anew and not by subtraction; then the piece picked
+    const int64_t sp = mode == 1 && skip >= 0 && skip < A.V ? skip / (VT * VE) : -1;
+    int64_t look = sp;
+    double own = 0.0;
+    for (bool picked = false;;) {
+      if (look >= 0) {
+        piece_weights<VE>(A, d, L.pow16, look, mode, skip, g);
+        own = piece_sum<VE>(g, seg);
+      }
+      if (picked) break;
+      if (w == 0) {                                    // the pieces' running sum passes u W in piece `piece`
+        auto weight = [&](int64_t p) -> double {
+          if (p >= A.pieces) return 0.0;
+          if (mode == 2) return A.left[r * A.pieces + p];
+          if (mode == 1 && p == sp) return own;
+          const Stat a = A.st[d.t * A.pieces + p];
+          return a.s * expo(a.m, d.m, d.it, L.pow16);
+        };
+        double W = 0.0;
+        for (int64_t p0 = 0; p0 < A.pieces; p0 += 64) W += wave_sumd(weight(p0 + lane));
+        const double gl = fmax((double)A.u_next[r] * W, 0.0);
+        double c = 0.0, before = 0.0;
+        int64_t at = -1, lastp = -1;
+        double lastc = 0.0;
+        for (int64_t p0 = 0; p0 < A.pieces && at < 0; p0 += 64) {
+          const double x = weight(p0 + lane);
+          double y = x;
+#pragma unroll
+          for (int o = 1; o < 64; o <<= 1) {
+            const double z = __shfl_up(y, o, 64);
+            if (lane >= o) y += z;
           }
-          if (lane == 0) found = (int)(at >= 0 ? at : some);
+          const uint64_t over = __ballot(x > 0.0 && c + y > gl), any = __ballot(x > 0.0);
+          if (any) {
+            const int k = 63 - __clzll(any);
+            lastp = p0 + k;
+            lastc = c + __shfl(y - x, k, 64);
+          }
+          if (over) {
+            const int k = __ffsll((unsigned long long)over) - 1;
+            at = p0 + k;
+            before = c + __shfl(y - x, k, 64);
+          }
+          c += __shfl(y, 63, 64);
         }
-        __syncthreads();
-        break;
+        if (at < 0) { at = lastp; before = lastc; }    // u at 1 or past it: the last one with any weight
+        if (lane == 0) { total = W > 0.0 ? fmax(gl - before, 0.0) : -1.0; piece = (int)at; where = -1; }
       }
       __syncthreads();
+      if (total < 0.0 && mode != 0) {                  // nothing is left of p: p itself
+        mode = 0;
+        look = -1;
+        __syncthreads();
+        continue;
+      }
+      look = piece;
+      picked = true;
+      if (look < 0) break;
     }
-    if (found >= 0) pick = found;
+    if (look >= 0) {
+      const double gl = total;
+      double c = 0.0;
+      int hit = -1, lasts = -1;                        // the segment of 512 in which it passes; the last one with any weight
+#pragma unroll
+      for (int k = 0; k < VE / 2; ++k) {
+        if (seg[k] > 0.0) {
+          lasts = k;
+          if (hit < 0 && c + seg[k] > gl) hit = k;
+        }
+        if (hit < 0) c += seg[k];
+      }
+      if (hit < 0) {
+        hit = lasts;
+        c = INFINITY;                                  // any weight: the last one
+      }
+      if (hit >= 0 && (hit & 3) == w) {
+        double y[8];
+#pragma unroll
+        for (int k = 0; k < VE / 8; ++k)
+          if (k == hit >> 2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = g[k][e];
+          }
+        const double x = sum8(y);
+        double pre = x;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const double z = __shfl_up(pre, o, 64);
+          if (lane >= o) pre += z;
+        }
+        double run = c == INFINITY ? -INFINITY : c + (pre - x);
+        int at = -1, lastw = -1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          run += y[e];
+          if (y[e] > 0.0) lastw = e;
+          if (at < 0 && y[e] > 0.0 && run > gl) at = e;
+        }
+        const uint64_t over = __ballot(at >= 0), any = __ballot(lastw >= 0);
+        const int from = over ? __ffsll((unsigned long long)over) - 1 : any ? 63 - __clzll(any) : -1;
+        if (lane == from) where = 512 * hit + 8 * lane + (over ? at : lastw);
+      }
+      __syncthreads();
+      if (where >= 0) pick = look * (VT * VE) + where;
+    }
   }
-  for (int64_t t = s0 + tid; t < s1; t += PT) out[t] = t < tt ? tokens[t + 1] : t == tt ? pick : -1;
-  if (tid == 0) count[r] = (int32_t)(tt - s0 + 1);
+  for (int64_t t = d.s0 + tid; t < d.s1; t += VT) A.out[t] = t < d.t ? A.tokens[t + 1] : t == d.t ? pick : -1;
+  if (tid == 0) A.count[r] = (int32_t)(d.t - d.s0 + 1);
+}
+
+// 2,048-value pieces while all rows in them fill the chip about twice, else 8,192
+int verify_ve(int64_t T, int64_t V) { return T * ((V + 8 * VT - 1) / (8 * VT)) <= 1024 ? 8 : 32; }
+int64_t verify_pieces(int64_t T, int64_t V) { const int64_t n = VT * verify_ve(T, V); return (V + n - 1) / n; }
+
+template <int VE>
+int verify_launch(const VerifyArgs& A, hipStream_t s) {
+  int rc;
+  if (A.T > 0) {
+    hipLaunchKernelGGL(verify_stats_kernel<VE>, dim3((unsigned)A.pieces, (unsigned)A.T), dim3(VT), 0, s, A);
+    if ((rc = kv800::check_launch("verify_stats")) != KV800_OK) return rc;
+    if (A.q) {
+      hipLaunchKernelGGL(verify_residual_kernel<VE>, dim3((unsigned)A.pieces, (unsigned)A.R), dim3(VT), 0, s, A);
+      if ((rc = kv800::check_launch("verify_residual")) != KV800_OK) return rc;
+    }
+  }
+  hipLaunchKernelGGL(verify_pick_kernel<VE>, dim3((unsigned)A.R), dim3(VT), 0, s, A);
+  return kv800::check_launch("verify_pick");
 }
 
 }  // namespace
@@ -431,9 +636,9 @@ int lfm3_hip_conv_commit(uint16_t* state, const uint16_t* taps, const int64_t* q
   return kv800::check_launch("conv_commit");
 }
 
-int64_t lfm3_hip_verify_workspace(int64_t T, int64_t V) {
-  if (T <= 0 || V <= 0) return 0;
-  return T * ((V + lfm3::VP - 1) / lfm3::VP) * (int64_t)sizeof(lfm3::Stat);
+int64_t lfm3_hip_verify_workspace(int64_t R, int64_t T, int64_t V) {
+  if (R <= 0 || T <= 0 || V <= 0) return 0;
+  return lfm3::verify_pieces(T, V) * (T * (int64_t)sizeof(lfm3::Stat) + R * (int64_t)sizeof(double));
 }
 
 int lfm3_hip_verify_drafts(const uint16_t* logits, int64_t ld, const int64_t* tokens, const int64_t* qsl, const float* temp,
@@ -441,22 +646,15 @@ int lfm3_hip_verify_drafts(const uint16_t* logits, int64_t ld, const int64_t* to
                            int64_t T, int64_t V, int64_t* out, int32_t* count, void* ws, int64_t ws_bytes, void* stream) {
   KV800_REQUIRE(R >= 1 && T >= 0 && V > 0 && V < (1LL << 31) && ld >= V && (!draft_probs || ldq >= V),
                 "verify_drafts: needs R >= 1, 0 < V < 2^31 and row strides of at least V");
-  KV800_REQUIRE(R <= 0x7FFFFFFF && T <= 65535, "verify_drafts: at most 65,535 tokens a call");
+  KV800_REQUIRE(R <= 65535 && T <= 65535, "verify_drafts: at most 65,535 rows and tokens a call");
   KV800_REQUIRE(qsl && count && (T == 0 || (logits && tokens && temp && u && u_next && out)), "verify_drafts: null pointer");
-  KV800_REQUIRE(ws_bytes >= lfm3_hip_verify_workspace(T, V) && (T == 0 || (ws && (uintptr_t)ws % 16 == 0)),
+  KV800_REQUIRE(ws_bytes >= lfm3_hip_verify_workspace(R, T, V) && (T == 0 || (ws && (uintptr_t)ws % 16 == 0)),
                 "verify_drafts: the workspace is too small or not 16-byte aligned");
-  const int64_t pieces = (V + lfm3::VP - 1) / lfm3::VP;
+  lfm3::VerifyArgs A = {logits, ld, tokens, qsl, temp, u, u_next, draft_probs, ldq, R, T, V, lfm3::verify_pieces(T, V),
+                        reinterpret_cast<lfm3::Stat*>(ws), nullptr, out, count};
+  A.left = reinterpret_cast<double*>(A.st + T * A.pieces);
   const hipStream_t s = (hipStream_t)stream;
-  lfm3::Stat* st = reinterpret_cast<lfm3::Stat*>(ws);
-  if (T > 0) {
-    hipLaunchKernelGGL(lfm3::verify_stats_kernel, dim3((unsigned)pieces, (unsigned)T), dim3(lfm3::VT), 0, s, logits, ld, qsl, temp,
-                       R, T, V, pieces, st);
-    const int rc = kv800::check_launch("verify_stats");
-    if (rc != KV800_OK) return rc;
-  }
-  hipLaunchKernelGGL(lfm3::verify_pick_kernel, dim3((unsigned)R), dim3(lfm3::PT), 0, s, logits, ld, tokens, qsl, temp, u, u_next,
-                     draft_probs, ldq, R, T, V, pieces, st, out, count);
-  return kv800::check_launch("verify_pick");
+  return lfm3::verify_ve(T, V) == 8 ? lfm3::verify_launch<8>(A, s) : lfm3::verify_launch<32>(A, s);
 }
 
 }  // extern "C"

@@ -137,8 +137,13 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
 
+def _raw_stream(dev):
+    """The current stream of dev as an integer (without the Stream object that torch.cuda.current_stream makes, 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
+
+
 def _stream(dev):
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    return ctypes.c_void_p(_raw_stream(dev))
 
 
 class _Here:
@@ -358,15 +363,17 @@ def chunk_meta(bt, lens, qlens, ebs, tokens, held=None, free=None, taken=None):
         return ChunkMeta(torch.zeros(1, dtype=torch.int64, device=dev), pad, pad.clone(), torch.zeros_like(pad),
                          torch.empty(0, dtype=torch.int32, device=dev), held, taken)
     lens, qlens = lens.contiguous(), qlens.contiguous()
-    m = torch.empty(R + 1 + 3 * tokens + 1, dtype=torch.int64, device=dev)   # one allocation: qsl, slot, pos, row, taken
-    qsl, slot, pos, row, tk = m.split((R + 1, tokens, tokens, tokens, 1))
-    i32 = torch.empty((2 if grow else 1) * R, dtype=torch.int32, device=dev)
+    qsl, slot, pos, row, tk = torch.empty(R + 2 + 3 * tokens, dtype=torch.int64, device=dev).split((R + 1, tokens, tokens, tokens, 1))
+    l32 = torch.empty(R, dtype=torch.int32, device=dev)
+    after = torch.empty(R, dtype=torch.int32, device=dev) if grow else None
     with _on(dev):
-        _check(L.kv800_hip_chunk_meta(_ptr(bt), bt.stride(0) if R > 1 else max(bt.shape[1], 1), bt.shape[1], _ptr(lens),
-                                      _ptr(qlens), R, ebs, tokens, _ptr(held), _ptr(free), free.shape[0] if grow else 0,
-                                      _ptr(taken), _ptr(i32[R:]) if grow else None, _ptr(tk) if grow else None, _ptr(qsl),
-                                      _ptr(slot), _ptr(pos), _ptr(row), _ptr(i32), _stream(dev)))
-    return ChunkMeta(qsl, slot, pos, row, i32[:R], i32[R:] if grow else None, tk if grow else None)
+        _check(L.kv800_hip_chunk_meta(bt.data_ptr(), bt.stride(0) if R > 1 else max(bt.shape[1], 1), bt.shape[1],
+                                      lens.data_ptr(), qlens.data_ptr(), R, ebs, tokens, held.data_ptr() if grow else None,
+                                      free.data_ptr() if grow else None, free.shape[0] if grow else 0,
+                                      taken.data_ptr() if grow else None, after.data_ptr() if grow else None,
+                                      tk.data_ptr() if grow else None, qsl.data_ptr(), slot.data_ptr(), pos.data_ptr(),
+                                      row.data_ptr(), l32.data_ptr(), _raw_stream(dev)))
+    return ChunkMeta(qsl, slot, pos, row, l32, after, tk if grow else None)
 
 
 def page_offsets(bt, scale, add=0):
@@ -746,25 +753,25 @@ def rope_pairs(cos_t, sin_t):
     while it is cached; it is rebuilt when either tensor is modified in place (version counter) or replaced. A call on
     another stream than the one that built it waits for it; a table built while a graph is captured belongs to that graph
     alone, whose replays fill it."""
-    key = (str(cos_t.device), cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0])
+    key = (cos_t.device, cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0])
     ent = _PAIRS.get(key)
     ver = (cos_t._version, sin_t._version)
-    now = torch.cuda.current_stream(cos_t.device)
-    capturing = torch.cuda.is_current_stream_capturing()
+    now = _raw_stream(cos_t.device)
     if ent is not None and ent[0] is cos_t and ent[1] is sin_t and ent[2] == ver:
         _PAIRS.move_to_end(key)
-        if ent[4] != now and not capturing:   # a capture begins by waiting for the device
-            now.wait_event(ent[5])
-            ent[3].record_stream(now)
+        if ent[4] != now and not torch.cuda.is_current_stream_capturing():   # a capture begins by waiting for the device
+            stream = torch.cuda.current_stream(cos_t.device)
+            stream.wait_event(ent[5])
+            ent[3].record_stream(stream)
         return ent[3]
     L = ops()
     P = cos_t.shape[0]
     t = torch.empty(P, 32, dtype=torch.int32, device=cos_t.device)
     _check(L.kv800_hip_rope_table(_ptr(cos_t), _ptr(sin_t), P, _ptr(t), _stream(cos_t.device)))
-    if capturing:
+    if torch.cuda.is_current_stream_capturing():
         return t
     done = torch.cuda.Event()
-    done.record(now)
+    done.record(torch.cuda.current_stream(cos_t.device))
     _PAIRS[key] = (cos_t, sin_t, ver, t, now, done)
     _PAIRS.move_to_end(key)
     while len(_PAIRS) > 8:
@@ -894,9 +901,10 @@ def decode_chunk(P, q, qsl, cos_t, sin_t):
         cs2 = rope_pairs(cos_t, sin_t) if s.nqmax else None
         wsb = int(L.kv800_hip_decode_chunk_workspace(R, T, s.nqmax))
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-        _check(L.kv800_hip_decode_chunk(ctypes.byref(s), _ptr(q), _ptr(qsl), R, T, _ptr(cos_t), _ptr(sin_t),
-                                        cos_t.shape[0] if rot else 0, _ptr(cs2), qbytes, eelems, selems, _ptr(out), _ptr(ws),
-                                        wsb, _stream(dev)))
+        _check(L.kv800_hip_decode_chunk(ctypes.byref(s), q.data_ptr(), qsl.data_ptr(), R, T, cos_t.data_ptr() if rot else None,
+                                        sin_t.data_ptr() if rot else None, cos_t.shape[0] if rot else 0,
+                                        cs2.data_ptr() if cs2 is not None else None, qbytes, eelems, selems, out.data_ptr(),
+                                        ws.data_ptr() if wsb else None, wsb, _raw_stream(dev)))
     return out
 
 

@@ -9,13 +9,13 @@ import ctypes
 import torch
 
 from . import kv800_hip
-from .kv800_hip import _need, _on, _ptr, _stream
+from .kv800_hip import _need, _on, _raw_stream
 
 _VP, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 SIGNATURES = {
     "lfm3_hip_conv_chunk": (_I32, [_VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _VP, _VP, _VP]),
     "lfm3_hip_conv_commit": (_I32, [_VP, _VP, _VP, _VP, _I64, _I64, _I64, _VP]),
-    "lfm3_hip_verify_workspace": (_I64, [_I64, _I64]),
+    "lfm3_hip_verify_workspace": (_I64, [_I64, _I64, _I64]),
     "lfm3_hip_verify_drafts": (_I32, [_VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _I64,
                                       _VP]),
 }
@@ -63,13 +63,15 @@ def conv_chunk(bcx, conv_w, state, qsl):
         bcx = bcx.contiguous()
         if bcx.stride(0) % 8:      # an odd width: the three parts alone
             bcx = bcx[:, :3 * H].contiguous()
-    out = torch.empty(2, T, H, dtype=torch.bfloat16, device=dev)
+    out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
+    taps = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
     if T == 0 or R == 0 or H == 0:
-        return out.zero_().unbind(0)
+        return out.zero_(), taps.zero_()
+    conv_w = conv_w.contiguous()
     with _on(dev):
-        kv800_hip._check(L.lfm3_hip_conv_chunk(_ptr(bcx), bcx.stride(0), _ptr(conv_w.contiguous()), _ptr(state), _ptr(qsl), R, T,
-                                               H, _ptr(out[0]), _ptr(out[1]), _stream(dev)))
-    return out.unbind(0)
+        kv800_hip._check(L.lfm3_hip_conv_chunk(bcx.data_ptr(), bcx.stride(0), conv_w.data_ptr(), state.data_ptr(), qsl.data_ptr(),
+                                               R, T, H, out.data_ptr(), taps.data_ptr(), _raw_stream(dev)))
+    return out, taps
 
 
 def conv_commit(state, taps, qsl, kept):
@@ -87,7 +89,8 @@ def conv_commit(state, taps, qsl, kept):
         return
     taps, kept = taps.contiguous(), kept.contiguous()
     with _on(dev):
-        kv800_hip._check(L.lfm3_hip_conv_commit(_ptr(state), _ptr(taps), _ptr(qsl), _ptr(kept), R, taps.shape[0], H, _stream(dev)))
+        kv800_hip._check(L.lfm3_hip_conv_commit(state.data_ptr(), taps.data_ptr(), qsl.data_ptr(), kept.data_ptr(), R,
+                                                taps.shape[0], H, _raw_stream(dev)))
 
 
 def verify_drafts(logits, tokens, qsl, temperature, u, u_next, draft_probs=None):
@@ -118,13 +121,15 @@ def verify_drafts(logits, tokens, qsl, temperature, u, u_next, draft_probs=None)
     count = torch.empty(R, dtype=torch.int32, device=dev)
     if R == 0 or T == 0:
         return out.fill_(-1), count.zero_()
-    wsb = int(L.lfm3_hip_verify_workspace(T, V))
+    wsb = int(L.lfm3_hip_verify_workspace(R, T, V))
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    tokens, temperature, u, u_next = tokens.contiguous(), temperature.contiguous(), u.contiguous(), u_next.contiguous()
     with _on(dev):
         kv800_hip._check(L.lfm3_hip_verify_drafts(
-            _ptr(logits), logits.stride(0), _ptr(tokens.contiguous()), _ptr(qsl), _ptr(temperature.contiguous()),
-            _ptr(u.contiguous()), _ptr(u_next.contiguous()), _ptr(draft_probs),
-            0 if draft_probs is None else draft_probs.stride(0), R, T, V, _ptr(out), _ptr(count), _ptr(ws), wsb, _stream(dev)))
+            logits.data_ptr(), logits.stride(0), tokens.data_ptr(), qsl.data_ptr(), temperature.data_ptr(), u.data_ptr(),
+            u_next.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
+            0 if draft_probs is None else draft_probs.stride(0), R, T, V, out.data_ptr(), count.data_ptr(), ws.data_ptr(), wsb,
+            _raw_stream(dev)))
     return out, count
 
 

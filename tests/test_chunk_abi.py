@@ -87,8 +87,8 @@ def test_conv_host_checks(lib):
 
 
 def test_verify_host_checks(lib):
-    ws = lib.lfm3_hip_verify_workspace(4, 100)
-    assert ws > 0 and lib.lfm3_hip_verify_workspace(0, 100) == 0
+    ws = lib.lfm3_hip_verify_workspace(2, 4, 100)
+    assert ws > 0 and lib.lfm3_hip_verify_workspace(2, 0, 100) == 0
     f = lambda **k: lib.lfm3_hip_verify_drafts(*{**dict(x=A, ld=100, tok=A, qsl=A, temp=A, u=A, un=A, q=None, ldq=0, R=2, T=4, V=100, out=A,
                                                         cnt=A, ws=A, wsb=ws, s=None), **k}.values())
     for k in (dict(R=0), dict(T=-1), dict(V=0), dict(V=1 << 31), dict(ld=99), dict(q=A, ldq=99), dict(x=None), dict(tok=None),
