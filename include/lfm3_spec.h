@@ -37,7 +37,7 @@ int64_t lfm3_hip_verify_workspace(int64_t R, int64_t T, int64_t V);
  * kept iff u[t] q(d) < p(d), q = row t of draft_probs ((T, V) fp32, row stride ldq; NULL: all of it on d). At the first
  * draft that is not kept the row ends with a token of max(p - q, 0) (of p without d if NULL; of p where that is empty), a
  * row whose drafts are all kept with a token of p behind its last one: the first index whose running sum exceeds
- * u_next[r] times the whole. temp[r] not positive and finite, or a largest logit that is not finite: a draft is kept iff it is the
+ * u_next[r] times the whole. temp[r] not in (0, 1e30], or a largest logit that is not finite: a draft is kept iff it is the
  * largest logit (the first of equal ones; the first NaN ranks above every number) and the row ends with that one.
  * Drafts outside [0, V) are never kept. out (T) int64: row r's kept drafts and its last token at qsl[r] .., -1 in the rest
  * and in the padding; count (R) int32: how many (0 for a row without tokens). u (T), u_next (R) fp32 in [0, 1). Sums run in
