@@ -217,43 +217,63 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
   auto chunk = [&](const ChunkStage& S, int cc, int kpos) {
     f4 sc[2][CT];
     __builtin_amdgcn_s_setprio(3);
+    // 4 steps (tile u, kc dword d); a step's table reads are issued two steps ahead of their use, all operands of the
+    // stage before the first
+    uint2 kc[2];
+    u4v cs[2][2];
+    uint32_t kk[3][4], an[3][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      uint32_t kk[2][4], an[2][4];
-      const uint2 kc = *reinterpret_cast<const uint2*>(&S.kc[okc + 2048 * u]);
-      u4v cs[2];
+    for (int u = 0; u < 2; ++u) kc[u] = *reinterpret_cast<const uint2*>(&S.kc[okc + 2048 * u]);
 #pragma unroll
-      for (int d = 0; d < 2; ++d) cs[d] = *reinterpret_cast<const u4v*>(&S.cs[(ocs ^ (16 * d)) + 2048 * u]);
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        const uint32_t x = d ? kc.y : kc.x;
-        const uint32_t xr = (x << 2) & 0xCCCCCCCCu, xn = x & 0xCCCCCCCCu;
-        const char *br = lutc + 256 * (4 * d), *bn = lutc + 256 * (8 + 4 * d);
-        kk[d][0] = *reinterpret_cast<const uint32_t*>(br + byte_or<0>(xr, kg));
-        an[d][0] = *reinterpret_cast<const uint32_t*>(bn + byte_or<0>(xn, kg));
-        kk[d][1] = *reinterpret_cast<const uint32_t*>(br + 256 + byte_or<1>(xr, kg));
-        an[d][1] = *reinterpret_cast<const uint32_t*>(bn + 256 + byte_or<1>(xn, kg));
-        kk[d][2] = *reinterpret_cast<const uint32_t*>(br + 512 + byte_or<2>(xr, kg));
-        an[d][2] = *reinterpret_cast<const uint32_t*>(bn + 512 + byte_or<2>(xn, kg));
-        kk[d][3] = *reinterpret_cast<const uint32_t*>(br + 768 + byte_or<3>(xr, kg));
-        an[d][3] = *reinterpret_cast<const uint32_t*>(bn + 768 + byte_or<3>(xn, kg));
+      for (int d = 0; d < 2; ++d) cs[u][d] = *reinterpret_cast<const u4v*>(&S.cs[(ocs ^ (16 * d)) + 2048 * u]);
+    auto lookup = [&](const int st) {
+      const int u = st >> 1, d = st & 1, b = st % 3;
+      const uint32_t x = d ? kc[u].y : kc[u].x;
+      const uint32_t xr = (x << 2) & 0xCCCCCCCCu, xn = x & 0xCCCCCCCCu;
+      const char *br = lutc + 256 * (4 * d), *bn = lutc + 256 * (8 + 4 * d);
+      kk[b][0] = *reinterpret_cast<const uint32_t*>(br + byte_or<0>(xr, kg));
+      kk[b][1] = *reinterpret_cast<const uint32_t*>(br + 256 + byte_or<1>(xr, kg));
+      kk[b][2] = *reinterpret_cast<const uint32_t*>(br + 512 + byte_or<2>(xr, kg));
+      kk[b][3] = *reinterpret_cast<const uint32_t*>(br + 768 + byte_or<3>(xr, kg));
+      an[b][0] = *reinterpret_cast<const uint32_t*>(bn + byte_or<0>(xn, kg));
+      an[b][1] = *reinterpret_cast<const uint32_t*>(bn + 256 + byte_or<1>(xn, kg));
+      an[b][2] = *reinterpret_cast<const uint32_t*>(bn + 512 + byte_or<2>(xn, kg));
+      an[b][3] = *reinterpret_cast<const uint32_t*>(bn + 768 + byte_or<3>(xn, kg));
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    lookup(0);
+    lookup(1);
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      if (st + 2 < 4) lookup(st + 2);
+      const int u = st >> 1, d = st & 1, b = st % 3;
+      uint32_t c4[4], s4[4], ar[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c4[e] = cs[u][d][e];
+        s4[e] = __builtin_amdgcn_alignbit(cs[u][d][e], cs[u][d][e], 16);
       }
+      rope4(kk[b], c4, s4, ar);
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        uint32_t c4[4], s4[4], ar[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          c4[e] = cs[d][e];
-          s4[e] = __builtin_amdgcn_alignbit(cs[d][e], cs[d][e], 16);
-        }
-        rope4(kk[d], c4, s4, ar);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          sc[u][ct] = mfma_bf(pack8b(ar), bq[ct][d], d == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sc[u][ct]);
-          sc[u][ct] = mfma_bf(pack8b(an[d]), bq[ct][2 + d], sc[u][ct]);
-        }
+      for (int ct = 0; ct < CT; ++ct) {
+        sc[u][ct] = mfma_bf(pack8b(ar), bq[ct][d], d == 0 ? f4{0.f, 0.f, 0.f, 0.f} : sc[u][ct]);
+        sc[u][ct] = mfma_bf(pack8b(an[b]), bq[ct][2 + d], sc[u][ct]);
       }
     }
+    // what the softmax and P V read, issued under the last products
+    float4 vs4[2], vl4[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int tk = 32 * cc + 16 * u + 4 * g;
+      vs4[u] = *reinterpret_cast<const float4*>(&L.vs[h][tk]);
+      vl4[u] = *reinterpret_cast<const float4*>(&L.vl[h][tk]);
+    }
+    typedef __attribute__((address_space(3))) i2v lds_i2;
+    const i2v X = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(const_cast<uint8_t*>(S.vb) + ovb));
+    __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(2);
     if (kpos + 31 > pbase) {                           // a caller's NQ that reaches into the new tokens: mask by position
 #pragma unroll
@@ -265,20 +285,12 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
             if (kpos + 16 * u + 4 * g + i > pcol[ct]) sc[u][ct][i] = -INFINITY;
     }
     h8 Bw[CT];
-    float4 vs4[2], vl4[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int tk = 32 * cc + 16 * u + 4 * g;
-      vs4[u] = *reinterpret_cast<const float4*>(&L.vs[h][tk]);
-      vl4[u] = *reinterpret_cast<const float4*>(&L.vl[h][tk]);
-    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const f4 s0 = sc[0][ct], s1 = sc[1][ct];
       float tmax = maxn(maxn(maxn(s0[0], s0[1]), maxn(s0[2], s0[3])), maxn(maxn(s1[0], s1[1]), maxn(s1[2], s1[3])));
-      tmax = max4rows(tmax) * scale;
-      if (__any(tmax > m[ct] + QLAZY)) {
-        const float mn = fmaxf(m[ct], tmax);
+      if (__any(tmax * scale > m[ct] + QLAZY)) {       // a lane's own scores; the column's maximum only where it matters
+        const float mn = fmaxf(m[ct], max4rows(tmax + 0.f) * scale);
         const float al = __builtin_amdgcn_exp2f(m[ct] - mn);
         m[ct] = mn; lsum[ct] *= al; lvs[ct] *= al;
 #pragma unroll
@@ -298,8 +310,6 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
       Bw[ct] = pack8(pk2(wt[0][0], wt[0][2]), pk2(wt[0][1], wt[0][3]), pk2(wt[1][0], wt[1][2]), pk2(wt[1][1], wt[1][3]));
     }
     __builtin_amdgcn_s_setprio(0);
-    typedef __attribute__((address_space(3))) i2v lds_i2;
-    const i2v X = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(const_cast<uint8_t*>(S.vb) + ovb));
     const uint32_t x0 = (uint32_t)X.x, x1 = (uint32_t)X.x >> 8, x2 = (uint32_t)X.y, x3 = (uint32_t)X.y >> 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -483,6 +493,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   if (!find_tile<QT>(A, it, t)) return;
   const int N = __builtin_amdgcn_readfirstlane(A.P.N[t.row]), win = (int)A.P.win;
   const int pbase = N - t.c + t.q0, plast = pbase + t.nq - 1;
+  const bool wide = CT > 1 && t.nq > 4;                // a tile of up to 4 queries leaves the second column tile out
   // key list: sinks [0, cnt), exact positions lo_row .. + cnt2, then lo_tile ..
   int lo_row, lo_tile;
   if (win > 0) {
@@ -634,6 +645,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
+          if (ct > 0 && !wide) continue;
           f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int s = 0; s < 4; ++s) x = mfma_bf(as_b8(k[s]), bq[ct][s], x);
@@ -655,6 +667,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
       u4v bh[CT], bl[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
+        if (ct > 0 && !wide) continue;
         float xs[2][4], cm = -INFINITY;
         const int wlo = win > 0 ? pcol[ct] - win : -1;
 #pragma unroll
@@ -697,6 +710,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
                         __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 2, 3))};
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
+          if (ct > 0 && !wide) continue;
           acc[ct][j] = mfma_bf(as_b8(av), as_b8(bh[ct]), acc[ct][j]);
           acc[ct][j] = mfma_bf(as_b8(av), as_b8(bl[ct]), acc[ct][j]);
         }
@@ -720,6 +734,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
       if (g == 0) { L.m[w][16 * ct + n] = m[ct]; L.l[w][16 * ct + n] = lsum[ct]; }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+      if (ct > 0 && !wide) break;                      // uniform
       __syncthreads();                                 // the chunks, and the last column tile's join, are done
       float M = NEG_BIG, l = 0.f;
       for (int k = 0; k < NW; ++k) M = fmaxf(M, L.m[k][16 * ct + n]);
@@ -836,7 +851,8 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
 }
 
 // queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8
-int chunk_ct(int64_t R, int64_t T) { return T <= 4 * R ? 1 : 2; }
+// (layers without sub-blocks: while every row can bring one token only; their kernel passes over an empty second half).
+int chunk_ct(int64_t R, int64_t T, bool quant) { return T <= (quant ? 4 * R : R) ? 1 : 2; }
 
 int64_t chunk_cus() {
   static std::mutex mu;
@@ -858,7 +874,7 @@ int64_t chunk_cus() {
 struct ChunkPlan { int ct; int64_t G, I, cols, pre; };   // cols: partial columns; pre: int64 entries
 ChunkPlan chunk_plan(int64_t R, int64_t T, int64_t nqmax) {
   ChunkPlan p;
-  p.ct = chunk_ct(R, T);
+  p.ct = chunk_ct(R, T, nqmax > 0);
   p.I = R + T / (4 * p.ct);
   p.G = nqmax > 0 ? chunk_cus() * (p.ct == 1 ? 3 : 2) : 0;   // what is resident at 150 / 207 VGPRs
   p.cols = nqmax > 0 ? (p.G + 2 * p.I) * 64 * p.ct : 0;
