@@ -67,17 +67,20 @@ __device__ __forceinline__ int64_t row_of(const int64_t* qsl, int64_t R, int64_t
   return last_at(R, [&](int64_t i) { return qsl[i] <= t; });
 }
 
-// A tile: its row, the row's first token and queries, the tile's first query and queries
-struct Tile { int64_t row, t0; int c, q0, nq; };
+// A tile: its row, the row's first token, length and queries, the tile's first query and queries
+struct Tile { int64_t row, t0; int n, c, q0, nq; };
 template <int QT>
 __device__ __forceinline__ int64_t tile_number(const int64_t* qsl, int64_t T, int64_t r) { return r + min(qsl[r], T) / QT; }
 // Tile `it`: 64-way search for the last row whose first tile number is <= it, by a whole wave; false if the number has none.
 template <int QT>
 __device__ __forceinline__ bool find_tile(const ChunkArgs& A, int64_t it, Tile& t) {
   const int64_t lo = last_at(A.R, [&](int64_t i) { return tile_number<QT>(A.qsl, A.T, i) <= it; });
+  const int64_t a = A.qsl[lo], b = A.qsl[lo + 1];
+  const int n = A.P.N[lo];                             // asked for along with them
   t.row = lo;
-  t.t0 = min(A.qsl[lo], A.T);
-  t.c = (int)(min(A.qsl[lo + 1], A.T) - t.t0);
+  t.t0 = uniform64(min(a, A.T));
+  t.c = (int)(uniform64(min(b, A.T)) - t.t0);
+  t.n = __builtin_amdgcn_readfirstlane(n);
   t.q0 = (int)min((it - (lo + t.t0 / QT)) * QT, (int64_t)0x7FFFFFFF);
   t.nq = min(QT, t.c - t.q0);
   return t.nq > 0;
@@ -167,7 +170,7 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
   const int h = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
   const char* lutc = reinterpret_cast<const char*>(&L.lut[0][0]);
-  const int pbase = __builtin_amdgcn_readfirstlane(A.P.N[t.row] - t.c + t.q0);   // position of the tile's first query
+  const int pbase = t.n - t.c + t.q0;                 // position of the tile's first query
   int pcol[CT];
   b8 bq[CT][4];
 #pragma unroll
@@ -435,6 +438,7 @@ __global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
     t.row = r;
     t.t0 = uniform64(min(A.qsl[r], A.T));
     t.c = (int)(uniform64(min(A.qsl[r + 1], A.T)) - t.t0);
+    t.n = __builtin_amdgcn_readfirstlane(A.P.N[r]);
     t.q0 = (int)(tile * QT);
     t.nq = min(QT, t.c - t.q0);
     chunk_span<CT>(L, SA, SB, A, t, j0, j1, first ? (int64_t)blockIdx.x : A.G + tile_number<QT>(A.qsl, A.T, r) + tile);
@@ -462,13 +466,15 @@ struct alignas(16) ChunkXLds {
 };
 __device__ const uint4 chunk_zeros[16] = {};           // a row for tokens without a key: a zero weight needs a finite value
 
-// 16 bytes per lane from p to LDS bytes 16 lane .. of dst (the same for all lanes). The compiler does not see the load: whoever
-// reads dst waits for it by the memory counter (vm_wait), which retires loads in order; its own waits only come out
-// longer. As a builtin, every read of LDS waited for every such load, whichever array it fills.
-__device__ __forceinline__ void load_lds(const uint16_t* p, uint16_t* dst) {
-  typedef __attribute__((address_space(3))) uint16_t lds_u16;
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-               ::"v"(p), "s"(__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_u16*)dst)) : "memory", "m0");
+// 16 bytes per lane from p to LDS address dst + 16 lane (dst the same for all lanes). The compiler does not see the load:
+// whoever reads it waits by the memory counter (vm_wait), which retires loads in order; the compiler's own waits only come
+// out longer. As a builtin, every read of LDS waited for every such load, whichever array it fills.
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
+__device__ __forceinline__ uint32_t lds_addr(const uint16_t* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_u16*)p);
+}
+__device__ __forceinline__ void load_lds(const uint16_t* p, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(dst) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void vm_wait() {            // all but the N youngest loads are done
@@ -491,7 +497,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   const int h = blockIdx.x & 3;
   Tile t;
   if (!find_tile<QT>(A, it, t)) return;
-  const int N = __builtin_amdgcn_readfirstlane(A.P.N[t.row]), win = (int)A.P.win;
+  const int N = t.n, win = (int)A.P.win;
   const int pbase = N - t.c + t.q0, plast = pbase + t.nq - 1;
   const bool wide = CT > 1 && t.nq > 4;                // a tile of up to 4 queries leaves the second column tile out
   // key list: sinks [0, cnt), exact positions lo_row .. + cnt2, then lo_tile ..
@@ -512,8 +518,13 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   const bool rot = A.cos_t != nullptr;
   const int ebs = (int)A.P.ebs;
   const double iebs = 1.0 / (double)ebs;
+  const int64_t hoff = h * A.P.e_hs;
+  const int ets = (int)A.P.e_ts;
   const uint16_t* const zeros = reinterpret_cast<const uint16_t*>(chunk_zeros);
-  auto posof = [&](int i) { return i < cnt ? i : i < cnt + cnt2 ? lo_row + i - cnt : rest + i; };
+  auto posof = [&](int i) {
+    const int x = i < cnt + cnt2 ? lo_row - cnt : rest;
+    return i + (i < cnt ? 0 : x);
+  };
   // Lane l (and l ^ 32) looks after token l % 32 of a chunk. page(): its page's offset, asked for two chunks ahead, before the
   // rows of the chunk between: loads retire in order. locate(): its K and V row of head h.
   auto split = [&](int pos, int& pg, int& in) {        // pos = pg ebs + in
@@ -545,7 +556,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
       } else {
         int pg, in;
         split(pos, pg, in);
-        ko = base + h * A.P.e_hs + in * A.P.e_ts;
+        ko = base + hoff + (int64_t)in * ets;
         vo = ko + A.P.e_v;
         ok = base >= 0 && pg < A.P.eoff_stride && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
       }
@@ -555,6 +566,7 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
     r.ok = (uint32_t)__ballot(ok);
     return r;
   };
+  const uint32_t kl = lds_addr(Ks.r[w]), vl = lds_addr(Vs.r[w]);
   const int r4 = lane >> 4, pc = lane & 15;            // an instruction fills 4 rows: row r4, piece pc
   auto row_at = [&](const uint16_t* p, int t) {        // token t's pointer
     const uint64_t x = (uint64_t)p;
@@ -566,14 +578,14 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) src[i] = row_at(p, 4 * i + r4) + 8 * (pc ^ ((4 * i + r4) & 15));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load_lds(src[i], &Ks.r[w][512 * i]);
+    for (int i = 0; i < 8; ++i) load_lds(src[i], kl + 1024 * i);
   };
   auto load_v = [&](const uint16_t* p) {               // at p ^ 2 (t % 8): pairs of pieces stay together
     const uint16_t* src[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) src[i] = row_at(p, 4 * i + r4) + 8 * (pc ^ (2 * ((4 * i + r4) & 7)));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load_lds(src[i], &Vs.r[w][512 * i]);
+    for (int i = 0; i < 8; ++i) load_lds(src[i], vl + 1024 * i);
   };
   struct Rope { u4v c[2], s[2]; };                     // cos / sin of channels 8 g .. + 7 at token 16 u + n
   auto load_rope = [&](int c0, Rope& r) {
@@ -658,29 +670,36 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
         load_rope(c0 + STEP, rp);
         load_k(nx.k);
       }
-      const uint32_t tb = at.ok >> (4 * g);               // bit 16 u + i: token 16 u + 4 g + i
-      int kp[2][4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) kp[u][i] = ((tb >> (16 * u + i)) & 1u) ? posof(c0 + 16 * u + 4 * g + i) : 0x7FFFFFFF;
-      u4v bh[CT], bl[CT];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        if (ct > 0 && !wide) continue;
-        float xs[2][4], cm = -INFINITY;
-        const int wlo = win > 0 ? pcol[ct] - win : -1;
+      // a chunk whose keys are all there and seen by every query of the tile needs no mask
+      const int p0 = rest + c0;                        // position of the chunk's first key, behind the sinks
+      const bool plain = c0 >= cnt + cnt2;
+      const bool all = plain & (at.ok == 0xFFFFFFFFu) & (p0 + 31 <= pbase) & ((win == 0) | (p0 > plast - win));
+      if (!all) {
+        const uint32_t tb = at.ok >> (4 * g);          // bit 16 u + i: token 16 u + 4 g + i
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool keep = kp[u][i] <= pcol[ct] && (kp[u][i] > wlo || kp[u][i] < A.nsink);
-            xs[u][i] = keep ? sc[u][ct][i] * A.scale : -INFINITY;
-            cm = fmaxf(cm, xs[u][i]);
+            const int e = 16 * u + 4 * g + i;
+            int kp = p0 + e;
+            if (!plain) kp = posof(c0 + e);
+            kp = (tb >> (16 * u + i)) & 1u ? kp : 0x7FFFFFFF;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const int wlo = win > 0 ? pcol[ct] - win : -1;
+              const bool keep = (kp <= pcol[ct]) & ((kp > wlo) | (kp < A.nsink));
+              sc[u][ct][i] = keep ? sc[u][ct][i] : -INFINITY;
+            }
           }
-        cm = max4rows(cm);
-        if (__any(cm > m[ct])) {
-          const float mn = fmaxf(m[ct], cm), al = __builtin_amdgcn_exp2f(m[ct] - mn);
+      }
+      u4v bh[CT], bl[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        if (ct > 0 && !wide) continue;
+        const f4 s0 = sc[0][ct], s1 = sc[1][ct];
+        const float cm = maxn(maxn(maxn(s0[0], s0[1]), maxn(s0[2], s0[3])), maxn(maxn(s1[0], s1[1]), maxn(s1[2], s1[3])));
+        if (__any(cm * A.scale > m[ct])) {             // a lane's own scores; the column's maximum only where it matters
+          const float mn = fmaxf(m[ct], max4rows(cm + 0.f) * A.scale), al = __builtin_amdgcn_exp2f(m[ct] - mn);
           m[ct] = mn;
           lsum[ct] *= al;
 #pragma unroll
@@ -689,7 +708,8 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int u = k >> 1, i = 2 * (k & 1);
-          const float pa = __builtin_amdgcn_exp2f(xs[u][i] - m[ct]), pb = __builtin_amdgcn_exp2f(xs[u][i + 1] - m[ct]);
+          const float pa = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][i], A.scale, -m[ct]));
+          const float pb = __builtin_amdgcn_exp2f(fmaf(sc[u][ct][i + 1], A.scale, -m[ct]));
           lsum[ct] += pa + pb;
           bh[ct][k] = bfpk(pa, pb);
           bl[ct][k] = bfpk(pa - __uint_as_float(bh[ct][k] << 16), pb - __uint_as_float(bh[ct][k] & 0xFFFF0000u));
@@ -928,7 +948,9 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
   KV800_REQUIRE(q && qsl && out && P->epool && P->eoff && P->N, "decode_chunk: null pointer");
   KV800_REQUIRE(P->ebs > 0 && P->eoff_stride > 0 && P->win >= 0 && P->win < (1LL << 31) && P->nqmax >= 0,
                 "decode_chunk: bad page geometry, window or nqmax");
-  KV800_REQUIRE(P->e_hs % 8 == 0 && P->e_ts % 8 == 0 && P->e_v % 8 == 0, "decode_chunk: strides must be multiples of 8 elements");
+  KV800_REQUIRE(P->e_hs % 8 == 0 && P->e_ts % 8 == 0 && P->e_v % 8 == 0 && P->e_ts < (1LL << 31) &&
+                    P->e_ts > -(1LL << 31),
+                "decode_chunk: strides must be multiples of 8 elements, the token stride below 2^31");
   KV800_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)P->epool) % 16 == 0, "decode_chunk: q, out and epool must be 16-byte aligned");
   KV800_REQUIRE((cos_t == nullptr) == (sin_t == nullptr), "decode_chunk: cos and sin tables go together");
   KV800_REQUIRE(!cos_t || ((((uintptr_t)cos_t | (uintptr_t)sin_t) % 16) == 0 && rope_rows > 0),
