@@ -42,7 +42,7 @@ struct ChunkArgs {
   const uint32_t* cs2;
   int64_t rope_rows, qpool_bytes, epool_elems, sink_elems;
   int64_t G, I;                    // workgroups of the quantized list; tile numbers
-  int64_t* pre;                    // R + 1: the quantized list's entries before each row; then entries per workgroup
+  int32_t* pre;                    // R + 1: the quantized list's entries before each row; then entries per workgroup
   float *mo, *lo, *ao;             // partial slots: [slot][4 heads][16 CT columns] and, for ao, [128]
   uint16_t* out;
   float scale;                     // log2(e) / sqrt(128)
@@ -98,11 +98,12 @@ struct alignas(16) ChunkStage {
   uint8_t kc[QCH * 128], cs[QCH * 128], vb[QCH * 64];
 };
 struct QLutWords { uint32_t la, lb, sa, sb; };   // klo / ksc bytes of the table that the lane builds
+struct ListRow { int t0, c, n, nu; };                  // first token, queries, length, entries per tile
 struct alignas(16) ChunkQLds {
   uint32_t lut[4][1024];       // each wave's code tables of the sub-block it is in
   float vs[4][64], vl[4][64];  // decoded vsc / vlo of 64 tokens
-  int64_t ws[4];
-  int64_t row, pre;
+  int ws[4], row, pre;
+  ListRow at;
 };
 
 // 16 tables of 4 groups: block (kind, d, e) of 256 bytes holds the tables of channels 8 g + 4 d + e, g = 0..3, entry (ca, cb)
@@ -149,23 +150,17 @@ __device__ __forceinline__ uint32_t chunk_scales(rsrc_t rs, int t0, int h, int l
          ((uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rs, o, VSC_O + 2 * t0, 0) << 8);
 }
 
-// The list of (tile, sub-block) pairs, tile by tile: row r has tiles x sub-blocks of them.
+// The list of (tile, 64 tokens) pairs, tile by tile: row r has tiles x sub-blocks x 4 of them.
 // Sub-blocks past the host's bound, the offset table or the rope table are not read.
 __device__ __forceinline__ int row_nq(const ChunkArgs& A, int64_t r) { return min(max(A.P.NQ[r], 0), 1 << 22); }
 __device__ __forceinline__ int row_blocks(const ChunkArgs& A, int64_t r) {
   return (int)min(min((int64_t)row_nq(A, r), A.P.nqmax), min(A.P.boff_stride, A.rope_rows / BLK));
 }
-template <int QT>
-__device__ __forceinline__ int64_t row_pairs(const ChunkArgs& A, int64_t r) {
-  const int64_t c = min(A.qsl[r + 1], A.T) - min(A.qsl[r], A.T);
-  return (max(c, (int64_t)0) + QT - 1) / QT * row_blocks(A, r);
-}
-
-// Attention of one tile's columns of KV head h (the wave's) over sub-blocks [j0, j1) of its row, into partial slot `slot`.
+// Attention of one tile's columns of KV head h (the wave's) over tokens [64 u0, 64 u1) of its row, into partial slot `slot`.
 // As in decode_quant_kernel, with the wave's one head: K pairs by table lookup, RoPE by v_dot2_f32_bf16, Q K^T on bf16 MFMA
 // with exact products; fp32 online softmax; P V on fp16 MFMA over the bit planes, weights fp16(p vsc): 11 bits, an eighth of the output's own rounding.
 template <int CT>
-__device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkStage& SB, const ChunkArgs& A, const Tile& t, int j0, int j1, int64_t slot) {
+__device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkStage& SB, const ChunkArgs& A, const Tile& t, int u0, int u1, int64_t slot) {
   constexpr int NC = 16 * CT;
   const int h = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
@@ -324,7 +319,7 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
     asm volatile("" ::: "memory");
   };
 
-  // the span's 4 (j1 - j0) pairs of 32-token stages, one after the other; loads one stage ahead, tables and scales one pair
+  // the span's u1 - u0 pairs of 32-token stages, one after the other; loads one stage ahead, tables and scales one pair
   const int64_t* brow = A.P.boff + t.row * A.P.boff_stride;
   auto sanitize = [&](int64_t x, int jb) -> int64_t {
     const int64_t raw = uniform64(x);
@@ -332,14 +327,14 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
   };
   const rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(A.cs2), (short)0,
                                                       (int)min(A.rope_rows * 128, (int64_t)INT32_MAX), RSRC_WORD3);
-  const int np = 4 * (j1 - j0);
-  int jb = j0, pin = 0;
-  int64_t base = sanitize(brow[jb], jb), nraw = brow[min(jb + 1, j1 - 1)];
+  const int np = u1 - u0, jl = (u1 - 1) >> 2;          // pairs; the last sub-block
+  int jb = u0 >> 2, pin = u0 & 3;
+  int64_t base = sanitize(brow[jb], jb), nraw = brow[min(jb + 1, jl)];
   rsrc_t rs = sub_rsrc(A.P.qpool + (base < 0 ? 0 : base));
   int cpos = base < 0 ? 0 : jb * BLK;
-  stage_load(SA, rs, rc, cpos, 0, h, lane);
+  stage_load(SA, rs, rc, cpos, 64 * pin, h, lane);
   lut_build(L.lut[h], lane, lut_words(rs, h, lane));
-  stage_scales(chunk_scales(rs, 0, h, lane));
+  stage_scales(chunk_scales(rs, 64 * pin, h, lane));
   __syncthreads();
   for (int p = 0; p < np; ++p) {
     const bool more = p + 1 < np, cross = more && pin == 3;
@@ -352,7 +347,7 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
       nbase = sanitize(nraw, njb);
       nrs = sub_rsrc(A.P.qpool + (nbase < 0 ? 0 : nbase));
       ncpos = nbase < 0 ? 0 : njb * BLK;
-      nraw = brow[min(njb + 1, j1 - 1)];
+      nraw = brow[min(njb + 1, jl)];
     }
     const QLutWords nlw = lut_words(nrs, h, lane);
     const uint32_t nsc = chunk_scales(nrs, 64 * npin, h, lane);
@@ -387,63 +382,92 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
 // Workgroup w takes entries [w C, (w + 1) C) of the list, C = ceil(total / G). The part of a tile that it begins with goes
 // to slot w; a tile that starts inside its range goes to slot G + the tile's number (nobody else enters that tile from an
 // earlier entry).
+template <int QT>
+__device__ __forceinline__ ListRow list_row(const ChunkArgs& A, int64_t r) {
+  const int64_t a = A.qsl[r], b = A.qsl[r + 1];
+  const int n = A.P.N[r], nb = row_blocks(A, r);
+  ListRow x;
+  x.t0 = (int)min(a, A.T);
+  x.c = max((int)min(b, A.T) - x.t0, 0);
+  x.n = n;
+  x.nu = 4 * nb;
+  return x;
+}
+template <int QT>
+__device__ __forceinline__ int list_size(const ListRow& x) { return (x.c + QT - 1) / QT * x.nu; }
+
 template <int CT>
 __global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
   constexpr int QT = 4 * CT;
   __shared__ ChunkQLds L;
   __shared__ ChunkStage SA, SB;   // two objects: a read of one is not held for the other's loads
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-  // every workgroup sums the rows' entries itself: thread i takes the rows [i k, i k + k)
-  const int64_t k = (A.R + 255) / 256, ra = min((int64_t)tid * k, A.R), rb = min(ra + k, A.R);
-  int64_t mine = 0;
-  for (int64_t r = ra; r < rb; ++r) mine += row_pairs<QT>(A, r);
-  int64_t inc = mine;
+  // every workgroup sums the rows' entries itself: thread i takes the rows [i k, i k + k). The list has less than 2^31
+  // entries (the host's check).
+  const int R = (int)A.R, k = (R + 255) / 256, ra = min(tid * k, R), rb = min(ra + k, R);
+  ListRow first = {0, 0, 0, 0};
+  int mine = 0;
+  if (ra < rb) {
+    first = list_row<QT>(A, ra);
+    mine = list_size<QT>(first);
+  }
+  for (int r = ra + 1; r < rb; ++r) mine += list_size<QT>(list_row<QT>(A, r));
+  int inc = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t x = __shfl_up(inc, o, 64);
+    const int x = __shfl_up(inc, o, 64);
     if (lane >= o) inc += x;
   }
   if (lane == 63) L.ws[w] = inc;
   __syncthreads();
-  int64_t pre = inc - mine;
+  int pre = inc - mine;
   for (int i = 0; i < w; ++i) pre += L.ws[i];
-  const int64_t total = uniform64(L.ws[0] + L.ws[1] + L.ws[2] + L.ws[3]), C = (total + A.G - 1) / A.G;
+  const int total = __builtin_amdgcn_readfirstlane(L.ws[0] + L.ws[1] + L.ws[2] + L.ws[3]), G = (int)A.G, C = (total + G - 1) / G;
   if (blockIdx.x == 0) {                               // for the merge
-    int64_t x = pre;
-    for (int64_t r = ra; r < rb; ++r) { A.pre[r] = x; x += row_pairs<QT>(A, r); }
-    if (tid == 0) A.pre[A.R] = C;
-  }
-  int64_t v = (int64_t)blockIdx.x * C;
-  const int64_t v1 = min(v + C, total);
-  if (v >= v1) return;                                 // uniform
-  if (v >= pre && v < pre + mine) {                    // one thread
-    int64_t x = pre;
-    for (int64_t r = ra; r < rb; ++r) {
-      const int64_t y = row_pairs<QT>(A, r);
-      if (v < x + y) { L.row = r; L.pre = x; break; }
-      x += y;
+    int x = pre;
+    for (int r = ra; r < rb; ++r) {
+      A.pre[r] = x;
+      if (r + 1 < rb) x += list_size<QT>(list_row<QT>(A, r));
     }
+    if (tid == 0) A.pre[R] = C;
+  }
+  int v = (int)blockIdx.x * C;
+  const int v1 = min(v + C, total);
+  if (v >= v1) return;                                 // uniform
+  if (v >= pre && v < pre + mine) {                    // one thread: the row of the workgroup's first entry
+    ListRow y = first;
+    int x = pre, r = ra;
+    while (v >= x + list_size<QT>(y)) {
+      x += list_size<QT>(y);
+      y = list_row<QT>(A, ++r);
+    }
+    L.row = r;
+    L.pre = x;
+    L.at = y;
   }
   __syncthreads();
   // the walk over the list in scalars: the sub-blocks' buffer resources, offsets and loop bounds stay in SGPRs
-  int64_t r = uniform64(L.row), x = uniform64(L.pre);
-  bool first = true;
-  while (v < v1) {
-    const int64_t y = uniform64(row_pairs<QT>(A, r));
-    if (v >= x + y) { x += y; ++r; continue; }
-    const int nb = __builtin_amdgcn_readfirstlane(row_blocks(A, r));
-    const int64_t tile = (v - x) / nb;
-    const int j0 = (int)((v - x) - tile * nb), j1 = (int)min((int64_t)nb, j0 + (v1 - v));
-    Tile t;
-    t.row = r;
-    t.t0 = uniform64(min(A.qsl[r], A.T));
-    t.c = (int)(uniform64(min(A.qsl[r + 1], A.T)) - t.t0);
-    t.n = __builtin_amdgcn_readfirstlane(A.P.N[r]);
-    t.q0 = (int)(tile * QT);
-    t.nq = min(QT, t.c - t.q0);
-    chunk_span<CT>(L, SA, SB, A, t, j0, j1, first ? (int64_t)blockIdx.x : A.G + tile_number<QT>(A.qsl, A.T, r) + tile);
-    first = false;
-    v += j1 - j0;
+  auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  int r = scalar(L.row), x = scalar(L.pre);
+  ListRow y = L.at;
+  for (bool head = true;; head = false) {
+    const int c = scalar(y.c), nu = scalar(y.nu), sz = (c + QT - 1) / QT * nu;
+    while (v < v1 && v < x + sz) {
+      const int tile = (int)((unsigned)(v - x) / (unsigned)nu), u0 = v - x - tile * nu, u1 = min(nu, u0 + (v1 - v));
+      Tile t;
+      t.row = r;
+      t.t0 = scalar(y.t0);
+      t.n = scalar(y.n);
+      t.c = c;
+      t.q0 = tile * QT;
+      t.nq = min(QT, c - t.q0);
+      chunk_span<CT>(L, SA, SB, A, t, u0, u1, head ? (int64_t)blockIdx.x : A.G + r + (unsigned)t.t0 / QT + tile);
+      head = false;
+      v += u1 - u0;
+    }
+    if (v >= v1) return;
+    x += sz;
+    y = list_row<QT>(A, ++r);
   }
 }
 
@@ -798,32 +822,36 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
 }
 
 // ---------------------------------------------------------------- merge
-// One workgroup per (token, KV head), one wave per query head. Lanes take the partials' m and l side by side (64 at a time),
-// then the wave adds up the partials' accumulators, lane = dims 2 lane, 2 lane + 1, eight loads in flight.
-template <int CT>
+// WPC waves per (token, query head), the four heads of a KV head (WPC = 1) or one head (4) per workgroup: 4 where there are
+// few tokens, whose partials are many. Lanes take the partials' m and l side by side (64 at a time), then the wave adds up
+// the partials' accumulators, lane = dims 2 lane, 2 lane + 1, eight loads in flight.
+template <int CT, int WPC>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
   constexpr int QT = 4 * CT, NC = 16 * CT;
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = blockIdx.x & 3, dd = 2 * lane;
-  const int64_t tok = blockIdx.x >> 2;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(A.out + (tok * 16 + 4 * h + w) * 128 + dd);
+  __shared__ float jm[4], jl[4], jx[4][128];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, dd = 2 * lane;
+  const int64_t tok = blockIdx.x / (4 * WPC);
+  const int q = WPC == 1 ? 4 * (int)(blockIdx.x & 3) + w : (int)(blockIdx.x & 15), h = q >> 2;
+  const int part = WPC == 1 ? 0 : w;                   // this wave's share of the partials
+  uint32_t* dst = reinterpret_cast<uint32_t*>(A.out + (tok * 16 + q) * 128 + dd);
   if (tok >= min(A.qsl[A.R], A.T)) {                   // padding
-    *dst = 0u;
+    if (part == 0) *dst = 0u;
     return;
   }
   const int64_t row = row_of(A.qsl, A.R, tok), i = tok - A.qsl[row];
   const int64_t it = tile_number<QT>(A.qsl, A.T, row) + i / QT;
-  const int c = 4 * (int)(i % QT) + w;
-  const int64_t C = A.pre[A.R], nb = row_blocks(A, row);
-  const int64_t s = A.pre[row] + i / QT * nb, e = s + nb;        // the tile's entries of the list
-  const int64_t w0 = nb ? s / C : 0;
-  const int n = nb ? (int)((e - 1) / C - w0) + 1 : 0;            // partials of the quantized list
-  const bool mid = nb && w0 * C < s;                             // the first of them starts inside its workgroup's range
+  const int c = 4 * (int)(i % QT) + (q & 3);
+  const unsigned C = A.pre[A.R], nu = 4 * row_blocks(A, row);
+  const unsigned s = A.pre[row] + (unsigned)i / QT * nu, e = s + nu;   // the tile's entries of the list
+  const unsigned w0 = nu ? s / C : 0;
+  const int n = nu ? (int)((e - 1) / C - w0) + 1 : 0;            // partials of the quantized list
+  const bool mid = nu && w0 * C < s;                             // the first of them starts inside its workgroup's range
   auto slot = [&](int k) { return ((k == 0 && mid ? A.G + it : w0 + k) * 4 + h) * NC + c; };
   const int64_t cx = ((A.G + A.I + it) * 4 + h) * NC + c;
   const float mx = A.mo[cx], lx = A.lo[cx];
   const float2 ax = *reinterpret_cast<const float2*>(A.ao + cx * 128 + dd);
   float M = mx, l = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int k0 = 0; k0 < n; k0 += 64) {
+  for (int k0 = 64 * part; k0 < n; k0 += 64 * WPC) {
     const bool in = k0 + lane < n;
     const int64_t p = slot(in ? k0 + lane : 0);
     const float mk = in ? A.mo[p] : NEG_BIG, lk = in ? A.lo[p] : 0.f;
@@ -851,6 +879,22 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  if constexpr (WPC > 1) {                             // the waves' shares, in wave order
+    if (lane == 0) { jm[w] = M; jl[w] = l; }
+    *reinterpret_cast<float2*>(&jx[w][dd]) = make_float2(x0, x1);
+    __syncthreads();
+    if (w > 0) return;
+    float m2 = M;
+    for (int k = 1; k < WPC; ++k) m2 = fmaxf(m2, jm[k]);
+    l = x0 = x1 = 0.f;
+    for (int k = 0; k < WPC; ++k) {
+      const float f = __builtin_amdgcn_exp2f(jm[k] - m2);
+      l += f * jl[k];
+      x0 += f * jx[k][dd];
+      x1 += f * jx[k][dd + 1];
+    }
+    M = m2;
+  }
   const float fx = __builtin_amdgcn_exp2f(mx - M);
   l += fx * lx;
   {                                                    // H x: bit 0 of the dim in the lane, bits 1..6 across the lanes
@@ -891,14 +935,14 @@ int64_t chunk_cus() {
   return cache[dev];
 }
 
-struct ChunkPlan { int ct; int64_t G, I, cols, pre; };   // cols: partial columns; pre: int64 entries
+struct ChunkPlan { int ct; int64_t G, I, cols, pre; };   // cols: partial columns; pre: entries
 ChunkPlan chunk_plan(int64_t R, int64_t T, int64_t nqmax) {
   ChunkPlan p;
   p.ct = chunk_ct(R, T, nqmax > 0);
   p.I = R + T / (4 * p.ct);
   p.G = nqmax > 0 ? chunk_cus() * (p.ct == 1 ? 3 : 2) : 0;   // what is resident at 150 / 207 VGPRs
   p.cols = nqmax > 0 ? (p.G + 2 * p.I) * 64 * p.ct : 0;
-  p.pre = nqmax > 0 ? (R + 2) / 2 * 2 : 0;
+  p.pre = nqmax > 0 ? (R + 4) / 4 * 4 : 0;
   return p;
 }
 
@@ -922,7 +966,10 @@ int chunk_launch(const ChunkArgs& A, bool quant, hipStream_t s) {
   const int64_t cu = chunk_cus(), pairs = 4 * max(A.R, A.T / (4 * CT));
   rc = pairs <= 2 * cu ? chunk_exact<CT, 4>(A, quant, s) : pairs <= 4 * cu ? chunk_exact<CT, 2>(A, quant, s) : chunk_exact<CT, 1>(A, quant, s);
   if (rc != KV800_OK || !quant) return rc;
-  hipLaunchKernelGGL(chunk_merge_kernel<CT>, dim3((unsigned)(4 * A.T)), dim3(256), 0, s, A);
+  if (16 * A.T <= 4 * cu)
+    hipLaunchKernelGGL((chunk_merge_kernel<CT, 4>), dim3((unsigned)(16 * A.T)), dim3(256), 0, s, A);
+  else
+    hipLaunchKernelGGL((chunk_merge_kernel<CT, 1>), dim3((unsigned)(4 * A.T)), dim3(256), 0, s, A);
   return check_launch("chunk_merge");
 }
 
@@ -936,7 +983,7 @@ extern "C" {
 int64_t kv800_hip_decode_chunk_workspace(int64_t R, int64_t T, int64_t nqmax) {
   if (R <= 0 || T <= 0 || nqmax <= 0) return 0;
   const ChunkPlan p = chunk_plan(R, T, nqmax);
-  return p.pre * 8 + p.cols * 130 * 4;
+  return p.pre * 4 + p.cols * 130 * 4;
 }
 
 int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int64_t* qsl, int64_t R, int64_t T,
@@ -965,6 +1012,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
                 "decode_chunk: sinks need sv, skoff, svoff and 16-byte aligned buffers");
   const ChunkPlan p = chunk_plan(R, T, quant ? P->nqmax : 0);
   KV800_REQUIRE(p.I <= (1LL << 28) && T <= (1LL << 28) && P->ebs < (1LL << 30), "decode_chunk: too many rows and tokens");
+  KV800_REQUIRE(!quant || p.I <= 0x7FFFFFFFLL / 4 / P->nqmax, "decode_chunk: too many rows and sub-blocks");
   KV800_REQUIRE(!quant || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= kv800_hip_decode_chunk_workspace(R, T, P->nqmax)),
                 "decode_chunk: the workspace is too small or not 16-byte aligned");
   ChunkArgs A;
@@ -973,7 +1021,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
   A.cos_t = cos_t; A.sin_t = sin_t; A.cs2 = cs2;
   A.rope_rows = rope_rows; A.qpool_bytes = qpool_bytes; A.epool_elems = epool_elems; A.sink_elems = sink_elems;
   A.G = p.G; A.I = p.I;
-  A.pre = reinterpret_cast<int64_t*>(ws);
+  A.pre = reinterpret_cast<int32_t*>(ws);
   A.ao = quant ? reinterpret_cast<float*>(A.pre + p.pre) : nullptr;
   A.mo = quant ? A.ao + p.cols * 128 : nullptr;
   A.lo = quant ? A.mo + p.cols : nullptr;
