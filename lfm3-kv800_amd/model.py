@@ -25,6 +25,7 @@ import torch.nn.functional as F
 
 from . import kv800, kv800_hip
 from . import model_ops as mo
+from . import spec_ops as so
 from . import vllm_cache as vc
 
 CONV, FULL, SLIDE = "conv", "full", "slide"
@@ -123,8 +124,13 @@ class Lfm3Decoder:
             if L["type"] == CONV:
                 L["state"].copy_(torch.randn(L["state"].shape, generator=g, device=self.dev) * 0.1)
 
-    def _conv(self, L, n):
-        return F.linear(mo.conv_step(F.linear(n, L["in_proj"]), L["conv"], L["state"]), L["out_proj"])
+    def _conv(self, L, n, qsl=None):
+        bcx = F.linear(n, L["in_proj"])
+        if qsl is None:
+            y = mo.conv_step(bcx, L["conv"], L["state"])
+        else:
+            y, L["taps"] = so.conv_chunk(bcx, L["conv"], L["state"], qsl)
+        return F.linear(y, L["out_proj"])
 
     def _attention(self, l, L, n, pos):
         cfg = self.cfg
@@ -139,18 +145,34 @@ class Lfm3Decoder:
         """tokens (R,) int64, pos (R,) int64 the new tokens' positions (device); the attention object's begin_step
         has been called with the rows' lengths including this token. Returns (R, vocab) logits, fp32 (the bf16 LM-head
         output widened) or, with fp32=False, bf16."""
+        logits = self._layers(tokens, pos, None, self.fused_ffn)
+        return logits.float() if fp32 else logits
+
+    def chunk(self, tokens, meta):
+        """Logits (T, vocab) bf16 behind every token of a step whose rows bring any number of tokens: tokens (T,) int64, row
+        after row, meta the kv800_hip.ChunkMeta that the attention object's begin_chunk returned. The conv states stay where
+        they are until commit()."""
+        self.qsl = meta.qsl
+        return self._layers(tokens, meta.pos, meta.qsl, self.fused_ffn and glu_rows(tokens.shape[0]))
+
+    def commit(self, kept):
+        """Move the conv states on over the first kept[r] ((R,) int32) of each row's tokens of the last chunk()."""
+        for L in self.layers:
+            if L["type"] == CONV:
+                so.conv_commit(L["state"], L["taps"], self.qsl, kept)
+
+    def _layers(self, tokens, pos, qsl, fused_ffn):
         cfg = self.cfg
         x = self.embed[tokens]
         _, n = mo.add_rmsnorm(None, x, None, self.layers[0]["norm"], cfg.eps)
         for l, L in enumerate(self.layers):
-            h = self._conv(L, n) if L["type"] == CONV else self._attention(l, L, n, pos)
+            h = self._conv(L, n, qsl) if L["type"] == CONV else self._attention(l, L, n, pos)
             x, n = mo.add_rmsnorm(h, x, L["post_norm"], L["ffn_norm"], cfg.eps)
-            a = mo.linear(n, L["w13p"]) if self.fused_ffn else mo.silu_mul(F.linear(n, L["w13"]))
+            a = mo.linear(n, L["w13p"]) if fused_ffn else mo.silu_mul(F.linear(n, L["w13"]))
             h = F.linear(a, L["w2"])
             nxt = self.layers[l + 1]["norm"] if l + 1 < len(self.layers) else self.final_norm
             x, n = mo.add_rmsnorm(h, x, L["post_ffn_norm"], nxt, cfg.eps)
-        logits = F.linear(n, self.embed)
-        return logits.float() if fp32 else logits
+        return F.linear(n, self.embed)
 
     def greedy(self, tokens, pos):
         """One step's greedy tokens (R,) int64: the first index of each row's largest logit (one HIP launch on the
@@ -174,7 +196,7 @@ class PagedAttention800:
         self.dev, self.ebs = device, ebs
         self.lens = torch.tensor([int(x) for x in lens0], dtype=torch.int64)
         R = self.R = len(lens0)
-        nmax = int(self.lens.max()) + steps + 1
+        nmax = self.nmax = int(self.lens.max()) + steps + 1
         self.cos, self.sin = kernel_tables(nmax + 64, device)
         rng = torch.Generator().manual_seed(seed)
         lp = nmax // ebs + 1                                                   # logical exact pages per row
@@ -259,6 +281,16 @@ class PagedAttention800:
         vc.launch_flushes(full, {l.l: me[self.group_of[l.l]] for l in full}, mq)
         return mq.positions
 
+    def begin_chunk(self, lens, qlens, tokens, most, bound):
+        """Metadata of a step whose rows bring qlens (R,) int32 <= most new tokens each, to lengths lens (R,) int64, both on
+        the device; tokens: room for them; bound (R,): the host's bound of lens. Returns the step's kv800_hip.ChunkMeta."""
+        if int(bound.max()) > self.nmax:
+            raise ValueError(f"the caches hold {self.nmax} positions per row, the step may reach {int(bound.max())}")
+        me = {g: vc.chunk_step_meta(self.bt[g], lens, qlens, self.ebs, tokens, most, bound) for g in self.bt}
+        mq = vc.chunk_step_meta(self.qbt, lens, qlens, vc.QBLOCK, tokens, most, bound)
+        self.metas = (me, mq)
+        return mq.chunk
+
     def attend(self, l, q, k_pre, k_post, v):
         me, mq = self.metas
         layer = self.layers[l]
@@ -317,3 +349,38 @@ def decode_loop(model, attention, tokens, steps, graph=False):
         tokens = model.greedy(tokens, attention.begin_step())
         out.append(tokens)
     return torch.stack(out)
+
+
+def speculative_loop(model, attention, tokens, steps, draft, most, temperature=None, generator=None):
+    """Decode with drafted tokens: `steps` steps from `tokens` (R,) int64, each of which appends to every row its last token
+    and up to `most` drafts, keeps the drafts that the model confirms (spec_ops.verify_drafts) and takes one more token
+    behind them. draft(last (R,), lens (R,)) -> (drafts (R, most) int64, counts (R,) int32 of them in use, their
+    distributions (R, most, vocab) fp32 or None), all on the device; lens counts the positions in the caches. temperature
+    (R,) fp32, None: greedy. Lengths stay on the device, so a step does not wait for the one before; the attention must be a
+    PagedAttention800 with room for steps (most + 1) more positions, most < 128. Returns the rows' new tokens, a list of R
+    tensors, and the (steps, R) counts; attention.lens follows."""
+    dev, R = tokens.device, tokens.shape[0]
+    if not 0 <= most < 128:
+        raise ValueError("most must be in [0, 128)")
+    if temperature is None:
+        temperature = torch.zeros(R, dtype=torch.float32, device=dev)
+    lens = attention.lens.to(dev)
+    T, last, got = R * (most + 1), tokens, []
+    at = torch.arange(T, device=dev)
+    for s in range(steps):
+        drafts, counts, probs = draft(last, lens)
+        ql = (counts + 1).to(torch.int32)
+        meta = attention.begin_chunk(lens + ql, ql, T, most + 1, attention.lens + (s + 1) * (most + 1))
+        i = (at - meta.qsl[meta.row]).clamp(max=most)
+        tok = torch.cat((last[:, None], drafts), 1)[meta.row, i]
+        logits = model.chunk(tok, meta)
+        q = None if probs is None else probs[meta.row, i.clamp(max=most - 1)]
+        out, kept = so.verify_drafts(logits, tok, meta.qsl, temperature, torch.rand(T, device=dev, generator=generator),
+                                     torch.rand(R, device=dev, generator=generator), q)
+        model.commit(kept)
+        lens = lens + kept
+        last = out[meta.qsl[:-1] + kept - 1]
+        got.append((out, kept, meta.row))
+    attention.lens = lens.cpu()
+    rows = [torch.cat([out[(row == r) & (out >= 0)] for out, _, row in got]) if got else tokens[:0] for r in range(R)]
+    return rows, torch.stack([kept for _, kept, _ in got]) if got else torch.zeros(0, R, dtype=torch.int32, device=dev)

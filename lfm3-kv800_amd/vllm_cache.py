@@ -50,6 +50,8 @@ class StepMeta:
     num_decodes: int = None
     query_lens: torch.Tensor = None
     req_of_tok: torch.Tensor = None
+    chunk: object = None
+    most: int = 0
 
     @property
     def mixed(self):
@@ -114,8 +116,24 @@ def mixed_step_meta(block_table, seq_lens_cpu, query_lens_cpu, ebs, device, num_
                     query_lens=up(ql.to(torch.int32)), req_of_tok=up(req))
 
 
+def chunk_step_meta(block_table, seq_lens, query_lens, ebs, tokens, most, bound_cpu):
+    """StepMeta of a step whose rows bring any number of new tokens and whose lengths are known on the device alone (drafted
+    tokens to verify, of which the last step's kept ones set this step's lengths): seq_lens (R,) int64, the new tokens
+    included, and query_lens (R,) int32, block_table (R, blocks) int32, all on the device. tokens: room for the step's
+    tokens (the rest is padding); most, bound_cpu (R,): host bounds of query_lens and seq_lens. One launch
+    (kv800_hip.chunk_meta). Drafts may be taken back by a shorter length in the next step as long as most <= 128: what a
+    step flushes lies at least 128 tokens before its end, so among the kept ones."""
+    m = kv800_hip.chunk_meta(block_table, seq_lens, query_lens, ebs, tokens)
+    bound = torch.as_tensor(bound_cpu).to(torch.int64).cpu()
+    if bound.shape != seq_lens.shape or int(most) < 1:
+        raise ValueError("bound_cpu must be (R,) and most >= 1")
+    return StepMeta(block_table, m.slot, m.lens32, bound, m.pos, query_lens=query_lens, req_of_tok=m.row, chunk=m, most=int(most))
+
+
 def _max_flush(m):
     """Most sub-blocks any row of the step becomes eligible for (host values): nq(seq_len) - nq(seq_len - query_len)."""
+    if m.chunk is not None:
+        return -(-m.most // kv800.BLK)
     sl = m.seq_lens_cpu.to(torch.int64)
     ql = (m.query_start_loc_cpu[1:] - m.query_start_loc_cpu[:-1]) if m.mixed else torch.ones_like(sl)
     nq = lambda n: torch.clamp(n - kv800.LAG, min=0) // kv800.BLK
@@ -145,7 +163,10 @@ class KV800DecodeLayer:
         mx: this layer's exact-group metadata; mq: the quant group's (quantized layers, and the sink hosts of window
         layers); hosts: {layer: KV800DecodeLayer} holding the sink hosts' quant caches (window layers); cos_t / sin_t
         (P, 32) bf16 RoPE tables; max_new: most sub-blocks any row can become eligible for in a decode step (1).
-        A mixed step (mx.mixed) runs the decode rows and the extend rows of the batch (vllm_attn.py:244-402)."""
+        A mixed step (mx.mixed) runs the decode rows and the extend rows of the batch (vllm_attn.py:244-402), a chunk step
+        (chunk_step_meta) all rows as they are over the paged cache (kv800_hip.decode_chunk)."""
+        if mx.chunk is not None:
+            return self._forward_chunk(q, k, v, mx, mq, hosts, cos_t, sin_t)
         if mx.mixed:
             return self._forward_mixed(q, k, v, mx, mq, hosts, cos_t, sin_t)
         ev, ebs = self.ev, self.ebs
@@ -194,7 +215,7 @@ class KV800DecodeLayer:
         boff, NQ, NP, qbt64, aux, nqmax = _step_tables(mq)
         if self.win:
             skb, svb = self._sinks(hosts)
-            at = aux.index_select(0, mx.req_of_tok) if mx.mixed else aux
+            at = aux if mx.req_of_tok is None else aux.index_select(0, mx.req_of_tok)
             kv800_hip.write_exact(ev, mx.slot_mapping, k, v, pos=mx.positions, sk=skb, sv=svb, skoff=at, svoff=at)
             return
         kv800_hip.write_exact(ev, mx.slot_mapping, k, v)
@@ -245,6 +266,29 @@ class KV800DecodeLayer:
             out[t0:] = prefill_quant_rows(P, q[t0:T], k[t0:T], v[t0:T], eq, prev[nd:], cos_t, sin_t)
         return out
 
+    def _forward_chunk(self, q, k, v, mx, mq, hosts, cos_t, sin_t):
+        """A chunk step: write_step, then the attention of all new tokens over the cache: quantized layers over the
+        sub-blocks that a decode step of the row's first new token reads (nq(length before + 1)) and the exact rows from
+        there on, so that a row with one token is attended as in a decode step; window layers over sinks and window."""
+        ev = self.ev
+        R = mx.seq_lens.shape[0]
+        self.write_step(k, v, mx, mq, hosts)
+        boff, NQ, NP, qbt64, aux, nqmax = _step_tables(mq)
+        geo = dict(epool=ev, eoff=self._eoff(mx), ebs=self.ebs, e_hs=ev.stride(1), e_ts=ev.stride(2), e_v=128, N=mx.seq_lens)
+        if self.win:
+            skb, svb = self._sinks(hosts)
+            if self._zeros is None or self._zeros.shape[0] < R:
+                self._zeros = torch.zeros(max(R, 64), dtype=torch.int32, device=ev.device)
+            P = kv800.Paged(qpool=None, boff=None, sk=skb, sv=svb, skoff=aux, svoff=aux, NQ=self._zeros[:R], nqmax=0,
+                            win=kv800.WIN, **geo)
+        else:
+            if ("chunk",) not in mq.cache:
+                n = mq.seq_lens - mq.query_lens + 1
+                mq.cache[("chunk",)] = torch.clamp(n - kv800.LAG, min=0).div_(kv800.BLK, rounding_mode="floor")
+            P = kv800.Paged(qpool=self.qv, boff=boff, sk=None, sv=None, skoff=None, svoff=None, NQ=mq.cache[("chunk",)], nqmax=nqmax,
+                            win=0, **geo)
+        return kv800_hip.decode_chunk(P, q, mx.chunk.qsl, cos_t, sin_t)
+
     def _eoff(self, mx):
         """The exact group's page offsets for this cache's page stride (one launch per group and step)."""
         key = ("eoff", self.ev.stride(0))
@@ -290,7 +334,7 @@ class KV800SlideLayer:
     def forward(self, q, k, v, mx: StepMeta):
         """q (T, 16, 128) post-RoPE, k (T, 4, 128) POST-RoPE, v (T, 4, 128), bf16, one row per scheduled token;
         mx: the layer's sliding-group metadata. A mixed step's extend rows attend their last 255 positions and their
-        new rows (vllm_attn.py:351-402 with slide=True)."""
+        new rows (vllm_attn.py:351-402 with slide=True), a chunk step's rows the same, from the pages."""
         ev, ebs = self.ev, self.ebs
         R = mx.seq_lens.shape[0]
         key = ("eoff", ev.stride(0))
@@ -300,6 +344,10 @@ class KV800SlideLayer:
         self.write_step(k, v, mx)
         if self._zeros is None or self._zeros.shape[0] < R:
             self._zeros = torch.zeros(max(R, 64), dtype=torch.int32, device=ev.device)
+        if mx.chunk is not None:
+            P = kv800.Paged(qpool=None, boff=None, epool=ev, eoff=eoff, ebs=ebs, e_hs=ev.stride(1), e_ts=ev.stride(2), e_v=128,
+                            sk=None, sv=None, skoff=None, svoff=None, N=mx.seq_lens, NQ=self._zeros[:R], nqmax=0, win=kv800.WIN)
+            return kv800_hip.decode_chunk(P, q, mx.chunk.qsl, None, None)
         nd = mx.num_decodes if mx.mixed else R
         cos1, sin0 = self.identity_tables(int(mx.seq_lens_cpu.max()) + 1)
         out = torch.empty(q.shape[0], 16, 128, dtype=torch.bfloat16, device=q.device) if mx.mixed else None
@@ -328,7 +376,7 @@ def _step_tables(mq):
     counts each row's sub-blocks before its query_len new tokens (one for a decode step)."""
     if ("step",) not in mq.cache:
         nqmax = int(torch.clamp(mq.seq_lens_cpu.to(torch.int64) - kv800.LAG, min=0).max()) // kv800.BLK
-        nnew = mq.query_lens if mq.mixed else 1
+        nnew = 1 if mq.query_lens is None else mq.query_lens
         mq.cache[("step",)] = kv800_hip.step_tables(mq.block_table, QBLOCK, QPAGE, mq.seq_lens, nqmax, nnew=nnew,
                                                     aux_scale=QPAGE // 2, aux_add=AUX_BYTES // 2) + (nqmax,)
     return mq.cache[("step",)]
@@ -349,7 +397,7 @@ def launch_flushes(layers, metas, mq, max_new=1):
     group's StepMeta. Call once per step, before the step's first attention layer. A mixed step starts none (its
     extend rows flush sub-blocks made of this step's own tokens): each layer's forward flushes after its writes."""
     quant = [l for l in layers if not l.win]
-    if not quant or mq.mixed:
+    if not quant or mq.query_lens is not None:
         return
     dev = quant[0].ev.device
     main = torch.cuda.current_stream(dev)
