@@ -5,6 +5,8 @@
 //   verify_stats_kernel     per piece of a logits row: largest value, its index, sum of exponentials
 //   verify_residual_kernel  per piece of the logits row that ends a batch row: what p has over q
 //   verify_pick_kernel      per batch row: which drafts are kept, and the token behind them
+#include <type_traits>
+
 #include "kv800_common.h"
 #include "../../include/kv800_hip.h"
 #include "../../include/lfm3_spec.h"
@@ -75,17 +77,13 @@ conv_chunk_kernel(const uint16_t* __restrict__ bcx, int64_t stride, const uint16
 #pragma unroll
     for (int c = 0; c < 8; ++c) f[c] = kv800::bfround(b[c] * f[c]);
   };
-  float w[7][8];
+  uint32_t cwp[28];                                    // the 8 channels' 7 weights, two a register
   {
-    const uint4* s = reinterpret_cast<const uint4*>(cw + c0 * 7);                  // 8 channels x 7 taps
-    uint32_t x[28];
+    const uint4* s = reinterpret_cast<const uint4*>(cw + c0 * 7);
 #pragma unroll
-    for (int i = 0; i < 7; ++i) { const uint4 v = s[i]; x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w; }
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int k = 0; k < 7; ++k) w[k][c] = ((c * 7 + k) & 1) ? kv800::bf2f_hi(x[(c * 7 + k) / 2]) : kv800::bf2f_lo(x[(c * 7 + k) / 2]);
+    for (int i = 0; i < 7; ++i) { const uint4 v = s[i]; cwp[4 * i] = v.x; cwp[4 * i + 1] = v.y; cwp[4 * i + 2] = v.z; cwp[4 * i + 3] = v.w; }
   }
+  auto wt = [&](int k, int c) { const int e = c * 7 + k; return (e & 1) ? kv800::bf2f_hi(cwp[e / 2]) : kv800::bf2f_lo(cwp[e / 2]); };
   if (t0 < total) {
     const int64_t s0 = qsl[r];
     if (t0 - s0 < 6) from_state(r);
@@ -125,8 +123,8 @@ conv_chunk_kernel(const uint16_t* __restrict__ bcx, int64_t stride, const uint16
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
 #pragma unroll
-        for (int k = 0; k < 6; ++k) y[c] = fmaf(win[k][c], w[k][c], y[c]);
-        y[c] = fmaf(f[c], w[6][c], y[c]) * g[c];
+        for (int k = 0; k < 6; ++k) y[c] = fmaf(win[k][c], wt(k, c), y[c]);
+        y[c] = fmaf(f[c], wt(6, c), y[c]) * g[c];
       }
 #pragma unroll
       for (int k = 0; k < 5; ++k)
@@ -646,12 +644,21 @@ int lfm3_hip_conv_chunk(const uint16_t* bcx, int64_t stride, const uint16_t* con
   const int64_t ny = (H / 8 + 255) / 256;
   KV800_REQUIRE(T <= 0x7FFFFFFF && ny <= 65535, "conv_chunk: too large");
   const hipStream_t s = (hipStream_t)stream;
-  if (T * ny <= 4096)
-    hipLaunchKernelGGL(lfm3::conv_chunk_kernel<1>, dim3((unsigned)T, (unsigned)ny), dim3(256), 0, s, bcx, stride, conv_w, state,
-                       qsl, R, T, H, out, taps);
-  else
-    hipLaunchKernelGGL(lfm3::conv_chunk_kernel<16>, dim3((unsigned)((T + 15) / 16), (unsigned)ny), dim3(256), 0, s, bcx, stride,
+  // Tokens per workgroup, by the workgroups that one each would make: few, so that every CU has one and a token's taps are
+  // not formed again by its successors' workgroups more often than that costs; 16 where 8 make a round and a third.
+  // H = 2048, us with 1 / 2 / 4 / 8 / 16 / 32: T = 160: 4.2 5.2 6.3 8.5 13 23; 512: 6.7 5.0 5.6 8.1 13 23; 1,024: 14 9.2 8.7 8.3
+  // 14 23; 4,096: 45 29 23 17 20 31; 8,192: 78 52 41 36 31 34; 16,384: 148 104 82 69 75 71; 32,768: 288 198 155 141 143 151.
+  const int64_t n = T * ny;
+  const auto go = [&](auto tt) {
+    constexpr int TT = decltype(tt)::value;
+    hipLaunchKernelGGL(lfm3::conv_chunk_kernel<TT>, dim3((unsigned)((T + TT - 1) / TT), (unsigned)ny), dim3(256), 0, s, bcx, stride,
                        conv_w, state, qsl, R, T, H, out, taps);
+  };
+  if (n <= 256) go(std::integral_constant<int, 1>());
+  else if (n <= 512) go(std::integral_constant<int, 2>());
+  else if (n <= 1024) go(std::integral_constant<int, 4>());
+  else if (n > 6144 && n <= 12288) go(std::integral_constant<int, 16>());
+  else go(std::integral_constant<int, 8>());
   return kv800::check_launch("conv_chunk");
 }
 
