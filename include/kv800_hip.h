@@ -297,7 +297,8 @@ int kv800_hip_decode_noalloc(const kv800_paged_t* P, const uint16_t* q, int64_t 
  * cs2: kv800_hip_rope_table of the same rows (needed with sub-blocks). V of sub-blocks is not rounded to bf16. Offsets outside
  * the pools and positions past the tables are skipped. out (T, 16, 128) bf16; a query without keys and the padding
  * [qsl[R], T) get zeros. ws: kv800_hip_decode_chunk_workspace(R, T, nqmax) bytes (0 for nqmax = 0 or window layers), 16-byte
- * aligned, of this call alone. The result does not depend on the other rows of the call, but on their number by rounding. */
+ * aligned, of this call alone. What a query does not see does not reach it, NaN and infinities included; the other rows of a
+ * call change a row's result by rounding alone (where its keys are split). With sub-blocks rope_rows < 2^24. */
 int64_t kv800_hip_decode_chunk_workspace(int64_t R, int64_t T, int64_t nqmax);
 int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int64_t* qsl, int64_t R, int64_t T,
                            const uint16_t* cos_t, const uint16_t* sin_t, int64_t rope_rows, const uint32_t* cs2,

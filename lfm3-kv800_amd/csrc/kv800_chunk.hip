@@ -261,6 +261,15 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
         sc[u][ct] = mfma_bf(pack8b(an[b]), bq[ct][2 + d], sc[u][ct]);
       }
     }
+    // A weight of 0 does not take out a NaN scale: where queries do not see all of the chunk, such a token's scales become 0 and
+    // its scores NaN, for the queries that see it.
+    uint32_t odd = 0;
+    if (kpos + 31 > pbase) {
+      const int tk = 32 * cc + (lane & 31);
+      const bool bad = __builtin_isnan(L.vs[h][tk]) || __builtin_isnan(L.vl[h][tk]);
+      odd = (uint32_t)__ballot(bad);
+      if (bad) L.vs[h][tk] = L.vl[h][tk] = 0.f;
+    }
     // what the softmax and P V read, issued under the last products
     float4 vs4[2], vl4[2];
 #pragma unroll
@@ -281,6 +290,13 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (kpos + 16 * u + 4 * g + i > pcol[ct]) sc[u][ct][i] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((odd >> (16 * u + 4 * g + i)) & 1u && kpos + 16 * u + 4 * g + i <= pcol[ct]) sc[u][ct][i] = __builtin_nanf("");
     }
     h8 Bw[CT];
 #pragma unroll
@@ -397,7 +413,7 @@ template <int QT>
 __device__ __forceinline__ int list_size(const ListRow& x) { return (x.c + QT - 1) / QT * x.nu; }
 
 template <int CT>
-__global__ void __launch_bounds__(256, 2) chunk_quant_kernel(ChunkArgs A) {
+__global__ void __launch_bounds__(256, CT == 1 ? 3 : 2) chunk_quant_kernel(ChunkArgs A) {
   constexpr int QT = 4 * CT;
   __shared__ ChunkQLds L;
   __shared__ ChunkStage SA, SB;   // two objects: a read of one is not held for the other's loads
@@ -487,6 +503,7 @@ struct alignas(16) ChunkXRows { uint16_t r[NW][XCH * 128]; };
 template <int CT, int NW>
 struct alignas(16) ChunkXLds {
   float m[NW][16 * CT], l[NW][16 * CT];
+  int odd[NW];
 };
 __device__ const uint4 chunk_zeros[16] = {};           // a row for tokens without a key: a zero weight needs a finite value
 
@@ -505,25 +522,20 @@ __device__ __forceinline__ void vm_wait() {            // all but the N youngest
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// Queries [qa, qa + nq) of tile t, KV head h. Returns whether an infinity or NaN stands among values that not all of them see:
+// a weight of 0 does not take it out of a product, so the caller then has the queries one by one, whose lists hold no other
+// keys.
 template <int CT, int NW, bool DIRECT>
-__global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
-  constexpr int QT = 4 * CT, NC = 16 * CT, XROW = 132;
-  __shared__ ChunkXRows<NW> Ks, Vs;                    // two objects: a read of one is not held for the other's loads
-  __shared__ ChunkXLds<CT, NW> L;
+__device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& Vs, ChunkXLds<CT, NW>& L, const ChunkArgs& A,
+                                           const Tile& t, int64_t it, int h, int qa, int nq) {
+  constexpr int NC = 16 * CT, XROW = 132;
   static_assert((NW - 1) * 16 * XROW * 4 <= (int)sizeof(Ks) || NW == 1, "the join must fit");
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, n = lane & 15;
-  if (DIRECT && (int64_t)blockIdx.x == 4 * A.I) {      // the padding's output rows
-    const int64_t e0 = min(A.qsl[A.R], A.T) * 256;
-    for (int64_t i = e0 + tid; i < A.T * 256; i += 64 * NW) reinterpret_cast<u4v*>(A.out)[i] = u4v{0u, 0u, 0u, 0u};
-    return;
-  }
-  const int64_t it = blockIdx.x >> 2;
-  const int h = blockIdx.x & 3;
-  Tile t;
-  if (!find_tile<QT>(A, it, t)) return;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));                        // nothing that hangs on it is kept in registers for the next call
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int N = t.n, win = (int)A.P.win;
-  const int pbase = N - t.c + t.q0, plast = pbase + t.nq - 1;
-  const bool wide = CT > 1 && t.nq > 4;                // a tile of up to 4 queries leaves the second column tile out
+  const int pbase = N - t.c + t.q0 + qa, plast = pbase + nq - 1;
+  const bool wide = CT > 1 && nq > 4;                // a tile of up to 4 queries leaves the second column tile out
   // key list: sinks [0, cnt), exact positions lo_row .. + cnt2, then lo_tile ..
   int lo_row, lo_tile;
   if (win > 0) {
@@ -590,6 +602,11 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
     r.ok = (uint32_t)__ballot(ok);
     return r;
   };
+  auto key_at = [&](int c0, uint32_t ok, int e) {      // position of token e of the chunk; past every query if it has no key
+    const int kp = c0 >= cnt + cnt2 ? rest + c0 + e : posof(c0 + e);
+    return (ok >> e) & 1u ? kp : 0x7FFFFFFF;
+  };
+  auto sees = [&](int qp, int kp) { return (kp <= qp) & ((kp > (win > 0 ? qp - win : -1)) | (kp < A.nsink)); };
   const uint32_t kl = lds_addr(Ks.r[w]), vl = lds_addr(Vs.r[w]);
   const int r4 = lane >> 4, pc = lane & 15;            // an instruction fills 4 rows: row r4, piece pc
   auto row_at = [&](const uint16_t* p, int t) {        // token t's pointer
@@ -628,10 +645,11 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   for (int ct = 0; ct < CT; ++ct) {
     const int qi = 4 * ct + (n >> 2);
     pcol[ct] = pbase + qi;
-    const uint16_t* qr = A.q + ((t.t0 + t.q0 + min(qi, t.nq - 1)) * 16 + 4 * h + (n & 3)) * 128 + 8 * g;
+    const uint16_t* qr = A.q + ((t.t0 + t.q0 + qa + min(qi, nq - 1)) * 16 + 4 * h + (n & 3)) * 128 + 8 * g;
 #pragma unroll
     for (int s = 0; s < 4; ++s) bq[ct][s] = as_b8(*reinterpret_cast<const u4v*>(qr + 32 * s));
   }
+  bool odd = false;                                    // an infinity or NaN among values that not every query sees
   float m[CT], lsum[CT];
   f4 acc[CT][8];                                       // dims 16 j + 4 g + i of column n
 #pragma unroll
@@ -696,24 +714,15 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
       }
       // a chunk whose keys are all there and seen by every query of the tile needs no mask
       const int p0 = rest + c0;                        // position of the chunk's first key, behind the sinks
-      const bool plain = c0 >= cnt + cnt2;
-      const bool all = plain & (at.ok == 0xFFFFFFFFu) & (p0 + 31 <= pbase) & ((win == 0) | (p0 > plast - win));
+      const bool all = (c0 >= cnt + cnt2) & (at.ok == 0xFFFFFFFFu) & (p0 + 31 <= pbase) & ((win == 0) | (p0 > plast - win));
       if (!all) {
-        const uint32_t tb = at.ok >> (4 * g);          // bit 16 u + i: token 16 u + 4 g + i
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int e = 16 * u + 4 * g + i;
-            int kp = p0 + e;
-            if (!plain) kp = posof(c0 + e);
-            kp = (tb >> (16 * u + i)) & 1u ? kp : 0x7FFFFFFF;
+            const int kp = key_at(c0, at.ok, 16 * u + 4 * g + i);
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              const int wlo = win > 0 ? pcol[ct] - win : -1;
-              const bool keep = (kp <= pcol[ct]) & ((kp > wlo) | (kp < A.nsink));
-              sc[u][ct][i] = keep ? sc[u][ct][i] : -INFINITY;
-            }
+            for (int ct = 0; ct < CT; ++ct) sc[u][ct][i] = sees(pcol[ct], kp) ? sc[u][ct][i] : -INFINITY;
           }
       }
       u4v bh[CT], bl[CT];
@@ -743,11 +752,33 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
       // V^T: lane (g, n) gives 4 values of row 4 g + n / 4 from dim 16 j + 4 (n % 4) on
       uint16_t* vw = Vs.r[w];
       const int vrow = 4 * g + (n >> 2);
+      auto read_vt = [&](int j) {
+        const int o = vrow * 128 + 8 * ((2 * j + ((n & 3) >> 1)) ^ (2 * (vrow & 7))) + 4 * (n & 1);
+        const s4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[o]);
+        const s4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[o + 16 * 128]);
+        return u4v{__builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 0, 1)),
+                   __builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 2, 3)),
+                   __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 0, 1)),
+                   __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 2, 3))};
+      };
+      // A weight of 0 does not take out an infinity or NaN. Where a chunk has a mask, its values are looked over: the largest
+      // exponent of each half, all ones in infinities and NaN.
+      if (!all && !odd && nq > 1) {
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        us2 z = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const u4v x = *reinterpret_cast<const u4v*>(vw + 512 * i + 8 * lane);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) z = __builtin_elementwise_max(z, __builtin_bit_cast(us2, x[k] & 0x7F807F80u));
+        }
+        odd = __any((z.x == 0x7F80) | (z.y == 0x7F80));
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int at = vrow * 128 + 8 * ((2 * j + ((n & 3) >> 1)) ^ (2 * (vrow & 7))) + 4 * (n & 1);
-        const s4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[at]);
-        const s4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[at + 16 * 128]);
+        const int o = vrow * 128 + 8 * ((2 * j + ((n & 3) >> 1)) ^ (2 * (vrow & 7))) + 4 * (n & 1);
+        const s4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[o]);
+        const s4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[o + 16 * 128]);
         const u4v av = {__builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 0, 1)),
                         __builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 2, 3)),
                         __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 0, 1)),
@@ -771,15 +802,19 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) lsum[ct] = sum4rows(lsum[ct]);
+  bool any = odd;
   if constexpr (NW > 1) {
-    float (*O)[16][XROW] = reinterpret_cast<float (*)[16][XROW]>(&Ks);   // the other waves' accumulators, scaled alike
+    float (*O)[16][XROW] = reinterpret_cast<float (*)[16][XROW]>(Ks.r[0]);   // the other waves' accumulators, scaled alike
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
       if (g == 0) { L.m[w][16 * ct + n] = m[ct]; L.l[w][16 * ct + n] = lsum[ct]; }
+    L.odd[w] = odd;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       if (ct > 0 && !wide) break;                      // uniform
       __syncthreads();                                 // the chunks, and the last column tile's join, are done
+      if (ct == 0)
+        for (int k = 0; k < NW; ++k) any |= L.odd[k] != 0;
       float M = NEG_BIG, l = 0.f;
       for (int k = 0; k < NW; ++k) M = fmaxf(M, L.m[k][16 * ct + n]);
       for (int k = 0; k < NW; ++k) l += L.l[k][16 * ct + n] * __builtin_amdgcn_exp2f(L.m[k][16 * ct + n] - M);
@@ -798,26 +833,46 @@ __global__ void __launch_bounds__(64 * NW) chunk_exact_kernel(ChunkArgs A) {
           for (int k = 0; k < NW - 1; ++k) acc[ct][j] += *reinterpret_cast<const f4*>(&O[k][n][16 * j + 4 * g]);
       }
     }
-    if (w > 0) return;
+    if (w > 0) return any;
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int qi = 4 * ct + (n >> 2);
-    if (qi >= t.nq) continue;
+    if (qi >= nq) continue;
     if (DIRECT) {
       const float inv = lsum[ct] > 0.f ? 1.0f / lsum[ct] : 0.f;
-      uint16_t* o = A.out + ((t.t0 + t.q0 + qi) * 16 + 4 * h + (n & 3)) * 128 + 4 * g;
+      uint16_t* o = A.out + ((t.t0 + t.q0 + qa + qi) * 16 + 4 * h + (n & 3)) * 128 + 4 * g;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const f4 a = acc[ct][j];
         *reinterpret_cast<uint2*>(o + 16 * j) = make_uint2(bfpk(a[0] * inv, a[1] * inv), bfpk(a[2] * inv, a[3] * inv));
       }
     } else {
-      const int64_t col = ((A.G + A.I + it) * 4 + h) * NC + 16 * ct + n;
+      const int64_t col = ((A.G + A.I + it) * 4 + h) * NC + 4 * (qa + qi) + (n & 3);
       if (g == 0) { A.mo[col] = m[ct]; A.lo[col] = lsum[ct]; }
 #pragma unroll
       for (int j = 0; j < 8; ++j) *reinterpret_cast<f4*>(A.ao + col * 128 + 16 * j + 4 * g) = acc[ct][j];
     }
+  }
+  return any;
+}
+
+template <int CT, int NW, bool DIRECT>
+__global__ void __launch_bounds__(64 * NW, 2) chunk_exact_kernel(ChunkArgs A) {
+  __shared__ ChunkXRows<NW> Ks, Vs;                    // two objects: a read of one is not held for the other's loads
+  __shared__ ChunkXLds<CT, NW> L;
+  if (DIRECT && (int64_t)blockIdx.x == 4 * A.I) {      // the padding's output rows
+    const int64_t e0 = min(A.qsl[A.R], A.T) * 256;
+    for (int64_t i = e0 + threadIdx.x; i < A.T * 256; i += 64 * NW) reinterpret_cast<u4v*>(A.out)[i] = u4v{0u, 0u, 0u, 0u};
+    return;
+  }
+  const int64_t it = blockIdx.x >> 2;
+  Tile t;
+  if (!find_tile<4 * CT>(A, it, t)) return;
+  for (int k = -1; k < t.nq; ++k) {                    // all queries, or after them one by one
+    const bool odd = exact_tile<CT, NW, DIRECT>(Ks, Vs, L, A, t, it, blockIdx.x & 3, max(k, 0), k < 0 ? t.nq : 1);
+    if (k < 0 && !odd) return;                         // uniform
+    __syncthreads();
   }
 }
 
@@ -1007,6 +1062,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
     KV800_REQUIRE(P->qpool && P->boff && P->boff_stride > 0 && P->NQ && cos_t && cs2 && qpool_bytes >= SUB && (uintptr_t)cs2 % 16 == 0 &&
                       (uintptr_t)P->qpool % 16 == 0,
                   "decode_chunk: quantized layers need NQ, the quant pool (16-byte aligned, one sub-block at least), its offsets and the rope tables");
+  KV800_REQUIRE(!quant || rope_rows < (1LL << 24), "decode_chunk: rope tables of 2^24 rows or more are not addressed");   // 128 bytes a row of cs2
   const bool sinks = P->win > 0 && P->sk;
   KV800_REQUIRE(!sinks || (P->sv && P->skoff && P->svoff && (((uintptr_t)P->sk | (uintptr_t)P->sv) % 16) == 0),
                 "decode_chunk: sinks need sv, skoff, svoff and 16-byte aligned buffers");

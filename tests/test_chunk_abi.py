@@ -70,7 +70,7 @@ def test_decode_chunk_host_checks(lib):
                  (dict(epool=None), {}), (dict(eoff=None), {}), (dict(N=None), {}), (dict(NQ=None), {}), (dict(ebs=0), {}),
                  (dict(eoff_stride=0), {}), (dict(win=-1), {}), (dict(win=1 << 31), {}), (dict(nqmax=-1), {}), (dict(e_ts=1020), {}),
                  (dict(e_hs=4), {}), (dict(e_v=1), {}), (dict(qpool=None), {}), (dict(boff=None), {}), (dict(qpool=A + 4), {}),
-                 (dict(win=256, sk=A), {}), (dict(win=256, sk=A, sv=A + 2, skoff=A, svoff=A), {})):
+                 (dict(win=256, sk=A), {}), (dict(win=256, sk=A, sv=A + 2, skoff=A, svoff=A), {}), (None, dict(rr=1 << 24))):
         refused(lib, f(P, **k), b"decode_chunk")
 
 

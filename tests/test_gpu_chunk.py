@@ -107,6 +107,61 @@ def test_bad_offsets_are_skipped(hip):
     check(got, c.want(hip, lambda r, p: gone[r](p) | (p >= short)), "short rope table")
 
 
+def poison(c, r, pos, what, k=None, v=None):
+    """Exact position `pos` of row r, head `what`: its key and value set to k and v."""
+    at = int(c.P.eoff[r, pos // c.P.ebs]) + what * c.P.e_hs + (pos % c.P.ebs) * c.P.e_ts
+    flat = c.P.epool.view(-1)
+    if k is not None:
+        flat[at:at + 128] = k
+    if v is not None:
+        flat[at + c.P.e_v:at + c.P.e_v + 128:3] = v
+
+
+@pytest.mark.parametrize("win", [0, 256])
+@pytest.mark.parametrize("new", [[1, 3, 4, 2], [1, 9, 12, 35]])
+def test_values_that_a_query_does_not_see(hip, win, new):
+    """NaN and infinities at positions behind a query, or before its window, do not reach it; queries that see them give NaN or
+    infinities in the heads that read them, and nowhere else."""
+    c = ref.Cache(hip, [700, 390, 1000, 513], new, ebs=40, win=win, seed=21)
+    want, at = c.want(hip), 0
+    bad = torch.zeros(sum(new), 16, dtype=torch.bool)
+    for r, n in enumerate(new):
+        hits = [(c.N[r] - 1, 0, float("nan"), None), (c.N[r] - 1, 1, None, float("inf")), (c.N[r] - n // 2 - 1, 2, None, float("nan")),
+                (c.N[r] - 1, 3, float("inf"), float("-inf"))]
+        if win:
+            hits += [(c.first[r], 0, None, float("inf")), (c.first[r] + n // 2, 2, float("nan"), float("nan"))]
+        for pos, h, k, v in hits:
+            poison(c, r, pos, h, k, v)
+            for i in range(n):
+                q = c.prev[r] + i
+                if pos <= q and (not win or pos > q - win):
+                    bad[at + i, 4 * h:4 * h + 4] = True
+        at += n
+    got = hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+    seen = ~torch.isfinite(got).all(-1).cpu()
+    assert torch.equal(seen, bad)
+    check(got[~bad.to(got.device)], want[~bad.to(got.device)], f"values unseen, window {win}")
+
+
+def test_scales_that_a_query_does_not_see(hip):
+    """Sub-blocks that reach into the new tokens, with NaN scales there."""
+    c = ref.Cache(hip, [250, 700], [12, 70], flushed=[1, 3], seed=22)
+    want = c.want(hip)
+    nan = 0x7F
+    VLO, VSC = 256 * 128 + 256 * 64, 256 * 128 + 256 * 64 + 512
+    bad = torch.zeros(82, 16, dtype=torch.bool)
+    for r, j, t, h, o in ((0, 0, 254, 1, VSC), (1, 2, 740 - 512, 0, VLO), (1, 2, 767 - 512, 3, VSC)):
+        block = int(c.P.boff[r, j])
+        c.P.qpool.view(-1)[block + o + 2 * t + h // 2] = nan
+        first = [0, 12][r]
+        for i in range([12, 70][r]):
+            if j * 256 + t <= c.prev[r] + i:
+                bad[first + i, 8 * (h // 2):8 * (h // 2) + 8] = True
+    got = hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+    assert torch.equal(~torch.isfinite(got).all(-1).cpu(), bad)
+    check(got[~bad.to(got.device)], want[~bad.to(got.device)], "scales unseen")
+
+
 def test_a_query_without_keys(hip):
     c = ref.Cache(hip, [40, 300], [2, 2], seed=10)
     c.P.eoff[0] = -1
