@@ -413,10 +413,8 @@ template <int QT>
 __device__ __forceinline__ int list_size(const ListRow& x) { return (x.c + QT - 1) / QT * x.nu; }
 
 template <int CT>
-__global__ void __launch_bounds__(256, CT == 1 ? 3 : 2) chunk_quant_kernel(ChunkArgs A) {
+__device__ __forceinline__ void quant_part(ChunkQLds& L, ChunkStage& SA, ChunkStage& SB, const ChunkArgs& A, const unsigned wg) {
   constexpr int QT = 4 * CT;
-  __shared__ ChunkQLds L;
-  __shared__ ChunkStage SA, SB;   // two objects: a read of one is not held for the other's loads
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   // every workgroup sums the rows' entries itself: thread i takes the rows [i k, i k + k). The list has less than 2^31
   // entries (the host's check).
@@ -439,7 +437,7 @@ __global__ void __launch_bounds__(256, CT == 1 ? 3 : 2) chunk_quant_kernel(Chunk
   int pre = inc - mine;
   for (int i = 0; i < w; ++i) pre += L.ws[i];
   const int total = __builtin_amdgcn_readfirstlane(L.ws[0] + L.ws[1] + L.ws[2] + L.ws[3]), G = (int)A.G, C = (total + G - 1) / G;
-  if (blockIdx.x == 0) {                               // for the merge
+  if (wg == 0) {                               // for the merge
     int x = pre;
     for (int r = ra; r < rb; ++r) {
       A.pre[r] = x;
@@ -447,7 +445,7 @@ __global__ void __launch_bounds__(256, CT == 1 ? 3 : 2) chunk_quant_kernel(Chunk
     }
     if (tid == 0) A.pre[R] = C;
   }
-  int v = (int)blockIdx.x * C;
+  int v = (int)wg * C;
   const int v1 = min(v + C, total);
   if (v >= v1) return;                                 // uniform
   if (v >= pre && v < pre + mine) {                    // one thread: the row of the workgroup's first entry
@@ -477,7 +475,7 @@ __global__ void __launch_bounds__(256, CT == 1 ? 3 : 2) chunk_quant_kernel(Chunk
       t.c = c;
       t.q0 = tile * QT;
       t.nq = min(QT, c - t.q0);
-      chunk_span<CT>(L, SA, SB, A, t, u0, u1, head ? (int64_t)blockIdx.x : A.G + r + (unsigned)t.t0 / QT + tile);
+      chunk_span<CT>(L, SA, SB, A, t, u0, u1, head ? (int64_t)wg : A.G + r + (unsigned)t.t0 / QT + tile);
       head = false;
       v += u1 - u0;
     }
@@ -485,6 +483,12 @@ __global__ void __launch_bounds__(256, CT == 1 ? 3 : 2) chunk_quant_kernel(Chunk
     x += sz;
     y = list_row<QT>(A, ++r);
   }
+}
+
+__global__ void __launch_bounds__(256, 3) chunk_quant_kernel(ChunkArgs A) {
+  __shared__ ChunkQLds L;
+  __shared__ ChunkStage SA, SB;   // two objects: a read of one is not held for the other's loads
+  quant_part<1>(L, SA, SB, A, blockIdx.x);
 }
 
 // ---------------------------------------------------------------- exact rows and sinks
@@ -858,6 +862,18 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
 }
 
 template <int CT, int NW, bool DIRECT>
+__device__ __forceinline__ void exact_part(ChunkXRows<NW>& Ks, ChunkXRows<NW>& Vs, ChunkXLds<CT, NW>& L, const ChunkArgs& A,
+                                           const unsigned wg) {
+  const int64_t it = wg >> 2;
+  Tile t;
+  if (!find_tile<4 * CT>(A, it, t)) return;
+  for (int k = -1; k < t.nq; ++k) {                    // all queries, or after them one by one
+    const bool odd = exact_tile<CT, NW, DIRECT>(Ks, Vs, L, A, t, it, wg & 3, max(k, 0), k < 0 ? t.nq : 1);
+    if (k < 0 && !odd) return;                         // uniform
+    __syncthreads();
+  }
+}
+template <int CT, int NW, bool DIRECT>
 __global__ void __launch_bounds__(64 * NW, 2) chunk_exact_kernel(ChunkArgs A) {
   __shared__ ChunkXRows<NW> Ks, Vs;                    // two objects: a read of one is not held for the other's loads
   __shared__ ChunkXLds<CT, NW> L;
@@ -866,14 +882,21 @@ __global__ void __launch_bounds__(64 * NW, 2) chunk_exact_kernel(ChunkArgs A) {
     for (int64_t i = e0 + threadIdx.x; i < A.T * 256; i += 64 * NW) reinterpret_cast<u4v*>(A.out)[i] = u4v{0u, 0u, 0u, 0u};
     return;
   }
-  const int64_t it = blockIdx.x >> 2;
-  Tile t;
-  if (!find_tile<4 * CT>(A, it, t)) return;
-  for (int k = -1; k < t.nq; ++k) {                    // all queries, or after them one by one
-    const bool odd = exact_tile<CT, NW, DIRECT>(Ks, Vs, L, A, t, it, blockIdx.x & 3, max(k, 0), k < 0 ? t.nq : 1);
-    if (k < 0 && !odd) return;                         // uniform
-    __syncthreads();
-  }
+  exact_part<CT, NW, DIRECT>(Ks, Vs, L, A, blockIdx.x);
+}
+// Both in one launch, for few tiles: three of four waves per (tile, KV head), then the quantized list's workgroups.
+constexpr int BNW = 3;
+union ChunkBoth { ChunkStage s; ChunkXRows<BNW> x; };
+template <int CT>
+__global__ void __launch_bounds__(256, 2) chunk_both_kernel(ChunkArgs A) {
+  __shared__ ChunkQLds L;
+  __shared__ ChunkBoth a, b;
+  __shared__ ChunkXLds<CT, BNW> X;
+  const unsigned nx = 4 * (unsigned)A.I;
+  if (blockIdx.x >= nx)
+    quant_part<CT>(L, a.s, b.s, A, blockIdx.x - nx);
+  else if (threadIdx.x < 64 * BNW)
+    exact_part<CT, BNW, false>(a.x, b.x, X, A, blockIdx.x);
 }
 
 // ---------------------------------------------------------------- merge
@@ -969,7 +992,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
   *dst = bfpk((x0 * hn + fx * ax.x) * inv, (x1 * hn + fx * ax.y) * inv);
 }
 
-// queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8
+// Queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8
 // (layers without sub-blocks: while every row can bring one token only; their kernel passes over an empty second half).
 int chunk_ct(int64_t R, int64_t T, bool quant) { return T <= (quant ? 4 * R : R) ? 1 : 2; }
 
@@ -990,38 +1013,47 @@ int64_t chunk_cus() {
   return cache[dev];
 }
 
-struct ChunkPlan { int ct; int64_t G, I, cols, pre; };   // cols: partial columns; pre: entries
+struct ChunkPlan { int ct; bool both; int64_t G, I, cols, pre; };   // cols: partial columns; pre: entries
 ChunkPlan chunk_plan(int64_t R, int64_t T, int64_t nqmax) {
   ChunkPlan p;
   p.ct = chunk_ct(R, T, nqmax > 0);
   p.I = R + T / (4 * p.ct);
-  p.G = nqmax > 0 ? chunk_cus() * (p.ct == 1 ? 3 : 2) : 0;   // what is resident at 150 / 207 VGPRs
+  // One launch for both parts, except where tiles of 4 have long lists: alone, their quantized part has three workgroups on a
+  // CU instead of two. In us, one launch / two: 1 row x 5 at 16K tokens 25 / 35, 16 x 8 at 4K 39 / 45, 128 x 8 at 16K 266 / 270;
+  // tiles of 4: 1 x 1 at 4K 19 / 25, 64 x 1 at 1K 26 / 34, 64 x 4 at 4K 53 / 53, 32 x 4 at 16K 71 / 70, 64 x 4 at 16K 117 / 106.
+  p.both = nqmax > 0 && (p.ct == 2 || R * nqmax <= 8 * chunk_cus());
+  p.G = nqmax > 0 ? chunk_cus() * (p.both ? 2 : 3) : 0;   // what is resident: 256 registers and 68 KB, or 168 and 39 KB
   p.cols = nqmax > 0 ? (p.G + 2 * p.I) * 64 * p.ct : 0;
   p.pre = nqmax > 0 ? (R + 4) / 4 * 4 : 0;
   return p;
 }
 
-template <int CT, int NW>
-int chunk_exact(const ChunkArgs& A, bool quant, hipStream_t s) {
-  const unsigned nx = (unsigned)(4 * A.I);
-  if (quant)
-    hipLaunchKernelGGL((chunk_exact_kernel<CT, NW, false>), dim3(nx), dim3(64 * NW), 0, s, A);
-  else
-    hipLaunchKernelGGL((chunk_exact_kernel<CT, NW, true>), dim3(nx + 1), dim3(64 * NW), 0, s, A);
+template <int CT, int NW, bool DIRECT>
+int chunk_exact(const ChunkArgs& A, hipStream_t s) {
+  hipLaunchKernelGGL((chunk_exact_kernel<CT, NW, DIRECT>), dim3((unsigned)(4 * A.I + DIRECT)), dim3(64 * NW), 0, s, A);
   return check_launch("chunk_exact");
 }
-template <int CT>
-int chunk_launch(const ChunkArgs& A, bool quant, hipStream_t s) {
-  int rc;
-  if (quant) {
-    hipLaunchKernelGGL(chunk_quant_kernel<CT>, dim3((unsigned)A.G), dim3(256), 0, s, A);
-    if ((rc = check_launch("chunk_quant")) != KV800_OK) return rc;
-  }
-  // waves per (tile, KV head): as many as are resident at once, by the rows' (tile, head) pairs (70, 35 and 17 KB of LDS)
+// waves per (tile, KV head): as many as are resident at once, by the rows' (tile, head) pairs (66, 33 and 16 KB of LDS)
+template <int CT, bool DIRECT>
+int chunk_exact_all(const ChunkArgs& A, hipStream_t s) {
   const int64_t cu = chunk_cus(), pairs = 4 * max(A.R, A.T / (4 * CT));
-  rc = pairs <= 2 * cu ? chunk_exact<CT, 4>(A, quant, s) : pairs <= 4 * cu ? chunk_exact<CT, 2>(A, quant, s) : chunk_exact<CT, 1>(A, quant, s);
-  if (rc != KV800_OK || !quant) return rc;
-  if (16 * A.T <= 4 * cu)
+  return pairs <= 2 * cu ? chunk_exact<CT, 4, DIRECT>(A, s)
+                         : pairs <= 4 * cu ? chunk_exact<CT, 2, DIRECT>(A, s) : chunk_exact<CT, 1, DIRECT>(A, s);
+}
+template <int CT>
+int chunk_launch(const ChunkArgs& A, bool quant, bool both, hipStream_t s) {
+  if (!quant) return chunk_exact_all<CT, true>(A, s);
+  int rc = KV800_OK;
+  if (both) {
+    hipLaunchKernelGGL(chunk_both_kernel<CT>, dim3((unsigned)(4 * A.I + A.G)), dim3(256), 0, s, A);
+    rc = check_launch("chunk_both");
+  } else if constexpr (CT == 1) {
+    hipLaunchKernelGGL(chunk_quant_kernel, dim3((unsigned)A.G), dim3(256), 0, s, A);
+    rc = check_launch("chunk_quant");
+    if (rc == KV800_OK) rc = chunk_exact_all<1, false>(A, s);
+  }
+  if (rc != KV800_OK) return rc;
+  if (16 * A.T <= 4 * chunk_cus())
     hipLaunchKernelGGL((chunk_merge_kernel<CT, 4>), dim3((unsigned)(16 * A.T)), dim3(256), 0, s, A);
   else
     hipLaunchKernelGGL((chunk_merge_kernel<CT, 1>), dim3((unsigned)(4 * A.T)), dim3(256), 0, s, A);
@@ -1068,7 +1100,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
                 "decode_chunk: sinks need sv, skoff, svoff and 16-byte aligned buffers");
   const ChunkPlan p = chunk_plan(R, T, quant ? P->nqmax : 0);
   KV800_REQUIRE(p.I <= (1LL << 28) && T <= (1LL << 28) && P->ebs < (1LL << 30), "decode_chunk: too many rows and tokens");
-  KV800_REQUIRE(!quant || p.I <= 0x7FFFFFFFLL / 4 / P->nqmax, "decode_chunk: too many rows and sub-blocks");
+  KV800_REQUIRE(!quant || p.I <= (int64_t)0x7FFFFFFF / 4 / P->nqmax, "decode_chunk: too many rows and sub-blocks");
   KV800_REQUIRE(!quant || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= kv800_hip_decode_chunk_workspace(R, T, P->nqmax)),
                 "decode_chunk: the workspace is too small or not 16-byte aligned");
   ChunkArgs A;
@@ -1085,7 +1117,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
   A.scale = 1.4426950408889634f * 0.08838834764831845f;
   A.nsink = sinks ? NSINK : 0;
   const hipStream_t s = (hipStream_t)stream;
-  return p.ct == 1 ? chunk_launch<1>(A, quant, s) : chunk_launch<2>(A, quant, s);
+  return p.ct == 1 ? chunk_launch<1>(A, quant, p.both, s) : chunk_launch<2>(A, quant, p.both, s);
 }
 
 }  // extern "C"

@@ -42,6 +42,23 @@ def test_quantized(hip, rows, ebs, token_major):
     check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), c.want(hip), f"quantized {rows} ebs {ebs}")
 
 
+@pytest.mark.parametrize("rows", ["one", "edges", "empty rows", "more rows than a wave", "rows of one wave each"])
+def test_quantized_in_two_launches(hip, rows):
+    """Tiles of 4 under a bound on the blocks that allows long lists: the two parts have a launch each."""
+    prev, new = ROWS.get(rows) or ([(53 * i) % 1100 for i in range(300)], [i % 5 for i in range(300)])
+    c = ref.Cache(hip, prev, new, ebs=40, seed=len(rows))
+    c.P.nqmax = 8 * torch.cuda.get_device_properties(0).multi_processor_count // len(prev) + 1
+    want = c.want(hip)
+    check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), want, f"two launches {rows}")
+    r = next(i for i, n in enumerate(new) if n)
+    t = sum(new[:r + 1]) - 1                             # the row's last token, whose value is NaN
+    poison(c, r, c.N[r] - 1, 2, v=float("nan"))
+    got = hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+    assert torch.isnan(got[t, 8:12]).any(-1).all()
+    got[t, 8:12] = want[t, 8:12].to(got.dtype)
+    check(got, want, f"two launches {rows}, a value unseen")
+
+
 @pytest.mark.parametrize("rows", list(ROWS))
 @pytest.mark.parametrize("sinks,rot", [(True, True), (False, False)])
 def test_window(hip, rows, sinks, rot):
