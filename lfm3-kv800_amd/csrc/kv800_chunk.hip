@@ -591,7 +591,7 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
       if (i < cnt) {
         ko = sko + ((int64_t)i * 4 + h) * 128;
         vo = svo + ((int64_t)i * 4 + h) * 128;
-        ok = ko >= 0 && vo >= 0 && ko + 128 <= A.sink_elems && vo + 128 <= A.sink_elems;
+        ok = sko >= 0 && svo >= 0 && ko + 128 <= A.sink_elems && vo + 128 <= A.sink_elems;
         kb = A.P.sk; vb = A.P.sv;
       } else {
         int pg, in;

@@ -745,6 +745,7 @@ def combine(MO, LO, AO, ns):
 
 # ---------------------------------------------------------------- decode
 _PAIRS = OrderedDict()     # (device, cos ptr, sin ptr, rows) -> (cos_t, sin_t, versions, pair table, stream, event)
+_CAPTURED = {}             # pair tables that a captured graph may read: kept, whatever leaves _PAIRS
 
 
 def rope_pairs(cos_t, sin_t):
@@ -752,14 +753,17 @@ def rope_pairs(cos_t, sin_t):
     tensors. The entry holds the two tables themselves, so their storage cannot be freed and reused by other tensors
     while it is cached; it is rebuilt when either tensor is modified in place (version counter) or replaced. A call on
     another stream than the one that built it waits for it; a table built while a graph is captured belongs to that graph
-    alone, whose replays fill it."""
+    alone, whose replays fill it. A captured call that finds its table reads it as it is then, on every replay: tables
+    changed in place are captured anew."""
     key = (cos_t.device, cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0])
     ent = _PAIRS.get(key)
     ver = (cos_t._version, sin_t._version)
     now = _raw_stream(cos_t.device)
     if ent is not None and ent[0] is cos_t and ent[1] is sin_t and ent[2] == ver:
         _PAIRS.move_to_end(key)
-        if ent[4] != now and not torch.cuda.is_current_stream_capturing():   # a capture begins by waiting for the device
+        if torch.cuda.is_current_stream_capturing():     # a capture begins by waiting for the device
+            _CAPTURED[ent[3].data_ptr()] = ent[3]
+        elif ent[4] != now:
             stream = torch.cuda.current_stream(cos_t.device)
             stream.wait_event(ent[5])
             ent[3].record_stream(stream)

@@ -369,12 +369,12 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
     at = torch.arange(T, device=dev)
     for s in range(steps):
         drafts, counts, probs = draft(last, lens)
-        ql = (counts + 1).to(torch.int32)
+        ql = (counts.clamp(0, most) + 1).to(torch.int32)
         meta = attention.begin_chunk(lens + ql, ql, T, most + 1, attention.lens + (s + 1) * (most + 1))
         i = (at - meta.qsl[meta.row]).clamp(max=most)
         tok = torch.cat((last[:, None], drafts), 1)[meta.row, i]
         logits = model.chunk(tok, meta)
-        q = None if probs is None else probs[meta.row, i.clamp(max=most - 1)]
+        q = None if probs is None or not most else probs[meta.row, i.clamp(max=most - 1)]
         out, kept = so.verify_drafts(logits, tok, meta.qsl, temperature, torch.rand(T, device=dev, generator=generator),
                                      torch.rand(R, device=dev, generator=generator), q)
         model.commit(kept)

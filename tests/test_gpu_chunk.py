@@ -217,6 +217,82 @@ def test_attention_in_a_graph_and_on_another_stream(hip):
     check(got, c.want(hip), "another stream")
 
 
+def test_graphs_keep_their_rope_tables(hip):
+    """A call captured before its pair table exists makes it on every replay; one captured after keeps the table that it found,
+    however many others are made since."""
+    c = ref.Cache(hip, [700, 1400], [4, 3], seed=31)
+    want = c.want(hip)
+    hip.rope_pairs(torch.ones_like(c.cos), c.sin)
+    graphs = []
+    for _ in range(2):
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+        graphs.append((g, out))
+        hip.rope_pairs(c.cos, c.sin)
+    kept = [hip.rope_pairs(torch.rand_like(c.cos), c.sin) for _ in range(12)]
+    c.cos.add_(0)                                       # another version: the cached table is made anew
+    check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), want, "eager after the captures")
+    for k in range(3):
+        for g, out in graphs:
+            out.zero_()
+            g.replay()
+            kept.append(torch.full((c.cos.shape[0], 32), 0x7FC07FC0, dtype=torch.int32, device=c.dev))
+            torch.cuda.synchronize()
+            check(out, want, f"replay {k}")
+
+
+def test_rope_table_of_another_stream(hip):
+    """The table is made on one stream behind other work and used on a second at once."""
+    c = ref.Cache(hip, [700, 1400], [4, 3], seed=32)
+    want, cos = c.want(hip), torch.zeros_like(c.cos)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        x = torch.randn(4096, 4096, device=c.dev)
+        for _ in range(20):
+            x = x @ x * 1e-2
+        cos.copy_(c.cos)
+        hip.rope_pairs(cos, c.sin)
+        ready = torch.cuda.Event()
+        ready.record()
+    with torch.cuda.stream(b):
+        got = hip.decode_chunk(c.P, c.q, c.qsl, cos, c.sin)
+    torch.cuda.synchronize()
+    check(got, want, "a table of another stream")
+
+
+def test_offsets_past_32_bits(hip):
+    """Pages and sub-blocks that lie behind the first 2^32 bytes and 2^31 elements of their pools."""
+    c = ref.Cache(hip, [700, 1100], [4, 6], ebs=64, seed=33)
+    want = c.want(hip)
+    old, far = c.P.epool, (1 << 31) + 8 * 1024
+    big = torch.empty(far + old.numel(), dtype=torch.bfloat16, device=c.dev)
+    big[far:] = old.flatten()
+    c.P.epool, c.P.eoff = big, c.P.eoff + far
+    oldq, farq = c.P.qpool, (1 << 32) + 51200
+    bigq = torch.empty(farq + oldq.numel(), dtype=torch.uint8, device=c.dev)
+    bigq[farq:] = oldq.flatten()
+    c.P.qpool, c.P.boff = bigq, torch.where(c.P.boff < (1 << 50), c.P.boff + farq, c.P.boff)
+    check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), want, "far offsets")
+    w = ref.Cache(hip, [700, 1100], [4, 6], ebs=64, win=256, seed=33)
+    want = w.want(hip)
+    big[far:far + w.P.epool.numel()] = w.P.epool.flatten()
+    w.P.epool, w.P.eoff = big, w.P.eoff + far
+    check(hip.decode_chunk(w.P, w.q, w.qsl, w.cos, w.sin), want, "far offsets of a window")
+
+
+def test_sinks_outside_their_buffers(hip):
+    c = ref.Cache(hip, [700, 400], [4, 6], win=256, sinks=True, seed=34)
+    c.P.skoff = c.P.skoff.clone()
+    c.P.skoff[1] = c.P.sk.numel() - 3 * 512
+    got = hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+    check(got[:4], c.want(hip)[:4], "sinks in place")
+    c.P.skoff[1] = -1
+    check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), c.want(hip, lambda r, p: (p < 4) & (r == 1)), "sinks outside")
+
+
 def test_attention_of_nothing(hip):
     c = ref.Cache(hip, [300, 10], [2, 3], seed=14)
     empty = hip.decode_chunk(c.P, c.q[:0], torch.zeros(3, dtype=torch.int64, device=c.dev), c.cos, c.sin)
@@ -489,3 +565,34 @@ def test_verify_strides_graph_and_refusals(hip):
             so.verify_drafts(*[bad if k == i else t for k, t in enumerate(ok)])
     with pytest.raises(ValueError):
         so.verify_drafts(*ok, q.cuda()[:, :50])
+
+
+def test_step_operators_on_another_stream(hip):
+    """Tables, conv and verification on a stream of their own, from inputs that it made."""
+    from lfm3_kv800_amd import spec_ops as so
+    st = torch.cuda.Stream()
+    g = torch.Generator().manual_seed(41)
+    lens, ql = [70, 5, 300], [3, 0, 5]
+    bcx, w = torch.randn(8, 3 * 64, generator=g).to(torch.bfloat16), torch.randn(64, 7, generator=g).to(torch.bfloat16)
+    state, logits = torch.randn(3, 64, 6, generator=g).to(torch.bfloat16), torch.randn(8, 777, generator=g).to(torch.bfloat16)
+    tok, u, un = torch.randint(0, 777, (8,), generator=g), torch.rand(8, generator=g), torch.rand(3, generator=g)
+    temp = torch.tensor([1.0, 0.0, 0.7])
+    kept = torch.tensor([2, 0, 5], dtype=torch.int32)
+
+    def run():
+        d = "cuda"
+        bt = torch.arange(3 * 20, dtype=torch.int32, device=d).view(3, 20)
+        m = hip.chunk_meta(bt, torch.tensor(lens, device=d), torch.tensor(ql, dtype=torch.int32, device=d), 16, 8)
+        s = state.to(d)
+        out, taps = so.conv_chunk(bcx.to(d), w.to(d), s, m.qsl)
+        so.conv_commit(s, taps, m.qsl, kept.to(d))
+        ids, n = so.verify_drafts(logits.to(d), tok.to(d), m.qsl, temp.to(d), u.to(d), un.to(d))
+        return m.qsl, m.slot, m.pos, out, s, ids, n
+    here = run()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        there = run()
+    st.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(here, there))
+    want = ref.verify(logits, tok, here[0].tolist(), temp, u, un)
+    assert there[5].tolist() == want[0] and there[6].tolist() == want[1]

@@ -200,3 +200,17 @@ def test_chunk_step_refusals(hip):
         M.speculative_loop(model, attn, torch.tensor([1, 2], device=DEV), 1, None, 128)
     rows, counts = M.speculative_loop(model, attn, torch.tensor([1, 2], device=DEV), 0, None, 3)
     assert [len(t) for t in rows] == [0, 0] and counts.shape == (0, 2)
+
+
+def test_speculative_loop_without_drafts(hip):
+    """most = 0, with and without (empty) distributions: the one-token loop. Draft counts past `most` count as `most`."""
+    from lfm3_kv800_amd import model as M
+    first = torch.tensor([1, 2], device=DEV)
+    empty = torch.zeros(2, 0, dtype=torch.int64, device=DEV)
+    runs = []
+    for probs in (None, torch.zeros(2, 0, 8192, device=DEV)):
+        model, attn = build([300, 20], 8)
+        rows, counts = M.speculative_loop(model, attn, first, 4, lambda last, lens: (empty, torch.full((2,), 7, device=DEV), probs), 0)
+        assert counts.tolist() == [[1, 1]] * 4 and attn.lens.tolist() == [304, 24]
+        runs.append(torch.stack(rows).tolist())
+    assert runs[0] == runs[1]
