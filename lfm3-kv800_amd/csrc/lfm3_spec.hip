@@ -202,26 +202,17 @@ __device__ __forceinline__ double wave_sumd(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// exp((x - m) / temp) for x <= m, within 2^-42: y = (x - m) / temp = (16 e + j) ln2 / 16 + r, |r| <= ln2 / 32, from two fused
-// multiply-adds of x; 16 e + j is the low word of 16 y / ln2 + 1.5 2^52; 2^(j / 16) from a table of 16 in LDS (32 banks: any
-// lanes at once), exp(r) as its series to r^5 / 120 (the next term is 1.4e-13). What lies 800 temp below m, -inf among it,
-// is 2^-1154 and comes out as 0 (temp up to 1e30).
+// exp((x - m) / temp) for x <= m, within 2^-42: y = (x - m) / temp with the difference exact, so that a small temperature does
+// not enlarge its rounding, = (16 e + j) ln2 / 16 + r, |r| <= ln2 / 32; 16 e + j is the low word of 16 y / ln2 + 1.5 2^52; 2^(j / 16)
+// from a table of 16 in LDS (32 banks: any lanes at once), exp(r) as its series to r^5 / 120 (the next term is 1.4e-13). What
+// lies 800 temp below m, -inf among it, is 2^-1154 and comes out as 0.
 __device__ const double POW16[16] = {1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
-struct Expo { double it, c, it16, c16; float low; };
-__device__ __forceinline__ Expo expo_of(float m, double it, float tp) {
-  Expo E;
-  E.it = it;
-  E.c = -(double)m * it;
-  E.it16 = it * 23.083120654223414;                    // 16 / ln2
-  E.c16 = E.c * 23.083120654223414;
-  E.low = fmaxf(m - 800.f * tp, -3.4e38f);
-  return E;
-}
+struct Expo { double m, it; };
 __device__ __forceinline__ double expo(float x, const Expo& E, const double* pow16) {
   const double magic = 6755399441055744.0;             // 1.5 2^52
-  const double v = (double)kv800::vmax(x, E.low);
-  const double zz = fma(v, E.it16, E.c16) + magic;
-  const double r = fma(zz - magic, -0.043321698784996581, fma(v, E.it, E.c));   // ln2 / 16
+  const double y = __builtin_elementwise_max(((double)x - E.m) * E.it, -800.0);
+  const double zz = fma(y, 23.083120654223414, magic);   // 16 / ln2
+  const double r = fma(zz - magic, -0.043321698784996581, y);   // ln2 / 16
   const int k = (int)(uint32_t)__double_as_longlong(zz);
   double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
   p = fma(r, p, 1.0 / 6.0);
@@ -331,7 +322,7 @@ __global__ void __launch_bounds__(VT) verify_stats_kernel(VerifyArgs A) {
     if (ranks_before(rm[k], ri[k], bm, bi)) { bm = rm[k]; bi = ri[k]; }
   double s = 0.0;
   if (sampled(tp, bm)) {
-    const Expo E = expo_of(bm, 1.0 / (double)tp, tp);
+    const Expo E = {(double)bm, 1.0 / (double)tp};
 #pragma unroll
     for (int k = 0; k < VE / 8; ++k)
 #pragma unroll
@@ -350,7 +341,6 @@ struct Verdict {
   int at;              // where it is,
   double s;            // sum of exp((x - m) / temp)
   double it;           // 1 / temp
-  float tp;            // temp
   bool sample, full;   // sampled; all drafts kept
 };
 struct VerdictLds { long long stop; double pow16[16], s; float m; int at; };
@@ -359,7 +349,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
   Verdict d;
   d.s0 = min(A.qsl[r], A.T);
   d.s1 = min(A.qsl[r + 1], A.T);
-  const float tp = d.tp = A.temp[r];
+  const float tp = A.temp[r];
   d.it = 1.0 / (double)tp;
   if (tid < 16) L.pow16[tid] = POW16[tid];
   if (tid == 0) L.stop = d.s1 - 1;
@@ -382,7 +372,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
     if (sampled(tp, M))
       for (int64_t p = lane; p < A.pieces; p += 64) {
         const Stat a = A.st[t * A.pieces + p];
-        S += a.s * expo(a.m, expo_of(M, d.it, tp), L.pow16);
+        S += a.s * expo(a.m, Expo{(double)M, d.it}, L.pow16);
       }
     S = wave_sumd(S);
   };
@@ -395,7 +385,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
     const float xk = in ? bf2f(A.logits[t * A.ld + k]) : -INFINITY, ut = A.u[t];
     const double qk = A.q ? (in ? (double)A.q[t * A.ldq + k] : 0.0) : 1.0;
     combine(t, M, at, S);
-    const bool keep = sampled(tp, M) ? in && (double)ut * qk < expo(xk, expo_of(M, d.it, tp), L.pow16) / S : k == at;
+    const bool keep = sampled(tp, M) ? in && (double)ut * qk < expo(xk, Expo{(double)M, d.it}, L.pow16) / S : k == at;
     if (!keep) {
       if (lane == 0) atomicMin(&L.stop, (long long)t);
       break;
@@ -429,7 +419,7 @@ __device__ __forceinline__ void piece_weights(const VerifyArgs& A, const Verdict
   load_piece<VE>(A.logits + d.t * A.ld + v0, n, -INFINITY, x);
   if (mode == 2) load_piece<VE>(A.q + d.t * A.ldq + v0, n, 0.f, q);
   const double inv = 1.0 / d.s;
-  const Expo E = expo_of(d.m, d.it, d.tp);
+  const Expo E = {(double)d.m, d.it};
 #pragma unroll
   for (int k = 0; k < VE / 8; ++k)
 #pragma unroll
@@ -515,7 +505,7 @@ __global__ void __launch_bounds__(VT) verify_pick_kernel(VerifyArgs A) {
           if (mode == 2) return A.left[r * A.pieces + p];
           if (mode == 1 && p == sp) return own;
           const Stat a = A.st[d.t * A.pieces + p];
-          return a.s * expo(a.m, expo_of(d.m, d.it, d.tp), L.pow16);
+          return a.s * expo(a.m, Expo{(double)d.m, d.it}, L.pow16);
         };
         double W = 0.0;
         for (int64_t p0 = 0; p0 < A.pieces; p0 += 64) W += wave_sumd(weight(p0 + lane));

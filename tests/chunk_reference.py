@@ -165,7 +165,7 @@ def verify(logits, tokens, qsl, temp, u, u_next, q=None):
             top = int(nan[0]) if len(nan) else int((row == row.max()).nonzero()[0])
             tp, ok = float(temp[r]), not len(nan) and math.isfinite(float(row.max()))
             n += 1
-            if not (0 < tp <= 1e30) or not ok:
+            if not (0 < tp <= float(torch.tensor(1e30))) or not ok:     # the fp32 number nearest 1e30
                 keep, nxt = not last and d == top, top
             else:
                 e = torch.exp((row - row.max()) / tp)

@@ -515,6 +515,20 @@ def test_verify_borders(hip):
     assert run_verify(x, tokens, qsl, temp, u, un, q) == ref.verify(x, tokens, qsl, temp, u, un, q)
 
 
+@pytest.mark.parametrize("V", [700, 9000])
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_extreme_temperatures(hip, V, probs):
+    """Down to the smallest numbers a row goes by its largest logits (several equal ones share), up to 1e30 all count alike."""
+    temps = (1e-3, 1e-8, 1e-12, 1e-16, 1e-25, 1e-30, 1e-45, 1e3, 1e20, 1e30)
+    x, tokens, qsl, temp, u, un, q = verify_case([4] * 40, V, 12, probs, temps)
+    x[::2, 5::V // 3] = x.max(-1, keepdim=True).values[::2]
+    x[1::4, 9] = -torch.finfo(torch.bfloat16).max
+    near = torch.randint(0, 3, (160,), generator=torch.Generator().manual_seed(5)) * (V // 3) + 5
+    tokens = torch.where(torch.rand(160, generator=torch.Generator().manual_seed(6)) < 0.4, near, tokens)
+    case = (x, tokens, qsl, temp, u, un, q)
+    assert run_verify(*case) == ref.verify(*case)
+
+
 def test_verify_infinities_and_nan(hip):
     """Masked tokens (-inf, the lowest bf16) are never taken; a row whose largest logit is not finite goes by its index."""
     x, tokens, qsl, temp, u, un, q = verify_case([5] * 8, 9000, 4, True, (1.0, 0.7))
