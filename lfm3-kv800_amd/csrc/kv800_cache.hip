@@ -98,7 +98,8 @@ step_meta_kernel(const int32_t* __restrict__ bt, int64_t bt_stride, int64_t npag
 // gridDim.y-th piece of 256. It sums the earlier rows' counts itself (12 bytes a row, from the L2) and scans its own in
 // LDS; a token finds its row by 8 steps of a binary search there. Fresh table entries are read from the free list, not
 // from the table, so the order in which workgroups write the table does not matter.
-// Bound: launch and two dependent rounds of loads. 398 rows x 8 tokens: CHUNK_META_TIME.
+// Bound: launch and two dependent rounds of loads. 1 row: 3.4 us; 398 rows x 8 tokens
+// with growth: 6.4 us (59 KB).
 struct MetaArgs {
   int32_t* bt;
   int64_t bt_stride, npages;

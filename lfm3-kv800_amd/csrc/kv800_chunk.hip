@@ -12,11 +12,18 @@
 // unpacked and rotated once for all of a tile's queries. Tile k of row r has the number r + qsl[r] / QT + k (ascending over
 // the rows without a scan; at most R + T / QT numbers, of which some stay without a tile).
 //
-//   chunk_quant_kernel   the sub-blocks, one workgroup of 4 waves per equal share of the (tile, sub-block) list, wave = KV
+//   quant_part           the sub-blocks, one workgroup of 4 waves per equal share of the list of (tile, 64 tokens), wave = KV
 //                        head; writes a partial (m, l, acc) per tile that it enters
-//   chunk_exact_kernel   exact rows and sinks, one workgroup per (tile, KV head); writes a partial, or for layers without
+//   exact_part           exact rows and sinks, one workgroup per (tile, KV head); writes a partial, or for layers without
 //                        sub-blocks the output
+//   chunk_both_kernel    the two in one launch; chunk_quant_kernel, chunk_exact_kernel: in a launch each
 //   chunk_merge_kernel   partials of a (tile, KV head) joined, Hadamard transform of the quantized part, bf16 output
+//
+// What bounds it (rates of a large copy 5.1 TB/s, of a large read 6.0 TB/s): long lists of tiles of 4 take 2.2 times the
+// time of their bytes (64 rows x 32768 x 4 tokens, 451 MB: 168 us of quant_part), VALU instructions in 68 % of the cycles, which are
+// table lookups and rotation of the keys; each column's share of them falls with the tile, so that tiles of 8 take 1.5
+// times as long for twice the queries. Window layers read at 4.1 TB/s (398 rows x 5 tokens, 223 MB: 54 us). One row takes
+// 17 + 8 us for 5 tokens at 16384 positions: the latency of four dependent loads, of the lookups and of a second launch.
 #include <mutex>
 
 #include "kv800_attn.h"
@@ -132,7 +139,7 @@ __device__ __forceinline__ void lut_build(uint32_t* lut, int lane, const QLutWor
 // Wave w's part of a stage, straight into LDS: tokens 8 w .. + 7 of kc and cs, and (waves 0, 1) tokens 16 w .. + 15 of vb. Lane l
 // writes bytes 16 l .. + 15 of the wave's kilobyte and fetches the piece that belongs there, so that a load reads whole
 // lines: rows fetched straight into the operand layout (lane = token, 128 bytes apart) cost the L1 one line per lane, 460
-// per chunk and head, and held it busy 86 % of the time (64 rows x 32K x 4: 242 us; staged STAGED_US us).
+// per chunk and head, and held it busy 86 % of the time (64 rows x 32768 x 4: 242 us; staged 174 us).
 __device__ __forceinline__ void stage_load(ChunkStage& S, rsrc_t rs, rsrc_t rc, int cpos, int t0, int w, int lane) {
   typedef __attribute__((address_space(3))) void lds_v;
   const int o = (lane >> 3) * 128 + 16 * ((lane & 7) ^ (lane >> 3));
@@ -395,7 +402,9 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
   }
 }
 
-// Workgroup w takes entries [w C, (w + 1) C) of the list, C = ceil(total / G). The part of a tile that it begins with goes
+// Workgroup w takes entries [w C, (w + 1) C) of the list, C = ceil(total / G): equal shares, whatever the rows' lengths. Two
+// stages of loads, one ahead: three, two ahead, took 186 us against 167 (64 rows x 32768 x 4), their barriers and addresses
+// costing more than the waits that they saved. The part of a tile that it begins with goes
 // to slot w; a tile that starts inside its range goes to slot G + the tile's number (nobody else enters that tile from an
 // earlier entry).
 template <int QT>
@@ -500,7 +509,8 @@ __global__ void __launch_bounds__(256, 3) chunk_quant_kernel(ChunkArgs A) {
 // token, every lane is a cache line of its own: 1,280 line requests per chunk, and 398 rows of a window layer took
 // 80 us), in pieces of 16 bytes permuted within the row so that operand reads spread over the banks. One buffer for each: the
 // next chunk's K is requested when this one's scores are formed, its V when this one's V is read, so that each is
-// in flight for about half a chunk, and 17 KB a wave leave room for nine waves on a CU.
+// in flight for about half a chunk, and 16 KB a wave leave room for the eight waves that 256 registers allow on a CU.
+// Window layers, 398 rows x 5: 54 us (223 MB); sliding 64 x 16: 22 us, the latency of five chunks in a row.
 constexpr int XCH = 32;
 template <int NW>
 struct alignas(16) ChunkXRows { uint16_t r[NW][XCH * 128]; };
@@ -884,7 +894,9 @@ __global__ void __launch_bounds__(64 * NW, 2) chunk_exact_kernel(ChunkArgs A) {
   }
   exact_part<CT, NW, DIRECT>(Ks, Vs, L, A, blockIdx.x);
 }
-// Both in one launch, for few tiles: three of four waves per (tile, KV head), then the quantized list's workgroups.
+// Both in one launch: three of four waves per (tile, KV head), whose LDS (48 KB) lets two workgroups stay on a CU beside the tables,
+// then the quantized list's workgroups. The other order takes 20 us instead of 17 for 1 row x 5 at 16384, where the exact part
+// is the longer chain, and 44 instead of 47 for 16 x 4096 x 33.
 constexpr int BNW = 3;
 union ChunkBoth { ChunkStage s; ChunkXRows<BNW> x; };
 template <int CT>
@@ -901,7 +913,7 @@ __global__ void __launch_bounds__(256, 2) chunk_both_kernel(ChunkArgs A) {
 
 // ---------------------------------------------------------------- merge
 // WPC waves per (token, query head), the four heads of a KV head (WPC = 1) or one head (4) per workgroup: 4 where there are
-// few tokens, whose partials are many. Lanes take the partials' m and l side by side (64 at a time), then the wave adds up
+// few tokens, whose partials are many (1 x 16384 x 5, 256 partials each: 8 us against 21; 64 rows x 32768 x 4, twelve each: 13 us against 9). Lanes take the partials' m and l side by side (64 at a time), then the wave adds up
 // the partials' accumulators, lane = dims 2 lane, 2 lane + 1, eight loads in flight.
 template <int CT, int WPC>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
@@ -992,8 +1004,10 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
   *dst = bfpk((x0 * hn + fx * ax.x) * inv, (x1 * hn + fx * ax.y) * inv);
 }
 
-// Queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8
-// (layers without sub-blocks: while every row can bring one token only; their kernel passes over an empty second half).
+// Queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8, whose keys are unpacked once
+// for twice the queries (64 rows x 32768 x 4, its parts and merge together: 263 us in tiles of 8, half of them empty, 195 in tiles of 4).
+// Layers without sub-blocks: 4 only while every row brings one token; their kernel passes over an empty second half
+// (window, 398 rows x 5: 66 us in tiles of 4, 54 in tiles of 8).
 int chunk_ct(int64_t R, int64_t T, bool quant) { return T <= (quant ? 4 * R : R) ? 1 : 2; }
 
 int64_t chunk_cus() {
@@ -1033,12 +1047,14 @@ int chunk_exact(const ChunkArgs& A, hipStream_t s) {
   hipLaunchKernelGGL((chunk_exact_kernel<CT, NW, DIRECT>), dim3((unsigned)(4 * A.I + DIRECT)), dim3(64 * NW), 0, s, A);
   return check_launch("chunk_exact");
 }
-// waves per (tile, KV head): as many as are resident at once, by the rows' (tile, head) pairs (66, 33 and 16 KB of LDS)
+// Waves per (tile, KV head): as many as are resident at once (66, 33 and 16 KB of LDS), by the workgroups, of which those
+// without a tile leave soon. In us with 4 / 2 / 1 waves, window layers: 64 rows x 5 tokens (416 workgroups) 16.8 / 19.2 / 23.5,
+// 64 x 16 (768) 29.1 / 21.8 / 25.1, 128 x 1 (640) 18.4 / 15.8 / 16.6, 256 x 5 (1,664) 43.5 / 38.8 / 32.0.
 template <int CT, bool DIRECT>
 int chunk_exact_all(const ChunkArgs& A, hipStream_t s) {
-  const int64_t cu = chunk_cus(), pairs = 4 * max(A.R, A.T / (4 * CT));
-  return pairs <= 2 * cu ? chunk_exact<CT, 4, DIRECT>(A, s)
-                         : pairs <= 4 * cu ? chunk_exact<CT, 2, DIRECT>(A, s) : chunk_exact<CT, 1, DIRECT>(A, s);
+  const int64_t cu = chunk_cus(), wgs = 4 * A.I;
+  return wgs <= 2 * cu ? chunk_exact<CT, 4, DIRECT>(A, s)
+                       : wgs <= 4 * cu ? chunk_exact<CT, 2, DIRECT>(A, s) : chunk_exact<CT, 1, DIRECT>(A, s);
 }
 template <int CT>
 int chunk_launch(const ChunkArgs& A, bool quant, bool both, hipStream_t s) {
