@@ -4,7 +4,8 @@ Modules: kv800 (the reference's cache / quantizer / decode API, kv800.py, with t
 binding of the C-ABI library libkv800_hip.so built from csrc/ by build.py), vllm_cache (the vLLM attention backend's
 per-step cache work on the device: new-token rows, sinks, flush, decode tables, decode and prefill rows of a mixed
 batch), train (patch_for_training's fake quantization on the GPU), model / model_ops (an LFM3-shaped engine loop that
-drives every attention layer through the above).
+drives every attention layer through the above), spec_ops (model-side operators of steps with drafted tokens: short conv,
+verification).
 Kept free of torch imports, like the reference package (lfm3_kv800/__init__.py:1-6)."""
 import logging
 

@@ -19,9 +19,9 @@
 //   chunk_both_kernel    the two in one launch; chunk_quant_kernel, chunk_exact_kernel: in a launch each
 //   chunk_merge_kernel   partials of a (tile, KV head) joined, Hadamard transform of the quantized part, bf16 output
 //
-// What bounds it (rates of a large copy 5.1 TB/s, of a large read 6.0 TB/s): long lists of tiles of 4 take 2.2 times the
+// What bounds it (rates of a large copy 5.1 TB/s, of a large read 6.0 TB/s): long lists of tiles of 4 take about twice the
 // time of their bytes (64 rows x 32768 x 4 tokens, 451 MB: 168 us of quant_part), VALU instructions in 68 % of the cycles, which are
-// table lookups and rotation of the keys; each column's share of them falls with the tile, so that tiles of 8 take 1.5
+// table lookups and rotation of the keys; each column's share of them falls with the tile, so that tiles of 8 take 1.4
 // times as long for twice the queries. Window layers read at 4.1 TB/s (398 rows x 5 tokens, 223 MB: 54 us). One row takes
 // 17 + 8 us for 5 tokens at 16384 positions: the latency of four dependent loads, of the lookups and of a second launch.
 #include <mutex>
