@@ -23,7 +23,7 @@
 // time of their bytes (64 rows x 32768 x 4 tokens, 451 MB: 168 us of quant_part), VALU instructions in 68 % of the cycles, which are
 // table lookups and rotation of the keys; each column's share of them falls with the tile, so that tiles of 8 take 1.4
 // times as long for twice the queries. Window layers read at 4.1 TB/s (398 rows x 5 tokens, 223 MB: 54 us). One row takes
-// 17 + 8 us for 5 tokens at 16384 positions: the latency of four dependent loads, of the lookups and of a second launch.
+// 17 + 7 us for 5 tokens at 16384 positions: the latency of four dependent loads, of the lookups and of a second launch.
 #include <mutex>
 
 #include "kv800_attn.h"
@@ -912,15 +912,16 @@ __global__ void __launch_bounds__(256, 2) chunk_both_kernel(ChunkArgs A) {
 }
 
 // ---------------------------------------------------------------- merge
-// WPC waves per (token, query head), the four heads of a KV head (WPC = 1) or one head (4) per workgroup: 4 where there are
-// few tokens, whose partials are many (1 x 16384 x 5, 256 partials each: 8 us against 21; 64 rows x 32768 x 4, twelve each: 13 us against 9). Lanes take the partials' m and l side by side (64 at a time), then the wave adds up
-// the partials' accumulators, lane = dims 2 lane, 2 lane + 1, eight loads in flight.
+// WPC waves per (token, query head), the four heads of a KV head (WPC = 1) or one head (8) per workgroup: 8 for few tokens,
+// whose partials are many (the whole call with 8 / 1: 1 x 16384 x 5 tokens 23.2 / 37.9 us, 8 x 16384 x 4 36.8 / 38.2, 8 x 16384 x 8
+// 48.8 / 48.0, 16 x 1024 x 8 29.5 / 25.4). Lanes take the partials' m and l side by side, then the wave adds up the partials'
+// accumulators, lane = dims 2 lane, 2 lane + 1, eight loads in flight.
 template <int CT, int WPC>
-__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
+__global__ void __launch_bounds__(WPC == 1 ? 256 : 64 * WPC) chunk_merge_kernel(ChunkArgs A) {
   constexpr int QT = 4 * CT, NC = 16 * CT;
-  __shared__ float jm[4], jl[4], jx[4][128];
+  __shared__ float jm[WPC], jl[WPC], jx[WPC][128];
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, dd = 2 * lane;
-  const int64_t tok = blockIdx.x / (4 * WPC);
+  const int64_t tok = blockIdx.x / (WPC == 1 ? 4 : 16);
   const int q = WPC == 1 ? 4 * (int)(blockIdx.x & 3) + w : (int)(blockIdx.x & 15), h = q >> 2;
   const int part = WPC == 1 ? 0 : w;                   // this wave's share of the partials
   uint32_t* dst = reinterpret_cast<uint32_t*>(A.out + (tok * 16 + q) * 128 + dd);
@@ -941,8 +942,10 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
   const float mx = A.mo[cx], lx = A.lo[cx];
   const float2 ax = *reinterpret_cast<const float2*>(A.ao + cx * 128 + dd);
   float M = mx, l = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int k0 = 64 * part; k0 < n; k0 += 64 * WPC) {
-    const bool in = k0 + lane < n;
+  const int share = WPC == 1 ? 64 : min(64, max(8, (n + WPC - 1) / WPC));   // partials of a wave at a time
+  for (int k0 = share * part; k0 < n; k0 += share * WPC) {
+    const int kn = min(share, n - k0);
+    const bool in = lane < kn;
     const int64_t p = slot(in ? k0 + lane : 0);
     const float mk = in ? A.mo[p] : NEG_BIG, lk = in ? A.lo[p] : 0.f;
     float m2 = mk;
@@ -954,7 +957,6 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs A) {
     l = l * al + f * lk;                               // the lane's own share; M starts at the exact part's m
     x0 *= al;
     x1 *= al;
-    const int kn = min(64, n - k0);
     for (int k = 0; k < kn; k += 8) {
       float2 a[8];
 #pragma unroll
@@ -1069,8 +1071,8 @@ int chunk_launch(const ChunkArgs& A, bool quant, bool both, hipStream_t s) {
     if (rc == KV800_OK) rc = chunk_exact_all<1, false>(A, s);
   }
   if (rc != KV800_OK) return rc;
-  if (16 * A.T <= 4 * chunk_cus())
-    hipLaunchKernelGGL((chunk_merge_kernel<CT, 4>), dim3((unsigned)(16 * A.T)), dim3(256), 0, s, A);
+  if (8 * A.T <= chunk_cus())
+    hipLaunchKernelGGL((chunk_merge_kernel<CT, 8>), dim3((unsigned)(16 * A.T)), dim3(64 * 8), 0, s, A);
   else
     hipLaunchKernelGGL((chunk_merge_kernel<CT, 1>), dim3((unsigned)(4 * A.T)), dim3(256), 0, s, A);
   return check_launch("chunk_merge");

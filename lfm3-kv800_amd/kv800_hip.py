@@ -897,6 +897,8 @@ def decode_chunk(P, q, qsl, cos_t, sin_t):
     s, qbytes, eelems, selems = paged_struct(P, R)
     if P.eoff.shape[0] < R or (s.nqmax and P.boff.shape[0] < R) or (s.sk and min(P.skoff.shape[0], P.svoff.shape[0]) < R):
         raise ValueError("eoff, boff, skoff and svoff must cover the rows")
+    if R > 1 and any(t.stride(0) != 1 for t in ((P.N, P.NQ, P.skoff, P.svoff) if s.sk else (P.N, P.NQ))):
+        raise ValueError("N, NQ, skoff and svoff must be contiguous")
     if s.nqmax and not rot:
         raise ValueError("quantized layers need the rope tables")
     q, qsl = q.contiguous(), qsl.contiguous()

@@ -293,6 +293,20 @@ def test_sinks_outside_their_buffers(hip):
     check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), c.want(hip, lambda r, p: (p < 4) & (r == 1)), "sinks outside")
 
 
+def test_strided_lengths_are_refused(hip):
+    c = ref.Cache(hip, [700, 90], [3, 4], seed=35)
+    for name in ("N", "NQ"):
+        keep = getattr(c.P, name)
+        setattr(c.P, name, torch.stack([keep, keep], 1)[:, 0])
+        with pytest.raises(ValueError):
+            hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+        setattr(c.P, name, keep)
+    w = ref.Cache(hip, [700, 90], [3, 4], win=256, sinks=True, seed=35)
+    w.P.svoff = torch.stack([w.P.svoff, w.P.svoff], 1)[:, 0]
+    with pytest.raises(ValueError):
+        hip.decode_chunk(w.P, w.q, w.qsl, w.cos, w.sin)
+
+
 def test_attention_of_nothing(hip):
     c = ref.Cache(hip, [300, 10], [2, 3], seed=14)
     empty = hip.decode_chunk(c.P, c.q[:0], torch.zeros(3, dtype=torch.int64, device=c.dev), c.cos, c.sin)
