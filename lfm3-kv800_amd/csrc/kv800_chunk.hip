@@ -166,9 +166,9 @@ __device__ __forceinline__ int row_blocks(const ChunkArgs& A, int64_t r) {
 // Attention of one tile's columns of KV head h (the wave's) over tokens [64 u0, 64 u1) of its row, into partial slot `slot`.
 // As in decode_quant_kernel, with the wave's one head: K pairs by table lookup, RoPE by v_dot2_f32_bf16, Q K^T on bf16 MFMA
 // with exact products; fp32 online softmax; P V on fp16 MFMA over the bit planes, weights fp16(p vsc): 11 bits, an eighth of the output's own rounding.
-template <int CT>
+// NC: columns of a slot, of which the tile has 16 CT at most.
+template <int CT, int NC>
 __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkStage& SB, const ChunkArgs& A, const Tile& t, int u0, int u1, int64_t slot) {
-  constexpr int NC = 16 * CT;
   const int h = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
   const char* lutc = reinterpret_cast<const char*>(&L.lut[0][0]);
@@ -425,8 +425,8 @@ template <int CT>
 __device__ __forceinline__ void quant_part(ChunkQLds& L, ChunkStage& SA, ChunkStage& SB, const ChunkArgs& A, const unsigned wg) {
   constexpr int QT = 4 * CT;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-  // every workgroup sums the rows' entries itself: thread i takes the rows [i k, i k + k). The list has less than 2^31
-  // entries (the host's check).
+  // every workgroup sums the rows' entries itself: thread i takes the rows [i k, i k + k). The list's entries, and a
+  // workgroup's end past them, are below 2^31 (the host's check).
   const int R = (int)A.R, k = (R + 255) / 256, ra = min(tid * k, R), rb = min(ra + k, R);
   ListRow first = {0, 0, 0, 0};
   int mine = 0;
@@ -484,7 +484,13 @@ __device__ __forceinline__ void quant_part(ChunkQLds& L, ChunkStage& SA, ChunkSt
       t.c = c;
       t.q0 = tile * QT;
       t.nq = min(QT, c - t.q0);
-      chunk_span<CT>(L, SA, SB, A, t, u0, u1, head ? (int64_t)wg : A.G + r + (unsigned)t.t0 / QT + tile);
+      const int64_t slot = head ? (int64_t)wg : A.G + r + (unsigned)t.t0 / QT + tile;
+      // a tile of up to 4 queries in one column tile (192 rows with 1 to 8: 238 against 254 us, both with the exact part; shares
+      // weighted by the tiles' queries gave nothing more)
+      if (CT == 1 || t.nq > 4)
+        chunk_span<CT, 16 * CT>(L, SA, SB, A, t, u0, u1, slot);
+      else
+        chunk_span<1, 16 * CT>(L, SA, SB, A, t, u0, u1, slot);
       head = false;
       v += u1 - u0;
     }
@@ -1118,7 +1124,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
                 "decode_chunk: sinks need sv, skoff, svoff and 16-byte aligned buffers");
   const ChunkPlan p = chunk_plan(R, T, quant ? P->nqmax : 0);
   KV800_REQUIRE(p.I <= (1LL << 28) && T <= (1LL << 28) && P->ebs < (1LL << 30), "decode_chunk: too many rows and tokens");
-  KV800_REQUIRE(!quant || p.I <= (int64_t)0x7FFFFFFF / 4 / P->nqmax, "decode_chunk: too many rows and sub-blocks");
+  KV800_REQUIRE(!quant || p.I <= (int64_t)0x7F000000 / 4 / P->nqmax, "decode_chunk: too many rows and sub-blocks");
   KV800_REQUIRE(!quant || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= kv800_hip_decode_chunk_workspace(R, T, P->nqmax)),
                 "decode_chunk: the workspace is too small or not 16-byte aligned");
   ChunkArgs A;
