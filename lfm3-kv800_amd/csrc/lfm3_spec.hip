@@ -183,14 +183,14 @@ conv_commit_kernel(uint16_t* __restrict__ state, const uint16_t* __restrict__ ta
 
 // ---------------------------------------------------------------- verification of drafts
 // A logits row is cut into pieces; verify_stats gives each piece's largest value m, its index and s = sum exp((x - m) / temp).
-// verify_residual (drafts with a distribution) and verify_pick derive from these which row of logits ends a batch row, each
+// verify_residual (drafts with a distribution), else verify_pick, derives from these which row of logits ends a batch row, each
 // workgroup for itself; the first sums max(p - q, 0) over its piece of that row, the second picks the piece in which the
 // running sum passes u W and scans it. So every row of logits is read once, the deciding one of each batch row (and its
 // q) once more, and one piece of it again.
 // All in 64 bits: the running sums of neighbours among 65,536 tokens lie 1e-5 apart where 32-bit exponentials are
 // 1e-7 off, and the choice has to be the same whatever way a row is cut. Bound: the logits' bytes and the exponentials'
 // instructions: about 30 per value, half of them of 64 bits, take longer than the bytes. 256 rows, 722 logits rows of 65,536 with
-// the drafts' distributions (162 MB): stats 42, residual 23, pick 15 us; one row of 5: 4, 0 and 10 us, chains of dependent
+// the drafts' distributions (162 MB): stats 42, residual 19, pick 12 us; one row of 5: 4, 0 and 10 us, chains of dependent
 // loads and of 64-bit sums over lanes.
 constexpr int VT = 256;                                // threads; a piece holds VT x VE values, VE = 8 or 32 a thread
 struct Stat { double s; float m; int32_t at; };        // 16 bytes
@@ -228,38 +228,37 @@ __device__ __forceinline__ double expo(float x, const Expo& E, const double* pow
   return ldexp(p * pow16[k & 15], k >> 4);
 }
 
-// A thread's values of a piece: in group k of VE / 8, the 8 from index 8 (256 k + tid) on. 16-byte loads where a whole aligned
-// group is there, else one by one; what lies past n is `fill`.
-template <int VE>
-__device__ __forceinline__ void load_piece(const uint16_t* p, int n, float fill, float (&x)[VE / 8][8]) {
-  const bool al = ((uintptr_t)p & 15) == 0;
+// Eight values from index i of a piece of n on: 16-byte loads where they are all there and aligned, else one by one; what
+// lies past n is `fill`.
+__device__ __forceinline__ void load_group(const uint16_t* p, int i, int n, float fill, float (&x)[8]) {
+  if (((uintptr_t)p & 15) == 0 && i + 8 <= n) load8(p + i, x);
+  else {
 #pragma unroll
-  for (int k = 0; k < VE / 8; ++k) {
-    const int i = 8 * (VT * k + (int)threadIdx.x);
-    if (al && i + 8 <= n) load8(p + i, x[k]);
-    else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[k][e] = i + e < n ? bf2f(p[i + e]) : fill;
-    }
+    for (int e = 0; e < 8; ++e) x[e] = i + e < n ? bf2f(p[i + e]) : fill;
   }
 }
-template <int VE>
-__device__ __forceinline__ void load_piece(const float* p, int n, float fill, float (&x)[VE / 8][8]) {
-  const bool al = ((uintptr_t)p & 15) == 0;
+__device__ __forceinline__ void load_group(const float* p, int i, int n, float fill, float (&x)[8]) {
+  if (((uintptr_t)p & 15) == 0 && i + 8 <= n) {
+    const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
 #pragma unroll
-  for (int k = 0; k < VE / 8; ++k) {
-    const int i = 8 * (VT * k + (int)threadIdx.x);
-    if (al && i + 8 <= n) {
-      const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
-      x[k][0] = a.x; x[k][1] = a.y; x[k][2] = a.z; x[k][3] = a.w;
-      x[k][4] = b.x; x[k][5] = b.y; x[k][6] = b.z; x[k][7] = b.w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[k][e] = i + e < n ? p[i + e] : fill;
-    }
+    for (int e = 0; e < 8; ++e) x[e] = i + e < n ? p[i + e] : fill;
   }
 }
+// a thread's group k of a piece: the 8 values from here on
+__device__ __forceinline__ int group_at(int k) { return 8 * (VT * k + (int)threadIdx.x); }
 
+// What a batch row comes to, the same in every thread of the workgroup.
+struct Verdict {
+  int64_t s0, s1, t;   // the row's tokens; the logits row that ends it
+  float m;             // that row's largest logit,
+  int at;              // where it is,
+  double s;            // sum of exp((x - m) / temp)
+  double it;           // 1 / temp
+  bool sample, full;   // sampled; all drafts kept
+};
 struct VerifyArgs {
   const uint16_t* logits;
   int64_t ld;
@@ -268,6 +267,7 @@ struct VerifyArgs {
   int64_t ldq, R, T, V, pieces;
   Stat* st;            // (T, pieces)
   double* left;        // (R, pieces): sums of max(p - q, 0) over the deciding rows' pieces
+  Verdict* verdicts;   // (R): of the rows with drafts, where these have a distribution
   int64_t* out;
   int32_t* count;
 };
@@ -282,7 +282,8 @@ __global__ void __launch_bounds__(VT) verify_stats_kernel(VerifyArgs A) {
   if (t >= min(A.qsl[A.R], A.T)) return;               // uniform
   const int n = (int)min((int64_t)(VT * VE), A.V - v0);
   float x[VE / 8][8];
-  load_piece<VE>(A.logits + t * A.ld + v0, n, -INFINITY, x);
+#pragma unroll
+  for (int k = 0; k < VE / 8; ++k) load_group(A.logits + t * A.ld + v0, group_at(k), n, -INFINITY, x[k]);
   if (tid < 16) pow16[tid] = POW16[tid];
   const float tp = A.temp[row_of(A.qsl, A.R, t)];
   // the piece's largest value first (NaN wins), then the first index that has it, by the threads whose own largest it is: about
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(VT) verify_stats_kernel(VerifyArgs A) {
     for (int k = VE / 8 - 1; k >= 0; --k)
 #pragma unroll
       for (int e = 7; e >= 0; --e) {
-        const int i = 8 * (VT * k + tid) + e;
+        const int i = group_at(k) + e;
         bi = (x[k][e] == bm || x[k][e] != x[k][e]) && i < n ? i : bi;
       }
     atomicMin(&at, bi);                                // the smallest index, whatever the order
@@ -324,15 +325,6 @@ __global__ void __launch_bounds__(VT) verify_stats_kernel(VerifyArgs A) {
   if (tid == 0) A.st[t * A.pieces + blockIdx.x] = Stat{(rs[0] + rs[1]) + (rs[2] + rs[3]), bm, (int32_t)(v0 + at)};
 }
 
-// What a batch row comes to, the same in every thread of the workgroup.
-struct Verdict {
-  int64_t s0, s1, t;   // the row's tokens; the logits row that ends it
-  float m;             // that row's largest logit,
-  int at;              // where it is,
-  double s;            // sum of exp((x - m) / temp)
-  double it;           // 1 / temp
-  bool sample, full;   // sampled; all drafts kept
-};
 struct VerdictLds { long long stop; double pow16[16], s; float m; int at; };
 __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, VerdictLds& L) {
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
@@ -399,41 +391,43 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
   return d;
 }
 
-// Weights of a piece of the deciding row: MODE 0: exp((x - m) / temp); 1: the same without token `skip`; 2: max(p - q, 0).
+// Weights of group k of a piece of the deciding row: mode 0: exp((x - m) / temp); 1: the same without token `skip`; 2:
+// max(p - q, 0).
 template <int VE>
-__device__ __forceinline__ void piece_weights(const VerifyArgs& A, const Verdict& d, const double* pow16, int64_t piece, int mode,
-                                              int64_t skip, double (&g)[VE / 8][8]) {
+__device__ __forceinline__ void group_weights(const VerifyArgs& A, const Verdict& d, const double* pow16, int64_t piece, int k, int mode,
+                                              int64_t skip, double (&g)[8]) {
   const int64_t v0 = piece * (VT * VE);
-  const int n = (int)min((int64_t)(VT * VE), A.V - v0);
-  float x[VE / 8][8], q[VE / 8][8];
-  load_piece<VE>(A.logits + d.t * A.ld + v0, n, -INFINITY, x);
-  if (mode == 2) load_piece<VE>(A.q + d.t * A.ldq + v0, n, 0.f, q);
+  const int n = (int)min((int64_t)(VT * VE), A.V - v0), i = group_at(k);
+  float x[8], q[8];
+  load_group(A.logits + d.t * A.ld + v0, i, n, -INFINITY, x);
+  if (mode == 2) load_group(A.q + d.t * A.ldq + v0, i, n, 0.f, q);
   const double inv = 1.0 / d.s;
   const Expo E = {(double)d.m, d.it};
 #pragma unroll
-  for (int k = 0; k < VE / 8; ++k)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      double y = expo(x[k][e], E, pow16);
-      if (mode == 1) y = v0 + 8 * (VT * k + (int)threadIdx.x) + e == skip ? 0.0 : y;
-      if (mode == 2) {
-        y = y * inv - (double)q[k][e];
-        y = y > 0.0 ? y : 0.0;                         // and for a q that is NaN
-      }
-      g[k][e] = y;
+  for (int e = 0; e < 8; ++e) {
+    double y = expo(x[e], E, pow16);
+    if (mode == 1) y = v0 + i + e == skip ? 0.0 : y;
+    if (mode == 2) {
+      y = y * inv - (double)q[e];
+      y = y > 0.0 ? y : 0.0;                           // and for a q that is NaN
     }
+    g[e] = y;
+  }
 }
 __device__ __forceinline__ double sum8(const double (&g)[8]) {
   return ((g[0] + g[1]) + (g[2] + g[3])) + ((g[4] + g[5]) + (g[6] + g[7]));
 }
-// the piece's sum, in the order in which pick_in_piece takes it apart; the same in every thread
-template <int VE>
-__device__ __forceinline__ double piece_sum(const double (&g)[VE / 8][8], double* seg) {
+// The sum of a piece's weights, in the order in which pick_kernel takes it apart; group(k, g) gives a thread's weights of
+// group k. The same in every thread.
+template <int VE, typename F>
+__device__ __forceinline__ double piece_sum(double* seg, F group) {
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   __syncthreads();                                     // seg's last readers are done
 #pragma unroll
   for (int k = 0; k < VE / 8; ++k) {
-    const double s = wave_sumd(sum8(g[k]));
+    double g[8];
+    group(k, g);
+    const double s = wave_sumd(sum8(g));
     if (lane == 0) seg[4 * k + w] = s;                 // 64 lanes x 8 values from index 512 (4 k + w) on
   }
   __syncthreads();
@@ -444,16 +438,15 @@ __device__ __forceinline__ double piece_sum(const double (&g)[VE / 8][8], double
 }
 
 template <int VE>
-__global__ void __launch_bounds__(VT) verify_residual_kernel(VerifyArgs A) {
+__global__ void __launch_bounds__(VT, 8) verify_residual_kernel(VerifyArgs A) {
   __shared__ VerdictLds L;
   __shared__ double seg[VE / 2];
   const int64_t r = blockIdx.y;
   if (min(A.qsl[r + 1], A.T) - min(A.qsl[r], A.T) < 2) return;   // no drafts
   const Verdict d = decide(A, r, L);
+  if (blockIdx.x == 0 && threadIdx.x == 0) A.verdicts[r] = d;    // for verify_pick
   if (!d.sample || d.full) return;
-  double g[VE / 8][8];
-  piece_weights<VE>(A, d, L.pow16, blockIdx.x, 2, -1, g);
-  const double s = piece_sum<VE>(g, seg);
+  const double s = piece_sum<VE>(seg, [&](int k, double (&g)[8]) { group_weights<VE>(A, d, L.pow16, blockIdx.x, k, 2, -1, g); });
   if (threadIdx.x == 0) A.left[r * A.pieces + blockIdx.x] = s;
 }
 
@@ -473,7 +466,14 @@ __global__ void __launch_bounds__(VT) verify_pick_kernel(VerifyArgs A) {
       return;
     }
   }
-  const Verdict d = decide(A, r, L);
+  Verdict d;
+  if (A.q && min(A.qsl[r + 1], A.T) - min(A.qsl[r], A.T) >= 2) {   // verify_residual has it
+    d = A.verdicts[r];
+    if (tid < 16) L.pow16[tid] = POW16[tid];
+    __syncthreads();
+  } else {
+    d = decide(A, r, L);
+  }
   int64_t pick = d.at;
   if (d.sample) {                                      // uniform, like all of the branches below
     const int64_t skip = d.full || A.q ? -1 : A.tokens[d.t + 1];
@@ -485,8 +485,11 @@ __global__ void __launch_bounds__(VT) verify_pick_kernel(VerifyArgs A) {
     double own = 0.0;
     for (bool picked = false;;) {
       if (look >= 0) {
-        piece_weights<VE>(A, d, L.pow16, look, mode, skip, g);
-        own = piece_sum<VE>(g, seg);
+        own = piece_sum<VE>(seg, [&](int k, double (&gk)[8]) {
+          group_weights<VE>(A, d, L.pow16, look, k, mode, skip, gk);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[k][e] = gk[e];
+        });
       }
       if (picked) break;
       if (w == 0) {                                    // the pieces' running sum passes u W in piece `piece`
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(VT) verify_pick_kernel(VerifyArgs A) {
 }
 
 // 2,048-value pieces while all rows in them make up to 1,024 workgroups, else 8,192, whose sums and lookups of a piece's row are
-// fewer (256 rows, stats, residual and pick: 81 us, in small pieces 94; one row of 5: 14 us, in large pieces 22)
+// fewer (256 rows, stats, residual and pick: 73 us, in small pieces 91; one row of 5: 14 us, in large pieces 22)
 int verify_ve(int64_t T, int64_t V) { return T * ((V + 8 * VT - 1) / (8 * VT)) <= 1024 ? 8 : 32; }
 int64_t verify_pieces(int64_t T, int64_t V) { const int64_t n = VT * verify_ve(T, V); return (V + n - 1) / n; }
 
@@ -658,7 +661,7 @@ int lfm3_hip_conv_commit(uint16_t* state, const uint16_t* taps, const int64_t* q
 
 int64_t lfm3_hip_verify_workspace(int64_t R, int64_t T, int64_t V) {
   if (R <= 0 || T <= 0 || V <= 0) return 0;
-  return lfm3::verify_pieces(T, V) * (T * (int64_t)sizeof(lfm3::Stat) + R * (int64_t)sizeof(double));
+  return lfm3::verify_pieces(T, V) * (T * (int64_t)sizeof(lfm3::Stat) + R * (int64_t)sizeof(double)) + R * (int64_t)sizeof(lfm3::Verdict);
 }
 
 int lfm3_hip_verify_drafts(const uint16_t* logits, int64_t ld, const int64_t* tokens, const int64_t* qsl, const float* temp,
@@ -671,8 +674,9 @@ int lfm3_hip_verify_drafts(const uint16_t* logits, int64_t ld, const int64_t* to
   KV800_REQUIRE(ws_bytes >= lfm3_hip_verify_workspace(R, T, V) && (T == 0 || (ws && (uintptr_t)ws % 16 == 0)),
                 "verify_drafts: the workspace is too small or not 16-byte aligned");
   lfm3::VerifyArgs A = {logits, ld, tokens, qsl, temp, u, u_next, draft_probs, ldq, R, T, V, lfm3::verify_pieces(T, V),
-                        reinterpret_cast<lfm3::Stat*>(ws), nullptr, out, count};
+                        reinterpret_cast<lfm3::Stat*>(ws), nullptr, nullptr, out, count};
   A.left = reinterpret_cast<double*>(A.st + T * A.pieces);
+  A.verdicts = reinterpret_cast<lfm3::Verdict*>(A.left + R * A.pieces);
   const hipStream_t s = (hipStream_t)stream;
   return lfm3::verify_ve(T, V) == 8 ? lfm3::verify_launch<8>(A, s) : lfm3::verify_launch<32>(A, s);
 }
