@@ -54,6 +54,7 @@ struct ChunkArgs {
   uint16_t* out;
   float scale;                     // log2(e) / sqrt(128)
   int nsink;
+  bool xfirst;                     // one launch: the exact part's workgroups come first
 };
 
 // The last i in [0, n) with below(i), for a predicate that holds up to some index, 0 among them: 64-way search by a whole
@@ -900,9 +901,10 @@ __global__ void __launch_bounds__(64 * NW, 2) chunk_exact_kernel(ChunkArgs A) {
   }
   exact_part<CT, NW, DIRECT>(Ks, Vs, L, A, blockIdx.x);
 }
-// Both in one launch: three of four waves per (tile, KV head), whose LDS (48 KB) lets two workgroups stay on a CU beside the tables,
-// then the quantized list's workgroups. The other order takes 20 us instead of 17 for 1 row x 5 at 16384, where the exact part
-// is the longer chain, and 44 instead of 47 for 16 x 4096 x 33.
+// Both in one launch: three of four waves per (tile, KV head), whose LDS (48 KB) lets two workgroups stay on a CU beside the tables.
+// The exact part's workgroups come first while the quantized ones have up to three entries each, for they are the longer
+// chain then; behind them they fill the end. In us, exact first / last: 1 row x 5 tokens at 16384 (half an entry) 23.5 / 26.9,
+// 16 x 8 at 4096 (1.9) 37.8 / 40.6, 32 x 8 at 4096 (3.8) 52.3 / 47.5, 16 x 8 at 16384 (7.9) 64.9 / 60.6, 16 x 33 at 16384 173 / 166.
 constexpr int BNW = 3;
 union ChunkBoth { ChunkStage s; ChunkXRows<BNW> x; };
 template <int CT>
@@ -910,11 +912,11 @@ __global__ void __launch_bounds__(256, 2) chunk_both_kernel(ChunkArgs A) {
   __shared__ ChunkQLds L;
   __shared__ ChunkBoth a, b;
   __shared__ ChunkXLds<CT, BNW> X;
-  const unsigned nx = 4 * (unsigned)A.I;
-  if (blockIdx.x >= nx)
-    quant_part<CT>(L, a.s, b.s, A, blockIdx.x - nx);
+  const unsigned nx = 4 * (unsigned)A.I, nq = (unsigned)A.G, wg = blockIdx.x, q0 = A.xfirst ? nx : 0;
+  if (wg - q0 < nq)
+    quant_part<CT>(L, a.s, b.s, A, wg - q0);
   else if (threadIdx.x < 64 * BNW)
-    exact_part<CT, BNW, false>(a.x, b.x, X, A, blockIdx.x);
+    exact_part<CT, BNW, false>(a.x, b.x, X, A, A.xfirst ? wg : wg - nq);
 }
 
 // ---------------------------------------------------------------- merge
@@ -1140,6 +1142,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
   A.out = out;
   A.scale = 1.4426950408889634f * 0.08838834764831845f;
   A.nsink = sinks ? NSINK : 0;
+  A.xfirst = 4 * P->nqmax * max(R, T / (4 * p.ct)) <= 3 * p.G;
   const hipStream_t s = (hipStream_t)stream;
   return p.ct == 1 ? chunk_launch<1>(A, quant, p.both, s) : chunk_launch<2>(A, quant, p.both, s);
 }

@@ -771,11 +771,12 @@ def rope_pairs(cos_t, sin_t):
     L = ops()
     P = cos_t.shape[0]
     t = torch.empty(P, 32, dtype=torch.int32, device=cos_t.device)
-    _check(L.kv800_hip_rope_table(_ptr(cos_t), _ptr(sin_t), P, _ptr(t), _stream(cos_t.device)))
-    if torch.cuda.is_current_stream_capturing():
-        return t
-    done = torch.cuda.Event()
-    done.record(torch.cuda.current_stream(cos_t.device))
+    with _on(cos_t.device):
+        _check(L.kv800_hip_rope_table(_ptr(cos_t), _ptr(sin_t), P, _ptr(t), _stream(cos_t.device)))
+        if torch.cuda.is_current_stream_capturing():
+            return t
+        done = torch.cuda.Event()
+        done.record(torch.cuda.current_stream(cos_t.device))
     _PAIRS[key] = (cos_t, sin_t, ver, t, now, done)
     _PAIRS.move_to_end(key)
     while len(_PAIRS) > 8:

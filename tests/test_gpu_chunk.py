@@ -59,6 +59,17 @@ def test_quantized_in_two_launches(hip, rows):
     check(got, want, f"two launches {rows}, a value unseen")
 
 
+@pytest.mark.parametrize("rows", ["odd", "chunk", "edges"])
+def test_quantized_part_first(hip, rows):
+    """One launch in which the exact part's workgroups come last: a bound that allows more than three entries a workgroup, but
+    not the lists that get a launch of their own."""
+    c = ref.Cache(hip, *ROWS[rows], ebs=40, seed=len(rows))
+    c.P.nqmax = 8 * torch.cuda.get_device_properties(0).multi_processor_count // len(c.N)
+    check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), c.want(hip), f"quantized part first {rows}")
+    small = hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+    assert torch.equal(small, hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin))
+
+
 @pytest.mark.parametrize("rows", list(ROWS))
 @pytest.mark.parametrize("sinks,rot", [(True, True), (False, False)])
 def test_window(hip, rows, sinks, rot):
