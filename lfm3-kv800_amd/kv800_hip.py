@@ -363,7 +363,8 @@ def chunk_meta(bt, lens, qlens, ebs, tokens, held=None, free=None, taken=None):
         return ChunkMeta(torch.zeros(1, dtype=torch.int64, device=dev), pad, pad.clone(), torch.zeros_like(pad),
                          torch.empty(0, dtype=torch.int32, device=dev), held, taken)
     lens, qlens = lens.contiguous(), qlens.contiguous()
-    qsl, slot, pos, row, tk = torch.empty(R + 2 + 3 * tokens, dtype=torch.int64, device=dev).split((R + 1, tokens, tokens, tokens, 1))
+    qsl, slot, pos, row, tk = torch.empty(R + 2 + 3 * tokens, dtype=torch.int64, device=dev).split_with_sizes(
+        (R + 1, tokens, tokens, tokens, 1))
     l32 = torch.empty(R, dtype=torch.int32, device=dev)
     after = torch.empty(R, dtype=torch.int32, device=dev) if grow else None
     with _on(dev):
