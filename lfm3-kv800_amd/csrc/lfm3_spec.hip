@@ -190,7 +190,7 @@ conv_commit_kernel(uint16_t* __restrict__ state, const uint16_t* __restrict__ ta
 // All in 64 bits: the running sums of neighbours among 65,536 tokens lie 1e-5 apart where 32-bit exponentials are
 // 1e-7 off, and the choice has to be the same whatever way a row is cut. Bound: the logits' bytes and the exponentials'
 // instructions: about 30 per value, half of them of 64 bits, take longer than the bytes. 256 rows, 722 logits rows of 65,536 with
-// the drafts' distributions (162 MB): stats 42, residual 19, pick 12 us; one row of 5: 4, 0 and 10 us, chains of dependent
+// the drafts' distributions (162 MB): stats 40, residual 17, pick 11 us; one row of 5: 3.5, 0 and 8 us, chains of dependent
 // loads and of 64-bit sums over lanes.
 constexpr int VT = 256;                                // threads; a piece holds VT x VE values, VE = 8 or 32 a thread
 struct Stat { double s; float m; int32_t at; };        // 16 bytes
@@ -203,10 +203,42 @@ __device__ __forceinline__ bool ranks_before(float a, int ia, float b, int ib) {
 }
 // whether a row with largest logit m is sampled: a temperature in (0, 1e30] and a finite m; else its choice is m's index
 __device__ __forceinline__ bool sampled(float tp, float m) { return tp > 0.f && tp <= 1e30f && m - m == 0.f; }
+// Reductions over a wave, the same in every lane: partners within rows of 16 by DPP (neighbours 1 and 2 apart, then mirrored
+// halves and rows, whose lanes are alike by then), across the rows by lane swaps, which return the values of both sides.
+// (By __shfl_xor, through the LDS, and with the deciding token combined twice: 256 rows 73 us of kernels instead of 68, one
+// row 14 instead of 11.6.)
+constexpr int DPP_STEP[4] = {0xB1, 0x4E, 0x141, 0x140};   // quad_perm [1 0 3 2], [2 3 0 1], row_half_mirror, row_mirror
+template <int K>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, DPP_STEP[K], 0xF, 0xF, false); }
+struct Pair32 { uint32_t a, b; };
+template <int K>
+__device__ __forceinline__ Pair32 both_sides(uint32_t x) {   // step K: this lane's value and its partner's, or the two in lane order
+  if constexpr (K < 4) return {x, dpp<K>(x)};
+  else if constexpr (K == 4) { const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false); return {r[0], r[1]}; }
+  else { const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false); return {r[0], r[1]}; }
+}
+template <int K = 0>
 __device__ __forceinline__ double wave_sumd(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  const uint64_t x = __builtin_bit_cast(uint64_t, v);
+  const Pair32 lo = both_sides<K>((uint32_t)x), hi = both_sides<K>((uint32_t)(x >> 32));
+  v = __builtin_bit_cast(double, ((uint64_t)hi.a << 32) | lo.a) + __builtin_bit_cast(double, ((uint64_t)hi.b << 32) | lo.b);
+  if constexpr (K < 5) return wave_sumd<K + 1>(v);
+  else return v;
+}
+template <int K = 0>
+__device__ __forceinline__ float wave_maxn(float v) {        // NaN wins
+  const Pair32 x = both_sides<K>(__float_as_uint(v));
+  v = __builtin_elementwise_maximum(__uint_as_float(x.a), __uint_as_float(x.b));
+  if constexpr (K < 5) return wave_maxn<K + 1>(v);
+  else return v;
+}
+template <int K = 0>
+__device__ __forceinline__ void wave_first(float& m, int& at) {   // the first in rank of the lanes' (m, at)
+  const Pair32 x = both_sides<K>(__float_as_uint(m)), i = both_sides<K>((uint32_t)at);
+  const bool second = ranks_before(__uint_as_float(x.b), (int)i.b, __uint_as_float(x.a), (int)i.a);
+  m = __uint_as_float(second ? x.b : x.a);
+  at = (int)(second ? i.b : i.a);
+  if constexpr (K < 5) wave_first<K + 1>(m, at);
 }
 // exp((x - m) / temp) for x <= m, within 2^-42: y = (x - m) / temp with the difference exact, so that a small temperature does
 // not enlarge its rounding, = (16 e + j) ln2 / 16 + r, |r| <= ln2 / 32; 16 e + j is the low word of 16 y / ln2 + 1.5 2^52; 2^(j / 16)
@@ -293,9 +325,7 @@ __global__ void __launch_bounds__(VT) verify_stats_kernel(VerifyArgs A) {
   for (int k = 0; k < VE / 8; ++k)
 #pragma unroll
     for (int e = 0; e < 8; e += 2) own = __builtin_elementwise_maximum(own, __builtin_elementwise_maximum(x[k][e], x[k][e + 1]));
-  float bm = own;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) bm = __builtin_elementwise_maximum(bm, __shfl_xor(bm, o, 64));
+  float bm = wave_maxn(own);
   if (lane == 0) rm[w] = bm;
   if (tid == 0) at = 0x7FFFFFFF;
   __syncthreads();
@@ -344,12 +374,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
       const Stat a = A.st[t * A.pieces + p];
       if (ranks_before(a.m, a.at, M, at)) { M = a.m; at = a.at; }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor(M, o, 64);
-      const int i2 = __shfl_xor(at, o, 64);
-      if (ranks_before(m2, i2, M, at)) { M = m2; at = i2; }
-    }
+    wave_first(M, at);
     S = 0.0;
     if (sampled(tp, M))
       for (int64_t p = lane; p < A.pieces; p += 64) {
@@ -358,15 +383,20 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
       }
     S = wave_sumd(S);
   };
-  for (int64_t t = d.s0 + w; t < d.s1 - 1; t += VT / 64) {
-    float M;
-    int at;
-    double S;
-    const int64_t k = A.tokens[t + 1];
+  // the wave that looks at the row's deciding token leaves what it found: the token breaks its loop, or is the row's last
+  float M = -INFINITY;
+  int at = 0x7FFFFFFF;
+  double S = 0.0;
+  int64_t mine = -1;
+  for (int64_t t = d.s0 + w; t < d.s1; t += VT / 64) {
+    const bool judge = t < d.s1 - 1;
+    const int64_t k = judge ? A.tokens[t + 1] : -1;
     const bool in = k >= 0 && k < A.V;
-    const float xk = in ? bf2f(A.logits[t * A.ld + k]) : -INFINITY, ut = A.u[t];
+    const float xk = in ? bf2f(A.logits[t * A.ld + k]) : -INFINITY, ut = judge ? A.u[t] : 0.f;
     const double qk = A.q ? (in ? (double)A.q[t * A.ldq + k] : 0.0) : 1.0;
     combine(t, M, at, S);
+    mine = t;
+    if (!judge) break;
     const bool keep = sampled(tp, M) ? in && (double)ut * qk < expo(xk, Expo{(double)M, d.it}, L.pow16) / S : k == at;
     if (!keep) {
       if (lane == 0) atomicMin(&L.stop, (long long)t);
@@ -375,13 +405,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
   }
   __syncthreads();
   d.t = L.stop;
-  if (w == 0) {
-    float M;
-    int at;
-    double S;
-    combine(d.t, M, at, S);
-    if (lane == 0) { L.m = M; L.at = at; L.s = S; }
-  }
+  if (mine == d.t && lane == 0) { L.m = M; L.at = at; L.s = S; }
   __syncthreads();
   d.m = L.m;
   d.at = L.at;
@@ -593,7 +617,8 @@ __global__ void __launch_bounds__(VT) verify_pick_kernel(VerifyArgs A) {
 }
 
 // 2,048-value pieces while all rows in them make up to 1,024 workgroups, else 8,192, whose sums and lookups of a piece's row are
-// fewer (256 rows, stats, residual and pick: 73 us, in small pieces 91; one row of 5: 14 us, in large pieces 22)
+// fewer (256 rows, stats, residual and pick: 73 us, in small pieces 91; one row of 5: 14 us, in large pieces 22; before faster
+// reductions)
 int verify_ve(int64_t T, int64_t V) { return T * ((V + 8 * VT - 1) / (8 * VT)) <= 1024 ? 8 : 32; }
 int64_t verify_pieces(int64_t T, int64_t V) { const int64_t n = VT * verify_ve(T, V); return (V + n - 1) / n; }
 
