@@ -920,6 +920,34 @@ __global__ void __launch_bounds__(256, 2) chunk_both_kernel(ChunkArgs A) {
 }
 
 // ---------------------------------------------------------------- merge
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xF, 0xF, false));
+}
+// over a wave, the same in every lane: within rows of 16 by DPP (lanes 1 and 2 apart, mirrored halves, mirrored rows), then
+// across the rows
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp<0xB1>(x)); x = fmaxf(x, dpp<0x4E>(x)); x = fmaxf(x, dpp<0x141>(x)); x = fmaxf(x, dpp<0x140>(x));
+  return max4rows(x);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x += dpp<0xB1>(x); x += dpp<0x4E>(x); x += dpp<0x141>(x); x += dpp<0x140>(x);
+  return sum4rows(x);
+}
+// Walsh-Hadamard transform over the 64 lanes: lanes 1, 2, 4 (7 apart, then 3), 8 apart by DPP; 16 and 32 apart by swaps,
+// which return the lower lane's value first
+__device__ __forceinline__ float lane_hadamard(float x) {
+  const int lane = threadIdx.x & 63;
+  float p;
+  p = dpp<0xB1>(x); x = lane & 1 ? p - x : x + p;
+  p = dpp<0x4E>(x); x = lane & 2 ? p - x : x + p;
+  p = dpp<0x1B>(dpp<0x141>(x)); x = lane & 4 ? p - x : x + p;
+  p = dpp<0x128>(x); x = lane & 8 ? p - x : x + p;
+  float2 r = rows16(x);
+  x = lane & 16 ? r.x - r.y : r.x + r.y;
+  r = halves32(x);
+  return lane & 32 ? r.x - r.y : r.x + r.y;
+}
 // WPC waves per (token, query head), the four heads of a KV head (WPC = 1) or one head (8) per workgroup: 8 for few tokens,
 // whose partials are many (the whole call with 8 / 1: 1 x 16384 x 5 tokens 23.2 / 37.9 us, 8 x 16384 x 4 36.8 / 38.2, 8 x 16384 x 8
 // 48.8 / 48.0, 16 x 1024 x 8 29.5 / 25.4). Lanes take the partials' m and l side by side, then the wave adds up the partials'
@@ -956,10 +984,7 @@ __global__ void __launch_bounds__(WPC == 1 ? 256 : 64 * WPC) chunk_merge_kernel(
     const bool in = lane < kn;
     const int64_t p = slot(in ? k0 + lane : 0);
     const float mk = in ? A.mo[p] : NEG_BIG, lk = in ? A.lo[p] : 0.f;
-    float m2 = mk;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m2 = fmaxf(m2, __shfl_xor(m2, o, 64));
-    m2 = fmaxf(m2, M);
+    const float m2 = fmaxf(wave_max(mk), M);
     const float al = __builtin_amdgcn_exp2f(M - m2), f = __builtin_amdgcn_exp2f(mk - m2);
     M = m2;
     l = l * al + f * lk;                               // the lane's own share; M starts at the exact part's m
@@ -977,8 +1002,7 @@ __global__ void __launch_bounds__(WPC == 1 ? 256 : 64 * WPC) chunk_merge_kernel(
       }
     }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  l = wave_sum(l);
   if constexpr (WPC > 1) {                             // the waves' shares, in wave order
     if (lane == 0) { jm[w] = M; jl[w] = l; }
     *reinterpret_cast<float2*>(&jx[w][dd]) = make_float2(x0, x1);
@@ -1002,13 +1026,8 @@ __global__ void __launch_bounds__(WPC == 1 ? 256 : 64 * WPC) chunk_merge_kernel(
     x0 = a + b;
     x1 = a - b;
   }
-#pragma unroll
-  for (int k = 0; k < 6; ++k) {
-    const int msk = 1 << k;
-    const float p0 = __shfl_xor(x0, msk), p1 = __shfl_xor(x1, msk);
-    x0 = (lane & msk) ? p0 - x0 : x0 + p0;
-    x1 = (lane & msk) ? p1 - x1 : x1 + p1;
-  }
+  x0 = lane_hadamard(x0);
+  x1 = lane_hadamard(x1);
   const float hn = __uint_as_float(0x3DB504F3u);       // 1 / sqrt(128)
   const float inv = l > 0.f ? 1.0f / l : 0.f;
   *dst = bfpk((x0 * hn + fx * ax.x) * inv, (x1 * hn + fx * ax.y) * inv);
