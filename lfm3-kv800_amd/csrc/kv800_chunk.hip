@@ -23,7 +23,7 @@
 // time of their bytes (64 rows x 32768 x 4 tokens, 451 MB: 168 us of quant_part), VALU instructions in 68 % of the cycles, which are
 // table lookups and rotation of the keys; each column's share of them falls with the tile, so that tiles of 8 take 1.4
 // times as long for twice the queries. Window layers read at 4.1 TB/s (398 rows x 5 tokens, 223 MB: 54 us). One row takes
-// 17 + 7 us for 5 tokens at 16384 positions: the latency of four dependent loads, of the lookups and of a second launch.
+// 17 + 6 us for 5 tokens at 16384 positions: the latency of four dependent loads, of the lookups and of a second launch.
 #include <mutex>
 
 #include "kv800_attn.h"
