@@ -389,14 +389,14 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& A, int64_t r, Verdic
   double S = 0.0;
   int64_t mine = -1;
   for (int64_t t = d.s0 + w; t < d.s1; t += VT / 64) {
-    const bool judge = t < d.s1 - 1;
-    const int64_t k = judge ? A.tokens[t + 1] : -1;
+    const bool draft = t < d.s1 - 1;
+    const int64_t k = draft ? A.tokens[t + 1] : -1;
     const bool in = k >= 0 && k < A.V;
-    const float xk = in ? bf2f(A.logits[t * A.ld + k]) : -INFINITY, ut = judge ? A.u[t] : 0.f;
+    const float xk = in ? bf2f(A.logits[t * A.ld + k]) : -INFINITY, ut = draft ? A.u[t] : 0.f;
     const double qk = A.q ? (in ? (double)A.q[t * A.ldq + k] : 0.0) : 1.0;
     combine(t, M, at, S);
     mine = t;
-    if (!judge) break;
+    if (!draft) break;
     const bool keep = sampled(tp, M) ? in && (double)ut * qk < expo(xk, Expo{(double)M, d.it}, L.pow16) / S : k == at;
     if (!keep) {
       if (lane == 0) atomicMin(&L.stop, (long long)t);
