@@ -305,6 +305,14 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
                            int64_t qpool_bytes, int64_t epool_elems, int64_t sink_elems, uint16_t* out, void* ws,
                            int64_t ws_bytes, void* stream);
 
+/* kv800_hip_decode_chunk with the tables' widths apart from their row strides: a row of P->boff has boff_cols entries and one of
+ * P->eoff eoff_cols, whatever lies between two rows (columns of a wider table, one row of any stride). Nothing behind a row's
+ * entries is read. kv800_hip_decode_chunk takes the strides for the widths. */
+int kv800_hip_decode_chunk_sized(const kv800_paged_t* P, int64_t boff_cols, int64_t eoff_cols, const uint16_t* q, const int64_t* qsl,
+                                 int64_t R, int64_t T, const uint16_t* cos_t, const uint16_t* sin_t, int64_t rope_rows,
+                                 const uint32_t* cs2, int64_t qpool_bytes, int64_t epool_elems, int64_t sink_elems, uint16_t* out,
+                                 void* ws, int64_t ws_bytes, void* stream);
+
 /* Streaming read of bytes (a positive multiple of 16) from buf with `groups` workgroups (8 plain 16-byte loads in
  * flight per lane), writing one xor word per workgroup to out[0 .. groups). No counterpart in the reference: a
  * measurement aid, the read bandwidth the part sustains for plain loads, against which bench.py sets the kernels'

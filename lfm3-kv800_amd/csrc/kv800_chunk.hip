@@ -48,6 +48,7 @@ struct ChunkArgs {
   const uint16_t *cos_t, *sin_t;   // null: keys as stored
   const uint32_t* cs2;
   int64_t rope_rows, qpool_bytes, epool_elems, sink_elems;
+  int64_t bcols, ecols;            // entries of a row of boff and of eoff, whose rows may lie further apart
   int64_t G, I;                    // workgroups of the quantized list; tile numbers
   int32_t* pre;                    // R + 1: the quantized list's entries before each row; then entries per workgroup
   float *mo, *lo, *ao;             // partial slots: [slot][4 heads][16 CT columns] and, for ao, [128]
@@ -162,7 +163,7 @@ __device__ __forceinline__ uint32_t chunk_scales(rsrc_t rs, int t0, int h, int l
 // Sub-blocks past the host's bound, the offset table or the rope table are not read.
 __device__ __forceinline__ int row_nq(const ChunkArgs& A, int64_t r) { return min(max(A.P.NQ[r], 0), 1 << 22); }
 __device__ __forceinline__ int row_blocks(const ChunkArgs& A, int64_t r) {
-  return (int)min(min((int64_t)row_nq(A, r), A.P.nqmax), min(A.P.boff_stride, A.rope_rows / BLK));
+  return (int)min(min((int64_t)row_nq(A, r), A.P.nqmax), min(A.bcols, A.rope_rows / BLK));
 }
 // Attention of one tile's columns of KV head h (the wave's) over tokens [64 u0, 64 u1) of its row, into partial slot `slot`.
 // As in decode_quant_kernel, with the wave's one head: K pairs by table lookup, RoPE by v_dot2_f32_bf16, Q K^T on bf16 MFMA
@@ -594,7 +595,7 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
     const int i = c0 + (lane & 31);
     int pg = 0, in;
     if (i >= cnt && i < nk) split(posof(i), pg, in);
-    return et[min((int64_t)pg, A.P.eoff_stride - 1)];
+    return et[min((int64_t)pg, A.ecols - 1)];
   };
   struct Where { const uint16_t *k, *v; uint32_t ok; };   // bit t of ok: token t of the chunk has a key
   auto locate = [&](int c0, int64_t base) {
@@ -615,7 +616,7 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
         split(pos, pg, in);
         ko = base + hoff + (int64_t)in * ets;
         vo = ko + A.P.e_v;
-        ok = base >= 0 && pg < A.P.eoff_stride && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
+        ok = base >= 0 && pg < A.ecols && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
       }
       ok = ok && (!rot || pos < A.rope_rows);
       if (ok) { r.k = kb + ko; r.v = vb + vo; }
@@ -1122,10 +1123,19 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
                            const uint16_t* cos_t, const uint16_t* sin_t, int64_t rope_rows, const uint32_t* cs2,
                            int64_t qpool_bytes, int64_t epool_elems, int64_t sink_elems, uint16_t* out, void* ws,
                            int64_t ws_bytes, void* stream) {
+  KV800_REQUIRE(P, "decode_chunk: null pointer");
+  return kv800_hip_decode_chunk_sized(P, P->boff_stride, P->eoff_stride, q, qsl, R, T, cos_t, sin_t, rope_rows, cs2, qpool_bytes,
+                                      epool_elems, sink_elems, out, ws, ws_bytes, stream);
+}
+
+int kv800_hip_decode_chunk_sized(const kv800_paged_t* P, int64_t boff_cols, int64_t eoff_cols, const uint16_t* q, const int64_t* qsl,
+                                 int64_t R, int64_t T, const uint16_t* cos_t, const uint16_t* sin_t, int64_t rope_rows,
+                                 const uint32_t* cs2, int64_t qpool_bytes, int64_t epool_elems, int64_t sink_elems, uint16_t* out,
+                                 void* ws, int64_t ws_bytes, void* stream) {
   KV800_REQUIRE(P && R >= 0 && T >= 0 && (R > 0 || T == 0), "decode_chunk: bad row or token count");
   if (T == 0) return KV800_OK;
   KV800_REQUIRE(q && qsl && out && P->epool && P->eoff && P->N, "decode_chunk: null pointer");
-  KV800_REQUIRE(P->ebs > 0 && P->eoff_stride > 0 && P->win >= 0 && P->win < (1LL << 31) && P->nqmax >= 0,
+  KV800_REQUIRE(P->ebs > 0 && eoff_cols > 0 && P->eoff_stride >= 0 && P->win >= 0 && P->win < (1LL << 31) && P->nqmax >= 0,
                 "decode_chunk: bad page geometry, window or nqmax");
   KV800_REQUIRE(P->e_hs % 8 == 0 && P->e_ts % 8 == 0 && P->e_v % 8 == 0 && P->e_ts < (1LL << 31) &&
                     P->e_ts > -(1LL << 31),
@@ -1136,7 +1146,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
                 "decode_chunk: rope tables must be 16-byte aligned and not empty");
   const bool quant = P->win == 0 && P->nqmax > 0;
   if (quant)
-    KV800_REQUIRE(P->qpool && P->boff && P->boff_stride > 0 && P->NQ && cos_t && cs2 && qpool_bytes >= SUB && (uintptr_t)cs2 % 16 == 0 &&
+    KV800_REQUIRE(P->qpool && P->boff && boff_cols > 0 && P->boff_stride >= 0 && P->NQ && cos_t && cs2 && qpool_bytes >= SUB && (uintptr_t)cs2 % 16 == 0 &&
                       (uintptr_t)P->qpool % 16 == 0,
                   "decode_chunk: quantized layers need NQ, the quant pool (16-byte aligned, one sub-block at least), its offsets and the rope tables");
   KV800_REQUIRE(!quant || rope_rows < (1LL << 24), "decode_chunk: rope tables of 2^24 rows or more are not addressed");   // 128 bytes a row of cs2
@@ -1153,6 +1163,7 @@ int kv800_hip_decode_chunk(const kv800_paged_t* P, const uint16_t* q, const int6
   A.q = q; A.qsl = qsl; A.R = R; A.T = T;
   A.cos_t = cos_t; A.sin_t = sin_t; A.cs2 = cs2;
   A.rope_rows = rope_rows; A.qpool_bytes = qpool_bytes; A.epool_elems = epool_elems; A.sink_elems = sink_elems;
+  A.bcols = boff_cols; A.ecols = eoff_cols;
   A.G = p.G; A.I = p.I;
   A.pre = reinterpret_cast<int32_t*>(ws);
   A.ao = quant ? reinterpret_cast<float*>(A.pre + p.pre) : nullptr;

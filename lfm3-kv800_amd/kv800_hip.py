@@ -89,6 +89,8 @@ SIGNATURES = {
     "kv800_hip_decode_chunk_workspace": (_I64, [_I64, _I64, _I64]),
     "kv800_hip_decode_chunk": (_I32, [ctypes.POINTER(Paged), _VP, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _I64, _I64,
                                       _VP, _VP, _I64, _VP]),
+    "kv800_hip_decode_chunk_sized": (_I32, [ctypes.POINTER(Paged), _I64, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _I64,
+                                            _I64, _VP, _VP, _I64, _VP]),
 }
 
 
@@ -800,6 +802,12 @@ def plan(B, nqmax, spb=None, target=None):
     return ns.value, sp.value
 
 
+def _row_stride(t):
+    """The row stride of an (R, n) table, which the decode takes for its width: of a single row, whatever stride torch gives
+    it, n at least."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] == 1 else t.stride(0)
+
+
 def paged_struct(P, B):
     """kv800_paged_t of a kv800.Paged, plus the extents of its pools."""
     dev = P.epool.device
@@ -813,11 +821,11 @@ def paged_struct(P, B):
         _need(P.qpool, "qpool", torch.uint8, dev); _need(P.boff, "boff", torch.int64, dev)
         if P.boff.stride(-1) != 1:
             raise ValueError("boff rows must be contiguous")
-        s.qpool, s.boff, s.boff_stride = P.qpool.data_ptr(), P.boff.data_ptr(), P.boff.stride(0)
+        s.qpool, s.boff, s.boff_stride = P.qpool.data_ptr(), P.boff.data_ptr(), _row_stride(P.boff)
         qbytes = _extent(P.qpool)
     else:
         qbytes = 0
-    s.epool, s.eoff, s.eoff_stride = P.epool.data_ptr(), P.eoff.data_ptr(), P.eoff.stride(0)
+    s.epool, s.eoff, s.eoff_stride = P.epool.data_ptr(), P.eoff.data_ptr(), _row_stride(P.eoff)
     s.ebs, s.e_hs, s.e_ts, s.e_v = int(P.ebs), int(P.e_hs), int(P.e_ts), int(P.e_v)
     sink_elems = 0
     if P.win and P.sk is not None:
@@ -909,10 +917,11 @@ def decode_chunk(P, q, qsl, cos_t, sin_t):
         cs2 = rope_pairs(cos_t, sin_t) if s.nqmax else None
         wsb = int(L.kv800_hip_decode_chunk_workspace(R, T, s.nqmax))
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-        _check(L.kv800_hip_decode_chunk(ctypes.byref(s), q.data_ptr(), qsl.data_ptr(), R, T, cos_t.data_ptr() if rot else None,
-                                        sin_t.data_ptr() if rot else None, cos_t.shape[0] if rot else 0,
-                                        cs2.data_ptr() if cs2 is not None else None, qbytes, eelems, selems, out.data_ptr(),
-                                        ws.data_ptr() if wsb else None, wsb, _raw_stream(dev)))
+        _check(L.kv800_hip_decode_chunk_sized(ctypes.byref(s), P.boff.shape[1] if s.nqmax else 0, P.eoff.shape[1], q.data_ptr(),
+                                              qsl.data_ptr(), R, T, cos_t.data_ptr() if rot else None,
+                                              sin_t.data_ptr() if rot else None, cos_t.shape[0] if rot else 0,
+                                              cs2.data_ptr() if cs2 is not None else None, qbytes, eelems, selems, out.data_ptr(),
+                                              ws.data_ptr() if wsb else None, wsb, _raw_stream(dev)))
     return out
 
 
