@@ -570,7 +570,11 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
   const int cnt = max(0, min(min(A.nsink, lo_row), hi));
   const int cnt2 = win > 0 ? max(0, min(min(A.nsink, hi) - lo_row, lo_tile - lo_row)) : 0;
   const int rest = lo_tile - cnt - cnt2;               // list index i >= cnt + cnt2 is position rest + i
-  const int nk = cnt + cnt2 + max(0, hi - lo_tile);
+  // a length past the page or rope table: what lies behind it has no keys, and is not walked through. 4,096 are left so that
+  // the chunks asked for ahead stay below 2^31
+  int64_t held = min(A.ecols * A.P.ebs, (int64_t)0x7FFFFFFF - 4096);
+  if (A.cos_t) held = min(held, A.rope_rows);
+  const int nk = cnt + cnt2 + max(0, min(hi, (int)held) - lo_tile);
   const int64_t* et = A.P.eoff + t.row * A.P.eoff_stride;
   const int64_t sko = cnt ? A.P.skoff[t.row] : 0, svo = cnt ? A.P.svoff[t.row] : 0;
   const bool rot = A.cos_t != nullptr;
@@ -1154,7 +1158,7 @@ int kv800_hip_decode_chunk_sized(const kv800_paged_t* P, int64_t boff_cols, int6
   KV800_REQUIRE(!sinks || (P->sv && P->skoff && P->svoff && (((uintptr_t)P->sk | (uintptr_t)P->sv) % 16) == 0),
                 "decode_chunk: sinks need sv, skoff, svoff and 16-byte aligned buffers");
   const ChunkPlan p = chunk_plan(R, T, quant ? P->nqmax : 0);
-  KV800_REQUIRE(p.I <= (1LL << 28) && T <= (1LL << 28) && P->ebs < (1LL << 30), "decode_chunk: too many rows and tokens");
+  KV800_REQUIRE(p.I <= (1LL << 28) && T <= (1LL << 28) && P->ebs < (1LL << 30) && eoff_cols < (1LL << 32), "decode_chunk: too many rows, tokens or pages");
   KV800_REQUIRE(!quant || p.I <= (int64_t)0x7F000000 / 4 / P->nqmax, "decode_chunk: too many rows and sub-blocks");
   KV800_REQUIRE(!quant || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= kv800_hip_decode_chunk_workspace(R, T, P->nqmax)),
                 "decode_chunk: the workspace is too small or not 16-byte aligned");

@@ -78,3 +78,21 @@ def test_tables_without_columns_are_refused(hip):
         with pytest.raises((RuntimeError, ValueError)):
             hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
         setattr(c.P, name, keep)
+
+
+def test_lengths_far_past_the_tables(hip):
+    """A length of 2^31 - 1 over a short table: its positions alone, without a walk over the others."""
+    far = (1 << 31) - 1
+    c = ref.Cache(hip, [1500, 300], [4, 9], ebs=32, seed=57)
+    want = c.want(hip)
+    K, V, pos = c.row(hip, 0)
+    want[:4] = ref.attend(c.q[:4], K, V, pos, torch.arange(far - 4, far, device=c.dev))
+    c.P.N[0] = far
+    check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), want, "a far length")
+    w = ref.Cache(hip, [700, 300], [4, 9], ebs=32, win=256, sinks=True, seed=58)
+    want = w.want(hip)
+    K, V = w.P.sk[0].double(), w.P.sv[0].double()
+    pos = torch.arange(4, device=w.dev)
+    want[:4] = ref.attend(w.q[:4], ref.rotate(K, pos, w.cos, w.sin), V, pos, pos + 1000)
+    w.P.N[0] = far
+    check(hip.decode_chunk(w.P, w.q, w.qsl, w.cos, w.sin), want, "a far length of a window")
