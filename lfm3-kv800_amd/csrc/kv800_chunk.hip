@@ -48,13 +48,13 @@ struct ChunkArgs {
   const uint16_t *cos_t, *sin_t;   // null: keys as stored
   const uint32_t* cs2;
   int64_t rope_rows, qpool_bytes, epool_elems, sink_elems;
-  int64_t bcols, ecols;            // entries of a row of boff and of eoff, whose rows may lie further apart
   int64_t G, I;                    // workgroups of the quantized list; tile numbers
   int32_t* pre;                    // R + 1: the quantized list's entries before each row; then entries per workgroup
   float *mo, *lo, *ao;             // partial slots: [slot][4 heads][16 CT columns] and, for ao, [128]
   uint16_t* out;
   float scale;                     // log2(e) / sqrt(128)
   int nsink;
+  int held;                        // positions that the page and rope tables hold
   bool xfirst;                     // one launch: the exact part's workgroups come first
 };
 
@@ -160,10 +160,10 @@ __device__ __forceinline__ uint32_t chunk_scales(rsrc_t rs, int t0, int h, int l
 }
 
 // The list of (tile, 64 tokens) pairs, tile by tile: row r has tiles x sub-blocks x 4 of them.
-// Sub-blocks past the host's bound, the offset table or the rope table are not read.
+// Sub-blocks past the host's bound, the offset table or the rope table are not read: P.nqmax is the least of the three.
 __device__ __forceinline__ int row_nq(const ChunkArgs& A, int64_t r) { return min(max(A.P.NQ[r], 0), 1 << 22); }
 __device__ __forceinline__ int row_blocks(const ChunkArgs& A, int64_t r) {
-  return (int)min(min((int64_t)row_nq(A, r), A.P.nqmax), min(A.bcols, A.rope_rows / BLK));
+  return (int)min((int64_t)row_nq(A, r), A.P.nqmax);
 }
 // Attention of one tile's columns of KV head h (the wave's) over tokens [64 u0, 64 u1) of its row, into partial slot `slot`.
 // As in decode_quant_kernel, with the wave's one head: K pairs by table lookup, RoPE by v_dot2_f32_bf16, Q K^T on bf16 MFMA
@@ -566,15 +566,11 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
   } else {
     lo_row = lo_tile = A.P.NQ ? __builtin_amdgcn_readfirstlane(row_nq(A, t.row)) * BLK : 0;
   }
-  const int hi = min(N, plast + 1);
-  const int cnt = max(0, min(min(A.nsink, lo_row), hi));
+  const int cnt = max(0, min(min(A.nsink, lo_row), min(N, plast + 1)));
+  const int hi = min(min(N, plast + 1), A.held);       // what the tables do not hold is not walked through
   const int cnt2 = win > 0 ? max(0, min(min(A.nsink, hi) - lo_row, lo_tile - lo_row)) : 0;
   const int rest = lo_tile - cnt - cnt2;               // list index i >= cnt + cnt2 is position rest + i
-  // a length past the page or rope table: what lies behind it has no keys, and is not walked through. 4,096 are left so that
-  // the chunks asked for ahead stay below 2^31
-  int64_t held = min(A.ecols * A.P.ebs, (int64_t)0x7FFFFFFF - 4096);
-  if (A.cos_t) held = min(held, A.rope_rows);
-  const int nk = cnt + cnt2 + max(0, min(hi, (int)held) - lo_tile);
+  const int nk = cnt + cnt2 + max(0, hi - lo_tile);
   const int64_t* et = A.P.eoff + t.row * A.P.eoff_stride;
   const int64_t sko = cnt ? A.P.skoff[t.row] : 0, svo = cnt ? A.P.svoff[t.row] : 0;
   const bool rot = A.cos_t != nullptr;
@@ -599,7 +595,7 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
     const int i = c0 + (lane & 31);
     int pg = 0, in;
     if (i >= cnt && i < nk) split(posof(i), pg, in);
-    return et[min((int64_t)pg, A.ecols - 1)];
+    return et[pg];                                     // of a position below A.held, or the first
   };
   struct Where { const uint16_t *k, *v; uint32_t ok; };   // bit t of ok: token t of the chunk has a key
   auto locate = [&](int c0, int64_t base) {
@@ -620,7 +616,7 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
         split(pos, pg, in);
         ko = base + hoff + (int64_t)in * ets;
         vo = ko + A.P.e_v;
-        ok = base >= 0 && pg < A.ecols && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
+        ok = base >= 0 && ko >= 0 && vo >= 0 && ko + 128 <= A.epool_elems && vo + 128 <= A.epool_elems;
       }
       ok = ok && (!rot || pos < A.rope_rows);
       if (ok) { r.k = kb + ko; r.v = vb + vo; }
@@ -1167,7 +1163,7 @@ int kv800_hip_decode_chunk_sized(const kv800_paged_t* P, int64_t boff_cols, int6
   A.q = q; A.qsl = qsl; A.R = R; A.T = T;
   A.cos_t = cos_t; A.sin_t = sin_t; A.cs2 = cs2;
   A.rope_rows = rope_rows; A.qpool_bytes = qpool_bytes; A.epool_elems = epool_elems; A.sink_elems = sink_elems;
-  A.bcols = boff_cols; A.ecols = eoff_cols;
+  A.P.nqmax = quant ? min(min(P->nqmax, boff_cols), rope_rows / BLK) : 0;   // of the kernels; the plan goes by the caller's
   A.G = p.G; A.I = p.I;
   A.pre = reinterpret_cast<int32_t*>(ws);
   A.ao = quant ? reinterpret_cast<float*>(A.pre + p.pre) : nullptr;
@@ -1176,6 +1172,8 @@ int kv800_hip_decode_chunk_sized(const kv800_paged_t* P, int64_t boff_cols, int6
   A.out = out;
   A.scale = 1.4426950408889634f * 0.08838834764831845f;
   A.nsink = sinks ? NSINK : 0;
+  const int64_t pages = min(eoff_cols * P->ebs, (int64_t)0x7FFFFFFF - 4096);   // the chunks asked for ahead stay below 2^31
+  A.held = (int)(cos_t ? min(pages, rope_rows) : pages);
   A.xfirst = 4 * P->nqmax * max(R, T / (4 * p.ct)) <= 3 * p.G;
   const hipStream_t s = (hipStream_t)stream;
   return p.ct == 1 ? chunk_launch<1>(A, quant, p.both, s) : chunk_launch<2>(A, quant, p.both, s);
