@@ -40,6 +40,17 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {   // a value that all 
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xF, 0xF, false));
+}
+// over a wave, the same in every lane: within rows of 16 by DPP (lanes 1 and 2 apart, mirrored halves, mirrored rows), then
+// across the rows
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp<0xB1>(x)); x = fmaxf(x, dpp<0x4E>(x)); x = fmaxf(x, dpp<0x141>(x)); x = fmaxf(x, dpp<0x140>(x));
+  return max4rows(x);
+}
+
 struct ChunkArgs {
   kv800_paged_t P;
   const uint16_t* q;
@@ -96,9 +107,15 @@ __device__ __forceinline__ bool find_tile(const ChunkArgs& A, int64_t it, Tile& 
 }
 
 // ---------------------------------------------------------------- quantized sub-blocks
-// Log2 units by which a score may exceed the running max before the state is rescaled: weights p vsc <= 2^4 448 stay within
-// fp16, whose 11 bits round alike at every size; with the exact max a quarter of the chunks rescaled (52 instructions).
+// Log2 units by which a score may exceed the running max before the state is rescaled; with the exact max a quarter of the
+// chunks rescaled (52 instructions).
 constexpr float QLAZY = 4.f;
+// Weights p vsc go to the matrix product as fp16, held as p vsc 2^(WEXP - ve), 2^ve above every vsc of the span so far: 2^(QLAZY
+// + WEXP) = 2^15 at most, and 11 bits down to 2^-14, 2^-25 of a weight of 1 at the largest scale; what is below is off by
+// 2^-36 of that at most. fp16(p vsc) itself lost bits from 2^-14 on and all of them from 2^-25 on: behind one key 12 to 17 above the
+// others whose value is near zero, outputs were off by 6 to 700 %. Following the largest scale costs 0.4 % (192 ragged rows).
+constexpr int WEXP = 11;
+constexpr int VE_MIN = -9;     // the least e4m3 number
 constexpr int QCH = 32;        // tokens per stage
 // A stage as it lies in LDS: kc, (cos, sin) and vb rows of 32 tokens, all heads, in pieces of 16 bytes. Pieces are permuted
 // within a row so that the reads of one piece of 16 rows spread over the banks: piece p of token t at p ^ (t % 8), of vb rows
@@ -167,7 +184,8 @@ __device__ __forceinline__ int row_blocks(const ChunkArgs& A, int64_t r) {
 }
 // Attention of one tile's columns of KV head h (the wave's) over tokens [64 u0, 64 u1) of its row, into partial slot `slot`.
 // As in decode_quant_kernel, with the wave's one head: K pairs by table lookup, RoPE by v_dot2_f32_bf16, Q K^T on bf16 MFMA
-// with exact products; fp32 online softmax; P V on fp16 MFMA over the bit planes, weights fp16(p vsc): 11 bits, an eighth of the output's own rounding.
+// with exact products; fp32 online softmax; P V on fp16 MFMA over the bit planes, weights of 11 bits, an eighth of the output's own
+// rounding.
 // NC: columns of a slot, of which the tile has 16 CT at most.
 template <int CT, int NC>
 __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkStage& SB, const ChunkArgs& A, const Tile& t, int u0, int u1, int64_t slot) {
@@ -206,11 +224,26 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
     for (int i = 0; i < 8; ++i) acc[ct][i] = f4{0.f, 0.f, 0.f, 0.f};
   }
   const float scale = A.scale;
+  // 2^ve and what the scales are multiplied by before P V; the sums follow when ve grows. The fp32 sum of vlo needs none of it
+  int ve = VE_MIN;
+  float cap = 0x1p-9f, fac = 0x1p20f;                  // 2^ve, 2^(WEXP - ve)
   auto stage_scales = [&](uint32_t x) {
     float v[4];
     f8x4(x, v);
+    const float a = fabsf(v[1]);
+    if (__builtin_expect(__any(a > cap), 0)) {
+      const float top = wave_max(a);                   // a NaN scale is not among them
+      const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(top) >> 23) - 126);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[ct][i] *= ldexpf(1.f, ve - e);
+      ve = e;
+      cap = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ldexpf(1.f, e))));
+      fac = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ldexpf(1.f, WEXP - e))));
+    }
     L.vl[h][lane] = v[0];
-    L.vs[h][lane] = v[1];
+    L.vs[h][lane] = v[1] * fac;
   };
   const uint32_t kg = (uint32_t)h * 4096u + 16u * (uint32_t)g;
   // one 32-token chunk, tokens 32 cc .. of the staged 64; kpos: position of its first token
@@ -395,7 +428,7 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
       if (g == 0) { A.mo[col] = m[ct]; A.lo[col] = ls; }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {                    // plane i: dims 16 i + 4 g + r, bits worth 2^(i - 24)
-        const float ps = __uint_as_float((uint32_t)(127 + 24 - i) << 23);
+        const float ps = __uint_as_float((uint32_t)(127 + 24 - WEXP + ve - i) << 23);
         const f4 o = acc[ct][i];
         *reinterpret_cast<float4*>(A.ao + col * 128 + 16 * i + 4 * g) =
             make_float4(o[0] * ps + lv, o[1] * ps + lv, o[2] * ps + lv, o[3] * ps + lv);
@@ -921,16 +954,6 @@ __global__ void __launch_bounds__(256, 2) chunk_both_kernel(ChunkArgs A) {
 }
 
 // ---------------------------------------------------------------- merge
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xF, 0xF, false));
-}
-// over a wave, the same in every lane: within rows of 16 by DPP (lanes 1 and 2 apart, mirrored halves, mirrored rows), then
-// across the rows
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, dpp<0xB1>(x)); x = fmaxf(x, dpp<0x4E>(x)); x = fmaxf(x, dpp<0x141>(x)); x = fmaxf(x, dpp<0x140>(x));
-  return max4rows(x);
-}
 __device__ __forceinline__ float wave_sum(float x) {
   x += dpp<0xB1>(x); x += dpp<0x4E>(x); x += dpp<0x141>(x); x += dpp<0x140>(x);
   return sum4rows(x);
