@@ -59,17 +59,16 @@ def conv_chunk(bcx, conv_w, state, qsl):
     if bcx.dim() != 2 or bcx.shape[1] < 3 * H or tuple(conv_w.shape) != (H, 7):
         raise ValueError(f"bcx must be (T, >= {3 * H}) and conv_w ({H}, 7), got {tuple(bcx.shape)}, {tuple(conv_w.shape)}")
     T = bcx.shape[0]
-    if bcx.stride(-1) != 1 or bcx.stride(0) % 8 or bcx.stride(0) < 3 * H or bcx.data_ptr() % 16:
-        bcx = bcx.contiguous()
-        if bcx.stride(0) % 8:      # an odd width: the three parts alone
-            bcx = bcx[:, :3 * H].contiguous()
+    ld = bcx.stride(0) if T > 1 else 3 * H        # of a single row torch's stride may be anything
+    if H and (bcx.stride(1) != 1 or ld % 8 or ld < 3 * H or bcx.data_ptr() % 16):
+        bcx, ld = bcx[:, :3 * H].clone(memory_format=torch.contiguous_format), 3 * H
     out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
     taps = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
     if T == 0 or R == 0 or H == 0:
         return out.zero_(), taps.zero_()
-    conv_w = conv_w.contiguous()
+    conv_w = _whole(conv_w)
     with _on(dev):
-        kv800_hip._check(L.lfm3_hip_conv_chunk(bcx.data_ptr(), bcx.stride(0), conv_w.data_ptr(), state.data_ptr(), qsl.data_ptr(),
+        kv800_hip._check(L.lfm3_hip_conv_chunk(bcx.data_ptr(), ld, conv_w.data_ptr(), state.data_ptr(), qsl.data_ptr(),
                                                R, T, H, out.data_ptr(), taps.data_ptr(), _raw_stream(dev)))
     return out, taps
 
@@ -87,7 +86,7 @@ def conv_commit(state, taps, qsl, kept):
         raise ValueError(f"taps must be (T, {H}) and kept ({R},), got {tuple(taps.shape)}, {tuple(kept.shape)}")
     if R == 0 or H == 0 or taps.shape[0] == 0:
         return
-    taps, kept = taps.contiguous(), kept.contiguous()
+    taps, kept = _whole(taps), kept.contiguous()
     with _on(dev):
         kv800_hip._check(L.lfm3_hip_conv_commit(state.data_ptr(), taps.data_ptr(), qsl.data_ptr(), kept.data_ptr(), R,
                                                 taps.shape[0], H, _raw_stream(dev)))
@@ -115,8 +114,8 @@ def verify_drafts(logits, tokens, qsl, temperature, u, u_next, draft_probs=None)
         _need(draft_probs, "draft_probs", torch.float32, dev)
         if draft_probs.shape != (T, V):
             raise ValueError(f"draft_probs must be ({T}, {V}), got {tuple(draft_probs.shape)}")
-        draft_probs = _row_major(draft_probs)
-    logits = _row_major(logits)
+        draft_probs, ldq = _row_major(draft_probs)
+    logits, ld = _row_major(logits)
     out = torch.empty(T, dtype=torch.int64, device=dev)
     count = torch.empty(R, dtype=torch.int32, device=dev)
     if R == 0 or T == 0:
@@ -126,13 +125,22 @@ def verify_drafts(logits, tokens, qsl, temperature, u, u_next, draft_probs=None)
     tokens, temperature, u, u_next = tokens.contiguous(), temperature.contiguous(), u.contiguous(), u_next.contiguous()
     with _on(dev):
         kv800_hip._check(L.lfm3_hip_verify_drafts(
-            logits.data_ptr(), logits.stride(0), tokens.data_ptr(), qsl.data_ptr(), temperature.data_ptr(), u.data_ptr(),
+            logits.data_ptr(), ld, tokens.data_ptr(), qsl.data_ptr(), temperature.data_ptr(), u.data_ptr(),
             u_next.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
-            0 if draft_probs is None else draft_probs.stride(0), R, T, V, out.data_ptr(), count.data_ptr(), ws.data_ptr(), wsb,
+            0 if draft_probs is None else ldq, R, T, V, out.data_ptr(), count.data_ptr(), ws.data_ptr(), wsb,
             _raw_stream(dev)))
     return out, count
 
 
 def _row_major(x):
-    """x with contiguous rows that do not overlap."""
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+    """x with contiguous rows that do not overlap, and their stride (a size of one may have any stride in torch, and counts as
+    contiguous with it)."""
+    T, V = x.shape
+    ld = x.stride(0) if T > 1 else V
+    return (x, ld) if (V == 1 or x.stride(1) == 1) and ld >= V else (x.clone(memory_format=torch.contiguous_format), V)
+
+
+def _whole(x):
+    """x contiguous and 16-byte aligned."""
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
