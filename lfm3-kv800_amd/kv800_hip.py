@@ -17,6 +17,7 @@ from dataclasses import dataclass
 import numpy as np
 
 import torch
+from torch.multiprocessing.reductions import StorageWeakRef
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "_lib", "libkv800_hip.so")
@@ -748,7 +749,15 @@ def combine(MO, LO, AO, ns):
 
 # ---------------------------------------------------------------- decode
 _PAIRS = OrderedDict()     # (device, cos ptr, sin ptr, rows) -> (cos_t, sin_t, versions, pair table, stream, event)
-_CAPTURED = {}             # pair tables that a captured graph may read: kept, whatever leaves _PAIRS
+_CAPTURED = {}             # pair tables that a captured graph may read: data ptr -> (table, weak refs of cos' and sin's storage)
+
+
+def _keep_for_graph(cos_t, sin_t, t):
+    """Keep the pair table t, which a graph under capture will read, as long as cos_t and sin_t have their storage: the graph
+    reads these two itself, so it is not replayed without them. Tables of storages that are gone are let go."""
+    for k in [k for k, (_, *refs) in _CAPTURED.items() if any(w.expired() for w in refs)]:
+        del _CAPTURED[k]
+    _CAPTURED[t.data_ptr()] = (t, StorageWeakRef(cos_t.untyped_storage()), StorageWeakRef(sin_t.untyped_storage()))
 
 
 def rope_pairs(cos_t, sin_t):
@@ -765,7 +774,7 @@ def rope_pairs(cos_t, sin_t):
     if ent is not None and ent[0] is cos_t and ent[1] is sin_t and ent[2] == ver:
         _PAIRS.move_to_end(key)
         if torch.cuda.is_current_stream_capturing():     # a capture begins by waiting for the device
-            _CAPTURED[ent[3].data_ptr()] = ent[3]
+            _keep_for_graph(cos_t, sin_t, ent[3])
         elif ent[4] != now:
             stream = torch.cuda.current_stream(cos_t.device)
             stream.wait_event(ent[5])
