@@ -50,6 +50,9 @@ int kv800_hip_version(void);
 /* Message of the calling thread's last failure ("" if none). */
 const char* kv800_hip_last_error(void);
 
+/* id[0] = the number of the graph capture that the stream takes part in (no two captures of a process share one), 0 if none. */
+int kv800_hip_capture_id(void* stream, uint64_t* id);
+
 /* Quantize M dense sub-blocks. Replaces kv800.quantize_blocks (kv800.py:56-76).
  * k, v: (M, 256, 4, 128) bf16 (pre-RoPE K, unrotated V), contiguous. out: (M, 51200) bytes.
  * Bit-identical to the reference on CPU torch (fp8 e4m3fn RNE encode, IEEE division, v @ H as the sequential

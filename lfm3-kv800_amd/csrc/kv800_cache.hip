@@ -332,6 +332,19 @@ int kv800_hip_chunk_meta(int32_t* bt, int64_t bt_stride, int64_t npages, const i
   return check_launch("chunk_meta");
 }
 
+int kv800_hip_capture_id(void* stream, uint64_t* id) {
+  KV800_REQUIRE(id, "capture_id: null pointer");
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &st, &n) != hipSuccess) {
+    (void)hipGetLastError();
+    kv800::set_error("capture_id: no such stream");
+    return KV800_EHIP;
+  }
+  id[0] = st == hipStreamCaptureStatusActive ? n : 0;
+  return KV800_OK;
+}
+
 int kv800_hip_read_probe(const void* buf, int64_t bytes, uint32_t* out, int64_t groups, void* stream) {
   KV800_REQUIRE(buf && out, "read_probe: null pointer");
   KV800_REQUIRE(bytes >= 16 && bytes % 16 == 0 && ((uintptr_t)buf % 16) == 0,

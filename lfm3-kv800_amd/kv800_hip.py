@@ -43,6 +43,7 @@ _VP, _I64, _I32, _F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_
 SIGNATURES = {
     "kv800_hip_version": (_I32, []),
     "kv800_hip_last_error": (ctypes.c_char_p, []),
+    "kv800_hip_capture_id": (_I32, [_VP, ctypes.POINTER(ctypes.c_uint64)]),
     "kv800_hip_read_probe": (_I32, [_VP, _I64, _VP, _I64, _VP]),
     "kv800_hip_quantize_blocks": (_I32, [_VP, _VP, _I64, _VP, _VP]),
     "kv800_hip_flush": (_I32, [_VP, _VP, _I64, _I64, _I64, _I64, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _VP, _I64, _I64,
@@ -752,6 +753,14 @@ _PAIRS = OrderedDict()     # (device, cos ptr, sin ptr, rows) -> (cos_t, sin_t, 
 _CAPTURED = {}             # pair tables that a captured graph may read: data ptr -> (table, weak refs of cos' and sin's storage)
 
 
+_BUILDING = {}             # (capture, stream, key) -> (cos_t, sin_t, versions, pair table) of the captures under way
+
+
+def _capture_id(stream):
+    n = ctypes.c_uint64(0)
+    return n.value if ops().kv800_hip_capture_id(stream, ctypes.byref(n)) == 0 else 0
+
+
 def _keep_for_graph(cos_t, sin_t, t):
     """Keep the pair table t, which a graph under capture will read, as long as cos_t and sin_t have their storage: the graph
     reads these two itself, so it is not replayed without them. Tables of storages that are gone are let go."""
@@ -765,7 +774,7 @@ def rope_pairs(cos_t, sin_t):
     tensors. The entry holds the two tables themselves, so their storage cannot be freed and reused by other tensors
     while it is cached; it is rebuilt when either tensor is modified in place (version counter) or replaced. A call on
     another stream than the one that built it waits for it; a table built while a graph is captured belongs to that graph
-    alone, whose replays fill it. A captured call that finds its table reads it as it is then, on every replay: tables
+    alone, whose replays fill it once for all later calls of the capture on that stream. A captured call that finds its table reads it as it is then, on every replay: tables
     changed in place are captured anew."""
     key = (cos_t.device, cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0])
     ent = _PAIRS.get(key)
@@ -782,10 +791,19 @@ def rope_pairs(cos_t, sin_t):
         return ent[3]
     L = ops()
     P = cos_t.shape[0]
+    capturing = torch.cuda.is_current_stream_capturing()
+    cap = _capture_id(now) if capturing else 0
+    for k in [k for k in _BUILDING if _capture_id(k[1]) != k[0]]:      # captures that have ended
+        del _BUILDING[k]
+    mine = _BUILDING.get((cap, now, key))
+    if cap and mine is not None and mine[0] is cos_t and mine[1] is sin_t and mine[2] == ver:
+        return mine[3]
     t = torch.empty(P, 32, dtype=torch.int32, device=cos_t.device)
     with _on(cos_t.device):
         _check(L.kv800_hip_rope_table(_ptr(cos_t), _ptr(sin_t), P, _ptr(t), _stream(cos_t.device)))
-        if torch.cuda.is_current_stream_capturing():
+        if capturing:
+            if cap:
+                _BUILDING[cap, now, key] = (cos_t, sin_t, ver, t)
             return t
         done = torch.cuda.Event()
         done.record(torch.cuda.current_stream(cos_t.device))

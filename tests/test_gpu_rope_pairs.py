@@ -48,3 +48,51 @@ def test_a_captured_table_lives_as_long_as_what_it_is_made_of(hip):
     capture(lambda: hip.decode_chunk(other.P, other.q, other.qsl, other.cos, other.sin))
     gc.collect()
     assert table() is None and len(hip._CAPTURED) == before - 1
+
+
+def test_a_table_missing_at_capture_is_made_once(hip):
+    """Calls of one capture share the table that the first of them makes; it belongs to that capture, and every replay fills it."""
+    c = ref.Cache(hip, [700, 1400], [4, 3], seed=73)
+    want = c.want(hip)
+    hip.rope_pairs(torch.ones_like(c.cos), c.sin)     # the library's first launch
+    tables, graphs = [], []
+    for _ in range(2):
+        def step():
+            a = hip.rope_pairs(c.cos, c.sin)
+            outs = [hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin) for _ in range(2)]
+            b = hip.rope_pairs(c.cos, c.sin)
+            assert b is a
+            tables.append(a)
+            return outs
+        graphs.append(capture(step))
+    assert tables[0] is not tables[1]
+    eager = hip.rope_pairs(c.cos, c.sin)
+    assert eager is not tables[0] and eager is not tables[1] and not hip._BUILDING
+    check(hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin), want, "eager after the captures")
+    for k in range(3):
+        for (g, outs), t in zip(graphs, tables):
+            for x in (*outs, t):
+                x.zero_()
+            g.replay()
+            hip.rope_pairs(torch.rand_like(c.cos), c.sin)
+            torch.cuda.synchronize()
+            for out in outs:
+                check(out, want, f"replay {k}")
+
+
+def test_tables_changed_inside_a_capture(hip):
+    """A table written between two calls of a capture is paired anew by the second."""
+    c = ref.Cache(hip, [700, 1400], [4, 3], seed=74)
+    cos, want = c.cos.clone(), c.want(hip)
+    hip.rope_pairs(torch.ones_like(c.cos), c.sin)
+
+    def step():
+        c.cos.zero_()
+        hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+        c.cos.copy_(cos)
+        return hip.decode_chunk(c.P, c.q, c.qsl, c.cos, c.sin)
+    g, out = capture(step)
+    for k in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        check(out, want, f"replay {k}")
