@@ -362,6 +362,9 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
     dev, R = tokens.device, tokens.shape[0]
     if not 0 <= most < 128:
         raise ValueError("most must be in [0, 128)")
+    if steps > 0 and int(attention.lens.max()) + steps * (most + 1) > attention.nmax:
+        raise ValueError(f"the caches hold {attention.nmax} positions per row, the steps may reach "
+                         f"{int(attention.lens.max()) + steps * (most + 1)}")
     if temperature is None:
         temperature = torch.zeros(R, dtype=torch.float32, device=dev)
     lens = attention.lens.to(dev)
