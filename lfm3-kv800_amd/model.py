@@ -355,7 +355,8 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
     """Decode with drafted tokens: `steps` steps from `tokens` (R,) int64, each of which appends to every row its last token
     and up to `most` drafts, keeps the drafts that the model confirms (spec_ops.verify_drafts) and takes one more token
     behind them. draft(last (R,), lens (R,)) -> (drafts (R, most) int64, counts (R,) int32 of them in use, their
-    distributions (R, most, vocab) fp32 or None), all on the device; lens counts the positions in the caches. temperature
+    distributions (R, most, vocab) fp32 or None), all on the device; lens counts the positions in the caches. Drafts behind a
+    row's count may hold anything, one outside the vocabulary is never kept. temperature
     (R,) fp32, None: greedy. Lengths stay on the device, so a step does not wait for the one before; the attention must be a
     PagedAttention800 with room for steps (most + 1) more positions, most < 128. Returns the rows' new tokens, a list of R
     tensors, and the (steps, R) counts; attention.lens follows."""
@@ -376,7 +377,7 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
         meta = attention.begin_chunk(lens + ql, ql, T, most + 1, attention.lens + (s + 1) * (most + 1))
         i = (at - meta.qsl[meta.row]).clamp(max=most)
         tok = torch.cat((last[:, None], drafts), 1)[meta.row, i]
-        logits = model.chunk(tok, meta)
+        logits = model.chunk(tok.clamp(0, model.cfg.vocab - 1), meta)     # unused and foreign drafts: any token, never kept
         q = None if probs is None or not most else probs[meta.row, i.clamp(max=most - 1)]
         out, kept = so.verify_drafts(logits, tok, meta.qsl, temperature, torch.rand(T, device=dev, generator=generator),
                                      torch.rand(R, device=dev, generator=generator), q)
