@@ -266,6 +266,10 @@ class PagedAttention800:
         self.lens_dev = self.lens.to(self.dev)
         self.lens_bound = self.lens + steps
 
+    def thaw(self):
+        """Undo freeze(): the next step goes by `lens` again. A step recorded before keeps its own lengths and cannot follow."""
+        self.lens_dev = self.lens_bound = None
+
     def begin_step(self):
         """Metadata of the next decode step (every row appends one token) and the start of its flushes."""
         self.lens += 1
@@ -322,6 +326,7 @@ class DecodeGraph:
             logits = model.step(self.tokens, attention.begin_step(), fp32=False)
             self.tokens.copy_(mo.argmax(logits))
         attention.lens = lens          # recording ran no step
+        self.lens_dev = attention.lens_dev   # which the recorded step moves on
         self.logits = logits
         torch.cuda.current_stream(tokens.device).wait_stream(self.stream)
 
@@ -329,6 +334,8 @@ class DecodeGraph:
         """One decode step: returns the (R,) greedy tokens."""
         if self.left <= 0:
             raise RuntimeError("DecodeGraph: the steps it was recorded for are used up")
+        if self.attn.lens_dev is not self.lens_dev:
+            raise RuntimeError("DecodeGraph: the attention's lengths have moved on without it")
         self.left -= 1
         self.attn.lens += 1
         self.graph.replay()
@@ -385,6 +392,8 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
         lens = lens + kept
         last = out[meta.qsl[:-1] + kept - 1]
         got.append((out, kept, meta.row))
-    attention.lens = lens.cpu()
+    if steps > 0:
+        attention.lens = lens.cpu()
+        attention.thaw()
     rows = [torch.cat([out[(row == r) & (out >= 0)] for out, _, row in got]) if got else tokens[:0] for r in range(R)]
     return rows, torch.stack([kept for _, kept, _ in got]) if got else torch.zeros(0, R, dtype=torch.int32, device=dev)
