@@ -442,7 +442,6 @@ __device__ __forceinline__ void chunk_span(ChunkQLds& L, ChunkStage& SA, ChunkSt
 // costing more than the waits that they saved. The part of a tile that it begins with goes
 // to slot w; a tile that starts inside its range goes to slot G + the tile's number (nobody else enters that tile from an
 // earlier entry).
-template <int QT>
 __device__ __forceinline__ ListRow list_row(const ChunkArgs& A, int64_t r) {
   const int64_t a = A.qsl[r], b = A.qsl[r + 1];
   const int n = A.P.N[r], nb = row_blocks(A, r);
@@ -466,10 +465,10 @@ __device__ __forceinline__ void quant_part(ChunkQLds& L, ChunkStage& SA, ChunkSt
   ListRow first = {0, 0, 0, 0};
   int mine = 0;
   if (ra < rb) {
-    first = list_row<QT>(A, ra);
+    first = list_row(A, ra);
     mine = list_size<QT>(first);
   }
-  for (int r = ra + 1; r < rb; ++r) mine += list_size<QT>(list_row<QT>(A, r));
+  for (int r = ra + 1; r < rb; ++r) mine += list_size<QT>(list_row(A, r));
   int inc = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -485,7 +484,7 @@ __device__ __forceinline__ void quant_part(ChunkQLds& L, ChunkStage& SA, ChunkSt
     int x = pre;
     for (int r = ra; r < rb; ++r) {
       A.pre[r] = x;
-      if (r + 1 < rb) x += list_size<QT>(list_row<QT>(A, r));
+      if (r + 1 < rb) x += list_size<QT>(list_row(A, r));
     }
     if (tid == 0) A.pre[R] = C;
   }
@@ -497,7 +496,7 @@ __device__ __forceinline__ void quant_part(ChunkQLds& L, ChunkStage& SA, ChunkSt
     int x = pre, r = ra;
     while (v >= x + list_size<QT>(y)) {
       x += list_size<QT>(y);
-      y = list_row<QT>(A, ++r);
+      y = list_row(A, ++r);
     }
     L.row = r;
     L.pre = x;
@@ -531,7 +530,7 @@ __device__ __forceinline__ void quant_part(ChunkQLds& L, ChunkStage& SA, ChunkSt
     }
     if (v >= v1) return;
     x += sz;
-    y = list_row<QT>(A, ++r);
+    y = list_row(A, ++r);
   }
 }
 
@@ -807,15 +806,6 @@ __device__ __forceinline__ bool exact_tile(ChunkXRows<NW>& Ks, ChunkXRows<NW>& V
       // V^T: lane (g, n) gives 4 values of row 4 g + n / 4 from dim 16 j + 4 (n % 4) on
       uint16_t* vw = Vs.r[w];
       const int vrow = 4 * g + (n >> 2);
-      auto read_vt = [&](int j) {
-        const int o = vrow * 128 + 8 * ((2 * j + ((n & 3) >> 1)) ^ (2 * (vrow & 7))) + 4 * (n & 1);
-        const s4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[o]);
-        const s4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)&vw[o + 16 * 128]);
-        return u4v{__builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 0, 1)),
-                   __builtin_bit_cast(uint32_t, __builtin_shufflevector(t0, t0, 2, 3)),
-                   __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 0, 1)),
-                   __builtin_bit_cast(uint32_t, __builtin_shufflevector(t1, t1, 2, 3))};
-      };
       // A weight of 0 does not take out an infinity or NaN. Where a chunk has a mask, its values are looked over: the largest
       // exponent of each half, all ones in infinities and NaN.
       if (!all && !odd && nq > 1) {
