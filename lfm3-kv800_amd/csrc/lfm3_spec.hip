@@ -616,10 +616,11 @@ __global__ void __launch_bounds__(VT) verify_pick_kernel(VerifyArgs A) {
   if (tid == 0) A.count[r] = (int32_t)(d.t - d.s0 + 1);
 }
 
-// 2,048-value pieces while all rows in them make up to 1,024 workgroups, else 8,192, whose sums and lookups of a piece's row are
-// fewer (256 rows, stats, residual and pick: 73 us, in small pieces 91; one row of 5: 14 us, in large pieces 22; before faster
-// reductions)
-int verify_ve(int64_t T, int64_t V) { return T * ((V + 8 * VT - 1) / (8 * VT)) <= 1024 ? 8 : 32; }
+// Pieces of 2,048 values while all rows in them make up to 9,216 workgroups, else of 8,192, whose sums and lookups of a piece's
+// row are fewer. All kernels, us in small / large pieces, 65,536 logits, drafts without a distribution: 4 rows of logits 11.3 / 18.3,
+// 48 14.3 / 20.2, 128 20.0 / 24.2, 256 (8,192 workgroups) 30.2 / 34.1, 320 37.1 / 39.8, 448 46.2 / 46.6, 640 60.7 / 57.5, 1,280 106 / 91;
+// with one: 4 13.4 / 20.2, 128 24.5 / 26.4, 256 37.9 / 39.4, 320 (10,240) 46.9 / 45.1, 640 77 / 67, 1,280 139 / 107.
+int verify_ve(int64_t T, int64_t V) { return T * ((V + 8 * VT - 1) / (8 * VT)) <= 9216 ? 8 : 32; }
 int64_t verify_pieces(int64_t T, int64_t V) { const int64_t n = VT * verify_ve(T, V); return (V + n - 1) / n; }
 
 template <int VE>

@@ -76,24 +76,32 @@ def test_one_token_per_row(hip, rows, layer):
 # ---------------------------------------------------------------- verification
 def same(case):
     T, V = case[0].shape
-    assert T * -(-V // 2048) > 1024                       # pieces of 8,192
+    assert T * -(-V // 2048) > 9216                       # pieces of 8,192
     assert run_verify(*case) == ref.verify(*case)
 
 
-@pytest.mark.parametrize("V,new", [(65536, [5, 1, 0, 5, 9, 2, 7, 4]), (65536, [33]), (70001, [1] * 40), (24576, [3] * 40),
-                                   (8193, [2, 9, 40, 1] * 6)])
+@pytest.mark.parametrize("V,new", [(65536, [5, 1, 0, 5, 9, 2, 7, 4] * 9), (65536, [300]), (70001, [1] * 270), (24576, [3] * 260),
+                                   (8193, [2, 9, 40, 1] * 36)])
 @pytest.mark.parametrize("probs", [False, True])
 def test_verify_large_pieces(hip, V, new, probs):
     same(verify_case(new, V, V + len(new), probs, (0.8, 1.0, 0.0, 1.3), pad=3))
 
 
+@pytest.mark.parametrize("V,new", [(65536, [5, 0, 3] * 35), (20001, [4] * 230)])
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_many_small_pieces(hip, V, new, probs):
+    case = verify_case(new, V, V + len(new), probs, (0.8, 1.0, 0.0, 1.3), pad=3)
+    assert 8000 < case[0].shape[0] * -(-V // 2048) <= 9760     # about the border of the two sizes
+    assert run_verify(*case) == ref.verify(*case)
+
+
 @pytest.mark.parametrize("probs", [False, True])
 def test_verify_large_pieces_borders(hip, probs):
-    x, tokens, qsl, temp, u, un, q = verify_case([4] * 28, 20001, 3, probs, (1.0, 0.7))
+    x, tokens, qsl, temp, u, un, q = verify_case([4] * 240, 20001, 3, probs, (1.0, 0.7))
     for a, b in ((0.0, 0.0), (1 - 2 ** -24, 1 - 2 ** -24), (0.5, 0.0)):
         same((x, tokens, qsl, temp, torch.full_like(u, a), torch.full_like(un, b), q))
-    x[:56] = 1.5                                          # equal logits
-    temp = torch.tensor([1.0, 0.0, 0.5, float("nan"), float("inf"), -1.0, 1e-30] * 4)
+    x[:480] = 1.5                                         # equal logits
+    temp = torch.tensor([1.0, 0.0, 0.5, float("nan"), float("inf"), -1.0, 1e-30] * 35)[:240]
     tokens[5], tokens[9], tokens[14], tokens[18] = -1, 20001, 1 << 40, 20000
     same((x, tokens, qsl, temp, u, un, q))
 
@@ -102,18 +110,18 @@ def test_verify_large_pieces_borders(hip, probs):
 def test_verify_large_pieces_extreme_temperatures(hip, probs):
     temps = (1e-3, 1e-8, 1e-12, 1e-16, 1e-25, 1e-30, 1e-45, 1e3, 1e20, 1e30)
     V = 20001
-    x, tokens, qsl, temp, u, un, q = verify_case([4] * 40, V, 12, probs, temps)
+    x, tokens, qsl, temp, u, un, q = verify_case([4] * 240, V, 12, probs, temps)
     x[::2, 5::V // 3] = x.max(-1, keepdim=True).values[::2]
     x[1::4, 9] = -torch.finfo(torch.bfloat16).max
-    near = torch.randint(0, 3, (160,), generator=torch.Generator().manual_seed(5)) * (V // 3) + 5
-    tokens = torch.where(torch.rand(160, generator=torch.Generator().manual_seed(6)) < 0.4, near, tokens)
+    near = torch.randint(0, 3, (960,), generator=torch.Generator().manual_seed(5)) * (V // 3) + 5
+    tokens = torch.where(torch.rand(960, generator=torch.Generator().manual_seed(6)) < 0.4, near, tokens)
     same((x, tokens, qsl, temp, u, un, q))
 
 
 @pytest.mark.parametrize("probs", [False, True])
 def test_verify_large_pieces_infinities_and_nan(hip, probs):
     V = 60001
-    x, tokens, qsl, temp, u, un, q = verify_case([5] * 8, V, 4, probs, (1.0, 0.7))
+    x, tokens, qsl, temp, u, un, q = verify_case([5] * 64, V, 4, probs, (1.0, 0.7))
     x[:, 100:50000] = float("-inf")                       # whole pieces without a token
     x[5:10, :50] = torch.finfo(torch.bfloat16).min
     x[10:15, 40000] = float("inf")
@@ -123,20 +131,20 @@ def test_verify_large_pieces_infinities_and_nan(hip, probs):
     x[25:30, :V - 3] = float("-inf")                      # the last three alone
     if probs:
         q[30:35, 55000:] = float("nan")
-        q[35:] = 2.0                                      # above p everywhere
+        q[35:40] = 2.0                                    # above p everywhere
     same((x, tokens, qsl, temp, u, un, q))
 
 
 def test_verify_large_pieces_strides(hip):
     from lfm3_kv800_amd import spec_ops as so
-    V, new = 20001, [3] * 40
+    V, new = 20001, [3] * 320
     x, tokens, qsl, temp, u, un, q = verify_case(new, V, 9, True, (1.0, 0.0))
     want = ref.verify(x, tokens, qsl, temp, u, un, q)
     d = [t.cuda() for t in (tokens, torch.tensor(qsl), temp, u, un)]
     for at, width in ((1, V + 2), (8, V + 15), (5, V + 5)):
-        wide = torch.full((120, width), float("nan"), dtype=torch.bfloat16).cuda()
+        wide = torch.full((960, width), float("nan"), dtype=torch.bfloat16).cuda()
         wide[:, at:at + V] = x.cuda()
-        qw = torch.full((120, width + 4), float("nan")).cuda()
+        qw = torch.full((960, width + 4), float("nan")).cuda()
         qw[:, 4:4 + V] = q.cuda()
         out, count = so.verify_drafts(wide[:, at:at + V], *d, qw[:, 4:4 + V])
         assert (out.tolist(), count.tolist()) == want, at
