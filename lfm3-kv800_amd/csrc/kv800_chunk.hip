@@ -69,24 +69,6 @@ struct ChunkArgs {
   bool xfirst;                     // one launch: the exact part's workgroups come first
 };
 
-// The last i in [0, n) with below(i), for a predicate that holds up to some index, 0 among them: 64-way search by a whole
-// wave, the same result in every lane; n of a few hundred takes two dependent loads.
-template <typename F>
-__device__ __forceinline__ int64_t last_at(int64_t n, F below) {
-  const int lane = threadIdx.x & 63;
-  int64_t lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int64_t step = (hi - lo + 63) / 64, i = lo + lane * step;
-    const int c = __popcll(__ballot(i < hi && below(i < hi ? i : lo)));
-    lo += (c > 0 ? c - 1 : 0) * step;
-    hi = min(hi, lo + step);
-  }
-  return lo;
-}
-__device__ __forceinline__ int64_t row_of(const int64_t* qsl, int64_t R, int64_t t) {
-  return last_at(R, [&](int64_t i) { return qsl[i] <= t; });
-}
-
 // A tile: its row, the row's first token, length and queries, the tile's first query and queries
 struct Tile { int64_t row, t0; int n, c, q0, nq; };
 template <int QT>

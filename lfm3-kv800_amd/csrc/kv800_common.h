@@ -64,6 +64,32 @@ __device__ __forceinline__ float vmax3(float a, float b, float c) {
   return r;
 }
 
+// (a, ia) ranks before (b, ib): the larger value, the smaller index among equals; NaN ranks above every number, the
+// first NaN first (torch.argmax)
+__device__ __forceinline__ bool ranks_before(float a, int ia, float b, int ib) {
+  const bool na = a != a, nb = b != b;
+  if (na || nb) return na && (!nb || ia < ib);
+  return a > b || (a == b && ia < ib);
+}
+// The last i in [0, n) with below(i), for a predicate that holds up to some index, 0 among them: 64-way search by a whole
+// wave, the same result in every lane; n of a few hundred takes two dependent loads.
+template <typename F>
+__device__ __forceinline__ int64_t last_at(int64_t n, F below) {
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 63) / 64, i = lo + lane * step;
+    const int c = __popcll(__ballot(i < hi && below(i < hi ? i : lo)));
+    lo += (c > 0 ? c - 1 : 0) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+// The row that holds token t: the last one with qsl[row] <= t.
+__device__ __forceinline__ int64_t row_of(const int64_t* qsl, int64_t R, int64_t t) {
+  return last_at(R, [&](int64_t i) { return qsl[i] <= t; });
+}
+
 }  // namespace kv800
 
 // ---------------------------------------------------------------- host error plumbing

@@ -25,6 +25,7 @@ namespace {
 
 using kv800::bf2f;
 using kv800::f2bf;
+using kv800::ranks_before;
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -183,13 +184,6 @@ gate_mul_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ g, 
 }
 
 // ---------------------------------------------------------------- greedy token (one workgroup per row)
-// (a, ia) ranks before (b, ib): the larger value, the smaller index among equals; NaN ranks above every number, the
-// first NaN first (torch.argmax)
-__device__ __forceinline__ bool ranks_before(float a, int ia, float b, int ib) {
-  const bool na = a != a, nb = b != b;
-  if (na || nb) return na && (!nb || ia < ib);
-  return a > b || (a == b && ia < ib);
-}
 // thread t scans the 8-element pieces t, t + AT, ... of the row, eight loads at a time (a 65,536-wide row is one
 // round of loads for 1,024 threads, two for 512); the workgroup then reduces the AT bests (the order of the compares
 // does not matter: ranks_before breaks ties by index). 1,024 threads a row while every row has a CU of its own (one

@@ -16,6 +16,8 @@ namespace {
 
 using kv800::bf2f;
 using kv800::f2bf;
+using kv800::ranks_before;
+using kv800::row_of;
 
 __device__ __forceinline__ void load8(const uint16_t* p, float (&f)[8]) {
   const uint4 u = *reinterpret_cast<const uint4*>(p);
@@ -28,20 +30,6 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&f)[8]) {
   u.x = f2bf(f[0]) | (f2bf(f[1]) << 16); u.y = f2bf(f[2]) | (f2bf(f[3]) << 16);
   u.z = f2bf(f[4]) | (f2bf(f[5]) << 16); u.w = f2bf(f[6]) | (f2bf(f[7]) << 16);
   *reinterpret_cast<uint4*>(p) = u;
-}
-
-// The row that holds token t: the last r < R with qsl[r] <= t (qsl[0] = 0). 64-way search by the whole wave, the same
-// result in every lane: R of a few hundred takes two dependent loads.
-__device__ __forceinline__ int64_t row_of(const int64_t* __restrict__ qsl, int64_t R, int64_t t) {
-  const int lane = threadIdx.x & 63;
-  int64_t lo = 0, hi = R;                              // qsl[lo] <= t; qsl[hi] > t, or hi = R
-  while (hi - lo > 1) {
-    const int64_t step = (hi - lo + 63) / 64, i = lo + lane * step;
-    const int c = __popcll(__ballot(i < hi && qsl[i < hi ? i : lo] <= t));   // lane 0 probes lo
-    lo += (c > 0 ? c - 1 : 0) * step;
-    hi = min(hi, lo + step);
-  }
-  return lo;
 }
 
 // ---------------------------------------------------------------- short conv over a row's new tokens
@@ -195,12 +183,6 @@ conv_commit_kernel(uint16_t* __restrict__ state, const uint16_t* __restrict__ ta
 constexpr int VT = 256;                                // threads; a piece holds VT x VE values, VE = 8 or 32 a thread
 struct Stat { double s; float m; int32_t at; };        // 16 bytes
 
-// (a, ia) ranks before (b, ib): larger first, the smaller index among equals, the first NaN before every number
-__device__ __forceinline__ bool ranks_before(float a, int ia, float b, int ib) {
-  const bool na = a != a, nb = b != b;
-  if (na || nb) return na && (!nb || ia < ib);
-  return a > b || (a == b && ia < ib);
-}
 // whether a row with largest logit m is sampled: a temperature in (0, 1e30] and a finite m; else its choice is m's index
 __device__ __forceinline__ bool sampled(float tp, float m) { return tp > 0.f && tp <= 1e30f && m - m == 0.f; }
 // Reductions over a wave, the same in every lane: partners within rows of 16 by DPP (neighbours 1 and 2 apart, then mirrored
