@@ -20,10 +20,12 @@
 //   chunk_merge_kernel   partials of a (tile, KV head) joined, Hadamard transform of the quantized part, bf16 output
 //
 // What bounds it (rates of a large copy 5.1 TB/s, of a large read 6.0 TB/s): long lists of tiles of 4 take about twice the
-// time of their bytes (64 rows x 32768 x 4 tokens, 451 MB: 168 us of quant_part), VALU instructions in 68 % of the cycles, which are
-// table lookups and rotation of the keys; each column's share of them falls with the tile, so that tiles of 8 take 1.4
-// times as long for twice the queries. Window layers read at 4.1 TB/s (398 rows x 5 tokens, 223 MB: 54 us). One row takes
-// 17 + 6 us for 5 tokens at 16384 positions: the latency of four dependent loads, of the lookups and of a second launch.
+// time of their bytes (64 rows x 32768 x 4 tokens, 451 MB: 156 us of quant_part in a long run of calls, up to 230 from an idle
+// card, whose clock is low), VALU instructions in 69 % of the cycles, which are table lookups and rotation of the keys; it reads
+// 677 MB, for rows out of step need every position of the rope table at once, 4 MB beside the stream in each L2. Each column's
+// share of the instructions falls with the tile: tiles of 8 take 1.4 times as long for twice the queries. Window layers
+// read at 4.1 TB/s (398 rows x 5 tokens, 223 MB: 55 us). One row takes 17 + 6 us for 5 tokens at 16384 positions: the latency
+// of exact chunks and of lookups one after the other, and of a second launch.
 #include <mutex>
 
 #include "kv800_attn.h"
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(256, 3) chunk_quant_kernel(ChunkArgs A) {
 // 80 us), in pieces of 16 bytes permuted within the row so that operand reads spread over the banks. One buffer for each: the
 // next chunk's K is requested when this one's scores are formed, its V when this one's V is read, so that each is
 // in flight for about half a chunk, and 16 KB a wave leave room for the eight waves that 256 registers allow on a CU.
-// Window layers, 398 rows x 5: 54 us (223 MB); sliding 64 x 16: 22 us, the latency of five chunks in a row.
+// Window layers, 398 rows x 5: 55 us (223 MB); sliding 64 x 16: 21 us, the latency of five chunks in a row.
 constexpr int XCH = 32;
 template <int NW>
 struct alignas(16) ChunkXRows { uint16_t r[NW][XCH * 128]; };
@@ -1030,9 +1032,12 @@ __global__ void __launch_bounds__(WPC == 1 ? 256 : 64 * WPC) chunk_merge_kernel(
 }
 
 // Queries per tile: 4 (one MFMA column tile) while the rows bring up to 4 tokens on average, else 8, whose keys are unpacked once
-// for twice the queries (64 rows x 32768 x 4, its parts and merge together: 263 us in tiles of 8, half of them empty, 195 in tiles of 4).
+// for twice the queries. All kernels, us in tiles of 4 / 8: 16 rows x 4096 with 4 tokens each 29.8 / 30.8, with 5 35.4 / 37.1; 32 x
+// 16384 72.4 / 71.6, 117 / 88; 64 x 8192 79.4 / 76.7, 121 / 93; 192 x 4096 with 2, 4, 5, 8 102 / 109, 115 / 119, 181 / 145, 192 /
+// 179. Ragged rows about the border, 1 .. 5, 7, 8 tokens: 16 x 4096 24.2 / 30.0, 33.4 / 33.1, 36.0 / 34.7; 32 x 16384 81 / 76, 88 / 81,
+// 100 / 86; 192 x 4096 120 / 123, 128 / 128, 148 / 137: of tiles of 8, those of up to 4 queries take one column tile.
 // Layers without sub-blocks: 4 only while every row brings one token; their kernel passes over an empty second half
-// (window, 398 rows x 5: 66 us in tiles of 4, 54 in tiles of 8).
+// (window, 398 rows x 5: 66 us in tiles of 4, 55 in tiles of 8).
 int chunk_ct(int64_t R, int64_t T, bool quant) { return T <= (quant ? 4 * R : R) ? 1 : 2; }
 
 int64_t chunk_cus() {

@@ -43,8 +43,9 @@ __global__ void __launch_bounds__(256)
 conv_chunk_kernel(const uint16_t* __restrict__ bcx, int64_t stride, const uint16_t* __restrict__ cw,
                   const uint16_t* __restrict__ state, const int64_t* __restrict__ qsl, int64_t R, int64_t T, int64_t H,
                   uint16_t* __restrict__ out, uint16_t* __restrict__ taps) {
-  // workgroups go round the 8 XCDs: four tiles in a row to one of them, whose L2 then holds the taps that three of them
-  // read again (2,048 tokens 12.5 -> 11.0 us, 4,096 18.3 -> 17.0, 16,384 the same; a whole eighth to each: 69 -> 73)
+  // workgroups go round the 8 XCDs: four tiles in a row to one of them, so that three of them may find their first taps in its
+  // L2 (2,048 tokens 12.5 -> 11.0 us, 4,096 18.3 -> 17.0; 16,384 the same: 300 MB fetched, which is every such tap again; a
+  // whole eighth to each: 69 -> 73)
   const int64_t t0 = ((int64_t)((blockIdx.x >> 5) * 8 + (blockIdx.x & 7)) * 4 + ((blockIdx.x >> 3) & 3)) * TT;
   const int64_t c0 = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
   if (t0 >= T) return;                                 // uniform
@@ -178,7 +179,7 @@ conv_commit_kernel(uint16_t* __restrict__ state, const uint16_t* __restrict__ ta
 // All in 64 bits: the running sums of neighbours among 65,536 tokens lie 1e-5 apart where 32-bit exponentials are
 // 1e-7 off, and the choice has to be the same whatever way a row is cut. Bound: the logits' bytes and the exponentials'
 // instructions: about 30 per value, half of them of 64 bits, take longer than the bytes. 256 rows, 722 logits rows of 65,536 with
-// the drafts' distributions (162 MB): stats 40, residual 17, pick 11 us; one row of 5: 3.5, 0 and 8 us, chains of dependent
+// the drafts' distributions (162 MB): stats 37, residual 16, pick 10 us; one row of 5: 3.4, 0 and 8 us, chains of dependent
 // loads and of 64-bit sums over lanes.
 constexpr int VT = 256;                                // threads; a piece holds VT x VE values, VE = 8 or 32 a thread
 struct Stat { double s; float m; int32_t at; };        // 16 bytes
@@ -222,7 +223,8 @@ __device__ __forceinline__ void wave_first(float& m, int& at) {   // the first i
   at = (int)(second ? i.b : i.a);
   if constexpr (K < 5) wave_first<K + 1>(m, at);
 }
-// exp((x - m) / temp) for x <= m, within 2^-42: y = (x - m) / temp with the difference exact, so that a small temperature does
+// exp((x - m) / temp) for x <= m, within 2^-42, by a table of powers of two and a short series (Tang's table-driven
+// exponential): y = (x - m) / temp with the difference exact, so that a small temperature does
 // not enlarge its rounding, = (16 e + j) ln2 / 16 + r, |r| <= ln2 / 32; 16 e + j is the low word of 16 y / ln2 + 1.5 2^52; 2^(j / 16)
 // from a table of 16 in LDS (32 banks: any lanes at once), exp(r) as its series to r^5 / 120 (the next term is 1.4e-13). What
 // lies 800 temp below m, -inf among it, is 2^-1154 and comes out as 0.
@@ -637,9 +639,12 @@ int lfm3_hip_conv_chunk(const uint16_t* bcx, int64_t stride, const uint16_t* con
   KV800_REQUIRE(T <= 0x7FFFFFFF && ny <= 65535, "conv_chunk: too large");
   const hipStream_t s = (hipStream_t)stream;
   // Tokens per workgroup, by the workgroups that one each would make: few, so that every CU has one and a token's taps are
-  // not formed again by its successors' workgroups more often than that costs; 16 where 8 make a round and a third.
-  // H = 2048, us with 1 / 2 / 4 / 8 / 16 / 32: T = 160: 4.2 5.2 6.3 8.5 13 23; 512: 6.7 5.0 5.6 8.1 13 23; 1,024: 14 9.2 8.7 8.3
-  // 14 23; 4,096: 45 29 23 17 20 31; 8,192: 78 52 41 36 31 34; 16,384: 148 104 82 69 75 71; 32,768: 288 198 155 141 143 151.
+  // not formed again by its successors' workgroups more often than that costs; 16 where 8 make more than three rounds of the
+  // CUs and less than six.
+  // H = 2048, us with 1 / 2 / 4 / 8 / 16 / 32, the commit's 4.6 among them: T = 256: 9.0 9.2 10.5 11.3 17 26; 512: 10.3 9.7 10.8
+  // 12.4 16 27; 1,024: 13.9 11.3 11.5 13.1 17 26; 1,280: 15.8 13.3 13.5 14.0 18 33; 4,096: 31 26 25.0 21.9 23.6 35; 6,144: 41 34 31 29.7
+  // 27.9 36; 7,168: 46 38 36 37.3 30.6 37; 10,240: 62 50 46 45.8 41.7 42; 12,288: 72 58 54 52.3 48.1 46; 13,312: 83 71 61 61.9 64.1 61;
+  // 16,384: 123 101 82 72.0 77.6 70; 32,768: 252 194 156 147 149 158.
   const int64_t n = T * ny;
   const auto go = [&](auto tt) {
     constexpr int TT = decltype(tt)::value;

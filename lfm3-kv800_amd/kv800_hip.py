@@ -914,7 +914,7 @@ def decode_chunk(P, q, qsl, cos_t, sin_t):
     positions, P.N[r] of them in all; their K / V rows are in the exact pages already. P.NQ: the sub-blocks flushed before
     these tokens, P.nqmax the host's bound of it; window layers (P.win > 0) read the exact pages and, with P.sk, the
     sinks. cos_t / sin_t (P, 32) bf16, or None: keys as stored. Returns (T, 16, 128) bf16, zeros for the tokens behind the
-    last row's. For chunks of many tokens the assembled prefill (prefill_keys, prefill) takes less time."""
+    last row's. From about 128 new tokens a row on the assembled prefill (prefill_keys, prefill) takes less time."""
     L = ops()
     dev = q.device
     _need(q, "q", torch.bfloat16, dev); _need(qsl, "qsl", torch.int64, dev)

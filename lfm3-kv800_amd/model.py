@@ -365,7 +365,9 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
     distributions (R, most, vocab) fp32 or None), all on the device; lens counts the positions in the caches. Drafts behind a
     row's count may hold anything, one outside the vocabulary is never kept. temperature
     (R,) fp32, None: greedy. Lengths stay on the device, so a step does not wait for the one before; the attention must be a
-    PagedAttention800 with room for steps (most + 1) more positions, most < 128. Returns the rows' new tokens, a list of R
+    PagedAttention800 with room for steps (most + 1) more positions, most < 128. Greedy tokens are those of the one-token loop
+    up to near-ties: the short conv rounds once a sum and not every product, and a block that becomes eligible inside a chunk
+    is read exact by that chunk. Returns the rows' new tokens, a list of R
     tensors, and the (steps, R) counts; attention.lens follows."""
     dev, R = tokens.device, tokens.shape[0]
     if not 0 <= most < 128:
