@@ -774,8 +774,8 @@ def rope_pairs(cos_t, sin_t):
     tensors. The entry holds the two tables themselves, so their storage cannot be freed and reused by other tensors
     while it is cached; it is rebuilt when either tensor is modified in place (version counter) or replaced. A call on
     another stream than the one that built it waits for it; a table built while a graph is captured belongs to that graph
-    alone, whose replays fill it once for all later calls of the capture on that stream. A captured call that finds its table reads it as it is then, on every replay: tables
-    changed in place are captured anew."""
+    alone, whose replays fill it once for all later calls of the capture on that stream. A captured call that finds its
+    table reads it as it is then, on every replay: tables changed in place are captured anew."""
     key = (cos_t.device, cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0])
     ent = _PAIRS.get(key)
     ver = (cos_t._version, sin_t._version)

@@ -13,6 +13,9 @@ def test_drafts_outside_the_vocabulary_do_not_reach_the_embedding(monkeypatch):
     class Attention:
         lens, nmax = torch.tensor([10, 20]), 100
 
+        def thaw(self):
+            pass
+
         def begin_chunk(self, lens, ql, tokens, most, bound):
             qsl = torch.cat([torch.zeros(1, dtype=torch.int64), ql.long().cumsum(0)])
             row = torch.searchsorted(qsl[1:], torch.arange(tokens), right=True)
