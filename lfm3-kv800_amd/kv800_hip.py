@@ -848,11 +848,11 @@ def paged_struct(P, B):
         _need(P.qpool, "qpool", torch.uint8, dev); _need(P.boff, "boff", torch.int64, dev)
         if P.boff.stride(-1) != 1:
             raise ValueError("boff rows must be contiguous")
-        s.qpool, s.boff, s.boff_stride = P.qpool.data_ptr(), P.boff.data_ptr(), _row_stride(P.boff)
+        s.qpool, s.boff, s.boff_stride = P.qpool.data_ptr(), P.boff.data_ptr(), _row_stride(P.boff) if B == 1 else P.boff.stride(0)
         qbytes = _extent(P.qpool)
     else:
         qbytes = 0
-    s.epool, s.eoff, s.eoff_stride = P.epool.data_ptr(), P.eoff.data_ptr(), _row_stride(P.eoff)
+    s.epool, s.eoff, s.eoff_stride = P.epool.data_ptr(), P.eoff.data_ptr(), _row_stride(P.eoff) if B == 1 else P.eoff.stride(0)
     s.ebs, s.e_hs, s.e_ts, s.e_v = int(P.ebs), int(P.e_hs), int(P.e_ts), int(P.e_v)
     sink_elems = 0
     if P.win and P.sk is not None:
