@@ -1,0 +1,448 @@
+// kv8_attn.hip -- attention over the paged 8-bit cache (include/kv8_hip.h), gfx950.
+//
+//   attend_kernel  softmax(scale q . k) v of a step's tokens, a list of (query tile, KV head, 128 positions) in equal shares
+//   merge_kernel   joins what several workgroups have of one (query tile, KV head)
+//
+// Both products run on the bf16 matrix instruction: a code times its power of two is exact in bf16, two codes an instruction, so
+// that scores are those of the held keys in fp32 and a weight is rounded to 8 bits once. The fp8 instructions with block scales
+// would take the codes as they are, but drop products below about 2^-13 of the largest one of a sum: next to a strong channel,
+// scores of 300 were 0.02 off.
+// Operands of 16 x 16 x 32 (lane l: row or column l % 16, g = l / 16): k = 8 g + j. Output: column l % 16, rows 4 g + i. Scores are
+// taken transposed (keys x queries): with the keys of a tile in the cache's slot order the lane's scores are those of the 16
+// tokens 16 g .. of a block, in order, and the lane reads the values of the same: weights never leave their lane.
+#include "kv8_common.h"
+#include "kv800_attn.h"
+
+namespace kv8 {
+namespace {
+
+using kv800::f4;
+
+constexpr int COLS = 16;              // (query, query head) pairs of a tile
+constexpr int STEP = 128;             // positions of a wave's step: two blocks
+
+struct Attend {
+  Cache C;
+  const uint16_t* q;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int bt_cols;
+  const int64_t* lens;
+  const int64_t* qsl;
+  int R;
+  int64_t T;
+  int G, TQ;                          // query heads per KV head, queries per tile
+  int64_t window;
+  float sl2;                          // scale log2(e)
+  uint16_t* out;
+  float* part;                        // 2 slots per workgroup of COLS x (D + 2) floats, NULL: no item is split
+};
+
+struct Row {
+  int64_t q0, p0, n;                  // first token, its position, positions (those the table covers)
+  int c, tiles, st0, steps;           // new tokens, query tiles, first step, steps
+};
+__device__ __forceinline__ Row row_at(const Attend& A, int r) {
+  Row w;
+  w.q0 = max(A.qsl[r], (int64_t)0);
+  const int64_t c = min(A.qsl[r + 1], A.T) - w.q0, n = A.lens[r];
+  w.c = (int)max(c, (int64_t)0);
+  w.p0 = n - w.c;
+  w.n = max(min(n, (int64_t)A.bt_cols * A.C.blocks * BLK), (int64_t)0);
+  w.tiles = (w.c + A.TQ - 1) / A.TQ;
+  const int64_t lo = A.window > 0 ? max(w.p0 + 1 - A.window, (int64_t)0) : 0;
+  w.st0 = (int)(min(lo, w.n) / STEP);
+  w.steps = max((int)((w.n + STEP - 1) / STEP) - w.st0, 1);              // 1 also without keys: the outputs are written
+  return w;
+}
+__device__ __forceinline__ int64_t cost_of(const Attend& A, const Row& w) { return (int64_t)w.tiles * A.C.heads * w.steps; }
+
+// Prefix sums of the rows' list entries: pre[i] those before thread i's `per` rows, pre[256] all.
+struct List {
+  int64_t pre[257];
+  int64_t wave[4];
+};
+__device__ __forceinline__ void scan_rows(const Attend& A, List& L, int per) {
+  const int tid = threadIdx.x;
+  int64_t s = 0;
+  for (int r = tid * per; r < min((tid + 1) * per, A.R); ++r) s += cost_of(A, row_at(A, r));
+  int64_t x = s;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = __shfl_up(x, o);
+    if ((tid & 63) >= o) x += y;
+  }
+  if ((tid & 63) == 63) L.wave[tid >> 6] = x;
+  __syncthreads();
+  int64_t before = 0;
+  for (int w = 0; w < (tid >> 6); ++w) before += L.wave[w];
+  L.pre[tid + 1] = before + x;
+  if (tid == 0) L.pre[0] = 0;
+  __syncthreads();
+}
+// Row that holds list entry x and the entries before that row.
+__device__ __forceinline__ int find_row(const Attend& A, const List& L, int per, int64_t x, int64_t& before) {
+  int lo = 0, hi = 256;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) / 2;
+    if (L.pre[m] <= x) lo = m;
+    else hi = m;
+  }
+  int r = lo * per;
+  before = L.pre[lo];
+  for (; r + 1 < A.R; ++r) {
+    const int64_t c = cost_of(A, row_at(A, r));
+    if (x < before + c) break;
+    before += c;
+  }
+  return r;
+}
+
+// 1 in each byte of w that is a NaN code (0x7F, 0xFF)
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7; }
+// eight codes in bf16, times the power of two f; exact
+__device__ __forceinline__ kv800::b8 wide8(uint32_t a, uint32_t b, float f) {
+  const kv800::bf2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, f, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, f, true),
+                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, f, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, f, true)};
+  return kv800::b8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+}
+
+// One workgroup takes entries [w W / NG, (w + 1) W / NG) of the list (row, query tile, head, step); without `part` (no item is
+// split) workgroup w is item w. The four waves take every fourth step of an item, each with its own maximum, sum and output, and
+// are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
+template <int D>
+__global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
+  constexpr int NT = D / 16, NK = D / 32, LD = D + 4;
+  __shared__ List L;
+  __shared__ __align__(16) float so[4][COLS][LD];
+  __shared__ float sm[4][COLS], sl[4][COLS];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, rr = lane & 15, g = lane >> 4;
+  const int64_t w = blockIdx.x, NG = gridDim.x;
+
+  for (int64_t t = max(A.qsl[A.R], (int64_t)0) + w; t < A.T; t += NG)     // the padding
+    for (int i = tid; i < A.C.heads * A.G * D / 8; i += 256)
+      reinterpret_cast<uint4*>(A.out + t * A.C.heads * A.G * D)[i] = make_uint4(0, 0, 0, 0);
+
+  scan_rows(A, L, per);
+  const int64_t W = L.pre[256];
+  int64_t x = w * W / NG;
+  const int64_t end = (w + 1) * W / NG;
+  if (x >= end) return;
+  int64_t before;
+  int r = find_row(A, L, per, x, before);
+  Row row = row_at(A, r);
+  while (x < end) {
+    while (x >= before + cost_of(A, row)) {
+      before += cost_of(A, row);
+      row = row_at(A, ++r);
+    }
+    const int64_t item = (x - before) / row.steps, at = before + item * row.steps;
+    const int s0 = (int)(x - at), s1 = (int)min((int64_t)row.steps, end - at);
+    const int h = (int)(item % A.C.heads), tile = (int)(item / A.C.heads);
+
+    // ---- the queries of the lane's column
+    const int i = tile * A.TQ + rr / A.G, hq = h * A.G + rr % A.G;
+    const bool have = rr < A.TQ * A.G && i < row.c;
+    const int64_t qp = row.p0 + i, qlo = A.window > 0 ? qp - A.window : -1;   // sees positions (qlo, qp]
+    kv800::b8 qr[NK];        // dims 16 g .. of the lower and (D = 128) upper 64, 8 an instruction
+#pragma unroll
+    for (int e = 0; e < NK; ++e) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (have) u = *reinterpret_cast<const uint4*>(A.q + ((row.q0 + i) * A.C.heads * A.G + hq) * D + (e >> 1) * 64 + 16 * g + 8 * (e & 1));
+      qr[e] = kv800::as_b8(kv800::u4v{u.x, u.y, u.z, u.w});
+    }
+    f4 o[NT];
+#pragma unroll
+    for (int d = 0; d < NT; ++d) o[d] = f4{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, l = 0.f;
+
+    // positions that some query of the tile sees, (tlo, thi], and those that all of them see, [alo, ahi)
+    const int ilast = min(row.c, (tile + 1) * A.TQ) - 1;
+    const int64_t thi = min(row.p0 + ilast, row.n - 1), tlo = A.window > 0 ? row.p0 + tile * A.TQ - A.window : -1;
+    const int64_t ahi = min(row.p0 + tile * A.TQ + 1, row.n), alo = A.window > 0 ? row.p0 + ilast - A.window + 1 : 0;
+
+    for (int st = row.st0 + s0 + wv; st < row.st0 + s1; st += 4) {
+      const int64_t pos = (int64_t)st * STEP;
+      if (pos > thi || pos + STEP <= tlo + 1) continue;
+      // ---- codes of the two blocks; a block that no query sees, or without a page, is not read
+      uint4 kk[8][D / 64], vv[NT][2];
+      float sc[2][2];
+      bool on[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int64_t bp = pos + u * BLK, bi = bp / BLK, col = bi / A.C.blocks;
+        on[u] = bp <= thi && bp + BLK > tlo + 1 && col < A.bt_cols;
+        int64_t page = 0;
+        if (on[u]) {
+          page = A.bt[(int64_t)r * A.bt_stride + col];
+          on[u] = page >= 0 && page < A.C.pages;
+        }
+        if (on[u]) {
+          const int ub = (int)(bi % A.C.blocks);
+          const uint8_t* base = block_of<D>(A.C, page, h, ub);
+          const uint8_t* ex = exps_of(A.C, page, h, ub);
+          sc[u][0] = pow2(held_exponent(ex[0]));
+          sc[u][1] = pow2(held_exponent(ex[1]));
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e)
+              kk[4 * u + a][e] = *reinterpret_cast<const uint4*>(base + ((4 * e + g) * BLK + 16 * a + rr) * 16);
+#pragma unroll
+          for (int d = 0; d < NT; ++d) vv[d][u] = *reinterpret_cast<const uint4*>(base + BLK * D + (g * D + 16 * d + rr) * 16);
+        } else {
+          sc[u][0] = sc[u][1] = 1.f;
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) kk[4 * u + a][e] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int d = 0; d < NT; ++d) vv[d][u] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      // ---- scores of the lane's column: tile a holds tokens 64 (a / 4) + 16 g + 4 (a % 4) + j
+      float s[32];
+#pragma unroll
+      for (int a = 0; a < 8; ++a) {
+        f4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) {
+          c = kv800::mfma_bf(wide8(kk[a][e].x, kk[a][e].y, sc[a >> 2][0]), qr[2 * e], c);
+          c = kv800::mfma_bf(wide8(kk[a][e].z, kk[a][e].w, sc[a >> 2][0]), qr[2 * e + 1], c);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[4 * a + j] = c[j] * A.sl2;
+      }
+      const bool edge = pos < alo || pos + STEP > ahi || !on[0] || !on[1];
+      if (edge) {
+#pragma unroll
+        for (int a = 0; a < 8; ++a)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int64_t t = pos + 64 * (a >> 2) + 16 * g + 4 * (a & 3) + j;
+            if (t > qp || t <= qlo || t >= row.n || !on[a >> 2]) s[4 * a + j] = -INFINITY;
+          }
+      }
+      float mt = s[0];
+#pragma unroll
+      for (int j = 1; j < 32; ++j) mt = fmaxf(mt, s[j]);
+      mt = kv800::max4rows(mt);
+      const float Mn = fmaxf(M, ceilf(mt));
+      if (__any(Mn > M)) {
+        const float alpha = Mn > M ? __builtin_amdgcn_exp2f(M - Mn) : 1.f;    // M = -inf: 0
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[d][j] *= alpha;
+        M = Mn;
+      }
+      // ---- weights
+      const float M0 = M > -INFINITY ? M : 0.f;
+      uint32_t pw[16];
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float p0 = __builtin_amdgcn_exp2f(s[2 * j] - M0), p1 = __builtin_amdgcn_exp2f(s[2 * j + 1] - M0);
+        sum += p0 + p1;
+        pw[j] = kv800::bfpk(p0, p1);
+      }
+      if (__any(sum != sum)) {   // a column whose every key so far is NaN has no maximum, yet its sum counts
+        if (kv800::max4rows(sum != sum ? 1.f : 0.f) > 0.f && M == -INFINITY) M = 0.f;
+      }
+      l += sum;
+      // ---- in a step with a mask, codes that not every query sees: a weight of 0 does not take out a NaN
+      bool poison = false;
+      if (edge) {
+        auto clean = [&](uint32_t& x) {
+          const uint32_t nb = nan_bytes(x);
+          poison |= nb != 0;
+          x &= ~(nb * 255u);
+        };
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) { clean(vv[d][u].x); clean(vv[d][u].y); clean(vv[d][u].z); clean(vv[d][u].w); }
+        poison = __any(poison);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const kv800::b8 pa = kv800::as_b8(kv800::u4v{pw[8 * u], pw[8 * u + 1], pw[8 * u + 2], pw[8 * u + 3]});
+        const kv800::b8 pb = kv800::as_b8(kv800::u4v{pw[8 * u + 4], pw[8 * u + 5], pw[8 * u + 6], pw[8 * u + 7]});
+#pragma unroll
+        for (int d = 0; d < NT; ++d) {
+          o[d] = kv800::mfma_bf(wide8(vv[d][u].x, vv[d][u].y, sc[u][1]), pa, o[d]);
+          o[d] = kv800::mfma_bf(wide8(vv[d][u].z, vv[d][u].w, sc[u][1]), pb, o[d]);
+        }
+      }
+      if (poison) {        // NaN values taken out above go to the queries that see them
+        for (int t = 0; t < STEP; ++t) {
+          const int64_t tp = pos + t;
+          if (!on[t >> 6] || tp > thi) continue;
+          const int64_t bi = tp / BLK;
+          const uint8_t* base = block_of<D>(A.C, A.bt[(int64_t)r * A.bt_stride + bi / A.C.blocks], h, (int)(bi % A.C.blocks)) + BLK * D;
+          if (tp <= qp && tp > qlo && tp < row.n)
+            for (int d = 0; d < NT; ++d)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if ((base[((t >> 4 & 3) * D + 16 * d + 4 * g + j) * 16 + (t & 15)] & 0x7F) == 0x7F) o[d][j] = NAN;
+        }
+      }
+    }
+    // ---- the four waves' parts
+    l = kv800::sum4rows(l);
+    if (g == 0) { sm[wv][rr] = M; sl[wv][rr] = l; }
+#pragma unroll
+    for (int d = 0; d < NT; ++d) *reinterpret_cast<f4*>(&so[wv][rr][16 * d + 4 * g]) = o[d];
+    __syncthreads();
+    {
+      const int c = tid >> 4, d0 = (tid & 15) * (D / 16);
+      float m = sm[0][c];
+#pragma unroll
+      for (int k = 1; k < 4; ++k) m = fmaxf(m, sm[k][c]);
+      float ls = 0.f, acc[D / 16];
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = sm[k][c] > -INFINITY ? __builtin_amdgcn_exp2f(sm[k][c] - m) : 0.f;
+        if (sm[k][c] > -INFINITY) {
+          ls += f * sl[k][c];
+#pragma unroll
+          for (int e = 0; e < D / 16; ++e) acc[e] += f * so[k][c][d0 + e];
+        }
+      }
+      if (s0 == 0 && s1 == row.steps) {
+        const int ic = tile * A.TQ + c / A.G;
+        if (c < A.TQ * A.G && ic < row.c) {
+          const float inv = ls == 0.f ? 0.f : 1.f / ls;
+          uint16_t* dst = A.out + ((row.q0 + ic) * A.C.heads * A.G + h * A.G + c % A.G) * D + d0;
+          uint32_t y[D / 32];
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) y[e] = kv800::bfpk(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+          if (D == 128) *reinterpret_cast<uint4*>(dst) = make_uint4(y[0], y[1], y[D / 32 - 2], y[D / 32 - 1]);
+          else *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[1]);
+        }
+      } else {
+        float* pt = A.part + ((2 * w + (s0 == 0 ? 1 : 0)) * COLS + c) * (D + 2);
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) pt[d0 + e] = acc[e];
+        if (d0 == 0) { pt[D] = m; pt[D + 1] = ls; }
+      }
+    }
+    __syncthreads();
+    x = at + s1;
+  }
+}
+
+// One workgroup per (workgroup of the list, column): if that one began an item that others finish, its part and theirs, in order.
+template <int D>
+__global__ void __launch_bounds__(256) merge_kernel(Attend A, int per) {
+  __shared__ List L;
+  __shared__ float red[256 / D][D], rl[256 / D];
+  const int64_t w = blockIdx.x, NG = gridDim.x;
+  const int c = blockIdx.y, tid = threadIdx.x;
+  scan_rows(A, L, per);
+  const int64_t W = L.pre[256], a = w * W / NG, end = (w + 1) * W / NG;
+  if (a >= end) return;                            // uniform, as the returns below
+  int64_t before;
+  const int r = find_row(A, L, per, end - 1, before);
+  const Row row = row_at(A, r);
+  const int64_t item = (end - 1 - before) / row.steps, at = before + item * row.steps;
+  if (at < a || at + row.steps <= end) return;     // the last item began earlier, or is whole here
+  const int h = (int)(item % A.C.heads), tile = (int)(item / A.C.heads), i = tile * A.TQ + c / A.G;
+  if (c >= A.TQ * A.G || i >= row.c) return;
+  const int64_t wl = ((at + row.steps) * NG + W - 1) / W - 1;   // the workgroup with the item's last entry: the least w' with (w' + 1) W / NG >= its end
+  const int d = tid % D, part = tid / D;
+  auto slot = [&](int64_t k) { return A.part + ((2 * k + (k == w ? 1 : 0)) * COLS + c) * (D + 2); };
+  float m = -INFINITY;
+  for (int64_t k = w; k <= wl; ++k) {
+    if (k * W / NG == (k + 1) * W / NG) continue;
+    m = fmaxf(m, slot(k)[D]);
+  }
+  float acc = 0.f, l = 0.f;
+  for (int64_t k = w + part; k <= wl; k += 256 / D) {
+    if (k * W / NG == (k + 1) * W / NG) continue;
+    const float* s = slot(k);
+    const float mk = s[D];
+    if (mk > -INFINITY) {
+      const float f = __builtin_amdgcn_exp2f(mk - m);
+      acc += f * s[d];
+      l += f * s[D + 1];
+    }
+  }
+  red[part][d] = acc;
+  if (d == 0) rl[part] = l;
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int k = 1; k < 256 / D; ++k) { acc += red[k][d]; l += rl[k]; }
+  A.out[((row.q0 + i) * A.C.heads * A.G + h * A.G + c % A.G) * D + d] = (uint16_t)kv800::f2bf(l == 0.f ? 0.f : acc / l);
+}
+
+// ---------------------------------------------------------------- host
+struct Plan {
+  int TQ, G;
+  int64_t groups;
+  bool split;
+};
+Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
+  Plan p;
+  p.G = (int)(heads / c->kv_heads);
+  p.TQ = COLS / p.G;
+  const int64_t tiles = (T + p.TQ - 1) / p.TQ + (T < R ? T : R);          // of all rows, at most
+  int64_t steps = (bt_cols * c->blocks * BLK + STEP - 1) / STEP;          // of an item, at most
+  if (window > 0) {
+    const int64_t most = (window + T + STEP - 2) / STEP + 1;
+    steps = most < steps ? most : steps;
+  }
+  const int64_t entries = tiles * c->kv_heads * (steps > 0 ? steps : 1);
+  p.groups = (entries + 3) / 4;
+  if (p.groups > 512) p.groups = 512;
+  p.split = true;
+  return p;
+}
+
+}  // namespace
+}  // namespace kv8
+
+extern "C" {
+
+int64_t kv8_hip_attend_workspace(const kv8_cache_t* cache, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
+  if (!kv8::valid(cache) || heads <= 0 || heads % cache->kv_heads || heads / cache->kv_heads > kv8::COLS || R <= 0 || T <= 0) return 0;
+  const kv8::Plan p = kv8::plan(cache, heads, R, T, bt_cols, window);
+  return p.split ? p.groups * 2 * kv8::COLS * (cache->dim + 2) * 4 : 0;
+}
+
+int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, const int32_t* bt, int64_t bt_stride,
+                   int64_t bt_cols, const int64_t* lens, const int64_t* qsl, int64_t R, int64_t T, int64_t window,
+                   float scale, uint16_t* out, void* ws, int64_t ws_bytes, void* stream) {
+  KV800_REQUIRE(kv8::valid(cache), "kv8_attend: bad cache descriptor");
+  KV800_REQUIRE(R >= 0 && T >= 0 && bt_cols >= 0 && bt_stride >= 0 && window >= 0, "kv8_attend: negative size");
+  KV800_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads / cache->kv_heads <= kv8::COLS,
+                "kv8_attend: heads must be a multiple of the cache's, up to 16 times");
+  KV800_REQUIRE(bt_cols <= INT32_MAX / (cache->blocks * kv8::BLK), "kv8_attend: the table covers 2^31 positions or more");
+  KV800_REQUIRE(R <= INT32_MAX / 512 && T <= INT32_MAX / 512, "kv8_attend: too many tokens or rows");
+  if (T == 0) return KV800_OK;
+  KV800_REQUIRE(R > 0, "kv8_attend: tokens without rows");
+  KV800_REQUIRE(q && lens && qsl && out && (bt || bt_cols == 0), "kv8_attend: null pointer");
+  KV800_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0, "kv8_attend: q and out must be 16-byte aligned");
+  const kv8::Plan p = kv8::plan(cache, heads, R, T, bt_cols, window);
+  const int64_t need = kv8_hip_attend_workspace(cache, heads, R, T, bt_cols, window);
+  KV800_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), "kv8_attend: %lld bytes of 16-byte aligned workspace needed",
+                (long long)need);
+  kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window,
+                   scale * 1.4426950408889634f, out, (float*)ws};
+  const int per = (int)((R + 255) / 256);
+  const dim3 grid((unsigned)p.groups);
+  if (cache->dim == 128) hipLaunchKernelGGL(kv8::attend_kernel<128>, grid, dim3(256), 0, (hipStream_t)stream, A, per);
+  else hipLaunchKernelGGL(kv8::attend_kernel<64>, grid, dim3(256), 0, (hipStream_t)stream, A, per);
+  int rc = kv800::check_launch("kv8_attend");
+  if (rc != KV800_OK || !p.split) return rc;
+  const dim3 mg((unsigned)p.groups, kv8::COLS);
+  if (cache->dim == 128) hipLaunchKernelGGL(kv8::merge_kernel<128>, mg, dim3(256), 0, (hipStream_t)stream, A, per);
+  else hipLaunchKernelGGL(kv8::merge_kernel<64>, mg, dim3(256), 0, (hipStream_t)stream, A, per);
+  return kv800::check_launch("kv8_attend merge");
+}
+
+}  // extern "C"
