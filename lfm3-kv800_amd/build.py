@@ -19,7 +19,7 @@ ARCH = "gfx950"
 SOURCES = {"kv800_quant.hip": ["-ffp-contract=off", "-mllvm", "-amdgpu-mfma-vgpr-form"], "kv800_decode.hip": ["-fno-strict-aliasing", "-mllvm", "-amdgpu-mfma-vgpr-form"],
            "kv800_chunk.hip": ["-fno-strict-aliasing", "-mllvm", "-amdgpu-mfma-vgpr-form"],
            "kv800_cache.hip": [], "kv800_prefill.hip": [], "lfm3_model.hip": [], "lfm3_gemm.hip": [], "lfm3_spec.hip": [],
-           "kv8_cache.hip": [], "kv8_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+           "kv8_cache.hip": [], "lfm3_int8.hip": [], "kv8_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 COMMON = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", INCLUDE, "-I", CSRC]
 
