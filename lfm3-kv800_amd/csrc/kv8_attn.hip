@@ -20,6 +20,7 @@ using kv800::f4;
 
 constexpr int COLS = 16;              // (query, query head) pairs of a tile
 constexpr int STEP = 128;             // positions of a wave's step: two blocks
+constexpr float LAZY = 8.f;           // log2 units by which a running maximum may lag over a long list of keys
 
 struct Attend {
   Cache C;
@@ -33,7 +34,8 @@ struct Attend {
   int64_t T;
   int G, TQ;                          // query heads per KV head, queries per tile
   int64_t window;
-  float sl2;                          // scale log2(e)
+  float sl2;                          // |scale| log2(e)
+  uint32_t flip;                      // sign bits of two bf16 for a negative scale: q changes its sign
   uint16_t* out;
   float* part;                        // 2 slots per workgroup of COLS x (D + 2) floats, NULL: no item is split
 };
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
     for (int e = 0; e < NK; ++e) {
       uint4 u = make_uint4(0, 0, 0, 0);
       if (have) u = *reinterpret_cast<const uint4*>(A.q + ((row.q0 + i) * A.C.heads * A.G + hq) * D + (e >> 1) * 64 + 16 * g + 8 * (e & 1));
-      qr[e] = kv800::as_b8(kv800::u4v{u.x, u.y, u.z, u.w});
+      qr[e] = kv800::as_b8(kv800::u4v{u.x ^ A.flip, u.y ^ A.flip, u.z ^ A.flip, u.w ^ A.flip});
     }
     f4 o[NT];
 #pragma unroll
@@ -380,6 +382,249 @@ __global__ void __launch_bounds__(256) merge_kernel(Attend A, int per) {
   A.out[((row.q0 + i) * A.C.heads * A.G + h * A.G + c % A.G) * D + d] = (uint16_t)kv800::f2bf(l == 0.f ? 0.f : acc / l);
 }
 
+// ---------------------------------------------------------------- many new tokens a row
+__global__ void __launch_bounds__(256) zero_padding_kernel(const int64_t* __restrict__ total, int64_t T, int64_t width, uint16_t* __restrict__ out) {
+  for (int64_t t = max(*total, (int64_t)0) + blockIdx.x; t < T; t += gridDim.x)
+    for (int64_t i = threadIdx.x; i < width / 8; i += 256) reinterpret_cast<uint4*>(out + t * width)[i] = make_uint4(0, 0, 0, 0);
+}
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ f16v mfma32(kv800::u4v a, kv800::u4v b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(kv800::as_b8(a), kv800::as_b8(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float halves_max(float x) {
+  const float2 p = kv800::halves32(x);
+  return fmaxf(p.x, p.y);
+}
+
+// One workgroup: NW waves of 32 columns ((query, query head) of one KV head), all over the same blocks of 64 tokens, which go
+// through LDS in bf16, two buffers: the next block's codes, loaded a block earlier, are widened and stored while the present
+// one is multiplied, one barrier a block. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 (lane l: row or column l % 32, k = 8 (l / 32) + j;
+// output column l % 32, rows 8 b + 4 (l / 32) + i), so a column's weights and sums stay in its two lanes. Row 8 b + 4 h + i of
+// key tile a is token 32 a + 16 (b / 2) + 8 h + 4 (b % 2) + i: the lane's weights are then those of 8 tokens side by side, half
+// of a piece of the values.
+template <int D, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int64_t ntiles, int splits, float* __restrict__ part) {
+  constexpr int NT = D / 32, NK = D / 16, NP = 4 * D / (64 * NW);          // dim tiles, k-steps, pieces of K (and V) a thread stages
+  constexpr int KB = BLK * D * 2;                                          // bytes of a block's keys in bf16
+  __shared__ __align__(16) uint8_t lds[2][2 * KB];
+  __shared__ int flag[2];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, cl = lane & 31, hf = lane >> 5;
+  const int H = A.C.heads, Hq = H * A.G;
+  // workgroup b runs on XCD b % 8: where the heads divide 8, an XCD has one head and every (8 / heads)-th tile of it, so that
+  // its L2 holds one head's blocks; the last tiles first, which see the most
+  int64_t b = blockIdx.x;
+  const int sp = (int)(b % splits);
+  b /= splits;
+  int h;
+  int64_t ti;
+  if (8 % H == 0 && splits == 1) {
+    const int xs = 8 / H, x = (int)(b & 7);
+    h = x / xs;
+    ti = (b >> 3) * xs + x % xs;
+  } else {
+    h = (int)(b % H);
+    ti = b / H;
+  }
+  if (ti >= ntiles) return;                                               // uniform, as every return
+  ti = ntiles - 1 - ti;
+  const int64_t r = kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / TQ + i <= ti; });
+  const Row row = row_at(A, (int)r);
+  const int64_t tile = ti - (row.q0 / TQ + r);
+  if (tile < 0 || tile * TQ >= row.c) return;
+  const int i0 = (int)tile * TQ, ilast = min(row.c, i0 + TQ) - 1;         // queries [i0, ilast] of the row
+  const int cc = wv * 32 + cl, iq = i0 + cc / A.G, hq = h * A.G + cc % A.G;
+  const bool have = cc < TQ * A.G && iq <= ilast;
+  const int64_t qp = row.p0 + iq, qlo = A.window > 0 ? qp - A.window : -1;
+  const bool busy = __any(have);                                          // waves without a column stage only
+
+  kv800::u4v qr[NK];
+#pragma unroll
+  for (int s = 0; s < NK; ++s) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (have) u = *reinterpret_cast<const uint4*>(A.q + ((row.q0 + iq) * Hq + hq) * D + 16 * s + 8 * hf);
+    qr[s] = kv800::u4v{u.x ^ A.flip, u.y ^ A.flip, u.z ^ A.flip, u.w ^ A.flip};
+  }
+  // blocks that some query sees, and positions that all of them see
+  const int64_t thi = min(row.p0 + ilast, row.n - 1), tlo = A.window > 0 ? max(row.p0 + i0 - A.window + 1, (int64_t)0) : 0;
+  const int64_t ahi = min(row.p0 + i0 + 1, row.n), alo = A.window > 0 ? row.p0 + ilast - A.window + 1 : 0;
+  int b0 = (int)(tlo / BLK), b1 = thi < tlo ? b0 : (int)(thi / BLK) + 1;
+  {
+    const int per = (b1 - b0 + splits - 1) / splits;
+    b0 = min(b1, b0 + sp * per);
+    b1 = min(b1, b0 + per);
+  }
+
+  // ---- staging: the codes of block bi into registers, later widened into LDS
+  uint4 rk[NP], rv[NP];
+  float sk = 1.f, sv = 1.f;
+  auto page_of = [&](int bi) -> int {
+    const int col = bi / A.C.blocks;
+    const int p = bi < b1 && col < A.bt_cols ? A.bt[r * A.bt_stride + col] : -1;
+    return p < A.C.pages ? p : -1;
+  };
+  auto load = [&](int bi, int page) {
+    if (page >= 0) {
+      const uint8_t* base = block_of<D>(A.C, page, h, bi % A.C.blocks);
+      const uint8_t* ex = exps_of(A.C, page, h, bi % A.C.blocks);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        rk[j] = *reinterpret_cast<const uint4*>(base + (tid + j * 64 * NW) * 16);
+        rv[j] = *reinterpret_cast<const uint4*>(base + BLK * D + (tid + j * 64 * NW) * 16);
+      }
+      sk = pow2(held_exponent(ex[0]));
+      sv = pow2(held_exponent(ex[1]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) rk[j] = rv[j] = make_uint4(0, 0, 0, 0);
+      sk = sv = 1.f;
+    }
+  };
+  auto is_edge = [&](int bi) { return (int64_t)bi * BLK < alo || (int64_t)bi * BLK + BLK > ahi; };
+  auto store = [&](int bi, int buf) {
+    if (is_edge(bi)) {      // a weight of 0 does not take out a NaN: NaN values leave the block, and are dealt out afterwards
+      bool any = false;
+      auto clean = [&](uint32_t& x) {
+        const uint32_t nb = nan_bytes(x);
+        any |= nb != 0;
+        x &= ~(nb * 255u);
+      };
+#pragma unroll
+      for (int j = 0; j < NP; ++j) { clean(rv[j].x); clean(rv[j].y); clean(rv[j].z); clean(rv[j].w); }
+      if (any) flag[buf] = bi;
+    }
+    uint8_t* kd = lds[buf];
+    uint8_t* vd = lds[buf] + KB;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const int p = tid + j * 64 * NW;
+      const int dg = p >> 6, slot = p & 63, a4 = slot >> 4, g = (slot >> 2) & 3;
+      const int at = 32 * (g >> 1) + 8 * (2 * (g & 1) + (a4 & 1)) + 4 * (a4 >> 1) + (slot & 3);
+      *reinterpret_cast<kv800::b8*>(kd + ((dg * 2) * BLK + at) * 16) = wide8(rk[j].x, rk[j].y, sk);
+      *reinterpret_cast<kv800::b8*>(kd + ((dg * 2 + 1) * BLK + at) * 16) = wide8(rk[j].z, rk[j].w, sk);
+      const int tg = p / D, d = p % D;
+      *reinterpret_cast<kv800::b8*>(vd + ((tg * 2) * D + d) * 16) = wide8(rv[j].x, rv[j].y, sv);
+      *reinterpret_cast<kv800::b8*>(vd + ((tg * 2 + 1) * D + d) * 16) = wide8(rv[j].z, rv[j].w, sv);
+    }
+  };
+
+  f16v o[NT];
+#pragma unroll
+  for (int d = 0; d < NT; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+  float m = have ? -1e30f : 1e30f, l = 0.f;       // columns without a query never ask for a rescale
+  const float lazy = part || A.window > 0 ? 0.f : LAZY;
+
+  if (tid < 2) flag[tid] = -1;
+  int page = page_of(b0), now = page, next = page_of(b0 + 1);
+  if (b0 < b1) load(b0, page);
+  __syncthreads();
+  if (b0 < b1) store(b0, b0 & 1);
+  load(b0 + 1, next);
+  __syncthreads();
+  for (int bi = b0; bi < b1; ++bi) {
+    const int buf = bi & 1;
+    const int after = page_of(bi + 2);
+    if (bi + 1 < b1) {
+      store(bi + 1, buf ^ 1);
+      load(bi + 2, after);
+    }
+    if (busy) {
+      const uint8_t* kd = lds[buf] + (hf * BLK + cl) * 16;
+      __builtin_amdgcn_s_setprio(0);
+      f16v s[2];
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const kv800::u4v x = *reinterpret_cast<const kv800::u4v*>(kd + (2 * k * BLK + 32 * a) * 16);
+          const f16v zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          s[a] = mfma32(x, qr[k], k == 0 ? zero : s[a]);
+        }
+      const bool edge = now < 0 || is_edge(bi);
+      if (edge) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int64_t t = (int64_t)bi * BLK + 32 * a + 16 * (v >> 3) + 8 * hf + (v & 7);
+            if (t > qp || t <= qlo || t >= row.n || now < 0) s[a][v] = -INFINITY;
+          }
+      }
+      __builtin_amdgcn_s_setprio(2);
+      float mt = -INFINITY;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) mt = fmaxf(fmaxf(mt, s[a][v]), s[a][v + 1]);
+      mt = halves_max(mt) * A.sl2;
+      if (__any(mt > m + lazy)) {
+        const float mn = fmaxf(m, mt), alpha = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < NT; ++d) o[d] *= alpha;
+      }
+      __builtin_amdgcn_s_setprio(1);
+      const uint8_t* vd = lds[buf] + KB + (hf * D + cl) * 16;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], A.sl2, -m));
+          sum += p[e];
+        }
+        const kv800::u4v pw = {kv800::bfpk(p[0], p[1]), kv800::bfpk(p[2], p[3]), kv800::bfpk(p[4], p[5]), kv800::bfpk(p[6], p[7])};
+#pragma unroll
+        for (int d = 0; d < NT; ++d) {
+          const kv800::u4v x = *reinterpret_cast<const kv800::u4v*>(vd + (2 * k * D + 32 * d) * 16);
+          o[d] = mfma32(x, pw, o[d]);
+        }
+      }
+      l += sum;
+      if (edge && now >= 0 && flag[buf] == bi) {
+        const uint8_t* base = block_of<D>(A.C, now, h, bi % A.C.blocks) + BLK * D;
+        for (int t = 0; t < BLK; ++t) {
+          const int64_t tp = (int64_t)bi * BLK + t;
+          if (tp <= qp && tp > qlo && tp < row.n)
+#pragma unroll
+            for (int d = 0; d < NT; ++d)
+#pragma unroll
+              for (int v = 0; v < 16; ++v)
+                if ((base[((t >> 4) * D + 32 * d + 8 * (v >> 2) + 4 * hf + (v & 3)) * 16 + (t & 15)] & 0x7F) == 0x7F) o[d][v] = NAN;
+        }
+      }
+    }
+    now = next;
+    next = after;
+    __syncthreads();
+  }
+  const float2 ls = kv800::halves32(l);
+  l = ls.x + ls.y;
+  if (!have) return;
+  if (part) {
+    float* pp = part + (((row.q0 + iq) * Hq + hq) * splits + sp) * (D + 4);
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<f4*>(pp + 32 * d + 8 * c + 4 * hf) = f4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
+    if (hf == 0) { pp[D] = m; pp[D + 1] = l; }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* dst = A.out + ((row.q0 + iq) * Hq + hq) * D + 4 * hf;
+#pragma unroll
+  for (int d = 0; d < NT; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<uint2*>(dst + 32 * d + 8 * c) =
+          make_uint2(kv800::bfpk(o[d][4 * c] * inv, o[d][4 * c + 1] * inv), kv800::bfpk(o[d][4 * c + 2] * inv, o[d][4 * c + 3] * inv));
+}
+
 // ---------------------------------------------------------------- host
 struct Plan {
   int TQ, G;
@@ -421,6 +666,7 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
   KV800_REQUIRE(R >= 0 && T >= 0 && bt_cols >= 0 && bt_stride >= 0 && window >= 0, "kv8_attend: negative size");
   KV800_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads / cache->kv_heads <= kv8::COLS,
                 "kv8_attend: heads must be a multiple of the cache's, up to 16 times");
+  KV800_REQUIRE(fabsf(scale) > 0.f && fabsf(scale) < INFINITY, "kv8_attend: scale must be finite and not 0");
   KV800_REQUIRE(bt_cols <= INT32_MAX / (cache->blocks * kv8::BLK), "kv8_attend: the table covers 2^31 positions or more");
   KV800_REQUIRE(R <= INT32_MAX / 512 && T <= INT32_MAX / 512, "kv8_attend: too many tokens or rows");
   if (T == 0) return KV800_OK;
@@ -432,8 +678,17 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
   KV800_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), "kv8_attend: %lld bytes of 16-byte aligned workspace needed",
                 (long long)need);
   kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window,
-                   scale * 1.4426950408889634f, out, (float*)ws};
+                   fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, out, (float*)ws};
   const int per = (int)((R + 255) / 256);
+  if (T * p.G >= 64 * R) {
+    const int NW = 4, TQ = 32 * NW / p.G;
+    const int64_t ntiles = T / TQ + R, xs = 8 % cache->kv_heads == 0 ? 8 / cache->kv_heads : 1;
+    const dim3 grid((unsigned)((ntiles + xs - 1) / xs * xs * cache->kv_heads));
+    hipLaunchKernelGGL(kv8::zero_padding_kernel, dim3(64), dim3(256), 0, (hipStream_t)stream, qsl + R, T, heads * cache->dim, out);
+    if (cache->dim == 128) hipLaunchKernelGGL((kv8::prompt_kernel<128, 4>), grid, dim3(64 * NW), 0, (hipStream_t)stream, A, TQ, ntiles, 1, nullptr);
+    else hipLaunchKernelGGL((kv8::prompt_kernel<64, 4>), grid, dim3(64 * NW), 0, (hipStream_t)stream, A, TQ, ntiles, 1, nullptr);
+    return kv800::check_launch("kv8_attend prompt");
+  }
   const dim3 grid((unsigned)p.groups);
   if (cache->dim == 128) hipLaunchKernelGGL(kv8::attend_kernel<128>, grid, dim3(256), 0, (hipStream_t)stream, A, per);
   else hipLaunchKernelGGL(kv8::attend_kernel<64>, grid, dim3(256), 0, (hipStream_t)stream, A, per);

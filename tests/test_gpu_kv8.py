@@ -112,7 +112,7 @@ def check_attend(kv8, data, exps, q, bt, lens, qsl, window=0, scale=None):
 
 
 ATTENDS = [([0], [1]), ([62], [1]), ([63], [2]), ([127], [1]), ([128], [1]), ([700, 0, 5, 1300], [1, 1, 1, 1]), ([40, 300, 0, 129], [3, 0, 17, 6]),
-           ([0, 70], [150, 40]), ([2500], [5])]
+           ([0, 70], [150, 40]), ([2500], [5]), ([0], [300]), ([513, 64, 9, 200], [129, 0, 200, 1]), ([1000], [65])]
 
 
 @pytest.mark.parametrize("window", [0, 1, 100, 256])
@@ -141,6 +141,30 @@ def test_attend_sees_nothing_else(kv8):
         q = torch.randn(T, 8, 128, generator=g).to(torch.bfloat16)
         got = check_attend(kv8, data, exps, q, bt, lens, qsl, window)
         assert not got[:4].isnan().any() and got[4:8, :4, 7].isnan().all() and not got[4:8, :4, :7].isnan().any()
+
+
+def test_prompt_sees_nothing_else(kv8):
+    """The same in prompt chunks, at their causal edge and at the window's."""
+    for window, D in ((0, 128), (90, 64)):
+        data, exps, bt, lens, qsl, T, g = rows(kv8, 19, [70, 0], [150, 131], 1, D, 64)
+        K, V = ref.tables(D)
+        for r in range(2):
+            n, c = int(lens[r]), int(qsl[r + 1] - qsl[r])
+            for p in list(range(n, -(-n // 64) * 64)) + ([p for p in range(max(0, n - c - 1 - window))] if window else []):
+                data[int(bt[r, p // 64]), :, 0, 0, K[p % 64]] = 0x7F
+                data[int(bt[r, p // 64]), :, 0, 1, V[p % 64]] = 0xFF
+        data[int(bt[0, 2]), 0, 0, 1, V[140 % 64, 9]] = 0xFF
+        data[int(bt[1, 1]), 0, 0, 0, K[80 % 64, 33]] = 0x7F
+        q = torch.randn(T, 4, D, generator=g).to(torch.bfloat16)
+        got = check_attend(kv8, data, exps, q, bt, lens, qsl, window)
+        assert not got[:70].isnan().any() and got[70, :, 9].isnan().all() and not got[150:230].isnan().any() and got[230].isnan().all()
+
+
+def test_negative_scale(kv8):
+    for new in ([2, 1], [100, 80]):
+        data, exps, bt, lens, qsl, T, g = rows(kv8, 6, [200, 10], new, 2, 64, 64)
+        q = torch.randn(T, 4, 64, generator=g).to(torch.bfloat16)
+        check_attend(kv8, data, exps, q, bt, lens, qsl, scale=-0.1)
 
 
 def test_attend_all_nan(kv8):

@@ -74,7 +74,7 @@ def test_attend_host_checks(lib):
     for k in BAD:
         refused(lib, f(desc(**k)), b"descriptor")
     for k in (dict(q=None), dict(out=None), dict(bt=None), dict(lens=None), dict(qsl=None), dict(q=A + 8), dict(out=A + 8), dict(heads=0), dict(heads=6), dict(heads=68),
-              dict(R=0), dict(R=-1), dict(T=-1), dict(win=-1), dict(bc=1 << 24), dict(ws=None), dict(ws=A + 8), dict(wsb=need - 1)):
+              dict(R=0), dict(R=-1), dict(T=-1), dict(win=-1), dict(scale=0.0), dict(scale=float('inf')), dict(scale=float('nan')), dict(bc=1 << 24), dict(ws=None), dict(ws=A + 8), dict(wsb=need - 1)):
         refused(lib, f(**k), b"kv8_attend")
     assert f(T=0) == 0
     for k in (dict(heads=0), dict(heads=6), dict(heads=68), dict(R=0), dict(T=0)):
