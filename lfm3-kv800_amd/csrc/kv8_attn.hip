@@ -10,6 +10,8 @@
 // Operands of 16 x 16 x 32 (lane l: row or column l % 16, g = l / 16): k = 8 g + j. Output: column l % 16, rows 4 g + i. Scores are
 // taken transposed (keys x queries): with the keys of a tile in the cache's slot order the lane's scores are those of the 16
 // tokens 16 g .. of a block, in order, and the lane reads the values of the same: weights never leave their lane.
+#include <type_traits>
+
 #include "kv8_common.h"
 #include "kv800_attn.h"
 
@@ -22,6 +24,9 @@ constexpr int COLS = 16;              // (query, query head) pairs of a tile
 constexpr int STEP = 128;             // positions of a wave's step: two blocks
 constexpr float LAZY = 8.f;           // log2 units by which a running maximum may lag over a long list of keys
 
+struct Desc {                         // of a workgroup whose last item others finish: where that item's outputs go
+  int token, queries, head, last;     // first token, its queries, KV head, last workgroup; last -1: none
+};
 struct Attend {
   Cache C;
   const uint16_t* q;
@@ -37,12 +42,14 @@ struct Attend {
   float sl2;                          // |scale| log2(e)
   uint32_t flip;                      // sign bits of two bf16 for a negative scale: q changes its sign
   uint16_t* out;
-  float* part;                        // 2 slots per workgroup of COLS x (D + 2) floats, NULL: no item is split
+  float* part;                        // 2 slots per workgroup of COLS parts: of an item that others began, of one that others finish
+  Desc* desc;                         // one per workgroup
 };
 
 struct Row {
   int64_t q0, p0, n;                  // first token, its position, positions (those the table covers)
-  int c, tiles, st0, steps;           // new tokens, query tiles, first step, steps
+  int64_t b0;                         // first block that its first query sees
+  int c, tiles, steps;                // new tokens, query tiles, steps from that block on
 };
 __device__ __forceinline__ Row row_at(const Attend& A, int r) {
   Row w;
@@ -53,8 +60,8 @@ __device__ __forceinline__ Row row_at(const Attend& A, int r) {
   w.n = max(min(n, (int64_t)A.bt_cols * A.C.blocks * BLK), (int64_t)0);
   w.tiles = (w.c + A.TQ - 1) / A.TQ;
   const int64_t lo = A.window > 0 ? max(w.p0 + 1 - A.window, (int64_t)0) : 0;
-  w.st0 = (int)(min(lo, w.n) / STEP);
-  w.steps = max((int)((w.n + STEP - 1) / STEP) - w.st0, 1);              // 1 also without keys: the outputs are written
+  w.b0 = min(lo, w.n) / BLK;
+  w.steps = max((int)((w.n - w.b0 * BLK + STEP - 1) / STEP), 1);         // 1 also without keys: the outputs are written
   return w;
 }
 __device__ __forceinline__ int64_t cost_of(const Attend& A, const Row& w) { return (int64_t)w.tiles * A.C.heads * w.steps; }
@@ -109,38 +116,63 @@ __device__ __forceinline__ kv800::b8 wide8(uint32_t a, uint32_t b, float f) {
   return kv800::b8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
 }
 
-// One workgroup takes entries [w W / NG, (w + 1) W / NG) of the list (row, query tile, head, step); without `part` (no item is
-// split) workgroup w is item w. The four waves take every fourth step of an item, each with its own maximum, sum and output, and
-// are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
+// A part of one column: D sums of weighted values, the maximum (log2 units), the sum of weights, relative to it; PART floats.
 template <int D>
+constexpr int PART = D + 4;
+
+// LIST: one workgroup takes entries [w W / NG, (w + 1) W / NG) of the W of the list (row, query tile, head, step); else workgroup w is one
+// (query tile, head), found by the tiles' numbers qsl[r] / TQ + r on. The four waves take every fourth step of an item, each with its
+// own maximum, sum and output, and are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
+template <int D, bool LIST>
 __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
   constexpr int NT = D / 16, NK = D / 32, LD = D + 4;
-  __shared__ List L;
+  __shared__ typename std::conditional<LIST, List, int>::type L;
   __shared__ __align__(16) float so[4][COLS][LD];
   __shared__ float sm[4][COLS], sl[4][COLS];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, rr = lane & 15, g = lane >> 4;
-  const int64_t w = blockIdx.x, NG = gridDim.x;
+  const int64_t w = blockIdx.x;
 
-  for (int64_t t = max(A.qsl[A.R], (int64_t)0) + w; t < A.T; t += NG)     // the padding
+  for (int64_t t = max(A.qsl[A.R], (int64_t)0) + w; t < A.T; t += gridDim.x)     // the padding
     for (int i = tid; i < A.C.heads * A.G * D / 8; i += 256)
       reinterpret_cast<uint4*>(A.out + t * A.C.heads * A.G * D)[i] = make_uint4(0, 0, 0, 0);
 
-  scan_rows(A, L, per);
-  const int64_t W = L.pre[256];
-  int64_t x = w * W / NG;
-  const int64_t end = (w + 1) * W / NG;
-  if (x >= end) return;
-  int64_t before;
-  int r = find_row(A, L, per, x, before);
-  Row row = row_at(A, r);
+  int64_t x = 0, end = 1, before = 0, W = 0, NG = 1;
+  int r;
+  Row row;
+  if constexpr (LIST) {
+    if (tid == 0) A.desc[w].last = -1;
+    scan_rows(A, L, per);
+    W = L.pre[256];
+    NG = min((int64_t)gridDim.x, W);               // no workgroup between two others is without entries
+    if (w >= NG) return;
+    x = w * W / NG;
+    end = (w + 1) * W / NG;
+    r = find_row(A, L, per, x, before);
+    row = row_at(A, r);
+  } else {
+    const int64_t ti = w / A.C.heads;
+    r = (int)kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / A.TQ + i <= ti; });
+    row = row_at(A, r);
+    if (ti - (row.q0 / A.TQ + r) >= row.tiles) return;
+  }
   while (x < end) {
-    while (x >= before + cost_of(A, row)) {
-      before += cost_of(A, row);
-      row = row_at(A, ++r);
+    int64_t at = 0;
+    int s0 = 0, s1 = row.steps, h, tile;
+    if constexpr (LIST) {
+      while (x >= before + cost_of(A, row)) {
+        before += cost_of(A, row);
+        row = row_at(A, ++r);
+      }
+      const int64_t item = (x - before) / row.steps;
+      at = before + item * row.steps;
+      s0 = (int)(x - at);
+      s1 = (int)min((int64_t)row.steps, end - at);
+      h = (int)(item % A.C.heads);
+      tile = (int)(item / A.C.heads);
+    } else {
+      h = (int)(w % A.C.heads);
+      tile = (int)(w / A.C.heads - (row.q0 / A.TQ + r));
     }
-    const int64_t item = (x - before) / row.steps, at = before + item * row.steps;
-    const int s0 = (int)(x - at), s1 = (int)min((int64_t)row.steps, end - at);
-    const int h = (int)(item % A.C.heads), tile = (int)(item / A.C.heads);
 
     // ---- the queries of the lane's column
     const int i = tile * A.TQ + rr / A.G, hq = h * A.G + rr % A.G;
@@ -163,8 +195,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
     const int64_t thi = min(row.p0 + ilast, row.n - 1), tlo = A.window > 0 ? row.p0 + tile * A.TQ - A.window : -1;
     const int64_t ahi = min(row.p0 + tile * A.TQ + 1, row.n), alo = A.window > 0 ? row.p0 + ilast - A.window + 1 : 0;
 
-    for (int st = row.st0 + s0 + wv; st < row.st0 + s1; st += 4) {
-      const int64_t pos = (int64_t)st * STEP;
+    for (int st = s0 + wv; st < s1; st += 4) {
+      const int64_t pos = row.b0 * BLK + (int64_t)st * STEP;
       if (pos > thi || pos + STEP <= tlo + 1) continue;
       // ---- codes of the two blocks; a block that no query sees, or without a page, is not read
       uint4 kk[8][D / 64], vv[NT][2];
@@ -326,60 +358,70 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
           else *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[1]);
         }
       } else {
-        float* pt = A.part + ((2 * w + (s0 == 0 ? 1 : 0)) * COLS + c) * (D + 2);
+        float* pt = A.part + ((2 * w + (s0 == 0 ? 1 : 0)) * COLS + c) * PART<D>;
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) pt[d0 + e] = acc[e];
         if (d0 == 0) { pt[D] = m; pt[D + 1] = ls; }
+        // the item's last entry: the least w' with (w' + 1) W / NG at or behind its end
+        if (s0 == 0 && tid == 0)
+          A.desc[w] = {(int)row.q0 + tile * A.TQ, min(A.TQ, row.c - tile * A.TQ), h, (int)(((at + row.steps) * NG + W - 1) / W - 1)};
       }
     }
+    if constexpr (!LIST) return;
     __syncthreads();
     x = at + s1;
   }
 }
 
-// One workgroup per (workgroup of the list, column): if that one began an item that others finish, its part and theirs, in order.
-template <int D>
-__global__ void __launch_bounds__(256) merge_kernel(Attend A, int per) {
-  __shared__ List L;
-  __shared__ float red[256 / D][D], rl[256 / D];
-  const int64_t w = blockIdx.x, NG = gridDim.x;
-  const int c = blockIdx.y, tid = threadIdx.x;
-  scan_rows(A, L, per);
-  const int64_t W = L.pre[256], a = w * W / NG, end = (w + 1) * W / NG;
-  if (a >= end) return;                            // uniform, as the returns below
-  int64_t before;
-  const int r = find_row(A, L, per, end - 1, before);
-  const Row row = row_at(A, r);
-  const int64_t item = (end - 1 - before) / row.steps, at = before + item * row.steps;
-  if (at < a || at + row.steps <= end) return;     // the last item began earlier, or is whole here
-  const int h = (int)(item % A.C.heads), tile = (int)(item / A.C.heads), i = tile * A.TQ + c / A.G;
-  if (c >= A.TQ * A.G || i >= row.c) return;
-  const int64_t wl = ((at + row.steps) * NG + W - 1) / W - 1;   // the workgroup with the item's last entry: the least w' with (w' + 1) W / NG >= its end
-  const int d = tid % D, part = tid / D;
-  auto slot = [&](int64_t k) { return A.part + ((2 * k + (k == w ? 1 : 0)) * COLS + c) * (D + 2); };
+// ---------------------------------------------------------------- joining parts
+// A wave joins `count` parts, in order: the maxima side by side, then D / 64 channels a lane. Writes the column's output.
+template <int D, typename Slot>
+__device__ __forceinline__ void join(int count, Slot slot, uint16_t* __restrict__ out) {
+  const int lane = threadIdx.x & 63;
   float m = -INFINITY;
-  for (int64_t k = w; k <= wl; ++k) {
-    if (k * W / NG == (k + 1) * W / NG) continue;
-    m = fmaxf(m, slot(k)[D]);
-  }
-  float acc = 0.f, l = 0.f;
-  for (int64_t k = w + part; k <= wl; k += 256 / D) {
-    if (k * W / NG == (k + 1) * W / NG) continue;
+  for (int k = lane; k < count; k += 64) m = fmaxf(m, slot(k)[D]);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (m == -INFINITY) m = 0.f;                     // no part has keys: all sums are 0
+  float a0 = 0.f, a1 = 0.f, l = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < count; ++k) {
     const float* s = slot(k);
-    const float mk = s[D];
-    if (mk > -INFINITY) {
-      const float f = __builtin_amdgcn_exp2f(mk - m);
-      acc += f * s[d];
-      l += f * s[D + 1];
+    const float f = __builtin_amdgcn_exp2f(s[D] - m);
+    l += f * s[D + 1];
+    if (D == 128) {
+      const float2 v = *reinterpret_cast<const float2*>(s + 2 * lane);
+      a0 += f * v.x;
+      a1 += f * v.y;
+    } else {
+      a0 += f * s[lane];
     }
   }
-  red[part][d] = acc;
-  if (d == 0) rl[part] = l;
-  __syncthreads();
-  if (part) return;
-#pragma unroll
-  for (int k = 1; k < 256 / D; ++k) { acc += red[k][d]; l += rl[k]; }
-  A.out[((row.q0 + i) * A.C.heads * A.G + h * A.G + c % A.G) * D + d] = (uint16_t)kv800::f2bf(l == 0.f ? 0.f : acc / l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (D == 128) reinterpret_cast<uint32_t*>(out)[lane] = kv800::bfpk(a0 * inv, a1 * inv);
+  else out[lane] = (uint16_t)kv800::f2bf(a0 * inv);
+}
+
+// One wave per (workgroup of the list, column): where that workgroup began an item that others finish, its part and theirs.
+template <int D>
+__global__ void __launch_bounds__(256) merge_kernel(Attend A) {
+  const int64_t w = blockIdx.x;
+  const Desc d = A.desc[w];
+  if (d.last < 0) return;
+  const int c = blockIdx.y * 4 + (threadIdx.x >> 6), i = c / A.G;
+  if (i >= d.queries) return;
+  const int Hq = A.C.heads * A.G;
+  join<D>(d.last - (int)w + 1, [&](int k) { return A.part + ((2 * (w + k) + (k == 0 ? 1 : 0)) * COLS + c) * PART<D>; },
+          A.out + ((int64_t)(d.token + i) * Hq + d.head * A.G + c % A.G) * D);
+}
+
+// One wave per (token, head) of the split prompt kernel.
+template <int D>
+__global__ void __launch_bounds__(256) merge_rows_kernel(const float* __restrict__ part, int splits, const int64_t* __restrict__ total, int heads,
+                                                         int64_t T, uint16_t* __restrict__ out) {
+  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (c >= min(*total, T) * heads) return;         // the padding has no parts
+  join<D>(splits, [&](int k) { return part + (c * splits + k) * PART<D>; }, out + c * D);
 }
 
 // ---------------------------------------------------------------- many new tokens a row
@@ -606,7 +648,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   l = ls.x + ls.y;
   if (!have) return;
   if (part) {
-    float* pp = part + (((row.q0 + iq) * Hq + hq) * splits + sp) * (D + 4);
+    float* pp = part + (((row.q0 + iq) * Hq + hq) * splits + sp) * PART<D>;
 #pragma unroll
     for (int d = 0; d < NT; ++d)
 #pragma unroll
@@ -626,26 +668,68 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
 }
 
 // ---------------------------------------------------------------- host
+// How a call runs. PROMPT: rows bring half a tile of the prompt kernel or more on average. DIRECT: few steps an item. A row that is
+// not as the mean has it is right all the same.
+enum Kind { LISTED, DIRECT, PROMPT };
 struct Plan {
-  int TQ, G;
-  int64_t groups;
-  bool split;
+  Kind kind;
+  int TQ, G, splits;
+  int64_t tiles, groups;              // query tiles of all rows at most; workgroups (LISTED)
+  int64_t bytes;                      // workspace
 };
+constexpr int NW = 4;                 // waves of the prompt kernel
 Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
   Plan p;
   p.G = (int)(heads / c->kv_heads);
-  p.TQ = COLS / p.G;
-  const int64_t tiles = (T + p.TQ - 1) / p.TQ + (T < R ? T : R);          // of all rows, at most
-  int64_t steps = (bt_cols * c->blocks * BLK + STEP - 1) / STEP;          // of an item, at most
-  if (window > 0) {
-    const int64_t most = (window + T + STEP - 2) / STEP + 1;
-    steps = most < steps ? most : steps;
+  p.splits = 1;
+  p.groups = 0;
+  p.bytes = 0;
+  const int64_t positions = bt_cols * c->blocks * BLK, mean = (T + R - 1) / R;
+  const int64_t seen = window > 0 && window + mean < positions ? window + mean : positions;   // of a row, or so
+  p.kind = T * p.G >= 64 * R ? PROMPT : seen <= 8 * STEP ? DIRECT : LISTED;
+  p.TQ = (p.kind == PROMPT ? 32 * NW : COLS) / p.G;
+  p.tiles = T / p.TQ + R;
+  if (p.kind == PROMPT) {
+    // few tiles: each split over its blocks, down to 8, for two workgroups a CU
+    const int64_t wgs = (mean + p.TQ - 1) / p.TQ * R * c->kv_heads, most = seen / (8 * BLK);
+    int64_t s = wgs > 0 ? 512 / wgs : 1;
+    if (s > most) s = most;
+    p.splits = (int)(s < 1 ? 1 : s);
+    if (p.splits > 1) p.bytes = T * heads * p.splits * (c->dim + 4) * 4;
+  } else if (p.kind == LISTED) {
+    const int64_t entries = p.tiles * c->kv_heads * ((positions + STEP - 1) / STEP + 1);
+    p.groups = (entries + 3) / 4 < 512 ? (entries + 3) / 4 : 512;
+    p.bytes = p.groups * (2 * COLS * (c->dim + 4) * 4 + (int64_t)sizeof(Desc));
   }
-  const int64_t entries = tiles * c->kv_heads * (steps > 0 ? steps : 1);
-  p.groups = (entries + 3) / 4;
-  if (p.groups > 512) p.groups = 512;
-  p.split = true;
   return p;
+}
+
+template <int D>
+int run(const Attend& A0, const Plan& p, int64_t heads, void* ws, hipStream_t s) {
+  Attend A = A0;
+  const int64_t H = A.C.heads;
+  if (p.kind == PROMPT) {
+    const int64_t xs = 8 % H == 0 && p.splits == 1 ? 8 / H : 1;
+    float* part = p.splits > 1 ? (float*)ws : nullptr;
+    hipLaunchKernelGGL(zero_padding_kernel, dim3(64), dim3(256), 0, s, A.qsl + A.R, A.T, heads * D, A.out);
+    hipLaunchKernelGGL((prompt_kernel<D, NW>), dim3((unsigned)((p.tiles + xs - 1) / xs * xs * H * p.splits)), dim3(64 * NW), 0, s, A, p.TQ,
+                       p.tiles, p.splits, part);
+    if (part)
+      hipLaunchKernelGGL(merge_rows_kernel<D>, dim3((unsigned)((A.T * heads + 3) / 4)), dim3(256), 0, s, part, p.splits, A.qsl + A.R,
+                         (int)heads, A.T, A.out);
+    return kv800::check_launch("kv8_attend prompt");
+  }
+  if (p.kind == DIRECT) {
+    hipLaunchKernelGGL((attend_kernel<D, false>), dim3((unsigned)(p.tiles * H)), dim3(256), 0, s, A, 0);
+    return kv800::check_launch("kv8_attend");
+  }
+  A.part = (float*)ws;
+  A.desc = (Desc*)(A.part + p.groups * 2 * COLS * PART<D>);
+  hipLaunchKernelGGL((attend_kernel<D, true>), dim3((unsigned)p.groups), dim3(256), 0, s, A, (A.R + 255) / 256);
+  const int rc = kv800::check_launch("kv8_attend");
+  if (rc != KV800_OK) return rc;
+  hipLaunchKernelGGL(merge_kernel<D>, dim3((unsigned)p.groups, COLS / 4), dim3(256), 0, s, A);
+  return kv800::check_launch("kv8_attend merge");
 }
 
 }  // namespace
@@ -655,8 +739,7 @@ extern "C" {
 
 int64_t kv8_hip_attend_workspace(const kv8_cache_t* cache, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
   if (!kv8::valid(cache) || heads <= 0 || heads % cache->kv_heads || heads / cache->kv_heads > kv8::COLS || R <= 0 || T <= 0) return 0;
-  const kv8::Plan p = kv8::plan(cache, heads, R, T, bt_cols, window);
-  return p.split ? p.groups * 2 * kv8::COLS * (cache->dim + 2) * 4 : 0;
+  return kv8::plan(cache, heads, R, T, bt_cols, window).bytes;
 }
 
 int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, const int32_t* bt, int64_t bt_stride,
@@ -674,30 +757,12 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
   KV800_REQUIRE(q && lens && qsl && out && (bt || bt_cols == 0), "kv8_attend: null pointer");
   KV800_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0, "kv8_attend: q and out must be 16-byte aligned");
   const kv8::Plan p = kv8::plan(cache, heads, R, T, bt_cols, window);
-  const int64_t need = kv8_hip_attend_workspace(cache, heads, R, T, bt_cols, window);
-  KV800_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), "kv8_attend: %lld bytes of 16-byte aligned workspace needed",
-                (long long)need);
-  kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window,
-                   fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, out, (float*)ws};
-  const int per = (int)((R + 255) / 256);
-  if (T * p.G >= 64 * R) {
-    const int NW = 4, TQ = 32 * NW / p.G;
-    const int64_t ntiles = T / TQ + R, xs = 8 % cache->kv_heads == 0 ? 8 / cache->kv_heads : 1;
-    const dim3 grid((unsigned)((ntiles + xs - 1) / xs * xs * cache->kv_heads));
-    hipLaunchKernelGGL(kv8::zero_padding_kernel, dim3(64), dim3(256), 0, (hipStream_t)stream, qsl + R, T, heads * cache->dim, out);
-    if (cache->dim == 128) hipLaunchKernelGGL((kv8::prompt_kernel<128, 4>), grid, dim3(64 * NW), 0, (hipStream_t)stream, A, TQ, ntiles, 1, nullptr);
-    else hipLaunchKernelGGL((kv8::prompt_kernel<64, 4>), grid, dim3(64 * NW), 0, (hipStream_t)stream, A, TQ, ntiles, 1, nullptr);
-    return kv800::check_launch("kv8_attend prompt");
-  }
-  const dim3 grid((unsigned)p.groups);
-  if (cache->dim == 128) hipLaunchKernelGGL(kv8::attend_kernel<128>, grid, dim3(256), 0, (hipStream_t)stream, A, per);
-  else hipLaunchKernelGGL(kv8::attend_kernel<64>, grid, dim3(256), 0, (hipStream_t)stream, A, per);
-  int rc = kv800::check_launch("kv8_attend");
-  if (rc != KV800_OK || !p.split) return rc;
-  const dim3 mg((unsigned)p.groups, kv8::COLS);
-  if (cache->dim == 128) hipLaunchKernelGGL(kv8::merge_kernel<128>, mg, dim3(256), 0, (hipStream_t)stream, A, per);
-  else hipLaunchKernelGGL(kv8::merge_kernel<64>, mg, dim3(256), 0, (hipStream_t)stream, A, per);
-  return kv800::check_launch("kv8_attend merge");
+  KV800_REQUIRE(p.tiles * cache->kv_heads * p.splits < INT32_MAX, "kv8_attend: too many tokens or rows");
+  KV800_REQUIRE(p.bytes == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.bytes), "kv8_attend: %lld bytes of 16-byte aligned workspace needed",
+                (long long)p.bytes);
+  const kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window,
+                         fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, out, nullptr, nullptr};
+  return cache->dim == 128 ? kv8::run<128>(A, p, heads, ws, (hipStream_t)stream) : kv8::run<64>(A, p, heads, ws, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -192,6 +192,16 @@ def test_attend_ranges(kv8, spread):
     assert not got[3:].any()
 
 
+@pytest.mark.parametrize("prev,new", [([5000], [1]), ([3000, 1, 400, 2047], [1, 2, 1, 1]), ([6000], [40]), ([4000, 700], [33, 100])], ids=str)
+@pytest.mark.parametrize("window", [0, 1500])
+def test_attend_split(kv8, prev, new, window):
+    """Long rows, whose keys several workgroups share, beside short ones, in tables wider than the rows."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 31, prev, new, 2, 128, 64, pad=3, cols=9)
+    q = (torch.randn(T, 8, 128, generator=g) * 2).to(torch.bfloat16)
+    got = check_attend(kv8, data, exps, q, bt, lens, qsl, window)
+    assert not got[int(qsl[-1]):].any()
+
+
 def test_attend_many_rows(kv8):
     """More rows than a workgroup has threads, some without tokens."""
     g = torch.Generator().manual_seed(1)

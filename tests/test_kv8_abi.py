@@ -67,9 +67,9 @@ def test_dequantize_host_checks(lib):
 
 
 def test_attend_host_checks(lib):
-    need = lib.kv8_hip_attend_workspace(desc(), 16, 2, 5, 4, 0)
+    need = lib.kv8_hip_attend_workspace(desc(), 16, 2, 5, 64, 0)
     assert need > 0
-    base = dict(q=A, heads=16, bt=A, bs=4, bc=4, lens=A, qsl=A, R=2, T=5, win=0, scale=0.1, out=A, ws=A, wsb=need, s=None)
+    base = dict(q=A, heads=16, bt=A, bs=64, bc=64, lens=A, qsl=A, R=2, T=5, win=0, scale=0.1, out=A, ws=A, wsb=need, s=None)
     f = lambda c=None, **k: lib.kv8_hip_attend(c or desc(), *{**base, **k}.values())
     for k in BAD:
         refused(lib, f(desc(**k)), b"descriptor")
@@ -78,7 +78,7 @@ def test_attend_host_checks(lib):
         refused(lib, f(**k), b"kv8_attend")
     assert f(T=0) == 0
     for k in (dict(heads=0), dict(heads=6), dict(heads=68), dict(R=0), dict(T=0)):
-        a = {**dict(heads=16, R=2, T=5, bc=4, win=0), **k}
+        a = {**dict(heads=16, R=2, T=5, bc=64, win=0), **k}
         assert lib.kv8_hip_attend_workspace(desc(), *a.values()) == 0
 
 
