@@ -2,7 +2,8 @@
 //
 //   layout_kernel    a weight into operand order, once
 //   quantize_kernel  tokens (or a weight's rows) to 8 bits, a scale for each
-//   product_kernel   the products, 4 waves of 64 x 64 outputs each
+//   few_kernel       products of few tokens: weights streamed, K split over a workgroup's waves
+//   many_kernel      products of many: 256 x 256 outputs a workgroup through LDS
 //
 // Sums of up to 65,536 products of 8-bit integers fit 32 bits, so they are exact and any split of K gives the same result; the
 // scales are applied once, in fp32.
@@ -46,15 +47,15 @@ __global__ void __launch_bounds__(256) layout_kernel(const int8_t* __restrict__ 
   *reinterpret_cast<uint4*>(wsh + i * 16) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// One wave per row. Up to 16 pieces of 512 channels stay in registers between the maximum and the codes; a longer row is read again.
+// One workgroup per row. Up to 4 pieces of 2,048 channels stay in registers between the maximum and the codes; a longer row is read again.
 // OPERAND: codes in operand order of tiles of 32 rows (nks blocks each), else row by row.
 template <bool OPERAND>
 __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t R, int64_t K, int64_t nks,
                                                        int8_t* __restrict__ q, float* __restrict__ scale) {
-  constexpr int HELD = 16;
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= R) return;
+  constexpr int HELD = 4, PIECE = 2048;
+  __shared__ uint32_t tops[4];
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x;
   const uint16_t* src = x + r * ldx;
   uint4 held[HELD];
   uint32_t top = 0;                                                      // magnitudes of bf16 order as integers; NaN above infinity
@@ -65,17 +66,20 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
   };
 #pragma unroll
   for (int j = 0; j < HELD; ++j) {
-    const int64_t k = j * 512 + lane * 8;
+    const int64_t k = j * PIECE + tid * 8;
     held[j] = make_uint4(0, 0, 0, 0);
     if (k < K) held[j] = *reinterpret_cast<const uint4*>(src + k);
   }
 #pragma unroll
   for (int j = 0; j < HELD; ++j) take(held[j]);
-  for (int64_t k = HELD * 512 + lane * 8; k < K; k += 512) take(*reinterpret_cast<const uint4*>(src + k));
+  for (int64_t k = HELD * PIECE + tid * 8; k < K; k += PIECE) take(*reinterpret_cast<const uint4*>(src + k));
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
   const float t = fmaxf(kv800::bf2f(top), LEAST), inv = 127.f / t;
-  if (lane == 0) scale[r] = top < 0x7F80u ? t / 127.f : __uint_as_float(0x7FC00000u);
+  if (tid == 0) scale[r] = top < 0x7F80u ? t / 127.f : __uint_as_float(0x7FC00000u);
   auto put = [&](int64_t k, const uint4& u) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     uint32_t o[2];
@@ -96,63 +100,257 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
   };
 #pragma unroll
   for (int j = 0; j < HELD; ++j) {
-    const int64_t k = j * 512 + lane * 8;
+    const int64_t k = j * PIECE + tid * 8;
     if (k < K) put(k, held[j]);
   }
-  for (int64_t k = HELD * 512 + lane * 8; k < K; k += 512) put(k, *reinterpret_cast<const uint4*>(src + k));
+  for (int64_t k = HELD * PIECE + tid * 8; k < K; k += PIECE) put(k, *reinterpret_cast<const uint4*>(src + k));
 }
 
-// One workgroup: 128 rows of the weight x 128 tokens, a wave 64 x 64, operands straight from memory (both lie in operand order).
-// Output of the instruction (weight rows x tokens): lane l holds token l % 32, rows 8 b + 4 (l / 32) + i.
-template <bool GATED>
-__global__ void __launch_bounds__(256) product_kernel(const int8_t* __restrict__ xq, const float* __restrict__ sx,
-                                                      const int8_t* __restrict__ wsh, const float* __restrict__ ssh, int64_t R,
-                                                      int64_t N, int64_t nt, int64_t mt, int64_t nks, uint16_t* __restrict__ y, int64_t ldy) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int64_t n0 = (int64_t)blockIdx.x * 4 + 2 * (wv & 1), m0 = (int64_t)blockIdx.y * 4 + 2 * (wv >> 1);
-  if (n0 >= nt || m0 >= mt) return;
-  const int8_t* wp[2];
-  const int8_t* xp[2];
+// tokens to 8 bits inside a product: the lane's 16 channels from k on (zeros past K), token row src
+__device__ __forceinline__ i4v quantized16(const uint16_t* src, int64_t k, int64_t K, float inv) {
+  i4v o = {0, 0, 0, 0};
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    wp[j] = wsh + (n0 + j) * nks * 1024 + lane * 16;                     // nt is even
-    xp[j] = xq + min(m0 + j, mt - 1) * nks * 1024 + lane * 16;           // a tile past the last is computed again, not stored
+  for (int p = 0; p < 2; ++p)
+    if (k + 8 * p < K) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + k + 8 * p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t b = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = e & 1 ? kv800::bf2f_hi(w[2 * i + (e >> 1)]) : kv800::bf2f_lo(w[2 * i + (e >> 1)]);
+          b |= ((uint32_t)(int)rintf(f * inv) & 0xFFu) << (8 * e);
+        }
+        o[2 * p + i] = (int)b;
+      }
+    }
+  return o;
+}
+
+struct Out {
+  uint16_t* y;
+  int64_t ldy, R, N;
+  bool wide;                 // rows on 8-byte boundaries
+};
+// Four outputs of token r from row n of the (padded) weight on; gated: g and u of output f on.
+__device__ __forceinline__ void put4(const Out& o, int64_t r, int64_t n, int64_t width, const float (&v)[4]) {
+  uint16_t* dst = o.y + r * o.ldy + n;
+  if (o.wide && n + 4 <= width) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(kv800::f2bf(v[0]) | (kv800::f2bf(v[1]) << 16), kv800::f2bf(v[2]) | (kv800::f2bf(v[3]) << 16));
+    return;
   }
-  i16v acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < width) dst[i] = (uint16_t)kv800::f2bf(v[i]);
+}
+__device__ __forceinline__ float gate(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+
+// Few tokens: one workgroup takes 64 rows of the weight x 32 WM tokens, its 8 waves an eighth of K each, so that every wave has
+// blocks of 1 KB in flight from its first instruction on; their sums meet in LDS, 32 tokens at a time. Output of the instruction
+// (weight rows x tokens): lane l holds token l % 32, rows 8 b + 4 (l / 32) + i.
+// FUSED (up to 32 tokens): the tokens are rounded to 8 bits by every workgroup for itself, while its first weights are on their way.
+constexpr int FEW = 8;       // waves
+template <int WM, bool GATED, bool FUSED>
+__global__ void __launch_bounds__(64 * FEW) few_kernel(const uint16_t* __restrict__ x, int64_t ldx, const int8_t* __restrict__ xq,
+                                                       const float* __restrict__ sx, const int8_t* __restrict__ wsh,
+                                                       const float* __restrict__ ssh, int64_t K, int64_t nks, Out o) {
+  constexpr int U = WM == 1 ? 8 : 4;               // k-steps in flight
+  __shared__ int4 part[FEW][2][4][64];
+  __shared__ int tops[32];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 2, m0 = (int64_t)blockIdx.y * WM;
+  const int per = (int)((nks + FEW - 1) / FEW), k0 = wv * per, k1 = min((int)nks, k0 + per);
+  const int8_t* wp = wsh + n0 * nks * 1024 + lane * 16;
+  const int tok = lane & 31;
+  i16v acc[2][WM];
 #pragma unroll
   for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < WM; ++b)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[a][b][v] = 0;
+  i4v wr[2][U];
+  auto weights = [&](int ks) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) wr[a][u] = *reinterpret_cast<const i4v*>(wp + (a * nks + min(ks + u, k1 - 1)) * 1024);
+  };
+  if (k0 < k1) weights(k0);
+  float inv = 0.f;
+  if (FUSED) {
+    if (tid < 32) tops[tid] = 0;
+    __syncthreads();
+    const int R = (int)o.R;
+    for (int r = 0; r < R; ++r) {
+      uint32_t top = 0;
+      for (int64_t k = tid * 8; k < K; k += 8 * 64 * FEW) {
+        const uint4 u = *reinterpret_cast<const uint4*>(x + r * ldx + k);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+      }
+#pragma unroll
+      for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+      if (lane == 0) atomicMax(&tops[r], (int)top);
+    }
+    __syncthreads();
+    inv = 127.f / fmaxf(kv800::bf2f((uint32_t)tops[tok]), LEAST);
+  }
+  for (int ks = k0; ks < k1; ks += U) {
+    i4v xr[WM][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int b = 0; b < WM; ++b) {
+        xr[b][u] = i4v{0, 0, 0, 0};
+        const int64_t r = (m0 + b) * 32 + tok;
+        if (r < o.R && ks + u < k1) {
+          if (FUSED) xr[b][u] = quantized16(x + r * ldx, 32 * (int64_t)(ks + u) + 16 * (lane >> 5), K, inv);
+          else xr[b][u] = *reinterpret_cast<const i4v*>(xq + ((m0 + b) * nks + ks + u) * 1024 + lane * 16);
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < WM; ++b) acc[a][b] = mfma(wr[a][u], xr[b][u], acc[a][b]);
+    if (ks + U < k1) weights(ks + U);
+  }
+#pragma unroll
+  for (int b = 0; b < WM; ++b) {
+    if (b) __syncthreads();
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) part[wv][a][q][lane] = make_int4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+    __syncthreads();
+    // thread: 4 rows of one token, of tile wv / 4 (gated: waves 0 .. 3, both tiles)
+    const int q = wv & 3, row = 8 * q + 4 * (lane >> 5);
+    const int64_t r = (m0 + b) * 32 + tok;
+    if (r >= o.R || (GATED && wv >= 4)) continue;
+    float s;
+    if (FUSED) s = tops[tok] < 0x7F80 ? fmaxf(kv800::bf2f((uint32_t)tops[tok]), LEAST) / 127.f : __uint_as_float(0x7FC00000u);
+    else s = sx[r];
+    auto sums = [&](int a, float (&f)[4]) {
+      int4 t = part[0][a][q][lane];
+#pragma unroll
+      for (int w = 1; w < FEW; ++w) {
+        const int4 p = part[w][a][q][lane];
+        t.x += p.x; t.y += p.y; t.z += p.z; t.w += p.w;
+      }
+      const float4 sc = *reinterpret_cast<const float4*>(ssh + (n0 + a) * 32 + row);
+      f[0] = (float)t.x * s * sc.x; f[1] = (float)t.y * s * sc.y; f[2] = (float)t.z * s * sc.z; f[3] = (float)t.w * s * sc.w;
+    };
+    float f[4];
+    if (GATED) {
+      float u[4];
+      sums(0, f);
+      sums(1, u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = gate(f[i], u[i]);
+      put4(o, r, n0 * 16 + row, o.N / 2, f);
+    } else {
+      sums(wv >> 2, f);
+      put4(o, r, (n0 + (wv >> 2)) * 32 + row, o.N, f);
+    }
+  }
+}
+
+// Many tokens: one workgroup takes 256 rows of the weight x 256 tokens, 128 channels a stage, two stages in LDS: the next one's
+// blocks are loaded straight into LDS while the present one is multiplied, one barrier a stage. A block lies in LDS as it does in memory, in
+// operand order, so that loads and reads go over consecutive addresses. 8 waves of 128 rows x 64 tokens: 6 blocks read from LDS for
+// 8 products.
+constexpr int TILE = 8, STAGE = 4, MANY = 8;       // tiles of 32 a side, k-steps a stage, waves
+struct alignas(16) Stage {
+  int8_t w[TILE * STAGE * 1024];
+  int8_t x[TILE * STAGE * 1024];
+};
+template <bool GATED>
+__global__ void __launch_bounds__(64 * MANY) many_kernel(const int8_t* __restrict__ xq, const float* __restrict__ sx,
+                                                         const int8_t* __restrict__ wsh, const float* __restrict__ ssh, int64_t nt,
+                                                         int64_t mt, int64_t nks, Out o) {
+  __shared__ Stage A, B;     // two objects: a read of one is not held for the other's loads
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, wn = wv & 1, wm = wv >> 1;
+  // workgroup b runs on XCD b % 8, which takes a contiguous run of the order (group of 8 token tiles, weight tile, token tile):
+  // the 32 workgroups that run there together share 4 weight tiles and 8 token tiles in its L2
+  const int nb = (int)gridDim.x, xcd = (int)blockIdx.x & 7, per = nb >> 3, rem = nb & 7;
+  const int L = xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3);
+  const int tn = (int)((nt + TILE - 1) / TILE), tm = (int)((mt + TILE - 1) / TILE);
+  const int grp = L / (8 * tn), gm = min(8, tm - 8 * grp), in = L - grp * 8 * tn;
+  const int64_t n0 = (int64_t)(in / gm) * TILE, m0 = (int64_t)(8 * grp + in % gm) * TILE;
+  auto load = [&](int64_t ks, Stage& S) {          // wave w: tile w of both sides
+    const int8_t* ws = wsh + (min(n0 + wv, nt - 1) * nks + ks) * 1024 + lane * 16;
+    const int8_t* xs = xq + (min(m0 + wv, mt - 1) * nks + ks) * 1024 + lane * 16;
+#pragma unroll
+    for (int k = 0; k < STAGE; ++k) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(ws + k * 1024),
+                                       (__attribute__((address_space(3))) void*)&S.w[(wv * STAGE + k) * 1024], 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(xs + k * 1024),
+                                       (__attribute__((address_space(3))) void*)&S.x[(wv * STAGE + k) * 1024], 16, 0, 0);
+    }
+    asm volatile("" ::"s"((uint32_t)(uintptr_t)&S) : "memory");   // the loads write S behind the compiler's view of it
+  };
+  i16v acc[4][2];
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[a][b][v] = 0;
-  for (int64_t ks = 0; ks < nks; ++ks) {
-    i4v a[2], b[2];
+  auto step = [&](int64_t ks, const Stage& S, Stage& next) {
+    if (ks + STAGE < nks) load(ks + STAGE, next);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) { a[j] = *reinterpret_cast<const i4v*>(wp[j] + ks * 1024); b[j] = *reinterpret_cast<const i4v*>(xp[j] + ks * 1024); }
+    for (int k = 0; k < STAGE; ++k) {
+      i4v a[4], b[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const i4v*>(&S.w[((4 * wn + i) * STAGE + k) * 1024 + lane * 16]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
+      for (int i = 0; i < 2; ++i) b[i] = *reinterpret_cast<const i4v*>(&S.x[((2 * wm + i) * STAGE + k) * 1024 + lane * 16]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
+    }
+    __syncthreads();         // ends the reads of S and waits for the loads into next
+  };
+  load(0, A);
+  __syncthreads();
+  for (int64_t ks = 0; ks < nks; ks += 2 * STAGE) {
+    step(ks, A, B);
+    if (ks + STAGE < nks) step(ks + STAGE, B, A);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int64_t r = (m0 + j) * 32 + (lane & 31);
-    if (m0 + j >= mt || r >= R) continue;
+    const int64_t r = (m0 + 2 * wm + j) * 32 + (lane & 31);
+    if (r >= o.R) continue;
     const float s = sx[r];
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int q = 0; q < 4; ++q) {
+      const int row = 8 * q + 4 * (lane >> 5);
+      auto scaled = [&](int i, float (&f)[4]) {
+        const float4 sc = *reinterpret_cast<const float4*>(ssh + (n0 + 4 * wn + i) * 32 + row);
+        f[0] = (float)acc[i][j][4 * q] * s * sc.x; f[1] = (float)acc[i][j][4 * q + 1] * s * sc.y;
+        f[2] = (float)acc[i][j][4 * q + 2] * s * sc.z; f[3] = (float)acc[i][j][4 * q + 3] * s * sc.w;
+      };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 8 * b + 4 * (lane >> 5) + i;
-        const float y0 = (float)acc[0][j][4 * b + i] * s * ssh[n0 * 32 + row], y1 = (float)acc[1][j][4 * b + i] * s * ssh[n0 * 32 + 32 + row];
+      for (int i = 0; i < 4; i += GATED ? 2 : 1) {
+        if (n0 + 4 * wn + i >= nt) continue;
+        float f[4];
+        scaled(i, f);
         if (GATED) {
-          const int64_t f = n0 * 16 + row;
-          if (f < N / 2) y[r * ldy + f] = (uint16_t)kv800::f2bf(y0 / (1.f + __expf(-y0)) * y1);
+          float u[4];
+          scaled(i + 1, u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = gate(f[e], u[e]);
+          put4(o, r, (n0 + 4 * wn + i) * 16 + row, o.N / 2, f);
         } else {
-          if (n0 * 32 + row < N) y[r * ldy + n0 * 32 + row] = (uint16_t)kv800::f2bf(y0);
-          if (n0 * 32 + 32 + row < N) y[r * ldy + n0 * 32 + 32 + row] = (uint16_t)kv800::f2bf(y1);
+          put4(o, r, (n0 + 4 * wn + i) * 32 + row, o.N, f);
         }
       }
+    }
   }
 }
 
@@ -164,6 +362,15 @@ bool sizes(int64_t R, int64_t N, int64_t K, int gated) {
   return R >= 0 && R <= (1 << 24) && N > 0 && N <= (1 << 24) && K > 0 && K <= K_MOST && K % 8 == 0 && (gated == 0 || (gated == 1 && N % 2 == 0));
 }
 
+// How a product runs: tokens rounded inside it, 32 or 64 tokens a workgroup of few_kernel, or many_kernel.
+enum Kind { FUSED, ONE, TWO, TILES };
+Kind kind_of(int64_t R, int64_t N, int64_t K, int gated) {
+  if (R <= 16) return FUSED;
+  const int64_t wgs = (padded_rows(N, gated) + 255) / 256 * ((R + 255) / 256);
+  if (wgs >= 192) return TILES;
+  return R <= 32 ? ONE : TWO;
+}
+
 }  // namespace
 }  // namespace lfm3
 
@@ -172,7 +379,7 @@ extern "C" {
 int lfm3_hip_int8_layout(const int8_t* w, int64_t ld, const float* scale, int64_t N, int64_t K, int gated, int8_t* wsh, float* ssh,
                          void* stream) {
   KV800_REQUIRE(lfm3::sizes(0, N, K, gated) && ld >= 0, "int8_layout: N up to 2^24 (even for a gated weight), K a multiple of 8 up to 65536");
-  KV800_REQUIRE(w && scale && wsh && ssh && (uintptr_t)wsh % 16 == 0, "int8_layout: null or unaligned pointer");
+  KV800_REQUIRE(w && scale && wsh && ssh && (uintptr_t)wsh % 16 == 0 && (uintptr_t)ssh % 16 == 0, "int8_layout: null or unaligned pointer");
   const int64_t Npad = lfm3::padded_rows(N, gated), nks = lfm3::round_up(K, 128) / 32, n = Npad / 32 * nks * 64;
   hipLaunchKernelGGL(lfm3::layout_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, w, ld, scale, N, K,
                      Npad, nks, gated, wsh, ssh);
@@ -182,13 +389,14 @@ int lfm3_hip_int8_layout(const int8_t* w, int64_t ld, const float* scale, int64_
 int lfm3_hip_int8_quantize(const uint16_t* w, int64_t ld, int64_t N, int64_t K, int8_t* w8, float* scale, void* stream) {
   KV800_REQUIRE(lfm3::sizes(0, N, K, 0) && ld % 8 == 0, "int8_quantize: N up to 2^24, K a multiple of 8 up to 65536, ld a multiple of 8");
   KV800_REQUIRE(w && w8 && scale && (uintptr_t)w % 16 == 0 && (uintptr_t)w8 % 8 == 0, "int8_quantize: null or unaligned pointer");
-  hipLaunchKernelGGL(lfm3::quantize_kernel<false>, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, (hipStream_t)stream, w, ld, N, K, 0,
+  hipLaunchKernelGGL(lfm3::quantize_kernel<false>, dim3((unsigned)N), dim3(256), 0, (hipStream_t)stream, w, ld, N, K, 0,
                      w8, scale);
   return kv800::check_launch("int8_quantize");
 }
 
 int64_t lfm3_hip_linear8_workspace(int64_t R, int64_t N, int64_t K, int gated) {
   if (!lfm3::sizes(R, N, K, gated) || R == 0) return 0;
+  if (lfm3::kind_of(R, N, K, gated) == lfm3::FUSED) return 0;
   const int64_t mpad = lfm3::round_up(R, 32);
   return mpad * lfm3::round_up(K, 128) + mpad * 4;
 }
@@ -199,23 +407,38 @@ int lfm3_hip_linear8(const uint16_t* x, int64_t ldx, const int8_t* wsh, const fl
                 "linear8: R and N up to 2^24 (N even for a gated weight), K a multiple of 8 up to 65536, gated 0 or 1");
   KV800_REQUIRE(ldx % 8 == 0 && ldy >= 0, "linear8: ldx must be a multiple of 8 and ldy >= 0");
   if (R == 0) return KV800_OK;
-  KV800_REQUIRE(x && wsh && ssh && y && (uintptr_t)x % 16 == 0 && (uintptr_t)wsh % 16 == 0, "linear8: null or unaligned pointer");
+  KV800_REQUIRE(x && wsh && ssh && y && (uintptr_t)x % 16 == 0 && (uintptr_t)wsh % 16 == 0 && (uintptr_t)ssh % 16 == 0, "linear8: null or unaligned pointer");
   const int64_t need = lfm3_hip_linear8_workspace(R, N, K, gated);
-  KV800_REQUIRE(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need, "linear8: %lld bytes of 16-byte aligned workspace needed", (long long)need);
+  KV800_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), "linear8: %lld bytes of 16-byte aligned workspace needed", (long long)need);
   const int64_t mt = lfm3::round_up(R, 32) / 32, nt = lfm3::padded_rows(N, gated) / 32, nks = lfm3::round_up(K, 128) / 32;
+  const lfm3::Out o = {y, ldy, R, N, ldy % 4 == 0 && (uintptr_t)y % 8 == 0};
+  const lfm3::Kind kind = lfm3::kind_of(R, N, K, gated);
+  hipStream_t st = (hipStream_t)stream;
   int8_t* xq = (int8_t*)ws;
   float* sx = (float*)(xq + mt * nks * 1024);
-  hipLaunchKernelGGL(lfm3::quantize_kernel<true>, dim3((unsigned)((R + 3) / 4)), dim3(256), 0, (hipStream_t)stream, x, ldx, R, K, nks,
-                     xq, sx);
-  int rc = kv800::check_launch("linear8 quantize");
-  if (rc != KV800_OK) return rc;
-  const dim3 grid((unsigned)((nt + 3) / 4), (unsigned)((mt + 3) / 4));
-  KV800_REQUIRE(grid.y <= 65535, "linear8: too many tokens");
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, xq, sx, wsh, ssh, R, N, nt, mt, nks, y, ldy);
+  if (kind != lfm3::FUSED) {
+    hipLaunchKernelGGL(lfm3::quantize_kernel<true>, dim3((unsigned)R), dim3(256), 0, st, x, ldx, R, K, nks, xq, sx);
+    const int rc = kv800::check_launch("linear8 quantize");
+    if (rc != KV800_OK) return rc;
+  }
+  auto few = [&](auto kernel, int64_t wm) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(nt / 2), (unsigned)((mt + wm - 1) / wm)), dim3(64 * lfm3::FEW), 0, st, x, ldx, xq, sx, wsh,
+                       ssh, K, nks, o);
   };
-  if (gated) go(lfm3::product_kernel<true>);
-  else go(lfm3::product_kernel<false>);
+  if (kind == lfm3::FUSED) {
+    if (gated) few(lfm3::few_kernel<1, true, true>, 1);
+    else few(lfm3::few_kernel<1, false, true>, 1);
+  } else if (kind == lfm3::ONE) {
+    if (gated) few(lfm3::few_kernel<1, true, false>, 1);
+    else few(lfm3::few_kernel<1, false, false>, 1);
+  } else if (kind == lfm3::TWO) {
+    if (gated) few(lfm3::few_kernel<2, true, false>, 2);
+    else few(lfm3::few_kernel<2, false, false>, 2);
+  } else {
+    const dim3 grid((unsigned)((nt + lfm3::TILE - 1) / lfm3::TILE * ((mt + lfm3::TILE - 1) / lfm3::TILE)));
+    if (gated) hipLaunchKernelGGL(lfm3::many_kernel<true>, grid, dim3(64 * lfm3::MANY), 0, st, xq, sx, wsh, ssh, nt, mt, nks, o);
+    else hipLaunchKernelGGL(lfm3::many_kernel<false>, grid, dim3(64 * lfm3::MANY), 0, st, xq, sx, wsh, ssh, nt, mt, nks, o);
+  }
   return kv800::check_launch("linear8");
 }
 
