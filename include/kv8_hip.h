@@ -29,7 +29,7 @@ typedef struct kv8_cache {
   uint8_t* data;
   uint8_t* exps;
   int64_t pages, kv_heads, blocks, dim;   /* blocks of 64 tokens a page; dim D: 64 or 128 */
-  int64_t page_stride, exp_stride;        /* bytes from page to page (page_stride a multiple of 16, data 16-byte aligned) */
+  int64_t page_stride, exp_stride;        /* bytes from page to page (a multiple of 16 and of 2; data 16-byte aligned, exps 2) */
 } kv8_cache_t;
 
 /* Append the step's tokens: k, v rows of kv_heads x D bf16, token and head strides in elements (multiples of 8, 16-byte

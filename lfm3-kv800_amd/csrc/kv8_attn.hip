@@ -46,6 +46,19 @@ struct Attend {
   Desc* desc;                         // one per workgroup
 };
 
+// What is the same for a whole wave and not written by the kernel: through the scalar cache, so that its arrival is not waited for in
+// the order of the vector loads.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)p; }
+__device__ __forceinline__ int64_t same(int64_t x) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+// the exponent bytes of keys and values at p (an even address): the low and high byte
+__device__ __forceinline__ uint32_t exps_load(const uint8_t* p) {
+  const uintptr_t a = (uintptr_t)p;
+  return scalar_load((const uint32_t*)(a & ~(uintptr_t)3)) >> (8 * (a & 2));
+}
+
 struct Row {
   int64_t q0, p0, n;                  // first token, its position, positions (those the table covers)
   int64_t b0;                         // first block that its first query sees
@@ -62,6 +75,13 @@ __device__ __forceinline__ Row row_at(const Attend& A, int r) {
   const int64_t lo = A.window > 0 ? max(w.p0 + 1 - A.window, (int64_t)0) : 0;
   w.b0 = min(lo, w.n) / BLK;
   w.steps = max((int)((w.n - w.b0 * BLK + STEP - 1) / STEP), 1);         // 1 also without keys: the outputs are written
+  return w;
+}
+// The same with r and all results in scalar registers.
+__device__ __forceinline__ Row uniform_row(const Attend& A, int r) {
+  Row w = row_at(A, r);
+  w.q0 = same(w.q0); w.p0 = same(w.p0); w.n = same(w.n); w.b0 = same(w.b0);
+  w.c = __builtin_amdgcn_readfirstlane(w.c); w.tiles = __builtin_amdgcn_readfirstlane(w.tiles); w.steps = __builtin_amdgcn_readfirstlane(w.steps);
   return w;
 }
 __device__ __forceinline__ int64_t cost_of(const Attend& A, const Row& w) { return (int64_t)w.tiles * A.C.heads * w.steps; }
@@ -129,7 +149,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
   __shared__ typename std::conditional<LIST, List, int>::type L;
   __shared__ __align__(16) float so[4][COLS][LD];
   __shared__ float sm[4][COLS], sl[4][COLS];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, rr = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), rr = lane & 15, g = lane >> 4;
   const int64_t w = blockIdx.x;
 
   for (int64_t t = max(A.qsl[A.R], (int64_t)0) + w; t < A.T; t += gridDim.x)     // the padding
@@ -147,12 +167,15 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
     if (w >= NG) return;
     x = w * W / NG;
     end = (w + 1) * W / NG;
-    r = find_row(A, L, per, x, before);
-    row = row_at(A, r);
+    r = __builtin_amdgcn_readfirstlane(find_row(A, L, per, x, before));
+    before = same(before);
+    x = same(x);
+    end = same(end);
+    row = uniform_row(A, r);
   } else {
     const int64_t ti = w / A.C.heads;
-    r = (int)kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / A.TQ + i <= ti; });
-    row = row_at(A, r);
+    r = (int)same(kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / A.TQ + i <= ti; }));
+    row = uniform_row(A, r);
     if (ti - (row.q0 / A.TQ + r) >= row.tiles) return;
   }
   while (x < end) {
@@ -161,7 +184,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
     if constexpr (LIST) {
       while (x >= before + cost_of(A, row)) {
         before += cost_of(A, row);
-        row = row_at(A, ++r);
+        row = uniform_row(A, ++r);
       }
       const int64_t item = (x - before) / row.steps;
       at = before + item * row.steps;
@@ -208,15 +231,15 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
         on[u] = bp <= thi && bp + BLK > tlo + 1 && col < A.bt_cols;
         int64_t page = 0;
         if (on[u]) {
-          page = A.bt[(int64_t)r * A.bt_stride + col];
+          page = scalar_load(A.bt + (int64_t)r * A.bt_stride + col);
           on[u] = page >= 0 && page < A.C.pages;
         }
         if (on[u]) {
           const int ub = (int)(bi % A.C.blocks);
           const uint8_t* base = block_of<D>(A.C, page, h, ub);
-          const uint8_t* ex = exps_of(A.C, page, h, ub);
-          sc[u][0] = pow2(held_exponent(ex[0]));
-          sc[u][1] = pow2(held_exponent(ex[1]));
+          const uint32_t ex = exps_load(exps_of(A.C, page, h, ub));
+          sc[u][0] = pow2(held_exponent((uint8_t)ex));
+          sc[u][1] = pow2(held_exponent((uint8_t)(ex >> 8)));
 #pragma unroll
           for (int a = 0; a < 4; ++a)
 #pragma unroll
@@ -470,8 +493,8 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   }
   if (ti >= ntiles) return;                                               // uniform, as every return
   ti = ntiles - 1 - ti;
-  const int64_t r = kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / TQ + i <= ti; });
-  const Row row = row_at(A, (int)r);
+  const int64_t r = same(kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / TQ + i <= ti; }));
+  const Row row = uniform_row(A, (int)r);
   const int64_t tile = ti - (row.q0 / TQ + r);
   if (tile < 0 || tile * TQ >= row.c) return;
   const int i0 = (int)tile * TQ, ilast = min(row.c, i0 + TQ) - 1;         // queries [i0, ilast] of the row
@@ -499,14 +522,14 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
 
   // ---- staging: the codes of block bi into registers, later widened into LDS
   uint4 rk[NP], rv[NP];
-  float sk = 1.f, sv = 1.f;
-  auto page_of = [&](int bi) -> int {
-    const int col = bi / A.C.blocks;
-    const int p = bi < b1 && col < A.bt_cols ? A.bt[r * A.bt_stride + col] : -1;
-    return p < A.C.pages ? p : -1;
+  uint32_t re = 0;
+  auto page_of = [&](int bi) {   // as the table has it; looked at a block later, when it has arrived
+    const int col = min(bi / A.C.blocks, A.bt_cols - 1);
+    return scalar_load(A.bt + r * A.bt_stride + col);
   };
+  auto valid = [&](int page, int bi) { return page >= 0 && page < A.C.pages && bi < b1; };
   auto load = [&](int bi, int page) {
-    if (page >= 0) {
+    if (valid(page, bi)) {
       const uint8_t* base = block_of<D>(A.C, page, h, bi % A.C.blocks);
       const uint8_t* ex = exps_of(A.C, page, h, bi % A.C.blocks);
 #pragma unroll
@@ -514,12 +537,11 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
         rk[j] = *reinterpret_cast<const uint4*>(base + (tid + j * 64 * NW) * 16);
         rv[j] = *reinterpret_cast<const uint4*>(base + BLK * D + (tid + j * 64 * NW) * 16);
       }
-      sk = pow2(held_exponent(ex[0]));
-      sv = pow2(held_exponent(ex[1]));
+      re = exps_load(ex);
     } else {
 #pragma unroll
       for (int j = 0; j < NP; ++j) rk[j] = rv[j] = make_uint4(0, 0, 0, 0);
-      sk = sv = 1.f;
+      re = 0;
     }
   };
   auto is_edge = [&](int bi) { return (int64_t)bi * BLK < alo || (int64_t)bi * BLK + BLK > ahi; };
@@ -535,6 +557,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
       for (int j = 0; j < NP; ++j) { clean(rv[j].x); clean(rv[j].y); clean(rv[j].z); clean(rv[j].w); }
       if (any) flag[buf] = bi;
     }
+    const float sk = pow2(held_exponent((uint8_t)re)), sv = pow2(held_exponent((uint8_t)(re >> 8)));
     uint8_t* kd = lds[buf];
     uint8_t* vd = lds[buf] + KB;
 #pragma unroll
@@ -559,19 +582,27 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   const float lazy = part || A.window > 0 ? 0.f : LAZY;
 
   if (tid < 2) flag[tid] = -1;
-  int page = page_of(b0), now = page, next = page_of(b0 + 1);
-  if (b0 < b1) load(b0, page);
+  int now = 0, next = 0, next2 = 0;               // pages of blocks bi, bi + 1, bi + 2
+  if (b0 < b1) {                                   // then the table has columns
+    now = page_of(b0);
+    next = page_of(b0 + 1);
+    next2 = page_of(b0 + 2);
+    load(b0, now);
+  }
   __syncthreads();
-  if (b0 < b1) store(b0, b0 & 1);
-  load(b0 + 1, next);
+  if (b0 < b1) {
+    store(b0, b0 & 1);
+    load(b0 + 1, next);
+  }
   __syncthreads();
   for (int bi = b0; bi < b1; ++bi) {
     const int buf = bi & 1;
-    const int after = page_of(bi + 2);
     if (bi + 1 < b1) {
       store(bi + 1, buf ^ 1);
-      load(bi + 2, after);
+      load(bi + 2, next2);
     }
+    const int after = page_of(bi + 3);
+    const bool held = valid(now, bi);
     if (busy) {
       const uint8_t* kd = lds[buf] + (hf * BLK + cl) * 16;
       __builtin_amdgcn_s_setprio(0);
@@ -584,14 +615,14 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
           const f16v zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
           s[a] = mfma32(x, qr[k], k == 0 ? zero : s[a]);
         }
-      const bool edge = now < 0 || is_edge(bi);
+      const bool edge = !held || is_edge(bi);
       if (edge) {
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
             const int64_t t = (int64_t)bi * BLK + 32 * a + 16 * (v >> 3) + 8 * hf + (v & 7);
-            if (t > qp || t <= qlo || t >= row.n || now < 0) s[a][v] = -INFINITY;
+            if (t > qp || t <= qlo || t >= row.n || !held) s[a][v] = -INFINITY;
           }
       }
       __builtin_amdgcn_s_setprio(2);
@@ -627,7 +658,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
         }
       }
       l += sum;
-      if (edge && now >= 0 && flag[buf] == bi) {
+      if (edge && held && flag[buf] == bi) {
         const uint8_t* base = block_of<D>(A.C, now, h, bi % A.C.blocks) + BLK * D;
         for (int t = 0; t < BLK; ++t) {
           const int64_t tp = (int64_t)bi * BLK + t;
@@ -641,7 +672,8 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
       }
     }
     now = next;
-    next = after;
+    next = next2;
+    next2 = after;
     __syncthreads();
   }
   const float2 ls = kv800::halves32(l);

@@ -60,7 +60,8 @@ inline bool valid(const kv8_cache_t* c) {
   return c && c->data && c->exps && (uintptr_t)c->data % 16 == 0 && c->pages > 0 && c->pages < INT32_MAX && c->kv_heads > 0 &&
          c->blocks > 0 && (c->dim == 64 || c->dim == 128) && c->kv_heads <= 65535 / 2 && c->blocks <= (1 << 20) &&
          c->kv_heads * c->blocks < (1 << 24) && c->page_stride % 16 == 0 &&
-         c->page_stride >= c->kv_heads * c->blocks * 2 * BLK * c->dim && c->exp_stride >= c->kv_heads * c->blocks * 2;
+         c->page_stride >= c->kv_heads * c->blocks * 2 * BLK * c->dim && c->exp_stride >= c->kv_heads * c->blocks * 2 &&
+         c->exp_stride % 2 == 0 && (uintptr_t)c->exps % 2 == 0;
 }
 inline Cache device_form(const kv8_cache_t* c) {
   return {c->data, c->exps, (int)c->pages, (int)c->kv_heads, (int)c->blocks, c->page_stride, c->exp_stride};

@@ -64,12 +64,13 @@ class Cache8:
             if not t[0].is_contiguous() or (P > 1 and t.stride(0) < t[0].numel()):
                 raise ValueError(f"{name}: a page must be contiguous, and pages may not overlap")
         ps = data.stride(0) if P > 1 else H * U * 2 * n
-        if ps % 16 or data.data_ptr() % 16:
-            raise ValueError("data must be 16-byte aligned, its pages a multiple of 16 bytes apart")
+        es = exps.stride(0) if P > 1 else H * U * 2
+        if ps % 16 or data.data_ptr() % 16 or es % 2 or exps.data_ptr() % 2:
+            raise ValueError("data must be 16-byte aligned, its pages a multiple of 16 bytes apart; exps 2-byte aligned, an even number apart")
         self.data, self.exps = data, exps
         self.pages, self.heads, self.blocks, self.dim = P, H, U, n // BLK
         self.bs = U * BLK
-        self._c = _Cache(data.data_ptr(), exps.data_ptr(), P, H, U, self.dim, ps, exps.stride(0) if P > 1 else H * U * 2)
+        self._c = _Cache(data.data_ptr(), exps.data_ptr(), P, H, U, self.dim, ps, es)
         self._p = ctypes.byref(self._c)
 
     @classmethod

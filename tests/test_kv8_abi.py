@@ -40,7 +40,7 @@ def desc(**k):
 
 
 BAD = [dict(data=None), dict(data=A + 8), dict(exps=None), dict(pages=0), dict(kv_heads=0), dict(blocks=0), dict(dim=96), dict(page_stride=4 * 2 * 2 * 8192 - 16),
-       dict(page_stride=4 * 2 * 2 * 8192 + 8), dict(exp_stride=15)]
+       dict(page_stride=4 * 2 * 2 * 8192 + 8), dict(exp_stride=15), dict(exp_stride=17), dict(exps=A + 1)]
 
 
 def refused(lib, rc, word):
