@@ -86,15 +86,16 @@ __device__ __forceinline__ Row uniform_row(const Attend& A, int r) {
 }
 __device__ __forceinline__ int64_t cost_of(const Attend& A, const Row& w) { return (int64_t)w.tiles * A.C.heads * w.steps; }
 
-// Prefix sums of the rows' list entries: pre[i] those before thread i's `per` rows, pre[256] all.
+// Prefix sums of what the rows count for: pre[i] of those before thread i's `per` rows, pre[256] all.
 struct List {
   int64_t pre[257];
   int64_t wave[4];
 };
-__device__ __forceinline__ void scan_rows(const Attend& A, List& L, int per) {
+template <typename F>
+__device__ __forceinline__ void scan_rows(const Attend& A, List& L, int per, F cost) {
   const int tid = threadIdx.x;
   int64_t s = 0;
-  for (int r = tid * per; r < min((tid + 1) * per, A.R); ++r) s += cost_of(A, row_at(A, r));
+  for (int r = tid * per; r < min((tid + 1) * per, A.R); ++r) s += cost(row_at(A, r));
   int64_t x = s;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -109,8 +110,9 @@ __device__ __forceinline__ void scan_rows(const Attend& A, List& L, int per) {
   if (tid == 0) L.pre[0] = 0;
   __syncthreads();
 }
-// Row that holds list entry x and the entries before that row.
-__device__ __forceinline__ int find_row(const Attend& A, const List& L, int per, int64_t x, int64_t& before) {
+// Row that holds number x of what was summed, and the sum before that row.
+template <typename F>
+__device__ __forceinline__ int find_row(const Attend& A, const List& L, int per, int64_t x, int64_t& before, F cost) {
   int lo = 0, hi = 256;
   while (hi - lo > 1) {
     const int m = (lo + hi) / 2;
@@ -120,7 +122,7 @@ __device__ __forceinline__ int find_row(const Attend& A, const List& L, int per,
   int r = lo * per;
   before = L.pre[lo];
   for (; r + 1 < A.R; ++r) {
-    const int64_t c = cost_of(A, row_at(A, r));
+    const int64_t c = cost(row_at(A, r));
     if (x < before + c) break;
     before += c;
   }
@@ -136,12 +138,20 @@ __device__ __forceinline__ kv800::b8 wide8(uint32_t a, uint32_t b, float f) {
   return kv800::b8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
 }
 
+// Zeros for the tokens behind the last row's, by all workgroups.
+template <int D>
+__device__ __forceinline__ void clear_padding(const Attend& A) {
+  for (int64_t t = max(A.qsl[A.R], (int64_t)0) + blockIdx.x; t < A.T; t += gridDim.x)
+    for (int i = threadIdx.x; i < A.C.heads * A.G * D / 8; i += blockDim.x)
+      reinterpret_cast<uint4*>(A.out + t * A.C.heads * A.G * D)[i] = make_uint4(0, 0, 0, 0);
+}
+
 // A part of one column: D sums of weighted values, the maximum (log2 units), the sum of weights, relative to it; PART floats.
 template <int D>
 constexpr int PART = D + 4;
 
 // LIST: one workgroup takes entries [w W / NG, (w + 1) W / NG) of the W of the list (row, query tile, head, step); else workgroup w is one
-// (query tile, head), found by the tiles' numbers qsl[r] / TQ + r on. The four waves take every fourth step of an item, each with its
+// (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one token. The four waves take every fourth step of an item, each with its
 // own maximum, sum and output, and are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
 template <int D, bool LIST>
 __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
@@ -152,31 +162,31 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), rr = lane & 15, g = lane >> 4;
   const int64_t w = blockIdx.x;
 
-  for (int64_t t = max(A.qsl[A.R], (int64_t)0) + w; t < A.T; t += gridDim.x)     // the padding
-    for (int i = tid; i < A.C.heads * A.G * D / 8; i += 256)
-      reinterpret_cast<uint4*>(A.out + t * A.C.heads * A.G * D)[i] = make_uint4(0, 0, 0, 0);
+  clear_padding<D>(A);
 
   int64_t x = 0, end = 1, before = 0, W = 0, NG = 1;
-  int r;
+  int r, tile0 = 0;
   Row row;
   if constexpr (LIST) {
     if (tid == 0) A.desc[w].last = -1;
-    scan_rows(A, L, per);
+    const auto cost = [&](const Row& w) { return cost_of(A, w); };
+    scan_rows(A, L, per, cost);
     W = L.pre[256];
     NG = min((int64_t)gridDim.x, W);               // no workgroup between two others is without entries
     if (w >= NG) return;
     x = w * W / NG;
     end = (w + 1) * W / NG;
-    r = __builtin_amdgcn_readfirstlane(find_row(A, L, per, x, before));
+    r = __builtin_amdgcn_readfirstlane(find_row(A, L, per, x, before, cost));
     before = same(before);
     x = same(x);
     end = same(end);
     row = uniform_row(A, r);
   } else {
     const int64_t ti = w / A.C.heads;
-    r = (int)same(kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / A.TQ + i <= ti; }));
+    r = (int)same(kv800::last_at(A.R, [&](int64_t i) { return (A.qsl[i] + i * (A.TQ - 1)) / A.TQ <= ti; }));
     row = uniform_row(A, r);
-    if (ti - (row.q0 / A.TQ + r) >= row.tiles) return;
+    tile0 = (int)((row.q0 + (int64_t)r * (A.TQ - 1)) / A.TQ);
+    if (ti - tile0 >= row.tiles) return;
   }
   while (x < end) {
     int64_t at = 0;
@@ -194,7 +204,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
       tile = (int)(item / A.C.heads);
     } else {
       h = (int)(w % A.C.heads);
-      tile = (int)(w / A.C.heads - (row.q0 / A.TQ + r));
+      tile = (int)(w / A.C.heads) - tile0;
     }
 
     // ---- the queries of the lane's column
@@ -448,10 +458,6 @@ __global__ void __launch_bounds__(256) merge_rows_kernel(const float* __restrict
 }
 
 // ---------------------------------------------------------------- many new tokens a row
-__global__ void __launch_bounds__(256) zero_padding_kernel(const int64_t* __restrict__ total, int64_t T, int64_t width, uint16_t* __restrict__ out) {
-  for (int64_t t = max(*total, (int64_t)0) + blockIdx.x; t < T; t += gridDim.x)
-    for (int64_t i = threadIdx.x; i < width / 8; i += 256) reinterpret_cast<uint4*>(out + t * width)[i] = make_uint4(0, 0, 0, 0);
-}
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 __device__ __forceinline__ f16v mfma32(kv800::u4v a, kv800::u4v b, f16v c) {
@@ -469,15 +475,21 @@ __device__ __forceinline__ float halves_max(float x) {
 // key tile a is token 32 a + 16 (b / 2) + 8 h + 4 (b % 2) + i: the lane's weights are then those of 8 tokens side by side, half
 // of a piece of the values.
 template <int D, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int64_t ntiles, int splits, float* __restrict__ part) {
+__global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int per, int splits, float* __restrict__ part) {
   constexpr int NT = D / 32, NK = D / 16, NP = 4 * D / (64 * NW);          // dim tiles, k-steps, pieces of K (and V) a thread stages
   constexpr int KB = BLK * D * 2;                                          // bytes of a block's keys in bf16
   __shared__ __align__(16) uint8_t lds[2][2 * KB];
   __shared__ int flag[2];
+  __shared__ List L;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, cl = lane & 31, hf = lane >> 5;
   const int H = A.C.heads, Hq = H * A.G;
-  // workgroup b runs on XCD b % 8: where the heads divide 8, an XCD has one head and every (8 / heads)-th tile of it, so that
-  // its L2 holds one head's blocks; the last tiles first, which see the most
+  clear_padding<D>(A);
+  // The rows' tiles side by side: idle workgroups are the last ones (at every other place they would leave half the chip's
+  // engines without work: 64 rows of 32 tokens over 4K 165 us). Workgroup b runs on XCD b % 8: where the heads divide 8, an XCD has
+  // one head and every (8 / heads)-th tile of it, so that its L2 holds one head's blocks; the last tiles first, which see the most.
+  const auto tiles = [&](const Row& w) { return (int64_t)((w.c + TQ - 1) / TQ); };
+  scan_rows(A, L, per, tiles);
+  const int64_t ntiles = same(L.pre[256]);
   int64_t b = blockIdx.x;
   const int sp = (int)(b % splits);
   b /= splits;
@@ -493,10 +505,10 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   }
   if (ti >= ntiles) return;                                               // uniform, as every return
   ti = ntiles - 1 - ti;
-  const int64_t r = same(kv800::last_at(A.R, [&](int64_t i) { return A.qsl[i] / TQ + i <= ti; }));
+  int64_t before;
+  const int64_t r = same(find_row(A, L, per, ti, before, tiles));
   const Row row = uniform_row(A, (int)r);
-  const int64_t tile = ti - (row.q0 / TQ + r);
-  if (tile < 0 || tile * TQ >= row.c) return;
+  const int64_t tile = ti - same(before);
   const int i0 = (int)tile * TQ, ilast = min(row.c, i0 + TQ) - 1;         // queries [i0, ilast] of the row
   const int cc = wv * 32 + cl, iq = i0 + cc / A.G, hq = h * A.G + cc % A.G;
   const bool have = cc < TQ * A.G && iq <= ilast;
@@ -515,9 +527,9 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   const int64_t ahi = min(row.p0 + i0 + 1, row.n), alo = A.window > 0 ? row.p0 + ilast - A.window + 1 : 0;
   int b0 = (int)(tlo / BLK), b1 = thi < tlo ? b0 : (int)(thi / BLK) + 1;
   {
-    const int per = (b1 - b0 + splits - 1) / splits;
-    b0 = min(b1, b0 + sp * per);
-    b1 = min(b1, b0 + per);
+    const int share = (b1 - b0 + splits - 1) / splits;
+    b0 = min(b1, b0 + sp * share);
+    b1 = min(b1, b0 + share);
   }
 
   // ---- staging: the codes of block bi into registers, later widened into LDS
@@ -720,7 +732,7 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
   const int64_t seen = window > 0 && window + mean < positions ? window + mean : positions;   // of a row, or so
   p.kind = T * p.G >= 64 * R ? PROMPT : seen <= 8 * STEP ? DIRECT : LISTED;
   p.TQ = (p.kind == PROMPT ? 32 * NW : COLS) / p.G;
-  p.tiles = T / p.TQ + R;
+  p.tiles = (T + R * (p.TQ - 1)) / p.TQ;
   if (p.kind == PROMPT) {
     // few tiles: each split over its blocks, down to 8, for two workgroups a CU
     const int64_t wgs = (mean + p.TQ - 1) / p.TQ * R * c->kv_heads, most = seen / (8 * BLK);
@@ -743,9 +755,8 @@ int run(const Attend& A0, const Plan& p, int64_t heads, void* ws, hipStream_t s)
   if (p.kind == PROMPT) {
     const int64_t xs = 8 % H == 0 && p.splits == 1 ? 8 / H : 1;
     float* part = p.splits > 1 ? (float*)ws : nullptr;
-    hipLaunchKernelGGL(zero_padding_kernel, dim3(64), dim3(256), 0, s, A.qsl + A.R, A.T, heads * D, A.out);
     hipLaunchKernelGGL((prompt_kernel<D, NW>), dim3((unsigned)((p.tiles + xs - 1) / xs * xs * H * p.splits)), dim3(64 * NW), 0, s, A, p.TQ,
-                       p.tiles, p.splits, part);
+                       (A.R + 255) / 256, p.splits, part);
     if (part)
       hipLaunchKernelGGL(merge_rows_kernel<D>, dim3((unsigned)((A.T * heads + 3) / 4)), dim3(256), 0, s, part, p.splits, A.qsl + A.R,
                          (int)heads, A.T, A.out);
