@@ -281,14 +281,17 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
         for (int j = 0; j < 4; ++j) s[4 * a + j] = c[j] * A.sl2;
       }
       const bool edge = pos < alo || pos + STEP > ahi || !on[0] || !on[1];
-      if (edge) {
+      if (edge) {          // tokens of the step that the column's query sees: [lo, hi)
+        int lo = (int)min(max(qlo + 1 - pos, (int64_t)0), (int64_t)STEP), hi = (int)min(max(min(qp + 1, row.n) - pos, (int64_t)0), (int64_t)STEP);
+        if (!on[0]) lo = max(lo, BLK);
+        if (!on[1]) hi = min(hi, BLK);
+        const int see0 = lo - 16 * g;
+        const uint32_t seen = (uint32_t)max(hi - lo, 0);
 #pragma unroll
         for (int a = 0; a < 8; ++a)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int64_t t = pos + 64 * (a >> 2) + 16 * g + 4 * (a & 3) + j;
-            if (t > qp || t <= qlo || t >= row.n || !on[a >> 2]) s[4 * a + j] = -INFINITY;
-          }
+          for (int j = 0; j < 4; ++j)
+            if ((uint32_t)(64 * (a >> 2) + 4 * (a & 3) + j - see0) >= seen) s[4 * a + j] = -INFINITY;
       }
       float mt = s[0];
 #pragma unroll
@@ -321,16 +324,21 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
       // ---- in a step with a mask, codes that not every query sees: a weight of 0 does not take out a NaN
       bool poison = false;
       if (edge) {
-        auto clean = [&](uint32_t& x) {
-          const uint32_t nb = nan_bytes(x);
-          poison |= nb != 0;
-          x &= ~(nb * 255u);
+        uint32_t top = 0;  // bit 7 of a byte: some value there is a NaN code
+        auto look = [&](const uint4& x) {
+          top |= ((x.x & 0x7F7F7F7Fu) + 0x01010101u) | ((x.y & 0x7F7F7F7Fu) + 0x01010101u);
+          top |= ((x.z & 0x7F7F7F7Fu) + 0x01010101u) | ((x.w & 0x7F7F7F7Fu) + 0x01010101u);
         };
 #pragma unroll
-        for (int d = 0; d < NT; ++d)
+        for (int d = 0; d < NT; ++d) { look(vv[d][0]); look(vv[d][1]); }
+        poison = __any((top & 0x80808080u) != 0);
+        if (poison) {
+          auto clean = [&](uint32_t& x) { x &= ~(nan_bytes(x) * 255u); };
 #pragma unroll
-          for (int u = 0; u < 2; ++u) { clean(vv[d][u].x); clean(vv[d][u].y); clean(vv[d][u].z); clean(vv[d][u].w); }
-        poison = __any(poison);
+          for (int d = 0; d < NT; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) { clean(vv[d][u].x); clean(vv[d][u].y); clean(vv[d][u].z); clean(vv[d][u].w); }
+        }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -609,15 +617,10 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   __syncthreads();
   for (int bi = b0; bi < b1; ++bi) {
     const int buf = bi & 1;
-    if (bi + 1 < b1) {
-      store(bi + 1, buf ^ 1);
-      load(bi + 2, next2);
-    }
     const int after = page_of(bi + 3);
     const bool held = valid(now, bi);
-    if (busy) {
+    {
       const uint8_t* kd = lds[buf] + (hf * BLK + cl) * 16;
-      __builtin_amdgcn_s_setprio(0);
       f16v s[2];
 #pragma unroll
       for (int k = 0; k < NK; ++k)
@@ -627,17 +630,22 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
           const f16v zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
           s[a] = mfma32(x, qr[k], k == 0 ? zero : s[a]);
         }
+      store(bi + 1, buf ^ 1);
+      load(bi + 2, next2);
       const bool edge = !held || is_edge(bi);
       if (edge) {
+        // tokens of the block that the lane's query sees: [lo, hi)
+        const int64_t bp = (int64_t)bi * BLK;
+        const int lo = (int)min(max(qlo + 1 - bp, (int64_t)0), (int64_t)BLK), hi = held ? (int)min(max(min(qp + 1, row.n) - bp, (int64_t)0), (int64_t)BLK) : 0;
+        const int see0 = lo - 8 * hf;
+        const uint32_t seen = (uint32_t)max(hi - lo, 0);
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const int64_t t = (int64_t)bi * BLK + 32 * a + 16 * (v >> 3) + 8 * hf + (v & 7);
-            if (t > qp || t <= qlo || t >= row.n || !held) s[a][v] = -INFINITY;
+            if ((uint32_t)(32 * a + 16 * (v >> 3) + (v & 7) - see0) >= seen) s[a][v] = -INFINITY;
           }
       }
-      __builtin_amdgcn_s_setprio(2);
       float mt = -INFINITY;
 #pragma unroll
       for (int a = 0; a < 2; ++a)
@@ -651,7 +659,6 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
 #pragma unroll
         for (int d = 0; d < NT; ++d) o[d] *= alpha;
       }
-      __builtin_amdgcn_s_setprio(1);
       const uint8_t* vd = lds[buf] + KB + (hf * D + cl) * 16;
       float sum = 0.f;
 #pragma unroll
