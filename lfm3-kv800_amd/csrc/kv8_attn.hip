@@ -21,7 +21,6 @@ namespace {
 using kv800::f4;
 
 constexpr int COLS = 16;              // (query, query head) pairs of a tile
-constexpr int STEP = 128;             // positions of a wave's step: two blocks
 constexpr float LAZY = 8.f;           // log2 units by which a running maximum may lag over a long list of keys
 
 struct Desc {                         // of a workgroup whose last item others finish: where that item's outputs go
@@ -39,6 +38,7 @@ struct Attend {
   int64_t T;
   int G, TQ;                          // query heads per KV head, queries per tile
   int64_t window;
+  int step;                           // positions of a wave's step
   float sl2;                          // |scale| log2(e)
   uint32_t flip;                      // sign bits of two bf16 for a negative scale: q changes its sign
   uint16_t* out;
@@ -74,7 +74,7 @@ __device__ __forceinline__ Row row_at(const Attend& A, int r) {
   w.tiles = (w.c + A.TQ - 1) / A.TQ;
   const int64_t lo = A.window > 0 ? max(w.p0 + 1 - A.window, (int64_t)0) : 0;
   w.b0 = min(lo, w.n) / BLK;
-  w.steps = max((int)((w.n - w.b0 * BLK + STEP - 1) / STEP), 1);         // 1 also without keys: the outputs are written
+  w.steps = max((int)((w.n - w.b0 * BLK + A.step - 1) / A.step), 1);         // 1 also without keys: the outputs are written
   return w;
 }
 // The same with r and all results in scalar registers.
@@ -153,8 +153,9 @@ constexpr int PART = D + 4;
 // LIST: one workgroup takes entries [w W / NG, (w + 1) W / NG) of the W of the list (row, query tile, head, step); else workgroup w is one
 // (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one token. The four waves take every fourth step of an item, each with its
 // own maximum, sum and output, and are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
-template <int D, bool LIST>
-__global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
+template <int D, bool LIST, int NB>
+__global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, int per) {
+  constexpr int STEP = NB * BLK;                   // positions of a wave's step
   constexpr int NT = D / 16, NK = D / 32, LD = D + 4;
   __shared__ typename std::conditional<LIST, List, int>::type L;
   __shared__ __align__(16) float so[4][COLS][LD];
@@ -183,7 +184,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
     row = uniform_row(A, r);
   } else {
     const int64_t ti = w / A.C.heads;
-    r = (int)same(kv800::last_at(A.R, [&](int64_t i) { return (A.qsl[i] + i * (A.TQ - 1)) / A.TQ <= ti; }));
+    const auto from = [&](int64_t i) { return (A.qsl[i] + i * (A.TQ - 1)) / A.TQ; };
+    r = (int)min(ti, (int64_t)A.R - 1);            // so it is where every row before has one tile
+    if (from(r) > ti || (r + 1 < A.R && from(r + 1) <= ti)) r = (int)kv800::last_at(A.R, [&](int64_t i) { return from(i) <= ti; });
+    r = __builtin_amdgcn_readfirstlane(r);
     row = uniform_row(A, r);
     tile0 = (int)((row.q0 + (int64_t)r * (A.TQ - 1)) / A.TQ);
     if (ti - tile0 >= row.tiles) return;
@@ -232,11 +236,11 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
       const int64_t pos = row.b0 * BLK + (int64_t)st * STEP;
       if (pos > thi || pos + STEP <= tlo + 1) continue;
       // ---- codes of the two blocks; a block that no query sees, or without a page, is not read
-      uint4 kk[8][D / 64], vv[NT][2];
-      float sc[2][2];
-      bool on[2];
+      uint4 kk[4 * NB][D / 64], vv[NT][NB];
+      float sc[NB][2];
+      bool on[NB];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < NB; ++u) {
         const int64_t bp = pos + u * BLK, bi = bp / BLK, col = bi / A.C.blocks;
         on[u] = bp <= thi && bp + BLK > tlo + 1 && col < A.bt_cols;
         int64_t page = 0;
@@ -268,9 +272,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
         }
       }
       // ---- scores of the lane's column: tile a holds tokens 64 (a / 4) + 16 g + 4 (a % 4) + j
-      float s[32];
+      float s[16 * NB];
 #pragma unroll
-      for (int a = 0; a < 8; ++a) {
+      for (int a = 0; a < 4 * NB; ++a) {
         f4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) {
@@ -280,22 +284,22 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[4 * a + j] = c[j] * A.sl2;
       }
-      const bool edge = pos < alo || pos + STEP > ahi || !on[0] || !on[1];
+      const bool edge = pos < alo || pos + STEP > ahi || !on[0] || !on[NB - 1];
       if (edge) {          // tokens of the step that the column's query sees: [lo, hi)
         int lo = (int)min(max(qlo + 1 - pos, (int64_t)0), (int64_t)STEP), hi = (int)min(max(min(qp + 1, row.n) - pos, (int64_t)0), (int64_t)STEP);
         if (!on[0]) lo = max(lo, BLK);
-        if (!on[1]) hi = min(hi, BLK);
+        if (!on[NB - 1]) hi = min(hi, STEP - BLK);
         const int see0 = lo - 16 * g;
         const uint32_t seen = (uint32_t)max(hi - lo, 0);
 #pragma unroll
-        for (int a = 0; a < 8; ++a)
+        for (int a = 0; a < 4 * NB; ++a)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if ((uint32_t)(64 * (a >> 2) + 4 * (a & 3) + j - see0) >= seen) s[4 * a + j] = -INFINITY;
       }
       float mt = s[0];
 #pragma unroll
-      for (int j = 1; j < 32; ++j) mt = fmaxf(mt, s[j]);
+      for (int j = 1; j < 16 * NB; ++j) mt = fmaxf(mt, s[j]);
       mt = kv800::max4rows(mt);
       const float Mn = fmaxf(M, ceilf(mt));
       if (__any(Mn > M)) {
@@ -309,10 +313,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
       }
       // ---- weights
       const float M0 = M > -INFINITY ? M : 0.f;
-      uint32_t pw[16];
+      uint32_t pw[8 * NB];
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 8 * NB; ++j) {
         const float p0 = __builtin_amdgcn_exp2f(s[2 * j] - M0), p1 = __builtin_amdgcn_exp2f(s[2 * j + 1] - M0);
         sum += p0 + p1;
         pw[j] = kv800::bfpk(p0, p1);
@@ -330,18 +334,20 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(Attend A, int per) {
           top |= ((x.z & 0x7F7F7F7Fu) + 0x01010101u) | ((x.w & 0x7F7F7F7Fu) + 0x01010101u);
         };
 #pragma unroll
-        for (int d = 0; d < NT; ++d) { look(vv[d][0]); look(vv[d][1]); }
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+          for (int u = 0; u < NB; ++u) look(vv[d][u]);
         poison = __any((top & 0x80808080u) != 0);
         if (poison) {
           auto clean = [&](uint32_t& x) { x &= ~(nan_bytes(x) * 255u); };
 #pragma unroll
           for (int d = 0; d < NT; ++d)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) { clean(vv[d][u].x); clean(vv[d][u].y); clean(vv[d][u].z); clean(vv[d][u].w); }
+            for (int u = 0; u < NB; ++u) { clean(vv[d][u].x); clean(vv[d][u].y); clean(vv[d][u].z); clean(vv[d][u].w); }
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < NB; ++u) {
         const kv800::b8 pa = kv800::as_b8(kv800::u4v{pw[8 * u], pw[8 * u + 1], pw[8 * u + 2], pw[8 * u + 3]});
         const kv800::b8 pb = kv800::as_b8(kv800::u4v{pw[8 * u + 4], pw[8 * u + 5], pw[8 * u + 6], pw[8 * u + 7]});
 #pragma unroll
@@ -724,10 +730,11 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
 enum Kind { LISTED, DIRECT, PROMPT };
 struct Plan {
   Kind kind;
-  int TQ, G, splits;
+  int TQ, G, splits, step;
   int64_t tiles, groups;              // query tiles of all rows at most; workgroups (LISTED)
   int64_t bytes;                      // workspace
 };
+constexpr int SD = 1, SL = 2;         // blocks a step
 constexpr int NW = 4;                 // waves of the prompt kernel
 Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
   Plan p;
@@ -737,7 +744,8 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
   p.bytes = 0;
   const int64_t positions = bt_cols * c->blocks * BLK, mean = (T + R - 1) / R;
   const int64_t seen = window > 0 && window + mean < positions ? window + mean : positions;   // of a row, or so
-  p.kind = T * p.G >= 64 * R ? PROMPT : seen <= 8 * STEP ? DIRECT : LISTED;
+  p.kind = T * p.G >= 64 * R ? PROMPT : seen <= 1024 ? DIRECT : LISTED;
+  p.step = p.kind == DIRECT ? SD * BLK : SL * BLK;
   p.TQ = (p.kind == PROMPT ? 32 * NW : COLS) / p.G;
   p.tiles = (T + R * (p.TQ - 1)) / p.TQ;
   if (p.kind == PROMPT) {
@@ -748,7 +756,7 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
     p.splits = (int)(s < 1 ? 1 : s);
     if (p.splits > 1) p.bytes = T * heads * p.splits * (c->dim + 4) * 4;
   } else if (p.kind == LISTED) {
-    const int64_t entries = p.tiles * c->kv_heads * ((positions + STEP - 1) / STEP + 1);
+    const int64_t entries = p.tiles * c->kv_heads * ((positions + p.step - 1) / p.step + 1);
     p.groups = (entries + 3) / 4 < 512 ? (entries + 3) / 4 : 512;
     p.bytes = p.groups * (2 * COLS * (c->dim + 4) * 4 + (int64_t)sizeof(Desc));
   }
@@ -770,12 +778,12 @@ int run(const Attend& A0, const Plan& p, int64_t heads, void* ws, hipStream_t s)
     return kv800::check_launch("kv8_attend prompt");
   }
   if (p.kind == DIRECT) {
-    hipLaunchKernelGGL((attend_kernel<D, false>), dim3((unsigned)(p.tiles * H)), dim3(256), 0, s, A, 0);
+    hipLaunchKernelGGL((attend_kernel<D, false, SD>), dim3((unsigned)(p.tiles * H)), dim3(256), 0, s, A, 0);
     return kv800::check_launch("kv8_attend");
   }
   A.part = (float*)ws;
   A.desc = (Desc*)(A.part + p.groups * 2 * COLS * PART<D>);
-  hipLaunchKernelGGL((attend_kernel<D, true>), dim3((unsigned)p.groups), dim3(256), 0, s, A, (A.R + 255) / 256);
+  hipLaunchKernelGGL((attend_kernel<D, true, SL>), dim3((unsigned)p.groups), dim3(256), 0, s, A, (A.R + 255) / 256);
   const int rc = kv800::check_launch("kv8_attend");
   if (rc != KV800_OK) return rc;
   hipLaunchKernelGGL(merge_kernel<D>, dim3((unsigned)p.groups, COLS / 4), dim3(256), 0, s, A);
@@ -810,7 +818,7 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
   KV800_REQUIRE(p.tiles * cache->kv_heads * p.splits < INT32_MAX, "kv8_attend: too many tokens or rows");
   KV800_REQUIRE(p.bytes == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.bytes), "kv8_attend: %lld bytes of 16-byte aligned workspace needed",
                 (long long)p.bytes);
-  const kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window,
+  const kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window, p.step,
                          fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, out, nullptr, nullptr};
   return cache->dim == 128 ? kv8::run<128>(A, p, heads, ws, (hipStream_t)stream) : kv8::run<64>(A, p, heads, ws, (hipStream_t)stream);
 }
