@@ -40,6 +40,18 @@ __device__ __forceinline__ uint32_t down4(uint32_t w, float f) {
 // slot of token t of a block's keys
 __device__ __forceinline__ int slot_of(int t) { return ((t >> 2) & 3) * 16 + (t >> 4) * 4 + (t & 3); }
 
+// The last i in [0, n) with below(i), for a predicate that holds up to some index, 0 among them, looked for around a guess first: one
+// load where it is within 31 of it, else as kv800::last_at. By a whole wave, the same result in every lane.
+template <typename F>
+__device__ __forceinline__ int64_t row_near(int64_t n, int64_t guess, F below) {
+  const int lane = threadIdx.x & 63;
+  const int64_t lo = max(min(guess - 31, n - 64), (int64_t)0), i = lo + lane;
+  const uint64_t yes = __ballot(i < n && below(i < n ? i : 0));
+  const int c = __popcll(yes);                                          // lanes 0 .. c - 1
+  if (c > 0 && (c < 64 || lo + 64 >= n)) return lo + c - 1;
+  return kv800::last_at(n, below);
+}
+
 struct Cache {
   uint8_t* data;
   uint8_t* exps;
