@@ -3,7 +3,7 @@
 //   layout_kernel    a weight into operand order, once
 //   quantize_kernel  tokens (or a weight's rows) to 8 bits, a scale for each
 //   few_kernel       products of few tokens: weights streamed, K split over a workgroup's waves
-//   many_kernel      products of many: 256 x 256 outputs a workgroup through LDS
+//   many_kernel      products of many: 256 x 128 outputs a workgroup through LDS
 //
 // Sums of up to 65,536 products of 8-bit integers fit 32 bits, so they are exact and any split of K gives the same result; the
 // scales are applied once, in fp32.
@@ -47,105 +47,126 @@ __global__ void __launch_bounds__(256) layout_kernel(const int8_t* __restrict__ 
   *reinterpret_cast<uint4*>(wsh + i * 16) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// One workgroup per row. Up to 4 pieces of 2,048 channels stay in registers between the maximum and the codes; a longer row is read again.
-// OPERAND: codes in operand order of tiles of 32 rows (nks blocks each), else row by row.
-template <bool OPERAND>
+// 16 channels to codes
+__device__ __forceinline__ uint4 codes16(const uint4 (&u)[2], float inv) {
+  const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float f = e & 1 ? kv800::bf2f_hi(w[2 * i + (e >> 1)]) : kv800::bf2f_lo(w[2 * i + (e >> 1)]);
+      o[i] |= ((uint32_t)(int)rintf(f * inv) & 0xFFu) << (8 * e);
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// largest magnitude of 16 channels as an integer: of bf16 they order as their bits do, NaN above infinity
+__device__ __forceinline__ uint32_t top16(const uint4 (&u)[2]) {
+  const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t = max(t, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+  return t;
+}
+
+// WAVES waves of the workgroup's 4 per row. Up to 2 pieces of 16 channels a lane stay in registers between the maximum and the codes;
+// a longer row is read again. OPERAND: codes in operand order of tiles of 32 rows (nks blocks each), else row by row.
+template <bool OPERAND, int WAVES>
 __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t R, int64_t K, int64_t nks,
                                                        int8_t* __restrict__ q, float* __restrict__ scale) {
-  constexpr int HELD = 4, PIECE = 2048;
+  constexpr int HELD = 2, LANES = 64 * WAVES;
   __shared__ uint32_t tops[4];
-  const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x, lt = tid % LANES;
+  const int64_t r = (int64_t)blockIdx.x * (4 / WAVES) + tid / LANES;
+  if (WAVES == 1 && r >= R) return;
   const uint16_t* src = x + r * ldx;
-  uint4 held[HELD];
-  uint32_t top = 0;                                                      // magnitudes of bf16 order as integers; NaN above infinity
-  auto take = [&](const uint4& u) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  auto take = [&](int64_t k, uint4 (&u)[2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+    for (int p = 0; p < 2; ++p) {
+      u[p] = make_uint4(0, 0, 0, 0);
+      if (k + 8 * p < K) u[p] = *reinterpret_cast<const uint4*>(src + k + 8 * p);
+    }
   };
+  uint4 held[HELD][2];
 #pragma unroll
-  for (int j = 0; j < HELD; ++j) {
-    const int64_t k = j * PIECE + tid * 8;
-    held[j] = make_uint4(0, 0, 0, 0);
-    if (k < K) held[j] = *reinterpret_cast<const uint4*>(src + k);
+  for (int j = 0; j < HELD; ++j) take((j * LANES + lt) * 16, held[j]);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) top = max(top, top16(held[j]));
+  for (int64_t k = (HELD * LANES + lt) * 16; k < K; k += LANES * 16) {
+    uint4 u[2];
+    take(k, u);
+    top = max(top, top16(u));
   }
-#pragma unroll
-  for (int j = 0; j < HELD; ++j) take(held[j]);
-  for (int64_t k = HELD * PIECE + tid * 8; k < K; k += PIECE) take(*reinterpret_cast<const uint4*>(src + k));
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-  if ((tid & 63) == 0) tops[tid >> 6] = top;
-  __syncthreads();
-  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+  if (WAVES > 1) {
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    __syncthreads();
+    top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+  }
   const float t = fmaxf(kv800::bf2f(top), LEAST), inv = 127.f / t;
-  if (tid == 0) scale[r] = top < 0x7F80u ? t / 127.f : __uint_as_float(0x7FC00000u);
-  auto put = [&](int64_t k, const uint4& u) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    uint32_t o[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t b = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float f = e & 1 ? kv800::bf2f_hi(w[2 * i + (e >> 1)]) : kv800::bf2f_lo(w[2 * i + (e >> 1)]);
-        b |= ((uint32_t)(int)rintf(f * inv) & 0xFFu) << (8 * e);
-      }
-      o[i] = b;
+  if (lt == 0) scale[r] = top < 0x7F80u ? t / 127.f : __uint_as_float(0x7FC00000u);
+  auto put = [&](int64_t k, const uint4 (&u)[2]) {
+    const uint4 o = codes16(u, inv);
+    if (OPERAND) {       // the row's padding to whole blocks meets zeros of the weight
+      *reinterpret_cast<uint4*>(q + (((r >> 5) * nks + (k >> 5)) * 64 + (r & 31) + 32 * ((k >> 4) & 1)) * 16) = o;
+    } else {
+      *reinterpret_cast<uint2*>(q + r * K + k) = make_uint2(o.x, o.y);
+      if (k + 8 < K) *reinterpret_cast<uint2*>(q + r * K + k + 8) = make_uint2(o.z, o.w);
     }
-    int8_t* dst;
-    if (OPERAND) dst = q + (((r >> 5) * nks + (k >> 5)) * 64 + (r & 31) + 32 * ((k >> 4) & 1)) * 16 + (k & 15);
-    else dst = q + r * K + k;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
   };
 #pragma unroll
   for (int j = 0; j < HELD; ++j) {
-    const int64_t k = j * PIECE + tid * 8;
+    const int64_t k = (j * LANES + lt) * 16;
     if (k < K) put(k, held[j]);
   }
-  for (int64_t k = HELD * PIECE + tid * 8; k < K; k += PIECE) put(k, *reinterpret_cast<const uint4*>(src + k));
+  for (int64_t k = (HELD * LANES + lt) * 16; k < K; k += LANES * 16) {
+    uint4 u[2];
+    take(k, u);
+    put(k, u);
+  }
 }
 
 // tokens to 8 bits inside a product: the lane's 16 channels from k on (zeros past K), token row src
 __device__ __forceinline__ i4v quantized16(const uint16_t* src, int64_t k, int64_t K, float inv) {
-  i4v o = {0, 0, 0, 0};
+  uint4 u[2];
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
-    if (k + 8 * p < K) {
-      const uint4 u = *reinterpret_cast<const uint4*>(src + k + 8 * p);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t b = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f = e & 1 ? kv800::bf2f_hi(w[2 * i + (e >> 1)]) : kv800::bf2f_lo(w[2 * i + (e >> 1)]);
-          b |= ((uint32_t)(int)rintf(f * inv) & 0xFFu) << (8 * e);
-        }
-        o[2 * p + i] = (int)b;
-      }
-    }
-  return o;
+  for (int p = 0; p < 2; ++p) {
+    u[p] = make_uint4(0, 0, 0, 0);
+    if (k + 8 * p < K) u[p] = *reinterpret_cast<const uint4*>(src + k + 8 * p);
+  }
+  return __builtin_bit_cast(i4v, codes16(u, inv));
+}
+
+// silu(g) u; the reciprocal is within an ulp, which the rounding to bf16 behind it does not show
+__device__ __forceinline__ float gate(float g, float u) {
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f)) * u;
+}
+__device__ __forceinline__ uint32_t bfpk(float a, float b) {   // two floats -> packed bf16 (round to nearest even)
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  const bf2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
 }
 
 struct Out {
   uint16_t* y;
   int64_t ldy, R, N;
-  bool wide;                 // rows on 8-byte boundaries
+  bool wide;                 // rows on 16-byte boundaries
 };
 // Four outputs of token r from row n of the (padded) weight on; gated: g and u of output f on.
 __device__ __forceinline__ void put4(const Out& o, int64_t r, int64_t n, int64_t width, const float (&v)[4]) {
   uint16_t* dst = o.y + r * o.ldy + n;
   if (o.wide && n + 4 <= width) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(kv800::f2bf(v[0]) | (kv800::f2bf(v[1]) << 16), kv800::f2bf(v[2]) | (kv800::f2bf(v[3]) << 16));
+    *reinterpret_cast<uint2*>(dst) = make_uint2(bfpk(v[0], v[1]), bfpk(v[2], v[3]));
     return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (n + i < width) dst[i] = (uint16_t)kv800::f2bf(v[i]);
+    if (n + i < width) dst[i] = (uint16_t)bfpk(v[i], 0.f);
 }
-__device__ __forceinline__ float gate(float g, float u) { return g / (1.f + __expf(-g)) * u; }
-
 // Few tokens: one workgroup takes 64 rows of the weight x 32 WM tokens, its 8 waves an eighth of K each, so that every wave has
 // blocks of 1 KB in flight from its first instruction on; their sums meet in LDS, 32 tokens at a time. Output of the instruction
 // (weight rows x tokens): lane l holds token l % 32, rows 8 b + 4 (l / 32) + i.
@@ -259,39 +280,51 @@ __global__ void __launch_bounds__(64 * FEW) few_kernel(const uint16_t* __restric
   }
 }
 
-// Many tokens: one workgroup takes 256 rows of the weight x 256 tokens, 128 channels a stage, two stages in LDS: the next one's
-// blocks are loaded straight into LDS while the present one is multiplied, one barrier a stage. A block lies in LDS as it does in memory, in
-// operand order, so that loads and reads go over consecutive addresses. 8 waves of 128 rows x 64 tokens: 6 blocks read from LDS for
-// 8 products.
-constexpr int TILE = 8, STAGE = 4, MANY = 8;       // tiles of 32 a side, k-steps a stage, waves
+// Many tokens: one workgroup of 4 waves takes 256 rows of the weight x 128 tokens, 64 channels a stage, three stages in LDS: a stage's
+// blocks are loaded straight into LDS two stages ahead, one barrier a stage. A block lies in LDS as it does in memory, in operand
+// order, so that loads and reads go over consecutive addresses. A wave has 128 rows x 64 tokens: 6 blocks read from LDS for 8 products.
+// Two workgroups share a CU, so that one's epilogue and barriers pass under the other's products: 8192 x 16384 x 2048 gated 300 us;
+// one workgroup of 8 waves for 256 x 256 with two stages of 128 channels 336.
+constexpr int TN = 8, TM = 4, STAGE = 2, MANY = 4;       // tiles of 32 of the weight and of tokens, k-steps a stage, waves
+constexpr int LOADS = (TN + TM) * STAGE / MANY;          // loads of a wave a stage
 struct alignas(16) Stage {
-  int8_t w[TILE * STAGE * 1024];
-  int8_t x[TILE * STAGE * 1024];
+  int8_t b[(TN + TM) * STAGE * 1024];                    // (tile, k-step): the weight's tiles, then the tokens'
 };
 template <bool GATED>
-__global__ void __launch_bounds__(64 * MANY) many_kernel(const int8_t* __restrict__ xq, const float* __restrict__ sx,
-                                                         const int8_t* __restrict__ wsh, const float* __restrict__ ssh, int64_t nt,
-                                                         int64_t mt, int64_t nks, Out o) {
-  __shared__ Stage A, B;     // two objects: a read of one is not held for the other's loads
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, wn = wv & 1, wm = wv >> 1;
+__global__ void __launch_bounds__(64 * MANY, 2) many_kernel(const int8_t* __restrict__ xq, const float* __restrict__ sx,
+                                                            const int8_t* __restrict__ wsh, const float* __restrict__ ssh, int64_t nt,
+                                                            int64_t mt, int64_t nks, Out o) {
+  __shared__ Stage A, B, C;  // three objects: a read of one is not held for the others' loads
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wv & 1, wm = wv >> 1;
   // workgroup b runs on XCD b % 8, which takes a contiguous run of the order (group of 8 token tiles, weight tile, token tile):
-  // the 32 workgroups that run there together share 4 weight tiles and 8 token tiles in its L2
+  // the 64 workgroups that run there together share 8 weight tiles and 8 token tiles in its L2
   const int nb = (int)gridDim.x, xcd = (int)blockIdx.x & 7, per = nb >> 3, rem = nb & 7;
   const int L = xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3);
-  const int tn = (int)((nt + TILE - 1) / TILE), tm = (int)((mt + TILE - 1) / TILE);
+  const int tn = (int)((nt + TN - 1) / TN), tm = (int)((mt + TM - 1) / TM);
   const int grp = L / (8 * tn), gm = min(8, tm - 8 * grp), in = L - grp * 8 * tn;
-  const int64_t n0 = (int64_t)(in / gm) * TILE, m0 = (int64_t)(8 * grp + in % gm) * TILE;
-  auto load = [&](int64_t ks, Stage& S) {          // wave w: tile w of both sides
-    const int8_t* ws = wsh + (min(n0 + wv, nt - 1) * nks + ks) * 1024 + lane * 16;
-    const int8_t* xs = xq + (min(m0 + wv, mt - 1) * nks + ks) * 1024 + lane * 16;
+  const int64_t n0 = (int64_t)(in / gm) * TN, m0 = (int64_t)(8 * grp + in % gm) * TM;
+  // the wave's loads: tiles wv, wv + MANY, ... of the stage; a tile past the last is the last one again, not stored
+  const int8_t* src[LOADS / STAGE];
 #pragma unroll
-    for (int k = 0; k < STAGE; ++k) {
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(ws + k * 1024),
-                                       (__attribute__((address_space(3))) void*)&S.w[(wv * STAGE + k) * 1024], 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(xs + k * 1024),
-                                       (__attribute__((address_space(3))) void*)&S.x[(wv * STAGE + k) * 1024], 16, 0, 0);
-    }
+  for (int i = 0; i < LOADS / STAGE; ++i) {
+    const int t = wv + i * MANY;
+    src[i] = (t < TN ? wsh + min(n0 + t, nt - 1) * nks * 1024 : xq + min(m0 + t - TN, mt - 1) * nks * 1024) + lane * 16;
+  }
+  auto load = [&](int64_t ks, Stage& S) {
+#pragma unroll
+    for (int i = 0; i < LOADS / STAGE; ++i)
+#pragma unroll
+      for (int k = 0; k < STAGE; ++k)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[i] + (ks + k) * 1024),
+                                         (__attribute__((address_space(3))) void*)&S.b[((wv + i * MANY) * STAGE + k) * 1024], 16, 0, 0);
     asm volatile("" ::"s"((uint32_t)(uintptr_t)&S) : "memory");   // the loads write S behind the compiler's view of it
+  };
+  // the wave's LDS reads are done and its loads, but for those of the last stage asked for; then all waves' are
+  auto meet = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | LOADS);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
   i16v acc[4][2];
 #pragma unroll
@@ -300,55 +333,90 @@ __global__ void __launch_bounds__(64 * MANY) many_kernel(const int8_t* __restric
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[a][b][v] = 0;
-  auto step = [&](int64_t ks, const Stage& S, Stage& next) {
-    if (ks + STAGE < nks) load(ks + STAGE, next);
+  // stage i from S, whose loads have arrived; those of stage i + 2 go out into `later`, whose reads ended at the last barrier (behind
+  // the last stage the last one again, so that the number of loads on their way is always the same)
+  const int n = (int)(nks / STAGE);
+  auto step = [&](int i, const Stage& S, Stage& later) {
+    load((int64_t)min(i + 2, n - 1) * STAGE, later);
+    i4v a[STAGE][4], b[STAGE][2];
 #pragma unroll
     for (int k = 0; k < STAGE; ++k) {
-      i4v a[4], b[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const i4v*>(&S.w[((4 * wn + i) * STAGE + k) * 1024 + lane * 16]);
+      for (int j = 0; j < 2; ++j) b[k][j] = *reinterpret_cast<const i4v*>(&S.b[((TN + 2 * wm + j) * STAGE + k) * 1024 + lane * 16]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) b[i] = *reinterpret_cast<const i4v*>(&S.x[((2 * wm + i) * STAGE + k) * 1024 + lane * 16]);
+      for (int i = 0; i < 4; ++i) a[k][i] = *reinterpret_cast<const i4v*>(&S.b[((4 * wn + i) * STAGE + k) * 1024 + lane * 16]);
+    }
+#pragma unroll
+    for (int k = 0; k < STAGE; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
-    }
-    __syncthreads();         // ends the reads of S and waits for the loads into next
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma(a[k][i], b[k][j], acc[i][j]);
+    // all of the stage's reads before its products: read one by one, each pair of products waited for its operand
+    __builtin_amdgcn_sched_group_barrier(0x100, 6 * STAGE, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 8 * STAGE, 0);
+    meet();
   };
   load(0, A);
-  __syncthreads();
-  for (int64_t ks = 0; ks < nks; ks += 2 * STAGE) {
-    step(ks, A, B);
-    if (ks + STAGE < nks) step(ks + STAGE, B, A);
+  load((int64_t)min(1, n - 1) * STAGE, B);
+  meet();
+  for (int i = 0;;) {
+    step(i, A, C);
+    if (++i == n) break;
+    step(i, B, A);
+    if (++i == n) break;
+    step(i, C, B);
+    if (++i == n) break;
   }
+  __builtin_amdgcn_s_waitcnt(0x0070);                    // nothing is on its way to LDS any more
+  __syncthreads();
+  // The outputs leave through LDS, so that a row's go out side by side (straight from the registers they are 16 bytes a line and store:
+  // 325 us): 64 tokens x 64 outputs a wave and pass, rows of 144 bytes.
+  constexpr int ROW = 144;
+  uint8_t* buf = reinterpret_cast<uint8_t*>(wv < 2 ? A.b : B.b) + (wv & 1) * 64 * ROW;
+  static_assert(2 * 64 * ROW <= (int)sizeof(Stage), "two waves' outputs fit a stage");
+  const int64_t width = GATED ? o.N / 2 : o.N, t0 = (m0 + 2 * wm) * 32;
+  float s[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t r = (m0 + 2 * wm + j) * 32 + (lane & 31);
-    if (r >= o.R) continue;
-    const float s = sx[r];
+  for (int j = 0; j < 2; ++j) s[j] = sx[min(t0 + 32 * j + (lane & 31), o.R - 1)];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int row = 8 * q + 4 * (lane >> 5);
-      auto scaled = [&](int i, float (&f)[4]) {
-        const float4 sc = *reinterpret_cast<const float4*>(ssh + (n0 + 4 * wn + i) * 32 + row);
-        f[0] = (float)acc[i][j][4 * q] * s * sc.x; f[1] = (float)acc[i][j][4 * q + 1] * s * sc.y;
-        f[2] = (float)acc[i][j][4 * q + 2] * s * sc.z; f[3] = (float)acc[i][j][4 * q + 3] * s * sc.w;
-      };
+  for (int pass = 0; pass < (GATED ? 1 : 2); ++pass) {
+    if (pass) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-      for (int i = 0; i < 4; i += GATED ? 2 : 1) {
-        if (n0 + 4 * wn + i >= nt) continue;
-        float f[4];
-        scaled(i, f);
-        if (GATED) {
-          float u[4];
-          scaled(i + 1, u);
+    for (int c = 0; c < 2; ++c)                          // 32 outputs: of tiles 2 c and 2 c + 1, or of tile 2 pass + c
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = gate(f[e], u[e]);
-          put4(o, r, (n0 + 4 * wn + i) * 16 + row, o.N / 2, f);
-        } else {
-          put4(o, r, (n0 + 4 * wn + i) * 32 + row, o.N, f);
+      for (int q = 0; q < 4; ++q) {
+        const int i = GATED ? 2 * c : 2 * pass + c, row = 8 * q + 4 * (lane >> 5);
+        const float4 k0 = *reinterpret_cast<const float4*>(ssh + min(n0 + 4 * wn + i, nt - 1) * 32 + row);
+        const float4 k1 = GATED ? *reinterpret_cast<const float4*>(ssh + min(n0 + 4 * wn + i + 1, nt - 1) * 32 + row) : k0;
+        const float ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[e] = (float)acc[i][j][4 * q + e] * s[j] * ka[e];
+            if (GATED) f[e] = gate(f[e], (float)acc[i + (GATED ? 1 : 0)][j][4 * q + e] * s[j] * kb[e]);
+          }
+          *reinterpret_cast<uint2*>(buf + (32 * j + (lane & 31)) * ROW + (32 * c + row) * 2) = make_uint2(bfpk(f[0], f[1]), bfpk(f[2], f[3]));
         }
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int64_t n = (GATED ? (n0 + 4 * wn) * 16 : (n0 + 4 * wn + 2 * pass) * 32) + (lane & 7) * 8;
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      const int tr = it * 8 + (lane >> 3);
+      const int64_t r = t0 + tr;
+      if (r >= o.R || n >= width) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(buf + tr * ROW + (lane & 7) * 16);
+      uint16_t* dst = o.y + r * o.ldy + n;
+      if (o.wide && n + 8 <= width) {
+        *reinterpret_cast<uint4*>(dst) = v;
+      } else {
+        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (n + i < width) dst[i] = (uint16_t)(e[i >> 1] >> (16 * (i & 1)));
       }
     }
   }
@@ -389,7 +457,7 @@ int lfm3_hip_int8_layout(const int8_t* w, int64_t ld, const float* scale, int64_
 int lfm3_hip_int8_quantize(const uint16_t* w, int64_t ld, int64_t N, int64_t K, int8_t* w8, float* scale, void* stream) {
   KV800_REQUIRE(lfm3::sizes(0, N, K, 0) && ld % 8 == 0, "int8_quantize: N up to 2^24, K a multiple of 8 up to 65536, ld a multiple of 8");
   KV800_REQUIRE(w && w8 && scale && (uintptr_t)w % 16 == 0 && (uintptr_t)w8 % 8 == 0, "int8_quantize: null or unaligned pointer");
-  hipLaunchKernelGGL(lfm3::quantize_kernel<false>, dim3((unsigned)N), dim3(256), 0, (hipStream_t)stream, w, ld, N, K, 0,
+  hipLaunchKernelGGL((lfm3::quantize_kernel<false, 4>), dim3((unsigned)N), dim3(256), 0, (hipStream_t)stream, w, ld, N, K, 0,
                      w8, scale);
   return kv800::check_launch("int8_quantize");
 }
@@ -411,13 +479,16 @@ int lfm3_hip_linear8(const uint16_t* x, int64_t ldx, const int8_t* wsh, const fl
   const int64_t need = lfm3_hip_linear8_workspace(R, N, K, gated);
   KV800_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), "linear8: %lld bytes of 16-byte aligned workspace needed", (long long)need);
   const int64_t mt = lfm3::round_up(R, 32) / 32, nt = lfm3::padded_rows(N, gated) / 32, nks = lfm3::round_up(K, 128) / 32;
-  const lfm3::Out o = {y, ldy, R, N, ldy % 4 == 0 && (uintptr_t)y % 8 == 0};
+  const lfm3::Out o = {y, ldy, R, N, ldy % 8 == 0 && (uintptr_t)y % 16 == 0};
   const lfm3::Kind kind = lfm3::kind_of(R, N, K, gated);
   hipStream_t st = (hipStream_t)stream;
   int8_t* xq = (int8_t*)ws;
   float* sx = (float*)(xq + mt * nks * 1024);
   if (kind != lfm3::FUSED) {
-    hipLaunchKernelGGL(lfm3::quantize_kernel<true>, dim3((unsigned)R), dim3(256), 0, st, x, ldx, R, K, nks, xq, sx);
+    if (R >= 1024 && K <= 2048)
+      hipLaunchKernelGGL((lfm3::quantize_kernel<true, 1>), dim3((unsigned)((R + 3) / 4)), dim3(256), 0, st, x, ldx, R, K, nks, xq, sx);
+    else
+      hipLaunchKernelGGL((lfm3::quantize_kernel<true, 4>), dim3((unsigned)R), dim3(256), 0, st, x, ldx, R, K, nks, xq, sx);
     const int rc = kv800::check_launch("linear8 quantize");
     if (rc != KV800_OK) return rc;
   }
@@ -435,7 +506,7 @@ int lfm3_hip_linear8(const uint16_t* x, int64_t ldx, const int8_t* wsh, const fl
     if (gated) few(lfm3::few_kernel<2, true, false>, 2);
     else few(lfm3::few_kernel<2, false, false>, 2);
   } else {
-    const dim3 grid((unsigned)((nt + lfm3::TILE - 1) / lfm3::TILE * ((mt + lfm3::TILE - 1) / lfm3::TILE)));
+    const dim3 grid((unsigned)((nt + lfm3::TN - 1) / lfm3::TN * ((mt + lfm3::TM - 1) / lfm3::TM)));
     if (gated) hipLaunchKernelGGL(lfm3::many_kernel<true>, grid, dim3(64 * lfm3::MANY), 0, st, xq, sx, wsh, ssh, nt, mt, nks, o);
     else hipLaunchKernelGGL(lfm3::many_kernel<false>, grid, dim3(64 * lfm3::MANY), 0, st, xq, sx, wsh, ssh, nt, mt, nks, o);
   }
