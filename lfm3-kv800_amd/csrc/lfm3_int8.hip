@@ -167,36 +167,35 @@ __device__ __forceinline__ void put4(const Out& o, int64_t r, int64_t n, int64_t
   for (int i = 0; i < 4; ++i)
     if (n + i < width) dst[i] = (uint16_t)bfpk(v[i], 0.f);
 }
-// Few tokens: one workgroup takes 64 rows of the weight x 32 WM tokens, its 8 waves an eighth of K each, so that every wave has
+// Few tokens: one workgroup takes 32 NT rows of the weight x 32 WM tokens, its 16 / NT waves a part of K each, so that every wave has
 // blocks of 1 KB in flight from its first instruction on; their sums meet in LDS, 32 tokens at a time. Output of the instruction
 // (weight rows x tokens): lane l holds token l % 32, rows 8 b + 4 (l / 32) + i.
 // FUSED (up to 32 tokens): the tokens are rounded to 8 bits by every workgroup for itself, while its first weights are on their way.
-constexpr int FEW = 8;       // waves
-template <int WM, bool GATED, bool FUSED>
-__global__ void __launch_bounds__(64 * FEW) few_kernel(const uint16_t* __restrict__ x, int64_t ldx, const int8_t* __restrict__ xq,
+template <int NT, int WM, bool GATED, bool FUSED>
+__global__ void __launch_bounds__(64 * 16 / NT) few_kernel(const uint16_t* __restrict__ x, int64_t ldx, const int8_t* __restrict__ xq,
                                                        const float* __restrict__ sx, const int8_t* __restrict__ wsh,
                                                        const float* __restrict__ ssh, int64_t K, int64_t nks, Out o) {
-  constexpr int U = WM == 1 ? 8 : 4;               // k-steps in flight
-  __shared__ int4 part[FEW][2][4][64];
+  constexpr int FEW = 16 / NT, U = WM == 1 && NT == 2 ? 8 : 4;   // waves; k-steps in flight
+  __shared__ int4 part[FEW][NT][4][64];
   __shared__ int tops[32];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int64_t n0 = (int64_t)blockIdx.x * 2, m0 = (int64_t)blockIdx.y * WM;
+  const int64_t n0 = (int64_t)blockIdx.x * NT, m0 = (int64_t)blockIdx.y * WM;
   const int per = (int)((nks + FEW - 1) / FEW), k0 = wv * per, k1 = min((int)nks, k0 + per);
   const int8_t* wp = wsh + n0 * nks * 1024 + lane * 16;
   const int tok = lane & 31;
-  i16v acc[2][WM];
+  i16v acc[NT][WM];
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int a = 0; a < NT; ++a)
 #pragma unroll
     for (int b = 0; b < WM; ++b)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[a][b][v] = 0;
-  i4v wr[2][U];
+  i4v wr[NT][U];
   auto weights = [&](int ks) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int a = 0; a < 2; ++a) wr[a][u] = *reinterpret_cast<const i4v*>(wp + (a * nks + min(ks + u, k1 - 1)) * 1024);
+      for (int a = 0; a < NT; ++a) wr[a][u] = *reinterpret_cast<const i4v*>(wp + (a * nks + min(ks + u, k1 - 1)) * 1024);
   };
   if (k0 < k1) weights(k0);
   float inv = 0.f;
@@ -235,7 +234,7 @@ __global__ void __launch_bounds__(64 * FEW) few_kernel(const uint16_t* __restric
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < NT; ++a)
 #pragma unroll
         for (int b = 0; b < WM; ++b) acc[a][b] = mfma(wr[a][u], xr[b][u], acc[a][b]);
     if (ks + U < k1) weights(ks + U);
@@ -244,14 +243,14 @@ __global__ void __launch_bounds__(64 * FEW) few_kernel(const uint16_t* __restric
   for (int b = 0; b < WM; ++b) {
     if (b) __syncthreads();
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < NT; ++a)
 #pragma unroll
       for (int q = 0; q < 4; ++q) part[wv][a][q][lane] = make_int4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
     __syncthreads();
     // thread: 4 rows of one token, of tile wv / 4 (gated: waves 0 .. 3, both tiles)
     const int q = wv & 3, row = 8 * q + 4 * (lane >> 5);
     const int64_t r = (m0 + b) * 32 + tok;
-    if (r >= o.R || (GATED && wv >= 4)) continue;
+    if (r >= o.R || wv >= (GATED ? 4 : 4 * NT)) continue;
     float s;
     if (FUSED) s = tops[tok] < 0x7F80 ? fmaxf(kv800::bf2f((uint32_t)tops[tok]), LEAST) / 127.f : __uint_as_float(0x7FC00000u);
     else s = sx[r];
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(64 * FEW) few_kernel(const uint16_t* __restric
     if (GATED) {
       float u[4];
       sums(0, f);
-      sums(1, u);
+      sums(NT - 1, u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = gate(f[i], u[i]);
       put4(o, r, n0 * 16 + row, o.N / 2, f);
@@ -430,13 +429,27 @@ bool sizes(int64_t R, int64_t N, int64_t K, int gated) {
   return R >= 0 && R <= (1 << 24) && N > 0 && N <= (1 << 24) && K > 0 && K <= K_MOST && K % 8 == 0 && (gated == 0 || (gated == 1 && N % 2 == 0));
 }
 
-// How a product runs: tokens rounded inside it, 32 or 64 tokens a workgroup of few_kernel, or many_kernel.
-enum Kind { FUSED, ONE, TWO, TILES };
-Kind kind_of(int64_t R, int64_t N, int64_t K, int gated) {
-  if (R <= 16) return FUSED;
-  const int64_t wgs = (padded_rows(N, gated) + 255) / 256 * ((R + 255) / 256);
-  if (wgs >= 192) return TILES;
-  return R <= 32 ? ONE : TWO;
+// How a product runs: in 256 x 128 tiles, or on few_kernel with nt tiles of the weight and wm of the tokens a workgroup, which rounds
+// the tokens itself or not. Times of whole calls on both sides of each rule, us (tokens x rows of the weight x K):
+//   tiles, from 112 on: 256 x 16384 x 2048 gated (128) 25.7, few 29.7; 512 x 6144 x 2048 (96) 26.9, few 21.2; 1024 x 2048 x 8192 (64) 80, few 40
+//   rounding inside: 1 x 16384 x 2048 gated 11.7, apart 12.9; 4 x 6144 x 2048 9.6, 13.1; 16 x 16384 x 2048 19.2, 12.8; 1 x 2048 x 8192
+//     18.0, 13.1; 4 x 65536 x 2048 47.5, 33.4
+//   16 waves on one tile of the weight: 256 x 2048 x 8192 18.6, 8 waves on two 21.8; 1024 x 2048 x 8192 50.6, 40.2
+//   32 tokens a workgroup: 64 x 2048 x 8192 13.2, 64 tokens 15.2; 256 x 2048 x 8192 19.1, 18.6
+struct How {
+  bool tiles, fused;
+  int nt, wm;
+};
+How how(int64_t R, int64_t N, int64_t K, int gated) {
+  const int64_t nt = padded_rows(N, gated) / 32, mt = (R + 31) / 32;
+  How h = {false, false, 2, mt > 1 ? 2 : 1};
+  h.tiles = ((nt + TN - 1) / TN) * ((mt + TM - 1) / TM) >= 112;
+  h.fused = !h.tiles && R <= 4 && K <= 4096 && nt <= 512;
+  if (!gated && (nt / 2) * ((mt + 1) / 2) < 256) {
+    h.nt = 1;
+    h.wm = nt * mt <= 256 ? 1 : 2;
+  }
+  return h;
 }
 
 }  // namespace
@@ -464,7 +477,7 @@ int lfm3_hip_int8_quantize(const uint16_t* w, int64_t ld, int64_t N, int64_t K, 
 
 int64_t lfm3_hip_linear8_workspace(int64_t R, int64_t N, int64_t K, int gated) {
   if (!lfm3::sizes(R, N, K, gated) || R == 0) return 0;
-  if (lfm3::kind_of(R, N, K, gated) == lfm3::FUSED) return 0;
+  if (lfm3::how(R, N, K, gated).fused) return 0;
   const int64_t mpad = lfm3::round_up(R, 32);
   return mpad * lfm3::round_up(K, 128) + mpad * 4;
 }
@@ -480,11 +493,11 @@ int lfm3_hip_linear8(const uint16_t* x, int64_t ldx, const int8_t* wsh, const fl
   KV800_REQUIRE(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need), "linear8: %lld bytes of 16-byte aligned workspace needed", (long long)need);
   const int64_t mt = lfm3::round_up(R, 32) / 32, nt = lfm3::padded_rows(N, gated) / 32, nks = lfm3::round_up(K, 128) / 32;
   const lfm3::Out o = {y, ldy, R, N, ldy % 8 == 0 && (uintptr_t)y % 16 == 0};
-  const lfm3::Kind kind = lfm3::kind_of(R, N, K, gated);
+  const lfm3::How h = lfm3::how(R, N, K, gated);
   hipStream_t st = (hipStream_t)stream;
   int8_t* xq = (int8_t*)ws;
   float* sx = (float*)(xq + mt * nks * 1024);
-  if (kind != lfm3::FUSED) {
+  if (!h.fused) {
     if (R >= 1024 && K <= 2048)
       hipLaunchKernelGGL((lfm3::quantize_kernel<true, 1>), dim3((unsigned)((R + 3) / 4)), dim3(256), 0, st, x, ldx, R, K, nks, xq, sx);
     else
@@ -492,19 +505,22 @@ int lfm3_hip_linear8(const uint16_t* x, int64_t ldx, const int8_t* wsh, const fl
     const int rc = kv800::check_launch("linear8 quantize");
     if (rc != KV800_OK) return rc;
   }
-  auto few = [&](auto kernel, int64_t wm) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(nt / 2), (unsigned)((mt + wm - 1) / wm)), dim3(64 * lfm3::FEW), 0, st, x, ldx, xq, sx, wsh,
-                       ssh, K, nks, o);
+  auto few = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(nt / h.nt), (unsigned)((mt + h.wm - 1) / h.wm)), dim3((unsigned)(1024 / h.nt)), 0, st, x, ldx, xq,
+                       sx, wsh, ssh, K, nks, o);
   };
-  if (kind == lfm3::FUSED) {
-    if (gated) few(lfm3::few_kernel<1, true, true>, 1);
-    else few(lfm3::few_kernel<1, false, true>, 1);
-  } else if (kind == lfm3::ONE) {
-    if (gated) few(lfm3::few_kernel<1, true, false>, 1);
-    else few(lfm3::few_kernel<1, false, false>, 1);
-  } else if (kind == lfm3::TWO) {
-    if (gated) few(lfm3::few_kernel<2, true, false>, 2);
-    else few(lfm3::few_kernel<2, false, false>, 2);
+  if (h.fused) {
+    if (gated) few(lfm3::few_kernel<2, 1, true, true>);
+    else if (h.nt == 1) few(lfm3::few_kernel<1, 1, false, true>);
+    else few(lfm3::few_kernel<2, 1, false, true>);
+  } else if (!h.tiles && h.wm == 1) {
+    if (gated) few(lfm3::few_kernel<2, 1, true, false>);
+    else if (h.nt == 1) few(lfm3::few_kernel<1, 1, false, false>);
+    else few(lfm3::few_kernel<2, 1, false, false>);
+  } else if (!h.tiles) {
+    if (gated) few(lfm3::few_kernel<2, 2, true, false>);
+    else if (h.nt == 1) few(lfm3::few_kernel<1, 2, false, false>);
+    else few(lfm3::few_kernel<2, 2, false, false>);
   } else {
     const dim3 grid((unsigned)((nt + lfm3::TN - 1) / lfm3::TN * ((mt + lfm3::TM - 1) / lfm3::TM)));
     if (gated) hipLaunchKernelGGL(lfm3::many_kernel<true>, grid, dim3(64 * lfm3::MANY), 0, st, xq, sx, wsh, ssh, nt, mt, nks, o);

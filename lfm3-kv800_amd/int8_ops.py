@@ -82,6 +82,7 @@ class Weight8:
         npad = 2 * (-(-(N // 2) // 32) * 32) if self.gated else -(-N // 64) * 64
         self.data = torch.empty(npad * (-(-K // 128) * 128), dtype=torch.int8, device=dev)
         self.scale = torch.empty(npad, dtype=torch.float32, device=dev)
+        self._ws = {}                                 # workspace bytes by the number of tokens
         with _on(dev):
             kv800_hip._check(L.lfm3_hip_int8_layout(w.data_ptr(), K, scale.data_ptr(), N, K, int(self.gated), self.data.data_ptr(),
                                                     self.scale.data_ptr(), _raw_stream(dev)))
@@ -100,9 +101,11 @@ def linear8(x, weight):
     if R == 0:
         return out
     x, ld = _rows16(x)
+    wsb = weight._ws.get(R)
+    if wsb is None:
+        wsb = weight._ws[R] = int(L.lfm3_hip_linear8_workspace(R, weight.n, weight.k, int(weight.gated)))
     with _on(dev):
-        wsb = int(L.lfm3_hip_linear8_workspace(R, weight.n, weight.k, int(weight.gated)))
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
         kv800_hip._check(L.lfm3_hip_linear8(x.data_ptr(), ld, weight.data.data_ptr(), weight.scale.data_ptr(), R, weight.n, weight.k,
-                                            int(weight.gated), out.data_ptr(), weight.width, ws.data_ptr(), wsb, _raw_stream(dev)))
+                                            int(weight.gated), out.data_ptr(), weight.width, ws.data_ptr() if wsb else None, wsb, _raw_stream(dev)))
     return out

@@ -69,7 +69,7 @@ class Cache8:
             raise ValueError("data must be 16-byte aligned, its pages a multiple of 16 bytes apart; exps 2-byte aligned, an even number apart")
         self.data, self.exps = data, exps
         self.pages, self.heads, self.blocks, self.dim = P, H, U, n // BLK
-        self.bs = U * BLK
+        self.bs, self.dev = U * BLK, data.device
         self._c = _Cache(data.data_ptr(), exps.data_ptr(), P, H, U, self.dim, ps, es)
         self._p = ctypes.byref(self._c)
 
@@ -83,8 +83,9 @@ class Cache8:
 
 
 def _step(cache, T, bt, lens, qsl):
-    dev = cache.data.device
-    _need(bt, "bt", torch.int32, dev); _need(lens, "lens", torch.int64, dev); _need(qsl, "qsl", torch.int64, dev)
+    dev, i64 = cache.dev, torch.int64
+    if not (bt.dtype is torch.int32 and lens.dtype is i64 and qsl.dtype is i64 and bt.device == dev and lens.device == dev and qsl.device == dev):
+        _need(bt, "bt", torch.int32, dev); _need(lens, "lens", i64, dev); _need(qsl, "qsl", i64, dev)
     if qsl.dim() != 1 or qsl.shape[0] < 1:
         raise ValueError("qsl must be (R + 1,)")
     R = qsl.shape[0] - 1
@@ -94,16 +95,21 @@ def _step(cache, T, bt, lens, qsl):
         raise ValueError("bt must have contiguous rows")
     if T and not R:
         raise ValueError("tokens without rows")
-    return dev, R, lens.contiguous(), qsl.contiguous()
+    return R, lens.contiguous(), qsl.contiguous()
 
 
 def _kv(x, name, cache, T):
     """x with channels side by side and aligned rows, and its token and head strides."""
-    _need(x, name, torch.bfloat16, cache.data.device)
+    if x.dtype is not torch.bfloat16 or x.device != cache.dev:
+        _need(x, name, torch.bfloat16, cache.dev)
     if x.shape != (T, cache.heads, cache.dim):
         raise ValueError(f"{name} must be ({T}, {cache.heads}, {cache.dim}), got {tuple(x.shape)}")
-    ts, hs = x.stride(0) if T > 1 else 0, x.stride(1) if cache.heads > 1 else 0     # of a single one torch's stride may be anything
-    if x.stride(2) != 1 or ts % 8 or hs % 8 or x.data_ptr() % 16:
+    ts, hs, one = x.stride()
+    if T <= 1:
+        ts = 0                                           # of a single one torch's stride may be anything
+    if cache.heads == 1:
+        hs = 0
+    if one != 1 or ts % 8 or hs % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
         ts, hs = cache.heads * cache.dim, cache.dim
     return x, ts, hs
@@ -119,14 +125,16 @@ def append(cache, k, v, bt, lens, qsl, cos_t=None, sin_t=None):
     if k.dim() != 3:
         raise ValueError(f"k must be (T, heads, D), got {tuple(k.shape)}")
     T = k.shape[0]
-    dev, R, lens, qsl = _step(cache, T, bt, lens, qsl)
+    dev = cache.dev
+    R, lens, qsl = _step(cache, T, bt, lens, qsl)
     k, kt, kh = _kv(k, "k", cache, T)
     v, vt, vh = _kv(v, "v", cache, T)
     rows = F = 0
     if (cos_t is None) != (sin_t is None):
         raise ValueError("cos_t and sin_t go together")
     if cos_t is not None:
-        _need(cos_t, "cos_t", torch.bfloat16, dev); _need(sin_t, "sin_t", torch.bfloat16, dev)
+        if not (cos_t.dtype is torch.bfloat16 and sin_t.dtype is torch.bfloat16 and cos_t.device == dev and sin_t.device == dev):
+            _need(cos_t, "cos_t", torch.bfloat16, dev); _need(sin_t, "sin_t", torch.bfloat16, dev)
         if cos_t.dim() != 2 or cos_t.shape != sin_t.shape or not cos_t.shape[0] or cos_t.shape[1] % 8 or not 0 < cos_t.shape[1] <= cache.dim // 2:
             raise ValueError(f"cos_t / sin_t must be (P, F) with F a multiple of 8 up to {cache.dim // 2}, got {tuple(cos_t.shape)}, {tuple(sin_t.shape)}")
         rows, F = cos_t.shape
@@ -143,9 +151,8 @@ def append(cache, k, v, bt, lens, qsl, cos_t=None, sin_t=None):
 def dequantize(cache):
     """(k, v) (pages, kv heads, page tokens, D) bf16: what the cache stands for (kv8_hip_dequantize)."""
     L = _lib()
-    dev = cache.data.device
-    k = torch.empty(cache.pages, cache.heads, cache.bs, cache.dim, dtype=torch.bfloat16, device=dev)
-    v = torch.empty_like(k)
+    dev = cache.dev
+    k, v = torch.empty(2, cache.pages, cache.heads, cache.bs, cache.dim, dtype=torch.bfloat16, device=dev).unbind(0)
     with _on(dev):
         kv800_hip._check(L.kv8_hip_dequantize(cache._p, k.data_ptr(), v.data_ptr(), _raw_stream(dev)))
     return k, v
@@ -157,11 +164,12 @@ def attend(cache, q, bt, lens, qsl, window=0, scale=None):
     window, the last `window` of them. scale: 1 / sqrt(D) if None. Returns (T, heads, D) bf16; zeros for queries without keys and
     for the padding."""
     L = _lib()
-    _need(q, "q", torch.bfloat16, cache.data.device)
+    _need(q, "q", torch.bfloat16, cache.dev)
     if q.dim() != 3 or q.shape[2] != cache.dim or not q.shape[1] or q.shape[1] % cache.heads or q.shape[1] > 16 * cache.heads:
         raise ValueError(f"q must be (T, heads, {cache.dim}) with heads a multiple of {cache.heads} up to {16 * cache.heads}, got {tuple(q.shape)}")
     T, heads = q.shape[:2]
-    dev, R, lens, qsl = _step(cache, T, bt, lens, qsl)
+    dev = cache.dev
+    R, lens, qsl = _step(cache, T, bt, lens, qsl)
     window = int(window)
     if window < 0:
         raise ValueError("window must be >= 0")
@@ -173,9 +181,9 @@ def attend(cache, q, bt, lens, qsl, window=0, scale=None):
     cols = bt.shape[1]
     with _on(dev):
         wsb = int(L.kv8_hip_attend_workspace(cache._p, heads, R, T, cols, window))
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
         kv800_hip._check(L.kv8_hip_attend(cache._p, q.data_ptr(), heads, bt.data_ptr(), bt.stride(0) if R > 1 else cols, cols,
-                                          lens.data_ptr(), qsl.data_ptr(), R, T, window, scale, out.data_ptr(), ws.data_ptr(), wsb,
+                                          lens.data_ptr(), qsl.data_ptr(), R, T, window, scale, out.data_ptr(), ws.data_ptr() if wsb else None, wsb,
                                           _raw_stream(dev)))
     return out
 

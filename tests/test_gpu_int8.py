@@ -34,7 +34,7 @@ def product(x, w, scale, gated):
 
 
 SIZES = [(1, 2, 8), (1, 64, 128), (3, 70, 136), (32, 32, 2048), (33, 66, 200), (64, 6144, 2048), (65, 130, 264), (127, 34, 8200), (128, 128, 128), (129, 3088, 1000),
-         (250, 1000, 384), (256, 2048, 8192), (300, 514, 640), (513, 258, 1032), (16, 100, 4160), (17, 100, 4160), (2048, 6160, 136), (1500, 9000, 264)]
+         (250, 1000, 384), (256, 2048, 8192), (300, 514, 640), (513, 258, 1032), (4, 100, 2048), (16, 100, 4160), (300, 12900, 264), (200, 70, 4104), (2048, 6160, 136), (1500, 9000, 264)]
 
 
 @pytest.mark.parametrize("gated", [False, True])
