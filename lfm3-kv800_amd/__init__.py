@@ -5,7 +5,8 @@ binding of the C-ABI library libkv800_hip.so built from csrc/ by build.py), vllm
 per-step cache work on the device: new-token rows, sinks, flush, decode tables, decode and prefill rows of a mixed
 batch), train (patch_for_training's fake quantization on the GPU), model / model_ops (an LFM3-shaped engine loop that
 drives every attention layer through the above), spec_ops (model-side operators of steps with drafted tokens: short conv,
-verification).
+verification), kv8 (paged 8-bit cache: append with rotation, attention, reading back), int8_ops (products of 8-bit weights and
+activations).
 Kept free of torch imports, like the reference package (lfm3_kv800/__init__.py:1-6)."""
 import logging
 

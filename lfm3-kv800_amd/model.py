@@ -13,6 +13,9 @@ LFM3_KV800=1 (vllm_model.py:268-304): 24 layers of width 2048, each `h += post_n
 The vocabulary and feed-forward sizes are not in the reference (its weights are not available offline): 65,536 and
 8,192 here, about 1.67 B parameters. Weights are random N(0, 0.02) in bf16, norm weights 1.
 
+With int8=True the layers' products run in 8-bit integers (int8_ops), and PagedAttention8 keeps every attention layer's keys and values
+in 8 bits (kv8): all 6 full-attention layers over their whole history, the sliding layers over their window.
+
 Attention goes through an object with begin_step() -> the new tokens' positions and attend(layer, q, k_pre, k_post, v)
 -> (R, 16, 128): PagedAttention800 (below) keeps vLLM's page geometry and runs every layer on libkv800_hip.so; tests
 substitute an oracle implementation to check the logits. Between the GEMMs, the model's elementwise work runs on the
@@ -23,7 +26,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import kv800, kv800_hip
+from . import int8_ops as i8
+from . import kv8, kv800, kv800_hip
 from . import model_ops as mo
 from . import spec_ops as so
 from . import vllm_cache as vc
@@ -79,6 +83,11 @@ def glu_rows(rows):
     return 128 < rows <= 256 or rows > 384
 
 
+def product(x, w):
+    """x W^T, (R, N) bf16, of a bf16 matrix or an int8_ops.Weight8."""
+    return i8.linear8(x, w) if isinstance(w, i8.Weight8) else F.linear(x, w)
+
+
 class Lfm3Decoder:
     """Random-init LFM3-shaped model for batched decode: step(tokens) appends one token to every row and returns the
     logits. The dense products are torch GEMMs; everything between them is one fused HIP kernel (model_ops): the
@@ -86,9 +95,10 @@ class Lfm3Decoder:
     the attention output gate. The FFN's up-projection and gated activation run as one HIP GEMM (model_ops.linear on
     a [g | u] weight) at the batch sizes where it beats the library product plus the activation kernel (glu_rows).
     conv_state: per conv layer (R, hidden, conv_len - 1) bf16. max_pos bounds the positions of the model's RoPE
-    tables."""
+    tables. int8: the layers' weights are quantized by rows and their products take tokens rounded to 8 bits (int8_ops.linear8, the
+    gated activation in the product's epilogue); embedding and LM head stay bf16."""
 
-    def __init__(self, cfg: Lfm3Config, attention, rows, device, seed=0, max_pos=65536):
+    def __init__(self, cfg: Lfm3Config, attention, rows, device, seed=0, max_pos=65536, int8=False):
         self.cfg, self.attn, self.R, self.dev = cfg, attention, rows, device
         g = torch.Generator(device=device).manual_seed(seed)
         H, D, G = cfg.hidden, cfg.head_dim, cfg.heads
@@ -101,7 +111,8 @@ class Lfm3Decoder:
         self.final_norm = ones(H)
         self.tables = {FULL: model_rope_tables(1e6, 32, max_pos, device),
                        SLIDE: model_rope_tables(1e4, 64, max_pos, device)}
-        self.fused_ffn = glu_rows(rows)
+        self.int8 = bool(int8)
+        self.fused_ffn = not self.int8 and glu_rows(rows)
         self.layers = []
         for l in range(cfg.layers):
             t = cfg.layer_type(l)
@@ -116,6 +127,10 @@ class Lfm3Decoder:
                 # q, k, v and the 16 output-gate logits from one product: rows [q | k | v | gate]
                 L.update(qkvg=torch.cat((w((G + 2 * cfg.kv_heads) * D, H), w(G, H))), q_norm=ones(D), k_norm=ones(D),
                          o_proj=w(H, G * D))
+            if self.int8:
+                for name in ("w13", "w2", "in_proj", "out_proj", "qkvg", "o_proj"):
+                    if name in L:
+                        L[name] = i8.Weight8(L[name], gated=name == "w13")
             self.layers.append(L)
 
     def randomize_conv_states(self, seed):
@@ -125,21 +140,21 @@ class Lfm3Decoder:
                 L["state"].copy_(torch.randn(L["state"].shape, generator=g, device=self.dev) * 0.1)
 
     def _conv(self, L, n, qsl=None):
-        bcx = F.linear(n, L["in_proj"])
+        bcx = product(n, L["in_proj"])
         if qsl is None:
             y = mo.conv_step(bcx, L["conv"], L["state"])
         else:
             y, L["taps"] = so.conv_chunk(bcx, L["conv"], L["state"], qsl)
-        return F.linear(y, L["out_proj"])
+        return product(y, L["out_proj"])
 
     def _attention(self, l, L, n, pos):
         cfg = self.cfg
-        qkvg = F.linear(n, L["qkvg"])                                                   # (R, 3088)
+        qkvg = product(n, L["qkvg"])                                                   # (R, 3088)
         cos, sin = self.tables[L["type"]]
         q, k_pre, k_rot, v = mo.qkv_post(qkvg, L["q_norm"], L["k_norm"], cos, sin, pos, cfg.eps)
         o = self.attn.attend(l, q, k_pre, k_rot, v)
         o = mo.gate_mul(o, qkvg[:, (cfg.heads + 2 * cfg.kv_heads) * cfg.head_dim:])
-        return F.linear(o.reshape(o.shape[0], -1), L["o_proj"])
+        return product(o.reshape(o.shape[0], -1), L["o_proj"])
 
     def step(self, tokens, pos, fp32=True):
         """tokens (R,) int64, pos (R,) int64 the new tokens' positions (device); the attention object's begin_step
@@ -168,8 +183,11 @@ class Lfm3Decoder:
         for l, L in enumerate(self.layers):
             h = self._conv(L, n, qsl) if L["type"] == CONV else self._attention(l, L, n, pos)
             x, n = mo.add_rmsnorm(h, x, L["post_norm"], L["ffn_norm"], cfg.eps)
-            a = mo.linear(n, L["w13p"]) if fused_ffn else mo.silu_mul(F.linear(n, L["w13"]))
-            h = F.linear(a, L["w2"])
+            if self.int8:
+                a = i8.linear8(n, L["w13"])
+            else:
+                a = mo.linear(n, L["w13p"]) if fused_ffn else mo.silu_mul(F.linear(n, L["w13"]))
+            h = product(a, L["w2"])
             nxt = self.layers[l + 1]["norm"] if l + 1 < len(self.layers) else self.final_norm
             x, n = mo.add_rmsnorm(h, x, L["post_ffn_norm"], nxt, cfg.eps)
         return F.linear(n, self.embed)
@@ -303,13 +321,94 @@ class PagedAttention800:
         return layer.forward(q, k_pre, v, me[self.group_of[l]], mq, hosts=self.layers, cos_t=self.cos, sin_t=self.sin)
 
 
+class PagedAttention8:
+    """The model's 11 attention layers over paged 8-bit caches (kv8): the 6 full layers over their whole history (no sinks, no
+    800h blocks), the 5 sliding layers over a window of 256. Keys are rotated on their way into the cache. One block table for the
+    full layers, one for the sliding ones, whose rows own a ring of `ring` shuffled pages that holds a chunk of FILL tokens and the
+    window before it. The same steps as PagedAttention800: begin_step / attend, begin_chunk / attend (rows with any number of
+    new tokens up to FILL: prompts, drafts), freeze / thaw for recorded steps, fill for synthetic histories. A draft that is taken back
+    may leave its block a larger exponent, so a loop with drafts can round a block's later tokens more coarsely than one without.
+
+    lens0: the rows' history lengths; steps: decode steps to provide for; bs: tokens per page."""
+
+    FILL = 2048
+
+    def __init__(self, lens0, steps, device, bs=128, seed=0):
+        self.dev = device
+        self.lens = torch.tensor([int(x) for x in lens0], dtype=torch.int64)
+        R = len(lens0)
+        nmax = self.nmax = int(self.lens.max()) + steps + 1
+        rng = torch.Generator().manual_seed(seed)
+        lp = (nmax - 1) // bs + 1
+        self.ring = min(lp, (self.FILL + kv800.WIN) // bs + 2)
+        perm = lambda n: torch.randperm(R * n, generator=rng).view(R, n).to(torch.int32)
+        self.bt = {FULL: perm(lp).to(device), SLIDE: perm(self.ring)[:, torch.arange(lp) % self.ring].contiguous().to(device)}
+        self.tables = {FULL: kernel_tables(nmax, device), SLIDE: model_rope_tables(1e4, 64, nmax, device)}
+        kind = {**{l: FULL for l in (*vc.QUANT_LAYERS, *vc.WINDOW_LAYERS)}, **{l: SLIDE for l in vc.SLIDE_LAYERS}}
+        self.kind = dict(sorted(kind.items()))
+        self.layers = {l: kv8.Cache8.empty(R * (lp if t == FULL else self.ring), 4, bs, 128, device) for l, t in self.kind.items()}
+        self.one = torch.arange(R + 1, dtype=torch.int64, device=device)      # starts of rows with one token each
+        self.step = None                                                      # (lens, qsl) of the present step
+        self.lens_dev = None                                                  # set by freeze()
+
+    def fill(self, history):
+        """Write every row's history into the caches, up to FILL positions per row at a time. history(l, r, p0, p1) -> (K, V)
+        (p1 - p0, 4, 128) bf16 on the device: pre-RoPE K for full layers, post-RoPE K for sliding layers."""
+        for c0 in range(0, int(self.lens.max()) if len(self.lens) else 0, self.FILL):
+            n = torch.clamp(self.lens, max=c0 + self.FILL)
+            new = torch.clamp(n - c0, min=0)
+            qsl = torch.cat((torch.zeros(1, dtype=torch.int64), new.cumsum(0))).to(self.dev)
+            n = n.to(self.dev)
+            for l, t in self.kind.items():
+                parts = [history(l, r, c0, c0 + c) for r, c in enumerate(new.tolist()) if c]
+                K, V = (torch.cat([p[i] for p in parts]) for i in (0, 1))
+                cos, sin = self.tables[FULL] if t == FULL else (None, None)
+                kv8.append(self.layers[l], K, V, self.bt[t], n, qsl, cos, sin)
+
+    def freeze(self, steps):
+        """Make the next `steps` decode steps replayable from one recorded step: the lengths then advance on the device."""
+        self.lens_dev = self.lens.to(self.dev)
+
+    def thaw(self):
+        """Undo freeze(): the next step goes by `lens` again."""
+        self.lens_dev = None
+
+    def begin_step(self):
+        """Metadata of the next decode step (every row appends one token): the new tokens' positions (R,) int64."""
+        self.lens += 1
+        if self.lens_dev is None:
+            lens = vc.step_lens(self.lens, self.dev)
+        else:
+            self.lens_dev += 1
+            lens = self.lens_dev
+        self.step = (lens, self.one)
+        return lens - 1
+
+    def begin_chunk(self, lens, qlens, tokens, most, bound):
+        """Metadata of a step whose rows bring qlens (R,) int32 <= most new tokens each, to lengths lens (R,) int64, both on
+        the device; tokens: room for them; bound (R,): the host's bound of lens. Returns the step's kv800_hip.ChunkMeta."""
+        if int(bound.max()) > self.nmax:
+            raise ValueError(f"the caches hold {self.nmax} positions per row, the step may reach {int(bound.max())}")
+        if most > self.FILL:
+            raise ValueError(f"a row may bring {self.FILL} tokens a step, not {most}")
+        m = kv800_hip.chunk_meta(self.bt[FULL], lens, qlens, self.layers[next(iter(self.layers))].bs, tokens)
+        self.step = (lens, m.qsl)
+        return m
+
+    def attend(self, l, q, k_pre, k_post, v):
+        lens, qsl = self.step
+        t, cache = self.kind[l], self.layers[l]
+        kv8.append(cache, k_pre, v, self.bt[t], lens, qsl, *self.tables[t])
+        return kv8.attend(cache, q, self.bt[t], lens, qsl, window=kv800.WIN if t == SLIDE else 0)
+
+
 class DecodeGraph:
     """Greedy decode with one HIP graph per step. Construction runs the first step eagerly on the graph's own stream
     (it builds the cached tables, library handles and the flush stream that the recorded step reuses; its tokens are
     `tokens` afterwards, its bf16 logits `first_logits`), then freezes the attention for `steps` further steps and records
     one step, whose input is the token buffer and whose greedy tokens are copied back into it. Each step() replays it:
     one graph launch instead of ~250 kernel launches from the host. `tokens` and `logits` (the last replay's bf16
-    logits) are buffers that the next step overwrites. The attention must be a PagedAttention800."""
+    logits) are buffers that the next step overwrites. The attention must be a PagedAttention800 or a PagedAttention8."""
 
     def __init__(self, model, attention, tokens, steps):
         self.attn, self.left = attention, int(steps)
@@ -344,7 +443,7 @@ class DecodeGraph:
 
 def decode_loop(model, attention, tokens, steps, graph=False):
     """Greedy decode: `steps` steps from `tokens` (R,) int64; returns the (steps, R) generated tokens. graph=True runs
-    the steps after the first as replays of one recorded step (DecodeGraph; PagedAttention800 only)."""
+    the steps after the first as replays of one recorded step (DecodeGraph; the paged attentions only)."""
     if graph and steps > 0:
         dg = DecodeGraph(model, attention, tokens, steps - 1)
         out = [dg.tokens.clone()]
@@ -365,7 +464,7 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
     distributions (R, most, vocab) fp32 or None), all on the device; lens counts the positions in the caches. Drafts behind a
     row's count may hold anything, one outside the vocabulary is never kept. temperature
     (R,) fp32, None: greedy. Lengths stay on the device, so a step does not wait for the one before; the attention must be a
-    PagedAttention800 with room for steps (most + 1) more positions, most < 128. Greedy tokens are those of the one-token loop
+    PagedAttention800 or PagedAttention8 with room for steps (most + 1) more positions, most < 128. Greedy tokens are those of the one-token loop
     up to near-ties: the short conv rounds once a sum and not every product, and a block that becomes eligible inside a chunk
     is read exact by that chunk. Returns the rows' new tokens, a list of R
     tensors, and the (steps, R) counts; attention.lens follows."""
