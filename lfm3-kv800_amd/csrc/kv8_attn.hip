@@ -1,7 +1,13 @@
 // kv8_attn.hip -- attention over the paged 8-bit cache (include/kv8_hip.h), gfx950.
 //
-//   attend_kernel  softmax(scale q . k) v of a step's tokens, a list of (query tile, KV head, 128 positions) in equal shares
-//   merge_kernel   joins what several workgroups have of one (query tile, KV head)
+//   attend_kernel      softmax(scale q . k) v of a step's tokens, a list of (query tile, KV head, positions) in equal shares
+//   merge_kernel       joins what several workgroups have of one (query tile, KV head)
+//   prompt_kernel      the same for many new tokens a row: tiles of 128 (query, query head), each block's values once through LDS
+//   merge_rows_kernel  joins what several workgroups have of one (token, head)
+//
+// With m the running maximum of a query's scores, l the sum of its weights and o that of the weighted values, a step of keys is
+//   m' = max(m, max s),  p = 2^(s - m'),  l' = 2^(m - m') l + sum p,  o' = 2^(m - m') o + p V;  o / l at the end,
+// in log2 units; parts of a row join by the same rule. All of m, l and o are fp32.
 //
 // Both products run on the bf16 matrix instruction: a code times its power of two is exact in bf16, two codes an instruction, so
 // that scores are those of the held keys in fp32 and a weight is rounded to 8 bits once. The fp8 instructions with block scales
@@ -10,6 +16,7 @@
 // Operands of 16 x 16 x 32 (lane l: row or column l % 16, g = l / 16): k = 8 g + j. Output: column l % 16, rows 4 g + i. Scores are
 // taken transposed (keys x queries): with the keys of a tile in the cache's slot order the lane's scores are those of the 16
 // tokens 16 g .. of a block, in order, and the lane reads the values of the same: weights never leave their lane.
+#include <cfloat>
 #include <type_traits>
 
 #include "kv8_common.h"
@@ -20,7 +27,7 @@ namespace {
 
 using kv800::f4;
 
-constexpr int COLS = 16;              // (query, query head) pairs of a tile
+constexpr int GROUP = 16;             // query heads a KV head may have
 constexpr float LAZY = 8.f;           // log2 units by which a running maximum may lag over a long list of keys
 
 struct Desc {                         // of a workgroup whose last item others finish: where that item's outputs go
@@ -36,13 +43,13 @@ struct Attend {
   const int64_t* qsl;
   int R;
   int64_t T;
-  int G, TQ;                          // query heads per KV head, queries per tile
+  int G, TQ;                          // query heads per KV head, queries per tile of 16 or 32 columns (query, query head)
   int64_t window;
   int step;                           // positions of a wave's step
   float sl2;                          // |scale| log2(e)
   uint32_t flip;                      // sign bits of two bf16 for a negative scale: q changes its sign
   uint16_t* out;
-  float* part;                        // 2 slots per workgroup of COLS parts: of an item that others began, of one that others finish
+  float* part;                        // 2 slots per workgroup of a tile's parts: of an item that others began, of one that others finish
   Desc* desc;                         // one per workgroup
 };
 
@@ -153,9 +160,9 @@ constexpr int PART = D + 4;
 // LIST: one workgroup takes entries [w W / NG, (w + 1) W / NG) of the W of the list (row, query tile, head, step); else workgroup w is one
 // (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one token. The four waves take every fourth step of an item, each with its
 // own maximum, sum and output, and are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
-template <int D, bool LIST, int NB>
-__global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, int per) {
-  constexpr int STEP = NB * BLK;                   // positions of a wave's step
+template <int D, bool LIST, int NB, int NC>
+__global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Attend A, int per) {
+  constexpr int STEP = NB * BLK, COLS = 16 * NC;   // positions of a wave's step; columns of a tile
   constexpr int NT = D / 16, NK = D / 32, LD = D + 4;
   __shared__ typename std::conditional<LIST, List, int>::type L;
   __shared__ __align__(16) float so[4][COLS][LD];
@@ -171,13 +178,31 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, 
   if constexpr (LIST) {
     if (tid == 0) A.desc[w].last = -1;
     const auto cost = [&](const Row& w) { return cost_of(A, w); };
-    scan_rows(A, L, per, cost);
-    W = L.pre[256];
+    int64_t incl = 0;                              // up to 64 rows: every wave for itself, lane r the sum to row r
+    if (A.R <= 64) {
+      incl = lane < A.R ? cost(row_at(A, lane)) : 0;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(incl, o);
+        if (lane >= o) incl += y;
+      }
+      W = __shfl(incl, 63);
+    } else {
+      scan_rows(A, L, per, cost);
+      W = L.pre[256];
+    }
+    W = same(W);
     NG = min((int64_t)gridDim.x, W);               // no workgroup between two others is without entries
     if (w >= NG) return;
     x = w * W / NG;
     end = (w + 1) * W / NG;
-    r = __builtin_amdgcn_readfirstlane(find_row(A, L, per, x, before, cost));
+    if (A.R <= 64) {
+      r = __popcll(__ballot(incl <= x));
+      before = r ? __shfl(incl, r - 1) : 0;
+    } else {
+      r = find_row(A, L, per, x, before, cost);
+    }
+    r = __builtin_amdgcn_readfirstlane(r);
     before = same(before);
     x = same(x);
     end = same(end);
@@ -211,21 +236,28 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, 
       tile = (int)(w / A.C.heads) - tile0;
     }
 
-    // ---- the queries of the lane's column
-    const int i = tile * A.TQ + rr / A.G, hq = h * A.G + rr % A.G;
-    const bool have = rr < A.TQ * A.G && i < row.c;
-    const int64_t qp = row.p0 + i, qlo = A.window > 0 ? qp - A.window : -1;   // sees positions (qlo, qp]
-    kv800::b8 qr[NK];        // dims 16 g .. of the lower and (D = 128) upper 64, 8 an instruction
+    // ---- the queries of the lane's columns
+    int64_t qp[NC], qlo[NC];     // the query sees positions (qlo, qp]
+    kv800::b8 qr[NC][NK];        // dims 16 g .. of the lower and (D = 128) upper 64, 8 an instruction
+    f4 o[NC][NT];
+    float M[NC], l[NC];
 #pragma unroll
-    for (int e = 0; e < NK; ++e) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (have) u = *reinterpret_cast<const uint4*>(A.q + ((row.q0 + i) * A.C.heads * A.G + hq) * D + (e >> 1) * 64 + 16 * g + 8 * (e & 1));
-      qr[e] = kv800::as_b8(kv800::u4v{u.x ^ A.flip, u.y ^ A.flip, u.z ^ A.flip, u.w ^ A.flip});
+    for (int n = 0; n < NC; ++n) {
+      const int c = 16 * n + rr, i = tile * A.TQ + c / A.G, hq = h * A.G + c % A.G;
+      const bool have = c < A.TQ * A.G && i < row.c;
+      qp[n] = row.p0 + i;
+      qlo[n] = A.window > 0 ? qp[n] - A.window : -1;
+#pragma unroll
+      for (int e = 0; e < NK; ++e) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (have) u = *reinterpret_cast<const uint4*>(A.q + ((row.q0 + i) * A.C.heads * A.G + hq) * D + (e >> 1) * 64 + 16 * g + 8 * (e & 1));
+        qr[n][e] = kv800::as_b8(kv800::u4v{u.x ^ A.flip, u.y ^ A.flip, u.z ^ A.flip, u.w ^ A.flip});
+      }
+#pragma unroll
+      for (int d = 0; d < NT; ++d) o[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+      M[n] = -INFINITY;
+      l[n] = 0.f;
     }
-    f4 o[NT];
-#pragma unroll
-    for (int d = 0; d < NT; ++d) o[d] = f4{0.f, 0.f, 0.f, 0.f};
-    float M = -INFINITY, l = 0.f;
 
     // positions that some query of the tile sees, (tlo, thi], and those that all of them see, [alo, ahi)
     const int ilast = min(row.c, (tile + 1) * A.TQ) - 1;
@@ -271,60 +303,68 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, 
           for (int d = 0; d < NT; ++d) vv[d][u] = make_uint4(0, 0, 0, 0);
         }
       }
-      // ---- scores of the lane's column: tile a holds tokens 64 (a / 4) + 16 g + 4 (a % 4) + j
-      float s[16 * NB];
+      // ---- scores of the lane's columns: tile a holds tokens 64 (a / 4) + 16 g + 4 (a % 4) + j
+      float s[NC][16 * NB];
 #pragma unroll
       for (int a = 0; a < 4 * NB; ++a) {
-        f4 c = {0.f, 0.f, 0.f, 0.f};
+        f4 c[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) c[n] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) {
-          c = kv800::mfma_bf(wide8(kk[a][e].x, kk[a][e].y, sc[a >> 2][0]), qr[2 * e], c);
-          c = kv800::mfma_bf(wide8(kk[a][e].z, kk[a][e].w, sc[a >> 2][0]), qr[2 * e + 1], c);
+          const kv800::b8 k0 = wide8(kk[a][e].x, kk[a][e].y, sc[a >> 2][0]), k1 = wide8(kk[a][e].z, kk[a][e].w, sc[a >> 2][0]);
+#pragma unroll
+          for (int n = 0; n < NC; ++n) c[n] = kv800::mfma_bf(k1, qr[n][2 * e + 1], kv800::mfma_bf(k0, qr[n][2 * e], c[n]));
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * a + j] = c[j] * A.sl2;
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][4 * a + j] = c[n][j] * A.sl2;
       }
       const bool edge = pos < alo || pos + STEP > ahi || !on[0] || !on[NB - 1];
-      if (edge) {          // tokens of the step that the column's query sees: [lo, hi)
-        int lo = (int)min(max(qlo + 1 - pos, (int64_t)0), (int64_t)STEP), hi = (int)min(max(min(qp + 1, row.n) - pos, (int64_t)0), (int64_t)STEP);
-        if (!on[0]) lo = max(lo, BLK);
-        if (!on[NB - 1]) hi = min(hi, STEP - BLK);
-        const int see0 = lo - 16 * g;
-        const uint32_t seen = (uint32_t)max(hi - lo, 0);
+      uint32_t pw[NC][8 * NB];
 #pragma unroll
-        for (int a = 0; a < 4 * NB; ++a)
+      for (int n = 0; n < NC; ++n) {
+        if (edge) {        // tokens of the step that the column's query sees: [lo, hi)
+          int lo = (int)min(max(qlo[n] + 1 - pos, (int64_t)0), (int64_t)STEP), hi = (int)min(max(min(qp[n] + 1, row.n) - pos, (int64_t)0), (int64_t)STEP);
+          if (!on[0]) lo = max(lo, BLK);
+          if (!on[NB - 1]) hi = min(hi, STEP - BLK);
+          const int see0 = lo - 16 * g;
+          const uint32_t seen = (uint32_t)max(hi - lo, 0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if ((uint32_t)(64 * (a >> 2) + 4 * (a & 3) + j - see0) >= seen) s[4 * a + j] = -INFINITY;
+          for (int a = 0; a < 4 * NB; ++a)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if ((uint32_t)(64 * (a >> 2) + 4 * (a & 3) + j - see0) >= seen) s[n][4 * a + j] = -INFINITY;
+        }
+        float mt = s[n][0];
+#pragma unroll
+        for (int j = 1; j < 16 * NB; ++j) mt = fmaxf(mt, s[n][j]);
+        mt = kv800::max4rows(mt);
+        const float Mn = fmaxf(M[n], ceilf(mt));
+        if (__any(Mn > M[n])) {
+          const float alpha = Mn > M[n] ? __builtin_amdgcn_exp2f(M[n] - Mn) : 1.f;    // M = -inf: 0
+          l[n] *= alpha;
+#pragma unroll
+          for (int d = 0; d < NT; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][d][j] *= alpha;
+          M[n] = Mn;
+        }
+        // ---- weights
+        const float M0 = M[n] > -INFINITY ? M[n] : 0.f;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8 * NB; ++j) {
+          const float p0 = __builtin_amdgcn_exp2f(s[n][2 * j] - M0), p1 = __builtin_amdgcn_exp2f(s[n][2 * j + 1] - M0);
+          sum += p0 + p1;
+          pw[n][j] = kv800::bfpk(p0, p1);
+        }
+        if (__any(sum != sum)) {   // a column whose every key so far is NaN has no maximum, yet its sum counts
+          if (kv800::max4rows(sum != sum ? 1.f : 0.f) > 0.f && M[n] == -INFINITY) M[n] = 0.f;
+        }
+        l[n] += sum;
       }
-      float mt = s[0];
-#pragma unroll
-      for (int j = 1; j < 16 * NB; ++j) mt = fmaxf(mt, s[j]);
-      mt = kv800::max4rows(mt);
-      const float Mn = fmaxf(M, ceilf(mt));
-      if (__any(Mn > M)) {
-        const float alpha = Mn > M ? __builtin_amdgcn_exp2f(M - Mn) : 1.f;    // M = -inf: 0
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < NT; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[d][j] *= alpha;
-        M = Mn;
-      }
-      // ---- weights
-      const float M0 = M > -INFINITY ? M : 0.f;
-      uint32_t pw[8 * NB];
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8 * NB; ++j) {
-        const float p0 = __builtin_amdgcn_exp2f(s[2 * j] - M0), p1 = __builtin_amdgcn_exp2f(s[2 * j + 1] - M0);
-        sum += p0 + p1;
-        pw[j] = kv800::bfpk(p0, p1);
-      }
-      if (__any(sum != sum)) {   // a column whose every key so far is NaN has no maximum, yet its sum counts
-        if (kv800::max4rows(sum != sum ? 1.f : 0.f) > 0.f && M == -INFINITY) M = 0.f;
-      }
-      l += sum;
       // ---- in a step with a mask, codes that not every query sees: a weight of 0 does not take out a NaN
       bool poison = false;
       if (edge) {
@@ -348,12 +388,17 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, 
       }
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
-        const kv800::b8 pa = kv800::as_b8(kv800::u4v{pw[8 * u], pw[8 * u + 1], pw[8 * u + 2], pw[8 * u + 3]});
-        const kv800::b8 pb = kv800::as_b8(kv800::u4v{pw[8 * u + 4], pw[8 * u + 5], pw[8 * u + 6], pw[8 * u + 7]});
+        kv800::b8 pa[NC], pb[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          pa[n] = kv800::as_b8(kv800::u4v{pw[n][8 * u], pw[n][8 * u + 1], pw[n][8 * u + 2], pw[n][8 * u + 3]});
+          pb[n] = kv800::as_b8(kv800::u4v{pw[n][8 * u + 4], pw[n][8 * u + 5], pw[n][8 * u + 6], pw[n][8 * u + 7]});
+        }
 #pragma unroll
         for (int d = 0; d < NT; ++d) {
-          o[d] = kv800::mfma_bf(wide8(vv[d][u].x, vv[d][u].y, sc[u][1]), pa, o[d]);
-          o[d] = kv800::mfma_bf(wide8(vv[d][u].z, vv[d][u].w, sc[u][1]), pb, o[d]);
+          const kv800::b8 v0 = wide8(vv[d][u].x, vv[d][u].y, sc[u][1]), v1 = wide8(vv[d][u].z, vv[d][u].w, sc[u][1]);
+#pragma unroll
+          for (int n = 0; n < NC; ++n) o[n][d] = kv800::mfma_bf(v1, pb[n], kv800::mfma_bf(v0, pa[n], o[n][d]));
         }
       }
       if (poison) {        // NaN values taken out above go to the queries that see them
@@ -362,22 +407,29 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, 
           if (!on[t >> 6] || tp > thi) continue;
           const int64_t bi = tp / BLK;
           const uint8_t* base = block_of<D>(A.C, A.bt[(int64_t)r * A.bt_stride + bi / A.C.blocks], h, (int)(bi % A.C.blocks)) + BLK * D;
-          if (tp <= qp && tp > qlo && tp < row.n)
-            for (int d = 0; d < NT; ++d)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if ((base[((t >> 4 & 3) * D + 16 * d + 4 * g + j) * 16 + (t & 15)] & 0x7F) == 0x7F) o[d][j] = NAN;
+          for (int n = 0; n < NC; ++n)
+            if (tp <= qp[n] && tp > qlo[n] && tp < row.n)
+#pragma unroll
+              for (int d = 0; d < NT; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if ((base[((t >> 4 & 3) * D + 16 * d + 4 * g + j) * 16 + (t & 15)] & 0x7F) == 0x7F) o[n][d][j] = NAN;
         }
       }
     }
     // ---- the four waves' parts
-    l = kv800::sum4rows(l);
-    if (g == 0) { sm[wv][rr] = M; sl[wv][rr] = l; }
 #pragma unroll
-    for (int d = 0; d < NT; ++d) *reinterpret_cast<f4*>(&so[wv][rr][16 * d + 4 * g]) = o[d];
+    for (int n = 0; n < NC; ++n) {
+      const float ls = kv800::sum4rows(l[n]);
+      if (g == 0) { sm[wv][16 * n + rr] = M[n]; sl[wv][16 * n + rr] = ls; }
+#pragma unroll
+      for (int d = 0; d < NT; ++d) *reinterpret_cast<f4*>(&so[wv][16 * n + rr][16 * d + 4 * g]) = o[n][d];
+    }
     __syncthreads();
-    {
-      const int c = tid >> 4, d0 = (tid & 15) * (D / 16);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int c = 16 * n + (tid >> 4), d0 = (tid & 15) * (D / 16);
       float m = sm[0][c];
 #pragma unroll
       for (int k = 1; k < 4; ++k) m = fmaxf(m, sm[k][c]);
@@ -410,7 +462,7 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attend_kernel(Attend A, 
         for (int e = 0; e < D / 16; ++e) pt[d0 + e] = acc[e];
         if (d0 == 0) { pt[D] = m; pt[D + 1] = ls; }
         // the item's last entry: the least w' with (w' + 1) W / NG at or behind its end
-        if (s0 == 0 && tid == 0)
+        if (s0 == 0 && tid == 0 && n == 0)
           A.desc[w] = {(int)row.q0 + tile * A.TQ, min(A.TQ, row.c - tile * A.TQ), h, (int)(((at + row.steps) * NG + W - 1) / W - 1)};
       }
     }
@@ -450,8 +502,9 @@ __device__ __forceinline__ void join(int count, Slot slot, uint16_t* __restrict_
 }
 
 // One wave per (workgroup of the list, column): where that workgroup began an item that others finish, its part and theirs.
-template <int D>
+template <int D, int NC>
 __global__ void __launch_bounds__(256) merge_kernel(Attend A) {
+  constexpr int COLS = 16 * NC;
   const int64_t w = blockIdx.x;
   const Desc d = A.desc[w];
   if (d.last < 0) return;
@@ -604,7 +657,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   for (int d = 0; d < NT; ++d)
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
-  float m = have ? -1e30f : 1e30f, l = 0.f;       // columns without a query never ask for a rescale
+  float m = have ? -FLT_MAX : FLT_MAX, l = 0.f;   // columns without a query never ask for a rescale
   const float lazy = part || A.window > 0 ? 0.f : LAZY;
 
   if (tid < 2) flag[tid] = -1;
@@ -730,11 +783,10 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
 enum Kind { LISTED, DIRECT, PROMPT };
 struct Plan {
   Kind kind;
-  int TQ, G, splits, step;
+  int TQ, G, splits, step, cols;
   int64_t tiles, groups;              // query tiles of all rows at most; workgroups (LISTED)
   int64_t bytes;                      // workspace
 };
-constexpr int SD = 1, SL = 2;         // blocks a step
 constexpr int NW = 4;                 // waves of the prompt kernel
 Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
   Plan p;
@@ -743,10 +795,17 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
   p.groups = 0;
   p.bytes = 0;
   const int64_t positions = bt_cols * c->blocks * BLK, mean = (T + R - 1) / R;
-  const int64_t seen = window > 0 && window + mean < positions ? window + mean : positions;   // of a row, or so
-  p.kind = T * p.G >= 64 * R ? PROMPT : seen <= 1024 ? DIRECT : LISTED;
-  p.step = p.kind == DIRECT ? SD * BLK : SL * BLK;
-  p.TQ = (p.kind == PROMPT ? 32 * NW : COLS) / p.G;
+  const int64_t seen = window > 0 && window < positions - mean ? window + mean : positions;   // of a row, or so
+  // Columns of a row and KV head, on average: the prompt kernel's tile has 128, the list's 16 or 32. Times, us, of 64 rows x 4,096 / 16 x
+  // 4,096 / 1 x 16,384 positions by tiles of 16, of 32, and as prompts: 16 columns 62, 64, 82 / 27, 27, 29 / 19, 23, 26; 32 columns 92, 66, 80 / 25, 32, 31 /
+  // 20, 25, 26; 48 columns 133, 92, 87 / 44, 30, 33 / 24, 47, 26; 64 columns 166, 92, 88 / 33, 31, 34 / 34, 48, 27.
+  const int64_t cols = T * p.G / R, items = R * c->kv_heads;
+  // (Sixteen rows of 4,096 positions with 1 to 33 tokens each: 36 us by tiles of 32, 32 as prompts, so 40 is where prompts begin.)
+  const bool wide = items * seen >= 1 << 19;
+  p.kind = cols >= 40 ? PROMPT : seen <= 1024 ? DIRECT : LISTED;
+  p.cols = p.kind == PROMPT ? 32 * NW : p.kind == LISTED && wide && cols > 16 ? 32 : 16;
+  p.TQ = p.cols / p.G;
+  p.step = p.kind == LISTED && p.cols == 16 ? 2 * BLK : BLK;
   p.tiles = (T + R * (p.TQ - 1)) / p.TQ;
   if (p.kind == PROMPT) {
     // few tiles: each split over its blocks, down to 8, for two workgroups a CU
@@ -758,7 +817,7 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
   } else if (p.kind == LISTED) {
     const int64_t entries = p.tiles * c->kv_heads * ((positions + p.step - 1) / p.step + 1);
     p.groups = (entries + 3) / 4 < 512 ? (entries + 3) / 4 : 512;
-    p.bytes = p.groups * (2 * COLS * (c->dim + 4) * 4 + (int64_t)sizeof(Desc));
+    p.bytes = p.groups * (2 * p.cols * (c->dim + 4) * 4 + (int64_t)sizeof(Desc));
   }
   return p;
 }
@@ -778,15 +837,19 @@ int run(const Attend& A0, const Plan& p, int64_t heads, void* ws, hipStream_t s)
     return kv800::check_launch("kv8_attend prompt");
   }
   if (p.kind == DIRECT) {
-    hipLaunchKernelGGL((attend_kernel<D, false, SD>), dim3((unsigned)(p.tiles * H)), dim3(256), 0, s, A, 0);
+    hipLaunchKernelGGL((attend_kernel<D, false, 1, 1>), dim3((unsigned)(p.tiles * H)), dim3(256), 0, s, A, 0);
     return kv800::check_launch("kv8_attend");
   }
   A.part = (float*)ws;
-  A.desc = (Desc*)(A.part + p.groups * 2 * COLS * PART<D>);
-  hipLaunchKernelGGL((attend_kernel<D, true, SL>), dim3((unsigned)p.groups), dim3(256), 0, s, A, (A.R + 255) / 256);
+  A.desc = (Desc*)(A.part + p.groups * 2 * p.cols * PART<D>);
+  const dim3 grid((unsigned)p.groups), mg((unsigned)p.groups, (unsigned)(p.cols / 4));
+  const int per = (A.R + 255) / 256;
+  if (p.cols == 32) hipLaunchKernelGGL((attend_kernel<D, true, 1, 2>), grid, dim3(256), 0, s, A, per);
+  else hipLaunchKernelGGL((attend_kernel<D, true, 2, 1>), grid, dim3(256), 0, s, A, per);
   const int rc = kv800::check_launch("kv8_attend");
   if (rc != KV800_OK) return rc;
-  hipLaunchKernelGGL(merge_kernel<D>, dim3((unsigned)p.groups, COLS / 4), dim3(256), 0, s, A);
+  if (p.cols == 32) hipLaunchKernelGGL((merge_kernel<D, 2>), mg, dim3(256), 0, s, A);
+  else hipLaunchKernelGGL((merge_kernel<D, 1>), mg, dim3(256), 0, s, A);
   return kv800::check_launch("kv8_attend merge");
 }
 
@@ -796,8 +859,8 @@ int run(const Attend& A0, const Plan& p, int64_t heads, void* ws, hipStream_t s)
 extern "C" {
 
 int64_t kv8_hip_attend_workspace(const kv8_cache_t* cache, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
-  if (!kv8::valid(cache) || heads <= 0 || heads % cache->kv_heads || heads / cache->kv_heads > kv8::COLS || R <= 0 || T <= 0) return 0;
-  return kv8::plan(cache, heads, R, T, bt_cols, window).bytes;
+  if (!kv8::valid(cache) || heads <= 0 || heads % cache->kv_heads || heads / cache->kv_heads > kv8::GROUP || R <= 0 || T <= 0) return 0;
+  return kv8::plan(cache, heads, R, T, bt_cols, window >= (int64_t)1 << 40 ? 0 : window).bytes;
 }
 
 int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, const int32_t* bt, int64_t bt_stride,
@@ -805,12 +868,13 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
                    float scale, uint16_t* out, void* ws, int64_t ws_bytes, void* stream) {
   KV800_REQUIRE(kv8::valid(cache), "kv8_attend: bad cache descriptor");
   KV800_REQUIRE(R >= 0 && T >= 0 && bt_cols >= 0 && bt_stride >= 0 && window >= 0, "kv8_attend: negative size");
-  KV800_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads / cache->kv_heads <= kv8::COLS,
+  KV800_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads / cache->kv_heads <= kv8::GROUP,
                 "kv8_attend: heads must be a multiple of the cache's, up to 16 times");
   KV800_REQUIRE(fabsf(scale) > 0.f && fabsf(scale) < INFINITY, "kv8_attend: scale must be finite and not 0");
   KV800_REQUIRE(bt_cols <= INT32_MAX / (cache->blocks * kv8::BLK), "kv8_attend: the table covers 2^31 positions or more");
   KV800_REQUIRE(R <= INT32_MAX / 512 && T <= INT32_MAX / 512, "kv8_attend: too many tokens or rows");
   if (T == 0) return KV800_OK;
+  if (window >= (int64_t)1 << 40) window = 0;      // more than any row has; sums with positions stay in 64 bits
   KV800_REQUIRE(R > 0, "kv8_attend: tokens without rows");
   KV800_REQUIRE(q && lens && qsl && out && (bt || bt_cols == 0), "kv8_attend: null pointer");
   KV800_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0, "kv8_attend: q and out must be 16-byte aligned");

@@ -170,7 +170,7 @@ def attend(cache, q, bt, lens, qsl, window=0, scale=None):
     T, heads = q.shape[:2]
     dev = cache.dev
     R, lens, qsl = _step(cache, T, bt, lens, qsl)
-    window = int(window)
+    window = min(int(window), 1 << 40)
     if window < 0:
         raise ValueError("window must be >= 0")
     scale = 1.0 / math.sqrt(cache.dim) if scale is None else float(scale)
