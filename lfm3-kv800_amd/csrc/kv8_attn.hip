@@ -879,7 +879,7 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
   KV800_REQUIRE(q && lens && qsl && out && (bt || bt_cols == 0), "kv8_attend: null pointer");
   KV800_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0, "kv8_attend: q and out must be 16-byte aligned");
   const kv8::Plan p = kv8::plan(cache, heads, R, T, bt_cols, window);
-  KV800_REQUIRE(p.tiles * cache->kv_heads * p.splits < INT32_MAX, "kv8_attend: too many tokens or rows");
+  KV800_REQUIRE(p.tiles * cache->kv_heads * p.splits < (1 << 24) - 64, "kv8_attend: too many tokens or rows");   // 2^32 threads a launch
   KV800_REQUIRE(p.bytes == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.bytes), "kv8_attend: %lld bytes of 16-byte aligned workspace needed",
                 (long long)p.bytes);
   const kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window, p.step,

@@ -237,7 +237,7 @@ int kv8_hip_append(const kv8_cache_t* cache, const uint16_t* k, int64_t k_ts, in
   KV800_REQUIRE(k && v && bt && lens && qsl, "kv8_append: null pointer");
   KV800_REQUIRE(k_ts % 8 == 0 && k_hs % 8 == 0 && v_ts % 8 == 0 && v_hs % 8 == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0,
                 "kv8_append: k and v need 16-byte aligned rows (strides multiples of 8)");
-  KV800_REQUIRE(R <= INT32_MAX / 4 && T <= (int64_t)INT32_MAX * 32, "kv8_append: too many tokens or rows");
+  KV800_REQUIRE(R < (1 << 30) && T < (1 << 30) && T + 126 * R < (1 << 30), "kv8_append: too many tokens or rows");   // 2^32 threads a launch
   KV800_REQUIRE((cos_t == nullptr) == (sin_t == nullptr), "kv8_append: cos_t and sin_t go together");
   KV800_REQUIRE(!cos_t || (freqs > 0 && freqs % 8 == 0 && freqs <= cache->dim / 2 && rope_rows > 0 && (uintptr_t)cos_t % 16 == 0 &&
                            (uintptr_t)sin_t % 16 == 0),

@@ -426,7 +426,7 @@ constexpr int64_t K_MOST = 65536;      // 127^2 K below 2^31
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 int64_t padded_rows(int64_t N, int gated) { return gated ? 2 * round_up(N / 2, 32) : round_up(N, 64); }
 bool sizes(int64_t R, int64_t N, int64_t K, int gated) {
-  return R >= 0 && R <= (1 << 24) && N > 0 && N <= (1 << 24) && K > 0 && K <= K_MOST && K % 8 == 0 && (gated == 0 || (gated == 1 && N % 2 == 0));
+  return R >= 0 && R < (1 << 24) && N > 0 && N < (1 << 24) && K > 0 && K <= K_MOST && K % 8 == 0 && (gated == 0 || (gated == 1 && N % 2 == 0));
 }
 
 // How a product runs: in 256 x 128 tiles, or on few_kernel with nt tiles of the weight and wm of the tokens a workgroup, which rounds
@@ -459,16 +459,17 @@ extern "C" {
 
 int lfm3_hip_int8_layout(const int8_t* w, int64_t ld, const float* scale, int64_t N, int64_t K, int gated, int8_t* wsh, float* ssh,
                          void* stream) {
-  KV800_REQUIRE(lfm3::sizes(0, N, K, gated) && ld >= 0, "int8_layout: N up to 2^24 (even for a gated weight), K a multiple of 8 up to 65536");
+  KV800_REQUIRE(lfm3::sizes(0, N, K, gated) && ld >= 0, "int8_layout: N below 2^24 (even for a gated weight), K a multiple of 8 up to 65536");
   KV800_REQUIRE(w && scale && wsh && ssh && (uintptr_t)wsh % 16 == 0 && (uintptr_t)ssh % 16 == 0, "int8_layout: null or unaligned pointer");
   const int64_t Npad = lfm3::padded_rows(N, gated), nks = lfm3::round_up(K, 128) / 32, n = Npad / 32 * nks * 64;
+  KV800_REQUIRE(n < (int64_t)1 << 32, "int8_layout: a weight of 64 GiB or more");   // 2^32 threads a launch
   hipLaunchKernelGGL(lfm3::layout_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, w, ld, scale, N, K,
                      Npad, nks, gated, wsh, ssh);
   return kv800::check_launch("int8_layout");
 }
 
 int lfm3_hip_int8_quantize(const uint16_t* w, int64_t ld, int64_t N, int64_t K, int8_t* w8, float* scale, void* stream) {
-  KV800_REQUIRE(lfm3::sizes(0, N, K, 0) && ld % 8 == 0, "int8_quantize: N up to 2^24, K a multiple of 8 up to 65536, ld a multiple of 8");
+  KV800_REQUIRE(lfm3::sizes(0, N, K, 0) && ld % 8 == 0, "int8_quantize: N below 2^24, K a multiple of 8 up to 65536, ld a multiple of 8");
   KV800_REQUIRE(w && w8 && scale && (uintptr_t)w % 16 == 0 && (uintptr_t)w8 % 8 == 0, "int8_quantize: null or unaligned pointer");
   hipLaunchKernelGGL((lfm3::quantize_kernel<false, 4>), dim3((unsigned)N), dim3(256), 0, (hipStream_t)stream, w, ld, N, K, 0,
                      w8, scale);
@@ -485,7 +486,7 @@ int64_t lfm3_hip_linear8_workspace(int64_t R, int64_t N, int64_t K, int gated) {
 int lfm3_hip_linear8(const uint16_t* x, int64_t ldx, const int8_t* wsh, const float* ssh, int64_t R, int64_t N, int64_t K,
                      int gated, uint16_t* y, int64_t ldy, void* ws, int64_t ws_bytes, void* stream) {
   KV800_REQUIRE(lfm3::sizes(R, N, K, gated),
-                "linear8: R and N up to 2^24 (N even for a gated weight), K a multiple of 8 up to 65536, gated 0 or 1");
+                "linear8: R and N below 2^24 (N even for a gated weight), K a multiple of 8 up to 65536, gated 0 or 1");
   KV800_REQUIRE(ldx % 8 == 0 && ldy >= 0, "linear8: ldx must be a multiple of 8 and ldy >= 0");
   if (R == 0) return KV800_OK;
   KV800_REQUIRE(x && wsh && ssh && y && (uintptr_t)x % 16 == 0 && (uintptr_t)wsh % 16 == 0 && (uintptr_t)ssh % 16 == 0, "linear8: null or unaligned pointer");

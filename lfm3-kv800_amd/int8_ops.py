@@ -63,7 +63,7 @@ class Weight8:
 
     def __init__(self, w, scale=None, gated=False):
         L = _lib()
-        if w.dim() != 2 or not w.shape[0] or not w.shape[1] or w.shape[1] % 8 or w.shape[1] > 65536 or w.shape[0] > 1 << 24:
+        if w.dim() != 2 or not w.shape[0] or not w.shape[1] or w.shape[1] % 8 or w.shape[1] > 65536 or w.shape[0] >= 1 << 24:
             raise ValueError(f"w must be (N, K) with K a multiple of 8 up to 65536, got {tuple(w.shape)}")
         self.gated = bool(gated)
         if self.gated and w.shape[0] % 2:

@@ -375,6 +375,8 @@ class PagedAttention8:
 
     def begin_step(self):
         """Metadata of the next decode step (every row appends one token): the new tokens' positions (R,) int64."""
+        if int(self.lens.max()) >= self.nmax:
+            raise ValueError(f"the caches hold {self.nmax} positions per row")
         self.lens += 1
         if self.lens_dev is None:
             lens = vc.step_lens(self.lens, self.dev)

@@ -107,3 +107,65 @@ def test_views(i8):
         assert ((i8.linear8(v, W).cpu().double() - want).abs() <= far).all()
     t = big[:, :256].t().contiguous().to(DEV).t()
     assert torch.equal(i8.linear8(t, W), i8.linear8(d[:, :256], W))
+
+
+@pytest.mark.parametrize("R,N,K,gated", [(1, 256, 512, True), (20, 512, 264, False), (256, 512, 2048, False), (1000, 8192, 256, True)], ids=str)
+def test_recorded_and_on_other_streams(i8, R, N, K, gated):
+    """Two products recorded into two graphs and replayed in turn on new tokens, with eager work between; the same on two streams at
+    once: equal bits."""
+    g = torch.Generator().manual_seed(R)
+    W = i8.Weight8((torch.randn(N, K, generator=g) * 0.05).to(torch.bfloat16).to(DEV), gated=gated)
+    xs = torch.randn(5, R, K, generator=g).to(torch.bfloat16).to(DEV)
+    want = [i8.linear8(x, W) for x in xs]
+    buf, graphs, outs = [xs[0].clone() for _ in range(2)], [], []
+    for n in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = i8.linear8(buf[n], W)
+        graphs.append(gr); outs.append(out)
+    for i in range(5):
+        for n in range(2):
+            buf[n].copy_(xs[(i + n) % 5])
+            graphs[n].replay()
+        i8.linear8(xs[0], W)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[i]) and torch.equal(outs[1], want[(i + 1) % 5]), i
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(5):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(i8.linear8(xs[i], W))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_weights_without_numbers(i8):
+    """A weight row with an infinity or NaN, or a scale that is none, gives NaN in its channel alone; rows of zeros give zeros."""
+    g = torch.Generator().manual_seed(4)
+    w = torch.randn(70, 136, generator=g).to(torch.bfloat16)
+    w[3, 5], w[40, 0], w[9] = math.inf, math.nan, 0
+    x = torch.randn(5, 136, generator=g).to(torch.bfloat16)
+    y = i8.linear8(x.to(DEV), i8.Weight8(w.to(DEV))).cpu().double()
+    q, s = quantized(w[[0, 9, 69]])
+    want, far = product(x, q, s[:, 0], False)
+    assert y[:, [3, 40]].isnan().all() and ((y[:, [0, 9, 69]] - want).abs() <= far).all() and not y[:, 9].any()
+    keep = [n for n in range(70) if n not in (3, 40)]
+    assert not y[:, keep].isnan().any()
+
+
+def test_calls_that_are_refused(i8):
+    w, s = torch.ones(64, 64, dtype=torch.int8, device=DEV), torch.ones(64, device=DEV)
+    b = torch.ones(64, 64, dtype=torch.bfloat16, device=DEV)
+    for a, kw in (((w, s[:63]), {}), ((w, s.double()), {}), ((w, s.cpu()), {}), ((w.cpu(), s.cpu()), {}), ((w.int(), s), {}), ((w,), {}), ((b.float(),), {}), ((b, s), {}),
+                  ((w[:, :60], s), {}), ((w[0], s), {}), ((w[:0], s[:0]), {}), ((w[:, :0], s), {}), ((w[:63], s[:63]), dict(gated=True))):
+        with pytest.raises((TypeError, ValueError)):
+            i8.Weight8(*a, **kw)
+    for a in (b.float(), b[:, :60], b[0], b[:0], b[:, :0], w):
+        with pytest.raises((TypeError, ValueError)):
+            i8.quantize_rows(a)
+    W = i8.Weight8(w, s)
+    for x in (b.float(), b.cpu(), b[:, :56], b[0], b[None]):
+        with pytest.raises((TypeError, ValueError)):
+            i8.linear8(x, W)
+    assert i8.linear8(b[:0], W).shape == (0, 64)
+    assert torch.equal(i8.linear8(b[:1].expand(9, 64), W), i8.linear8(b[:9], W))

@@ -210,3 +210,220 @@ def test_attend_many_rows(kv8):
     data, exps, bt, lens, qsl, T, g = rows(kv8, 5, prev, new, 1, 64, 64)
     q = torch.randn(T, 2, 64, generator=g).to(torch.bfloat16)
     check_attend(kv8, data, exps, q, bt, lens, qsl)
+
+
+@pytest.mark.parametrize("R", [64, 70])
+@pytest.mark.parametrize("G", [4, 3])
+def test_attend_drafts_of_many_rows(kv8, R, G):
+    """Tiles of 32 columns: a large step of drafts in tables wider than the rows, some of them empty, one token of NaN values that only
+    later queries see, up to 64 rows and beyond."""
+    g = torch.Generator().manual_seed(R)
+    prev = torch.randint(0, 260, (R,), generator=g).tolist()
+    prev[3], prev[R - 2] = 1000, 700
+    new = torch.randint(5, 10, (R,), generator=g).tolist()
+    new[0] = new[17] = 0
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 6, prev, new, 8, 64, 64, pad=2, cols=2)
+    assert R * 8 * bt.shape[1] * 64 >= 1 << 19
+    bad = prev[3] + 2
+    data[int(bt[3, bad // 64]), :, 0, 1, ref.tables(64)[1][bad % 64, 11]] = 0x7F
+    q = torch.randn(T, 8 * G, 64, generator=g).to(torch.bfloat16)
+    got = check_attend(kv8, data, exps, q, bt, lens, qsl)
+    a, b = int(qsl[3]), int(qsl[4])
+    assert not got[a:a + 2].isnan().any() and got[a + 2:b, :, 11].isnan().all() and not got[b:].isnan().any()
+    if R == 64 and G == 4:
+        check_attend(kv8, data, exps, q, bt, lens, qsl, window=1100)
+
+
+def test_attend_many_long_rows(kv8):
+    """More rows than lanes in lists of 128 positions."""
+    g = torch.Generator().manual_seed(8)
+    prev = torch.randint(0, 150, (300,), generator=g).tolist()
+    prev[7], prev[250] = 1500, 1200
+    new = torch.randint(0, 3, (300,), generator=g).tolist()
+    new[7] = 2
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 5, prev, new, 1, 64, 64)
+    q = torch.randn(T, 2, 64, generator=g).to(torch.bfloat16)
+    check_attend(kv8, data, exps, q, bt, lens, qsl)
+
+
+SHAPES = [([300, 64], [1, 1]), ([1500, 0], [1, 1]), ([2100, 5], [5, 2]), ([200, 90], [70, 64])]
+
+
+@pytest.mark.parametrize("prev,new", SHAPES, ids=str)
+def test_queries_that_are_no_numbers(kv8, prev, new):
+    """An infinity or NaN in one query stays with it; scores far below what exponents reach, on their own, are still a softmax's."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 41, prev, new, 2, 64, 64)
+    q = torch.randn(T, 8, 64, generator=g)
+    q[0, 1, 3], q[T - 1, 5, 9] = math.nan, math.inf
+    q = q.to(torch.bfloat16)
+    c = kv8.Cache8(data.to(DEV), exps.to(DEV))
+    got = kv8.attend(c, q.to(DEV), bt.to(DEV), lens.to(DEV), qsl.to(DEV)).cpu().double()
+    clean = q.clone()
+    clean[0, 1], clean[T - 1, 5] = 0, 0
+    want, far = ref.attend(data, exps, clean, bt, lens, qsl)
+    rest = torch.ones(T, 8, dtype=torch.bool)
+    rest[0, 1] = rest[T - 1, 5] = False
+    assert got[0, 1].isnan().all() and got[T - 1, 5].isnan().all()
+    assert float(((got - want).abs() / far)[rest].max()) <= 1.0
+    # keys of one value, so that all scores of a query are equal: about -2^114, the mean of what it sees
+    data[:, :, :, 0] = 0x38
+    exps[..., 0] = 247
+    q = torch.full((T, 8, 64), -2.0 ** -9)
+    check_attend(kv8, data, exps, q.to(torch.bfloat16), bt, lens, qsl, scale=2.0 ** -3)
+
+
+def test_lengths_and_tables_at_their_ends(kv8):
+    """Lengths past the table and before its first position, a table without columns, rows without tokens, no rows, no tokens."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 12, [100, 64, 30, 10], [3, 70, 0, 2], 2, 128, 64, pad=1)
+    lens = torch.tensor([400, 150, -7, 1])
+    x = torch.randn(T, 4, 128, generator=g).to(torch.bfloat16)
+    q = torch.randn(T, 8, 128, generator=g).to(torch.bfloat16)
+    want = ref.append(data, exps, x[:, :2], x[:, 2:], bt, lens, qsl)
+    c = kv8.Cache8(data.to(DEV), exps.to(DEV))
+    up = lambda *a: [t.to(DEV) for t in a]
+    kv8.append(c, *up(x[:, :2], x[:, 2:], bt, lens, qsl))
+    assert torch.equal(c.exps.cpu(), want[1]) and same(c.data.cpu(), want[0])
+    check_attend(kv8, *want, q, bt, lens, qsl)
+    none = torch.empty(4, 0, dtype=torch.int32)
+    kv8.append(c, *up(x[:, :2], x[:, 2:], none, lens, qsl))
+    assert torch.equal(c.exps.cpu(), want[1]) and same(c.data.cpu(), want[0])
+    assert not kv8.attend(c, *up(q, none, lens, qsl)).any()
+    e = torch.zeros(0, dtype=torch.int64)
+    one = torch.zeros(1, dtype=torch.int64)
+    kv8.append(c, *up(x[:0, :2], x[:0, 2:], bt[:0], e, one))
+    assert kv8.attend(c, *up(q[:0], bt[:0], e, one)).shape == (0, 8, 128)
+    assert torch.equal(c.exps.cpu(), want[1]) and same(c.data.cpu(), want[0])
+
+
+def test_views_of_everything(kv8):
+    """Pages apart in a pool, a table and queries that are views, keys that heads share, unaligned values; rows that share pages."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 14, [200, 130, 70], [1, 3, 2], 2, 128, 64)
+    bt[1, 0] = bt[0, 0]                                         # a prefix of 64 tokens in common
+    wide = torch.full((3, 9), -1, dtype=torch.int32)
+    wide[:, 2:2 + bt.shape[1]] = bt
+    P = data.shape[0]
+    pool, epool = torch.zeros(2 * P, *data.shape[1:], dtype=torch.uint8), torch.zeros(3 * P, *exps.shape[1:], dtype=torch.uint8)
+    pool[::2], epool[1::3] = data, exps
+    pd, ed = pool.to(DEV), epool.to(DEV)
+    c = kv8.Cache8(pd[::2], ed[1::3])
+    btd = wide.to(DEV)[:, 2:2 + bt.shape[1]]
+    k1 = torch.randn(T, 1, 128, generator=g).to(torch.bfloat16)
+    vv = torch.randn(T * 2 * 128 + 3, generator=g).to(torch.bfloat16)
+    kd, vd = k1.to(DEV).expand(T, 2, 128), vv.to(DEV)[3:].view(T, 2, 128)
+    kv8.append(c, kd, vd, btd, lens.to(DEV), qsl.to(DEV))
+    want = ref.append(data, exps, k1.expand(T, 2, 128), vv[3:].view(T, 2, 128), bt, lens, qsl)
+    assert torch.equal(ed.cpu()[1::3], want[1]) and same(pd.cpu()[::2], want[0])
+    assert not pd.cpu()[1::2].any() and not ed.cpu()[0::3].any() and not ed.cpu()[2::3].any()
+    q = torch.randn(8, T, 200, generator=g).to(torch.bfloat16)
+    qv = q.to(DEV).transpose(0, 1)[:, :, 5:133]
+    for scale in (None, -0.05):
+        o = kv8.attend(c, qv, btd, lens.to(DEV), qsl.to(DEV), scale=scale).cpu().double()
+        ow, far = ref.attend(*want, q.transpose(0, 1)[:, :, 5:133], bt, lens, qsl, scale=scale)
+        assert float(((o - ow).abs() / far).max()) <= 1.0
+    k, v = kv8.dequantize(c)
+    for got, held in zip((k, v), ref.values(*want)):
+        assert torch.equal(got.cpu().double(), held)
+
+
+def test_offsets_past_32_bits(kv8):
+    """Pages 2 GiB apart: bytes past 2^32 are the ones that a row's pages lie at."""
+    need = 3 * (1 << 31)
+    if torch.cuda.mem_get_info()[0] < need + (1 << 30):
+        pytest.skip("not enough memory")
+    pool = torch.empty(need, dtype=torch.uint8, device=DEV)
+    H, D, U = 2, 64, 1
+    dv = pool.as_strided((3, H, U, 2, 64 * D), (1 << 31, U * 2 * 64 * D, 2 * 64 * D, 64 * D, 1))
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 15, [100, 10], [2, 1], H, D, 64, spare=0)
+    assert data.shape[0] == 3
+    dv.copy_(data.to(DEV))
+    c = kv8.Cache8(dv, exps.to(DEV))
+    x = torch.randn(T, 2 * H, D, generator=g).to(torch.bfloat16)
+    xd = x.to(DEV)
+    kv8.append(c, xd[:, :H], xd[:, H:], bt.to(DEV), lens.to(DEV), qsl.to(DEV))
+    want = ref.append(data, exps, x[:, :H], x[:, H:], bt, lens, qsl)
+    assert torch.equal(c.exps.cpu(), want[1]) and same(dv.cpu(), want[0])
+    q = torch.randn(T, 8, D, generator=g).to(torch.bfloat16)
+    got = kv8.attend(c, q.to(DEV), bt.to(DEV), lens.to(DEV), qsl.to(DEV)).cpu().double()
+    ow, far = ref.attend(*want, q, bt, lens, qsl)
+    assert float(((got - ow).abs() / far).max()) <= 1.0
+    del c, dv, pool
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("prev,new", SHAPES + [([700, 600], [200, 129])], ids=str)
+def test_recorded_and_on_other_streams(kv8, prev, new):
+    """Append and attention recorded into two graphs and replayed in turn on new inputs, with eager work between; the same on two
+    streams at once: equal bits."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 16, prev, new, 2, 128, 64, pad=2)
+    xs = torch.randn(6, T, 4, 128, generator=g).to(torch.bfloat16).to(DEV)
+    qs = torch.randn(6, T, 8, 128, generator=g).to(torch.bfloat16).to(DEV)
+    btd, ld, qd = bt.to(DEV), lens.to(DEV), qsl.to(DEV)
+
+    def fresh():
+        return kv8.Cache8(data.to(DEV), exps.to(DEV))
+
+    def step(c, x, q):
+        kv8.append(c, x[:, :2], x[:, 2:], btd, ld, qd)
+        return kv8.attend(c, q, btd, ld, qd)
+
+    eager = fresh()
+    want = [step(eager, xs[i], qs[i]).clone() for i in range(6)]
+    caches, inputs, graphs, outs = [], [], [], []
+    for n in range(2):
+        c, x, q = fresh(), xs[0].clone(), qs[0].clone()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step(c, x, q)
+        torch.cuda.current_stream().wait_stream(s)
+        c.data.copy_(data)
+        c.exps.copy_(exps)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step(c, x, q)
+        caches.append(c); inputs.append((x, q)); graphs.append(gr); outs.append(out)
+    for i in range(6):
+        for n in range(2):
+            inputs[n][0].copy_(xs[i]); inputs[n][1].copy_(qs[i])
+            graphs[n].replay()
+        kv8.attend(eager, qs[0], btd, ld, qd)
+        torch.cuda.synchronize()
+        for n in range(2):
+            assert torch.equal(outs[n], want[i]), (i, n)
+    # two streams, the cache's work on each in turn with nothing of the other waited for
+    a, b = fresh(), fresh()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = {}
+    for i in range(6):
+        for c, s, key in ((a, sa, "a"), (b, sb, "b")):
+            with torch.cuda.stream(s):
+                got[key, i] = step(c, xs[i], qs[i])
+    torch.cuda.synchronize()
+    for i in range(6):
+        assert torch.equal(got["a", i], want[i]) and torch.equal(got["b", i], want[i])
+
+
+def test_calls_that_are_refused(kv8):
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 17, [10, 3], [1, 2], 2, 64, 64)
+    c = kv8.Cache8(data.to(DEV), exps.to(DEV))
+    k = torch.randn(T, 2, 64).to(torch.bfloat16).to(DEV)
+    q = torch.randn(T, 4, 64).to(torch.bfloat16).to(DEV)
+    btd, ld, qd = bt.to(DEV), lens.to(DEV), qsl.to(DEV)
+    cos = torch.ones(9, 16, dtype=torch.bfloat16, device=DEV)
+    ok = dict(k=k, v=k, bt=btd, lens=ld, qsl=qd, cos_t=None, sin_t=None)
+    ap = lambda **a: kv8.append(c, *{**ok, **a}.values())
+    for a in (dict(k=k.float()), dict(v=k.half()), dict(k=k.cpu()), dict(bt=btd.long()), dict(lens=ld.int()), dict(qsl=qd.int()), dict(bt=bt), dict(lens=lens),
+              dict(k=k[:2]), dict(v=k[:, :1]), dict(k=k[..., :32]), dict(k=k[0]), dict(bt=btd[:1]), dict(bt=btd[0]), dict(lens=ld[:1]), dict(qsl=qd[None]),
+              dict(qsl=qd[:0]), dict(cos_t=cos), dict(cos_t=cos, sin_t=cos[:, :8]), dict(cos_t=cos[:, :12], sin_t=cos[:, :12]), dict(cos_t=cos.float(), sin_t=cos),
+              dict(cos_t=cos[:0], sin_t=cos[:0]), dict(cos_t=cos[0], sin_t=cos[0]), dict(bt=btd.repeat(1, 4)[:, ::2]), dict(bt=btd[:0], lens=ld[:0], qsl=qd[:1])):
+        with pytest.raises((TypeError, ValueError)):
+            ap(**a)
+    at = lambda *a, **kw: kv8.attend(c, *a, **kw)
+    for a, kw in (((q.float(), btd, ld, qd), {}), ((q[:, :3], btd, ld, qd), {}), ((q[..., :32], btd, ld, qd), {}), ((q[0], btd, ld, qd), {}), ((q[:, :0], btd, ld, qd), {}),
+                  ((q.repeat(1, 9, 1), btd, ld, qd), {}), ((q.cpu(), btd, ld, qd), {}), ((q, btd, ld, qd), dict(window=-1)), ((q, btd, ld, qd), dict(scale=0.0)),
+                  ((q, btd, ld, qd), dict(scale=math.nan)), ((q, btd[:0], ld[:0], qd[:1]), {})):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            at(*a, **kw)
+    assert torch.equal(c.data.cpu(), data) and torch.equal(c.exps.cpu(), exps)
+    assert torch.equal(at(q, btd, ld, qd), at(q, btd, ld, qd, window=1 << 70))

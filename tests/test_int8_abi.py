@@ -38,7 +38,7 @@ def test_header_exported_and_bound(lib):
 
 def test_layout_and_quantize_host_checks(lib):
     f = lambda **k: lib.lfm3_hip_int8_layout(*{**dict(w=A, ld=64, s=A, N=10, K=64, gated=0, wsh=A, ssh=A, st=None), **k}.values())
-    for k in (dict(w=None), dict(s=None), dict(wsh=None), dict(wsh=A + 8), dict(ssh=None), dict(N=0), dict(N=(1 << 24) + 2), dict(K=0), dict(K=60), dict(K=65544),
+    for k in (dict(w=None), dict(s=None), dict(wsh=None), dict(wsh=A + 8), dict(ssh=None), dict(N=0), dict(N=(1 << 24) + 2), dict(N=1 << 24), dict(N=(1 << 23) + 2, K=8192), dict(K=0), dict(K=60), dict(K=65544),
               dict(gated=2), dict(gated=1, N=9), dict(ld=-1)):
         refused(lib, f(**k), b"int8_layout")
     g = lambda **k: lib.lfm3_hip_int8_quantize(*{**dict(w=A, ld=64, N=10, K=64, w8=A, s=A, st=None), **k}.values())
@@ -51,7 +51,7 @@ def test_linear8_host_checks(lib, R):
     need = lib.lfm3_hip_linear8_workspace(R, 96, 128, 0)
     assert need == 0 if R == 1 else need >= R * 128 + 4 * R
     f = lambda **k: lib.lfm3_hip_linear8(*{**dict(x=A, ldx=128, w=A, s=A, R=R, N=96, K=128, gated=0, y=A, ldy=96, ws=A, wsb=need, st=None), **k}.values())
-    for k in (dict(x=None), dict(x=A + 8), dict(ldx=132), dict(w=None), dict(w=A + 8), dict(s=None), dict(s=A + 4), dict(R=-1), dict(R=(1 << 24) + 1), dict(N=0), dict(K=0),
+    for k in (dict(x=None), dict(x=A + 8), dict(ldx=132), dict(w=None), dict(w=A + 8), dict(s=None), dict(s=A + 4), dict(R=-1), dict(R=(1 << 24) + 1), dict(R=1 << 24), dict(N=0), dict(K=0),
               dict(K=100), dict(K=65544), dict(gated=2), dict(gated=1, N=95), dict(y=None), dict(ldy=-1)) + ((dict(ws=None), dict(ws=A + 8), dict(wsb=need - 1)) if need else ()):
         refused(lib, f(**k), b"linear8")
     assert f(R=0) == 0

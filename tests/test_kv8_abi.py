@@ -53,7 +53,7 @@ def test_append_host_checks(lib):
     for k in BAD:
         refused(lib, f(desc(**k)), b"descriptor")
     for k in (dict(k=None), dict(v=None), dict(bt=None), dict(lens=None), dict(qsl=None), dict(k=A + 2), dict(kt=516), dict(vh=4), dict(R=-1), dict(T=-1),
-              dict(bc=-1), dict(cos=A), dict(cos=A, sin=A, rr=0, F=32), dict(cos=A, sin=A, rr=9, F=12), dict(cos=A, sin=A, rr=9, F=72)):
+              dict(bc=-1), dict(cos=A), dict(cos=A, sin=A, rr=0, F=32), dict(cos=A, sin=A, rr=9, F=12), dict(cos=A, sin=A, rr=9, F=72), dict(R=1 << 30), dict(T=1 << 30), dict(R=1 << 23, T=1 << 27), dict(R=(1 << 63) - 1), dict(T=(1 << 63) - 1)):
         refused(lib, f(**k), b"kv8_append")
     for k in (dict(R=0), dict(T=0), dict(bc=0)):
         assert f(**k) == 0
@@ -74,8 +74,11 @@ def test_attend_host_checks(lib):
     for k in BAD:
         refused(lib, f(desc(**k)), b"descriptor")
     for k in (dict(q=None), dict(out=None), dict(bt=None), dict(lens=None), dict(qsl=None), dict(q=A + 8), dict(out=A + 8), dict(heads=0), dict(heads=6), dict(heads=68),
-              dict(R=0), dict(R=-1), dict(T=-1), dict(win=-1), dict(scale=0.0), dict(scale=float('inf')), dict(scale=float('nan')), dict(bc=1 << 24), dict(ws=None), dict(ws=A + 8), dict(wsb=need - 1)):
+              dict(R=0), dict(R=-1), dict(T=-1), dict(win=-1), dict(scale=0.0), dict(scale=float('inf')), dict(scale=float('nan')), dict(bc=1 << 24), dict(ws=None), dict(ws=A + 8), dict(wsb=need - 1),
+              dict(R=1 << 22, T=1 << 22, bc=8), dict(R=1 << 40), dict(T=1 << 40)):
         refused(lib, f(**k), b"kv8_attend")
+    for win in (1 << 40, 1 << 62, (1 << 63) - 1):          # past every position: as without a window
+        assert lib.kv8_hip_attend_workspace(desc(), 16, 2, 5, 64, win) == need
     assert f(T=0) == 0
     for k in (dict(heads=0), dict(heads=6), dict(heads=68), dict(R=0), dict(T=0)):
         a = {**dict(heads=16, R=2, T=5, bc=64, win=0), **k}
