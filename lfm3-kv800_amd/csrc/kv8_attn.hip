@@ -157,7 +157,7 @@ __device__ __forceinline__ void clear_padding(const Attend& A) {
 template <int D>
 constexpr int PART = D + 4;
 
-// LIST: one workgroup takes entries [w W / NG, (w + 1) W / NG) of the W of the list (row, query tile, head, step); else workgroup w is one
+// LIST: one workgroup takes its share of the W entries of the list (row, query tile, head, step); else workgroup w is one
 // (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one token. The four waves take every fourth step of an item, each with its
 // own maximum, sum and output, and are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
 template <int D, bool LIST, int NB, int NC>
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
 
   clear_padding<D>(A);
 
-  int64_t x = 0, end = 1, before = 0, W = 0, NG = 1;
+  int64_t x = 0, end = 1, before = 0, W = 0, NG = 1, share = 1;
   int r, tile0 = 0;
   Row row;
   if constexpr (LIST) {
@@ -192,10 +192,13 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
       W = L.pre[256];
     }
     W = same(W);
-    NG = min((int64_t)gridDim.x, W);               // no workgroup between two others is without entries
-    if (w >= NG) return;
-    x = w * W / NG;
-    end = (w + 1) * W / NG;
+    // Up to 4 entries each, which run at once: as many for each, so that most items begin with a workgroup (1 x 16384, 4 tokens: 17.2 us,
+    // 20.8 in proportion); else in proportion, no two differing by more than one (16 x 4096, 8 tokens: 25.4, 29.2 with as many for each).
+    NG = min((int64_t)gridDim.x, W);
+    share = W <= 4 * (int64_t)gridDim.x ? (W + gridDim.x - 1) / gridDim.x : 0;
+    x = share ? w * share : w * W / NG;
+    if (w >= NG || x >= W) return;                 // no workgroup between two others is without entries
+    end = share ? min(x + share, W) : (w + 1) * W / NG;
     if (A.R <= 64) {
       r = __popcll(__ballot(incl <= x));
       before = r ? __shfl(incl, r - 1) : 0;
@@ -461,9 +464,9 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) pt[d0 + e] = acc[e];
         if (d0 == 0) { pt[D] = m; pt[D + 1] = ls; }
-        // the item's last entry: the least w' with (w' + 1) W / NG at or behind its end
+        // the item's last workgroup; in proportion: the least w' with (w' + 1) W / NG at or behind its end
         if (s0 == 0 && tid == 0 && n == 0)
-          A.desc[w] = {(int)row.q0 + tile * A.TQ, min(A.TQ, row.c - tile * A.TQ), h, (int)(((at + row.steps) * NG + W - 1) / W - 1)};
+          A.desc[w] = {(int)row.q0 + tile * A.TQ, min(A.TQ, row.c - tile * A.TQ), h, (int)(share ? (at + row.steps - 1) / share : ((at + row.steps) * NG + W - 1) / W - 1)};
       }
     }
     if constexpr (!LIST) return;
@@ -473,32 +476,53 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
 }
 
 // ---------------------------------------------------------------- joining parts
-// A wave joins `count` parts, in order: the maxima side by side, then D / 64 channels a lane. Writes the column's output.
+// A wave joins `count` parts, 64 at a time: their maxima and factors side by side, then two parts a load, D / 32 channels a lane, 16
+// parts on their way while the maxima are. The sums' order is that of the parts. Writes the column's output. (A part a load, 4 on
+// their way: 1 x 65536 positions, 128 parts an item, 35.7 us the whole call, 27.0 so.)
 template <int D, typename Slot>
 __device__ __forceinline__ void join(int count, Slot slot, uint16_t* __restrict__ out) {
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int k = lane; k < count; k += 64) m = fmaxf(m, slot(k)[D]);
+  constexpr int C = D / 32, AHEAD = 8;
+  typedef float fc __attribute__((ext_vector_type(C)));
+  const int lane = threadIdx.x & 63, half = lane >> 5, li = lane & 31;
+  fc acc = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int k0 = 0; k0 < count; k0 += 64) {
+    const int n = min(64, count - k0);
+    fc v[AHEAD];
+    auto load = [&](int j) {                       // behind the last part: that one again, times 0
 #pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if (m == -INFINITY) m = 0.f;                     // no part has keys: all sums are 0
-  float a0 = 0.f, a1 = 0.f, l = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < count; ++k) {
-    const float* s = slot(k);
-    const float f = __builtin_amdgcn_exp2f(s[D] - m);
-    l += f * s[D + 1];
-    if (D == 128) {
-      const float2 v = *reinterpret_cast<const float2*>(s + 2 * lane);
-      a0 += f * v.x;
-      a1 += f * v.y;
-    } else {
-      a0 += f * s[lane];
+      for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const fc*>(slot(k0 + min(j + 2 * i + half, n - 1)) + C * li);
+    };
+    const float2 ml = *reinterpret_cast<const float2*>(slot(k0 + min(lane, n - 1)) + D);
+    load(0);
+    float top = ml.x;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    top = fmaxf(m, top);
+    const float M0 = top > -INFINITY ? top : 0.f;  // no part has keys: all sums are 0
+    const float f = lane < n ? __builtin_amdgcn_exp2f(ml.x - M0) : 0.f, old = __builtin_amdgcn_exp2f(m - M0);
+    m = top;
+    l = l * old + f * ml.y;
+    acc *= old;
+    for (int j = 0;;) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) acc += __shfl(f, j + 2 * i + half) * v[i];
+      j += 2 * AHEAD;
+      if (j >= n) break;
+      load(j);
     }
   }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+#pragma unroll
+  for (int c = 0; c < C; ++c) acc[c] += __shfl_xor(acc[c], 32);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (D == 128) reinterpret_cast<uint32_t*>(out)[lane] = kv800::bfpk(a0 * inv, a1 * inv);
-  else out[lane] = (uint16_t)kv800::f2bf(a0 * inv);
+  uint32_t y[C / 2];
+#pragma unroll
+  for (int c = 0; c < C / 2; ++c) y[c] = kv800::bfpk(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+  if (half) return;
+  if (D == 128) reinterpret_cast<uint2*>(out)[li] = make_uint2(y[0], y[C / 2 - 1]);
+  else reinterpret_cast<uint32_t*>(out)[li] = y[0];
 }
 
 // One wave per (workgroup of the list, column): where that workgroup began an item that others finish, its part and theirs.
@@ -507,9 +531,9 @@ __global__ void __launch_bounds__(256) merge_kernel(Attend A) {
   constexpr int COLS = 16 * NC;
   const int64_t w = blockIdx.x;
   const Desc d = A.desc[w];
-  if (d.last < 0) return;
   const int c = blockIdx.y * 4 + (threadIdx.x >> 6), i = c / A.G;
-  if (i >= d.queries) return;
+  asm volatile("" ::"s"(d.token), "s"(d.queries), "s"(d.head));          // all of it in one load
+  if (d.last < 0 || i >= d.queries) return;
   const int Hq = A.C.heads * A.G;
   join<D>(d.last - (int)w + 1, [&](int k) { return A.part + ((2 * (w + k) + (k == 0 ? 1 : 0)) * COLS + c) * PART<D>; },
           A.out + ((int64_t)(d.token + i) * Hq + d.head * A.G + c % A.G) * D);
@@ -815,8 +839,13 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
     p.splits = (int)(s < 1 ? 1 : s);
     if (p.splits > 1) p.bytes = T * heads * p.splits * (c->dim + 4) * 4;
   } else if (p.kind == LISTED) {
-    const int64_t entries = p.tiles * c->kv_heads * ((positions + p.step - 1) / p.step + 1);
-    p.groups = (entries + 3) / 4 < 512 ? (entries + 3) / 4 : 512;
+    // One workgroup a CU, fewer rather than with less than 2 entries; two where all entries then run at once and the items are not so few
+    // that each has many parts. Times, us, with up to 256 / 512: 1 x 65536 22.4 / 27.3, 64 x 4096 57.9 / 61.3, 32 x 32768 190 / 194;
+    // 16 x 2048 18.6 / 17.1, 24 x 2500 23.4 / 19.7; 1 x 32768 18.8 / 22.3. Two also for many items, so that one's joins pass under the
+    // other's steps: 128 x 2048 62.9 / 60.8, 192 rows of up to 32768 186.2 / 183.7.
+    const int64_t entries = p.tiles * c->kv_heads * ((seen + p.step - 1) / p.step + (seen < positions ? 1 : 0));
+    p.groups = entries <= 1024 ? (entries + 1) / 2 : entries < 2048 ? (entries + 3) / 4 : items > 256 ? 512 : 256;
+    if (p.groups > 256 && items < 32) p.groups = 256;
     p.bytes = p.groups * (2 * p.cols * (c->dim + 4) * 4 + (int64_t)sizeof(Desc));
   }
   return p;
