@@ -158,8 +158,12 @@ template <int D>
 constexpr int PART = D + 4;
 
 // LIST: one workgroup takes its share of the W entries of the list (row, query tile, head, step); else workgroup w is one
-// (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one token. The four waves take every fourth step of an item, each with its
-// own maximum, sum and output, and are joined in LDS. Maxima are integers, so that their changes scale by exact powers of two.
+// (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one
+// token. The four waves take every fourth step of an item, each with its own maximum, sum and output, and are joined in LDS. Maxima are
+// integers, so that their changes scale by exact powers of two. Bound: HBM for large batches (32 rows of 32,768 190 us: 5.65 TB/s of
+// the cache), else the chain lengths - table - page - codes - join, 8 us, and the merge.
+// NB, NC: blocks of 64 positions a step, column tiles. A list by steps of 128 positions (1 x 32768 18.5 us, by 64 22.5; 8 x 4096 20.2,
+// 17.8); with 32 columns by 64, for the registers.
 template <int D, bool LIST, int NB, int NC>
 __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Attend A, int per) {
   constexpr int STEP = NB * BLK, COLS = 16 * NC;   // positions of a wave's step; columns of a tile
@@ -564,7 +568,8 @@ __device__ __forceinline__ float halves_max(float x) {
 // one is multiplied, one barrier a block. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 (lane l: row or column l % 32, k = 8 (l / 32) + j;
 // output column l % 32, rows 8 b + 4 (l / 32) + i), so a column's weights and sums stay in its two lanes. Row 8 b + 4 h + i of
 // key tile a is token 32 a + 16 (b / 2) + 8 h + 4 (b % 2) + i: the lane's weights are then those of 8 tokens side by side, half
-// of a piece of the values.
+// of a piece of the values. Two prompts of 8,192 tokens, 16 heads: 560 us, 985 TFLOP/s, bound by the issue of both vector and matrix
+// instructions (48 and 43 % busy), of which two waves a SIMD overlap little.
 template <int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int per, int splits, float* __restrict__ part) {
   constexpr int NT = D / 32, NK = D / 16, NP = 4 * D / (64 * NW);          // dim tiles, k-steps, pieces of K (and V) a thread stages
@@ -826,23 +831,28 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
   const int64_t cols = T * p.G / R, items = R * c->kv_heads;
   // (Sixteen rows of 4,096 positions with 1 to 33 tokens each: 36 us by tiles of 32, 32 as prompts, so 40 is where prompts begin.)
   const bool wide = items * seen >= 1 << 19;
-  p.kind = cols >= 40 ? PROMPT : seen <= 1024 ? DIRECT : LISTED;
+  // A workgroup an item without a list: short rows (1 x 1000 10.5 us, listed 14.9; 256 x 1000 51, 60), and of many rows with a token each
+  // longer ones (40 x 1800 18, 23; 100 x 4000 76, 93; 100 x 8000 145, 164; 32 x 8000 58, 56.5). With more tokens a row some of the items'
+  // numbers are idle workgroups: 128 x 4000 with 2 tokens 106, 102.5.
+  p.kind = cols >= 40 ? PROMPT : seen <= (T <= R && items >= 128 ? 8192 : 1024) ? DIRECT : LISTED;
   p.cols = p.kind == PROMPT ? 32 * NW : p.kind == LISTED && wide && cols > 16 ? 32 : 16;
   p.TQ = p.cols / p.G;
   p.step = p.kind == LISTED && p.cols == 16 ? 2 * BLK : BLK;
   p.tiles = (T + R * (p.TQ - 1)) / p.TQ;
   if (p.kind == PROMPT) {
-    // few tiles: each split over its blocks, down to 8, for two workgroups a CU
-    const int64_t wgs = (mean + p.TQ - 1) / p.TQ * R * c->kv_heads, most = seen / (8 * BLK);
-    int64_t s = wgs > 0 ? 512 / wgs : 1;
+    // Few tiles: each split over its blocks, down to 4, for two workgroups a CU. Times, us, so / unsplit: 64 new tokens of one row of 16,384
+    // 30 / 368, 24 of each of 16 of 4,096 38 / 103; 256 tiles, split in two, 45 / 32 (2 prompts of 1,024). Down to 8 blocks: one row of 2,048
+    // 23.5, 19.4 down to 4.
+    const int64_t wgs = (mean + p.TQ - 1) / p.TQ * R * c->kv_heads, most = seen / (4 * BLK);
+    int64_t s = wgs > 0 && wgs < 256 ? 512 / wgs : 1;
     if (s > most) s = most;
     p.splits = (int)(s < 1 ? 1 : s);
     if (p.splits > 1) p.bytes = T * heads * p.splits * (c->dim + 4) * 4;
   } else if (p.kind == LISTED) {
     // One workgroup a CU, fewer rather than with less than 2 entries; two where all entries then run at once and the items are not so few
-    // that each has many parts. Times, us, with up to 256 / 512: 1 x 65536 22.4 / 27.3, 64 x 4096 57.9 / 61.3, 32 x 32768 190 / 194;
-    // 16 x 2048 18.6 / 17.1, 24 x 2500 23.4 / 19.7; 1 x 32768 18.8 / 22.3. Two also for many items, so that one's joins pass under the
-    // other's steps: 128 x 2048 62.9 / 60.8, 192 rows of up to 32768 186.2 / 183.7.
+    // that each has many parts. Times, us, with up to 256 / 512: 1 x 65536 22.4 / 27.3, 64 x 4096 with 4 tokens 58 / 65, 32 x 32768 190 / 194;
+    // 24 x 2500 23.4 / 19.7; 1 x 32768 18.8 / 22.3. Two also for many items, so that one's joins pass under the
+    // other's steps: 128 x 2048 with 4 tokens 63.8 / 62.0, 192 rows of up to 32768 186.2 / 183.7.
     const int64_t entries = p.tiles * c->kv_heads * ((seen + p.step - 1) / p.step + (seen < positions ? 1 : 0));
     p.groups = entries <= 1024 ? (entries + 1) / 2 : entries < 2048 ? (entries + 3) / 4 : items > 256 ? 512 : 256;
     if (p.groups > 256 && items < 32) p.groups = 256;

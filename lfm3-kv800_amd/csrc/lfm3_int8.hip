@@ -499,6 +499,7 @@ int lfm3_hip_linear8(const uint16_t* x, int64_t ldx, const int8_t* wsh, const fl
   int8_t* xq = (int8_t*)ws;
   float* sx = (float*)(xq + mt * nks * 1024);
   if (!h.fused) {
+    // a wave a row: 8192 x 2048 x 2048 49.4 us, a workgroup a row 56; 1024 x 2048 x 8192 41.7, 40.4
     if (R >= 1024 && K <= 2048)
       hipLaunchKernelGGL((lfm3::quantize_kernel<true, 1>), dim3((unsigned)((R + 3) / 4)), dim3(256), 0, st, x, ldx, R, K, nks, xq, sx);
     else
