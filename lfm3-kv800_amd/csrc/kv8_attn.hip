@@ -45,7 +45,7 @@ struct Attend {
   int64_t T;
   int G, TQ;                          // query heads per KV head, queries per tile of 16 or 32 columns (query, query head)
   int64_t window;
-  int step;                           // positions of a wave's step
+  int shift;                          // log2 of the positions of a wave's step
   float sl2;                          // |scale| log2(e)
   uint32_t flip;                      // sign bits of two bf16 for a negative scale: q changes its sign
   uint16_t* out;
@@ -81,7 +81,7 @@ __device__ __forceinline__ Row row_at(const Attend& A, int r) {
   w.tiles = (w.c + A.TQ - 1) / A.TQ;
   const int64_t lo = A.window > 0 ? max(w.p0 + 1 - A.window, (int64_t)0) : 0;
   w.b0 = min(lo, w.n) / BLK;
-  w.steps = max((int)((w.n - w.b0 * BLK + A.step - 1) / A.step), 1);         // 1 also without keys: the outputs are written
+  w.steps = max((int)((w.n - w.b0 * BLK + (1 << A.shift) - 1) >> A.shift), 1);   // 1 also without keys: the outputs are written
   return w;
 }
 // The same with r and all results in scalar registers.
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
     end = same(end);
     row = uniform_row(A, r);
   } else {
-    const int64_t ti = w / A.C.heads;
+    const int64_t ti = (uint32_t)w / (uint32_t)A.C.heads;
     const auto from = [&](int64_t i) { return (A.qsl[i] + i * (A.TQ - 1)) / A.TQ; };
     r = (int)min(ti, (int64_t)A.R - 1);            // so it is where every row before has one tile
     if (from(r) > ti || (r + 1 < A.R && from(r + 1) <= ti)) r = (int)kv800::last_at(A.R, [&](int64_t i) { return from(i) <= ti; });
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
       h = (int)(item % A.C.heads);
       tile = (int)(item / A.C.heads);
     } else {
-      h = (int)(w % A.C.heads);
-      tile = (int)(w / A.C.heads) - tile0;
+      h = (int)((uint32_t)w % (uint32_t)A.C.heads);
+      tile = (int)((uint32_t)w / (uint32_t)A.C.heads) - tile0;
     }
 
     // ---- the queries of the lane's columns
@@ -280,15 +280,17 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
       bool on[NB];
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
-        const int64_t bp = pos + u * BLK, bi = bp / BLK, col = bi / A.C.blocks;
-        on[u] = bp <= thi && bp + BLK > tlo + 1 && col < A.bt_cols;
+        const int64_t bp = pos + u * BLK;
+        on[u] = bp <= thi && bp + BLK > tlo + 1;                           // then below 2^31, which a division in 64 bits is too long for
+        const uint32_t bi = (uint32_t)(bp / BLK), col = bi / (uint32_t)A.C.blocks;
+        on[u] = on[u] && col < (uint32_t)A.bt_cols;
         int64_t page = 0;
         if (on[u]) {
           page = scalar_load(A.bt + (int64_t)r * A.bt_stride + col);
           on[u] = page >= 0 && page < A.C.pages;
         }
         if (on[u]) {
-          const int ub = (int)(bi % A.C.blocks);
+          const int ub = (int)(bi - col * (uint32_t)A.C.blocks);
           const uint8_t* base = block_of<D>(A.C, page, h, ub);
           const uint32_t ex = exps_load(exps_of(A.C, page, h, ub));
           sc[u][0] = pow2(held_exponent((uint8_t)ex));
@@ -568,7 +570,7 @@ __device__ __forceinline__ float halves_max(float x) {
 // one is multiplied, one barrier a block. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 (lane l: row or column l % 32, k = 8 (l / 32) + j;
 // output column l % 32, rows 8 b + 4 (l / 32) + i), so a column's weights and sums stay in its two lanes. Row 8 b + 4 h + i of
 // key tile a is token 32 a + 16 (b / 2) + 8 h + 4 (b % 2) + i: the lane's weights are then those of 8 tokens side by side, half
-// of a piece of the values. Two prompts of 8,192 tokens, 16 heads: 560 us, 985 TFLOP/s, bound by the issue of both vector and matrix
+// of a piece of the values. Two prompts of 8,192 tokens, 16 heads: 550 us, 1 PFLOP/s, bound by the issue of both vector and matrix
 // instructions (48 and 43 % busy), of which two waves a SIMD overlap little.
 template <int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int per, int splits, float* __restrict__ part) {
@@ -609,7 +611,6 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   const int cc = wv * 32 + cl, iq = i0 + cc / A.G, hq = h * A.G + cc % A.G;
   const bool have = cc < TQ * A.G && iq <= ilast;
   const int64_t qp = row.p0 + iq, qlo = A.window > 0 ? qp - A.window : -1;
-  const bool busy = __any(have);                                          // waves without a column stage only
 
   kv800::u4v qr[NK];
 #pragma unroll
@@ -631,15 +632,20 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   // ---- staging: the codes of block bi into registers, later widened into LDS
   uint4 rk[NP], rv[NP];
   uint32_t re = 0;
-  auto page_of = [&](int bi) {   // as the table has it; looked at a block later, when it has arrived
-    const int col = min(bi / A.C.blocks, A.bt_cols - 1);
-    return scalar_load(A.bt + r * A.bt_stride + col);
+  // Places of blocks are counted on, not divided for: the loop's scalar instructions stand between the wave's products (562 -> 550 us
+  // for two prompts of 8,192).
+  struct Place { int col, u; };  // table column, block of the page
+  auto place = [&](int bi) { return Place{bi / A.C.blocks, bi % A.C.blocks}; };
+  auto onward = [&](Place& x) {
+    if (++x.u == A.C.blocks) { x.u = 0; ++x.col; }
   };
+  const int32_t* table = A.bt + r * A.bt_stride;
+  auto page_of = [&](const Place& x) { return scalar_load(table + min(x.col, A.bt_cols - 1)); };   // looked at a block later, when it has arrived
   auto valid = [&](int page, int bi) { return page >= 0 && page < A.C.pages && bi < b1; };
-  auto load = [&](int bi, int page) {
+  auto load = [&](int bi, int page, int u) {
     if (valid(page, bi)) {
-      const uint8_t* base = block_of<D>(A.C, page, h, bi % A.C.blocks);
-      const uint8_t* ex = exps_of(A.C, page, h, bi % A.C.blocks);
+      const uint8_t* base = block_of<D>(A.C, page, h, u);
+      const uint8_t* ex = exps_of(A.C, page, h, u);
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         rk[j] = *reinterpret_cast<const uint4*>(base + (tid + j * 64 * NW) * 16);
@@ -652,7 +658,8 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
       re = 0;
     }
   };
-  auto is_edge = [&](int bi) { return (int64_t)bi * BLK < alo || (int64_t)bi * BLK + BLK > ahi; };
+  const int in0 = (int)min((max(alo, (int64_t)0) + BLK - 1) / BLK, (int64_t)INT32_MAX), in1 = (int)min(max(ahi, (int64_t)0) / BLK, (int64_t)INT32_MAX);
+  auto is_edge = [&](int bi) { return bi < in0 || bi >= in1; };           // not every query sees all of the block
   auto store = [&](int bi, int buf) {
     if (is_edge(bi)) {      // a weight of 0 does not take out a NaN: NaN values leave the block, and are dealt out afterwards
       bool any = false;
@@ -692,20 +699,23 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   if (tid < 2) flag[tid] = -1;
   int now = 0, next = 0, next2 = 0;               // pages of blocks bi, bi + 1, bi + 2
   if (b0 < b1) {                                   // then the table has columns
-    now = page_of(b0);
-    next = page_of(b0 + 1);
-    next2 = page_of(b0 + 2);
-    load(b0, now);
+    now = page_of(place(b0));
+    next = page_of(place(b0 + 1));
+    next2 = page_of(place(b0 + 2));
+    load(b0, now, place(b0).u);
   }
   __syncthreads();
   if (b0 < b1) {
     store(b0, b0 & 1);
-    load(b0 + 1, next);
+    load(b0 + 1, next, place(b0 + 1).u);
   }
   __syncthreads();
+  Place ahead = place(b0 + 3);
+  int u2 = place(b0 + 2).u;                        // of block bi + 2
   for (int bi = b0; bi < b1; ++bi) {
     const int buf = bi & 1;
-    const int after = page_of(bi + 3);
+    const int after = page_of(ahead), u3 = ahead.u;
+    onward(ahead);
     const bool held = valid(now, bi);
     {
       const uint8_t* kd = lds[buf] + (hf * BLK + cl) * 16;
@@ -719,7 +729,8 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
           s[a] = mfma32(x, qr[k], k == 0 ? zero : s[a]);
         }
       store(bi + 1, buf ^ 1);
-      load(bi + 2, next2);
+      load(bi + 2, next2, u2);
+      u2 = u3;
       const bool edge = !held || is_edge(bi);
       if (edge) {
         // tokens of the block that the lane's query sees: [lo, hi)
@@ -921,7 +932,7 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
   KV800_REQUIRE(p.tiles * cache->kv_heads * p.splits < (1 << 24) - 64, "kv8_attend: too many tokens or rows");   // 2^32 threads a launch
   KV800_REQUIRE(p.bytes == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.bytes), "kv8_attend: %lld bytes of 16-byte aligned workspace needed",
                 (long long)p.bytes);
-  const kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window, p.step,
+  const kv8::Attend A = {kv8::device_form(cache), q, bt, bt_stride, (int)bt_cols, lens, qsl, (int)R, T, p.G, p.TQ, window, p.step == 2 * kv8::BLK ? 7 : 6,
                          fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, out, nullptr, nullptr};
   return cache->dim == 128 ? kv8::run<128>(A, p, heads, ws, (hipStream_t)stream) : kv8::run<64>(A, p, heads, ws, (hipStream_t)stream);
 }
