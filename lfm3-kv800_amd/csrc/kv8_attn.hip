@@ -160,7 +160,7 @@ constexpr int PART = D + 4;
 // LIST: one workgroup takes its share of the W entries of the list (row, query tile, head, step); else workgroup w is one
 // (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one
 // token. The four waves take every fourth step of an item, each with its own maximum, sum and output, and are joined in LDS. Maxima are
-// integers, so that their changes scale by exact powers of two. Bound: HBM for large batches (32 rows of 32,768 190 us: 5.65 TB/s of
+// integers, so that their changes scale by exact powers of two. Bound: HBM for large batches (32 rows of 32,768 188 us: 5.7 TB/s of
 // the cache), else the chain lengths - table - page - codes - join, 8 us, and the merge.
 // NB, NC: blocks of 64 positions a step, column tiles. A list by steps of 128 positions (1 x 32768 18.5 us, by 64 22.5; 8 x 4096 20.2,
 // 17.8); with 32 columns by 64, for the registers.
