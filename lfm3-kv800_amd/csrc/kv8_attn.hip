@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
       W = L.pre[256];
     }
     W = same(W);
+    if (W == 0) return;                            // no row has tokens
     // Up to 4 entries each, which run at once: as many for each, so that most items begin with a workgroup (1 x 16384, 4 tokens: 17.2 us,
     // 20.8 in proportion); else in proportion, no two differing by more than one (16 x 4096, 8 tokens: 25.4, 29.2 with as many for each).
     NG = min((int64_t)gridDim.x, W);
@@ -571,7 +572,7 @@ __device__ __forceinline__ float halves_max(float x) {
 // output column l % 32, rows 8 b + 4 (l / 32) + i), so a column's weights and sums stay in its two lanes. Row 8 b + 4 h + i of
 // key tile a is token 32 a + 16 (b / 2) + 8 h + 4 (b % 2) + i: the lane's weights are then those of 8 tokens side by side, half
 // of a piece of the values. Two prompts of 8,192 tokens, 16 heads: 550 us, 1 PFLOP/s, bound by the issue of both vector and matrix
-// instructions (48 and 43 % busy), of which two waves a SIMD overlap little.
+// instructions (50 and 46 % busy), of which two waves a SIMD overlap little.
 template <int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int per, int splits, float* __restrict__ part) {
   constexpr int NT = D / 32, NK = D / 16, NP = 4 * D / (64 * NW);          // dim tiles, k-steps, pieces of K (and V) a thread stages
@@ -828,6 +829,11 @@ struct Plan {
   int64_t bytes;                      // workspace
 };
 constexpr int NW = 4;                 // waves of the prompt kernel
+// Sizes whose sums and products stay in 64 bits below.
+bool fits(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_cols) {
+  return R <= INT32_MAX / 512 && T <= INT32_MAX / 512 && R * c->kv_heads < (1 << 24) && T * heads < (int64_t)1 << 32 &&
+         bt_cols <= INT32_MAX / (c->blocks * BLK);
+}
 Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
   Plan p;
   p.G = (int)(heads / c->kv_heads);
@@ -909,7 +915,9 @@ int run(const Attend& A0, const Plan& p, int64_t heads, void* ws, hipStream_t s)
 extern "C" {
 
 int64_t kv8_hip_attend_workspace(const kv8_cache_t* cache, int64_t heads, int64_t R, int64_t T, int64_t bt_cols, int64_t window) {
-  if (!kv8::valid(cache) || heads <= 0 || heads % cache->kv_heads || heads / cache->kv_heads > kv8::GROUP || R <= 0 || T <= 0) return 0;
+  if (!kv8::valid(cache) || heads <= 0 || heads % cache->kv_heads || heads / cache->kv_heads > kv8::GROUP || R <= 0 || T <= 0 || bt_cols < 0 ||
+      window < 0 || !kv8::fits(cache, heads, R, T, bt_cols))
+    return 0;
   return kv8::plan(cache, heads, R, T, bt_cols, window >= (int64_t)1 << 40 ? 0 : window).bytes;
 }
 
@@ -922,7 +930,7 @@ int kv8_hip_attend(const kv8_cache_t* cache, const uint16_t* q, int64_t heads, c
                 "kv8_attend: heads must be a multiple of the cache's, up to 16 times");
   KV800_REQUIRE(fabsf(scale) > 0.f && fabsf(scale) < INFINITY, "kv8_attend: scale must be finite and not 0");
   KV800_REQUIRE(bt_cols <= INT32_MAX / (cache->blocks * kv8::BLK), "kv8_attend: the table covers 2^31 positions or more");
-  KV800_REQUIRE(R <= INT32_MAX / 512 && T <= INT32_MAX / 512, "kv8_attend: too many tokens or rows");
+  KV800_REQUIRE(kv8::fits(cache, heads, R, T, bt_cols), "kv8_attend: too many tokens or rows");
   if (T == 0) return KV800_OK;
   if (window >= (int64_t)1 << 40) window = 0;      // more than any row has; sums with positions stay in 64 bits
   KV800_REQUIRE(R > 0, "kv8_attend: tokens without rows");

@@ -427,3 +427,14 @@ def test_calls_that_are_refused(kv8):
             at(*a, **kw)
     assert torch.equal(c.data.cpu(), data) and torch.equal(c.exps.cpu(), exps)
     assert torch.equal(at(q, btd, ld, qd), at(q, btd, ld, qd, window=1 << 70))
+
+
+@pytest.mark.parametrize("pad,prev", [(3, [700, 64]), (3, [3000, 64]), (200, [3000, 64]), (3, [100] * 70 + [1500])], ids=["direct", "list", "prompt", "rows"])
+def test_steps_of_padding(kv8, pad, prev):
+    """Rows that all bring nothing, in room for some tokens: zeros, and the cache stays."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 23, prev, [0] * len(prev), 2, 64, 64, pad=pad)
+    c = kv8.Cache8(data.to(DEV), exps.to(DEV))
+    x = torch.randn(T, 4, 64, generator=g).to(torch.bfloat16).to(DEV)
+    kv8.append(c, x[:, :2], x[:, 2:], bt.to(DEV), lens.to(DEV), qsl.to(DEV))
+    assert torch.equal(c.data.cpu(), data) and torch.equal(c.exps.cpu(), exps)
+    assert not kv8.attend(c, x, bt.to(DEV), lens.to(DEV), qsl.to(DEV)).any()

@@ -80,7 +80,8 @@ def test_attend_host_checks(lib):
     for win in (1 << 40, 1 << 62, (1 << 63) - 1):          # past every position: as without a window
         assert lib.kv8_hip_attend_workspace(desc(), 16, 2, 5, 64, win) == need
     assert f(T=0) == 0
-    for k in (dict(heads=0), dict(heads=6), dict(heads=68), dict(R=0), dict(T=0)):
+    for k in (dict(heads=0), dict(heads=6), dict(heads=68), dict(R=0), dict(T=0), dict(R=1 << 62), dict(T=1 << 62), dict(bc=1 << 62), dict(bc=-1), dict(win=-1),
+              dict(heads=64, T=1 << 27)):
         a = {**dict(heads=16, R=2, T=5, bc=64, win=0), **k}
         assert lib.kv8_hip_attend_workspace(desc(), *a.values()) == 0
 
