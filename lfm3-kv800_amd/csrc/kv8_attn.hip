@@ -74,9 +74,9 @@ struct Row {
 __device__ __forceinline__ Row row_at(const Attend& A, int r) {
   Row w;
   w.q0 = max(A.qsl[r], (int64_t)0);
-  const int64_t c = min(A.qsl[r + 1], A.T) - w.q0, n = A.lens[r];
-  w.c = (int)max(c, (int64_t)0);
-  w.p0 = n - w.c;
+  const int64_t q1 = A.qsl[r + 1], n = A.lens[r];
+  w.c = (int)max(min(q1, A.T) - w.q0, (int64_t)0);
+  w.p0 = n - max(q1 - w.q0, (int64_t)0);   // of tokens past T too, which are not there
   w.n = max(min(n, (int64_t)A.bt_cols * A.C.blocks * BLK), (int64_t)0);
   w.tiles = (w.c + A.TQ - 1) / A.TQ;
   const int64_t lo = A.window > 0 ? max(w.p0 + 1 - A.window, (int64_t)0) : 0;

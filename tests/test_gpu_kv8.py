@@ -438,3 +438,18 @@ def test_steps_of_padding(kv8, pad, prev):
     kv8.append(c, x[:, :2], x[:, 2:], bt.to(DEV), lens.to(DEV), qsl.to(DEV))
     assert torch.equal(c.data.cpu(), data) and torch.equal(c.exps.cpu(), exps)
     assert not kv8.attend(c, x, bt.to(DEV), lens.to(DEV), qsl.to(DEV)).any()
+
+
+@pytest.mark.parametrize("prev,new", SHAPES + [([60, 700], [20, 30])], ids=str)
+def test_rows_past_the_tokens(kv8, prev, new):
+    """Starts of rows past the tokens that are there: the present ones stand where the lengths put them."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 29, prev, new, 2, 64, 64)
+    T -= 1
+    x = torch.randn(T, 4, 64, generator=g).to(torch.bfloat16)
+    q = torch.randn(T, 8, 64, generator=g).to(torch.bfloat16)
+    want = ref.append(data, exps, x[:, :2], x[:, 2:], bt, lens, qsl)
+    c = kv8.Cache8(data.to(DEV), exps.to(DEV))
+    xd = x.to(DEV)
+    kv8.append(c, xd[:, :2], xd[:, 2:], bt.to(DEV), lens.to(DEV), qsl.to(DEV))
+    assert torch.equal(c.exps.cpu(), want[1]) and same(c.data.cpu(), want[0])
+    check_attend(kv8, *want, q, bt, lens, qsl)
