@@ -310,7 +310,7 @@ def _attend(s):
 def _linear(s):
     x = s["x"].float()
     top = x.abs().amax(-1, keepdim=True).clamp(min=2.0 ** -100)
-    y = (x * (torch.full_like(top, 127) / top)).round() @ s["w"].float().T.contiguous()
+    y = (x * (127 / top)).round() @ s["w"].float().T.contiguous()
     y = y * (top / 127) * s["sw"]
     if s["case"]["gated"]:
         g, u = y.chunk(2, 1)
