@@ -44,6 +44,8 @@ def quantize_rows(w):
     """(codes (N, K) int8, scale (N,) fp32) of a bf16 matrix: scale = max(max |w|, 2^-100) / 127 of a row, codes round(w / scale)
     (lfm3_hip_int8_quantize)."""
     L = _lib()
+    if w.device.type != "cuda":
+        raise ValueError(f"w must be on a GPU, got {w.device}")
     _need(w, "w", torch.bfloat16, w.device)
     if w.dim() != 2 or not w.shape[0] or not w.shape[1] or w.shape[1] % 8 or w.shape[1] > 65536:
         raise ValueError(f"w must be (N, K) with K a multiple of 8 up to 65536, got {tuple(w.shape)}")
@@ -68,11 +70,11 @@ class Weight8:
         self.gated = bool(gated)
         if self.gated and w.shape[0] % 2:
             raise ValueError(f"a gated weight has an even number of rows, got {w.shape[0]}")
-        if scale is None:
-            w, scale = quantize_rows(w)
         dev = w.device
         if dev.type != "cuda":
             raise ValueError(f"w must be on a GPU, got {dev}")
+        if scale is None:
+            w, scale = quantize_rows(w)
         _need(w, "w", torch.int8, dev); _need(scale, "scale", torch.float32, dev)
         N, K = self.n, self.k = w.shape
         if scale.shape != (N,):

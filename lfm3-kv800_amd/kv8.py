@@ -82,6 +82,13 @@ class Cache8:
                    torch.full((pages, heads, bs // BLK, 2), 127, dtype=torch.uint8, device=device))
 
 
+def _dev(cache):
+    """The cache's GPU. (A cache of host tensors may be described, not worked on.)"""
+    if cache.dev.type != "cuda":
+        raise ValueError(f"the cache must be on a GPU, got {cache.dev}")
+    return cache.dev
+
+
 def _step(cache, T, bt, lens, qsl):
     dev, i64 = cache.dev, torch.int64
     if not (bt.dtype is torch.int32 and lens.dtype is i64 and qsl.dtype is i64 and bt.device == dev and lens.device == dev and qsl.device == dev):
@@ -122,10 +129,10 @@ def append(cache, k, v, bt, lens, qsl, cos_t=None, sin_t=None):
     tokens whose position the table has no page for are dropped. A block's exponent never falls while the row's earlier tokens are
     in it: a larger token has their codes rounded again."""
     L = _lib()
+    dev = _dev(cache)
     if k.dim() != 3:
         raise ValueError(f"k must be (T, heads, D), got {tuple(k.shape)}")
     T = k.shape[0]
-    dev = cache.dev
     R, lens, qsl = _step(cache, T, bt, lens, qsl)
     k, kt, kh = _kv(k, "k", cache, T)
     v, vt, vh = _kv(v, "v", cache, T)
@@ -151,7 +158,7 @@ def append(cache, k, v, bt, lens, qsl, cos_t=None, sin_t=None):
 def dequantize(cache):
     """(k, v) (pages, kv heads, page tokens, D) bf16: what the cache stands for (kv8_hip_dequantize)."""
     L = _lib()
-    dev = cache.dev
+    dev = _dev(cache)
     k, v = torch.empty(2, cache.pages, cache.heads, cache.bs, cache.dim, dtype=torch.bfloat16, device=dev).unbind(0)
     with _on(dev):
         kv800_hip._check(L.kv8_hip_dequantize(cache._p, k.data_ptr(), v.data_ptr(), _raw_stream(dev)))
@@ -164,11 +171,11 @@ def attend(cache, q, bt, lens, qsl, window=0, scale=None):
     window, the last `window` of them. scale: 1 / sqrt(D) if None. Returns (T, heads, D) bf16; zeros for queries without keys and
     for the padding."""
     L = _lib()
-    _need(q, "q", torch.bfloat16, cache.dev)
+    dev = _dev(cache)
+    _need(q, "q", torch.bfloat16, dev)
     if q.dim() != 3 or q.shape[2] != cache.dim or not q.shape[1] or q.shape[1] % cache.heads or q.shape[1] > 16 * cache.heads:
         raise ValueError(f"q must be (T, heads, {cache.dim}) with heads a multiple of {cache.heads} up to {16 * cache.heads}, got {tuple(q.shape)}")
     T, heads = q.shape[:2]
-    dev = cache.dev
     R, lens, qsl = _step(cache, T, bt, lens, qsl)
     window = min(int(window), 1 << 40)
     if window < 0:

@@ -142,8 +142,13 @@ def _ptr(t):
 
 
 def _raw_stream(dev):
-    """The current stream of dev as an integer (without the Stream object that torch.cuda.current_stream makes, 2 us)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
+    """The current stream of dev as an integer (without the Stream object that torch.cuda.current_stream makes, 2 us). Every launch
+    asks for it, so that none gets the pointers of a host tensor, whose device has no index."""
+    if dev.index is not None:
+        return torch._C._cuda_getCurrentRawStream(dev.index)
+    if dev.type != "cuda":
+        raise ValueError(f"the tensors must be on a GPU, got {dev}")
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _stream(dev):
