@@ -365,8 +365,15 @@ class PagedAttention8:
                 cos, sin = self.tables[FULL] if t == FULL else (None, None)
                 kv8.append(self.layers[l], K, V, self.bt[t], n, qsl, cos, sin)
 
+    def provide(self, steps):
+        """Whether the caches hold `steps` more positions of every row; a ValueError if not."""
+        if int(self.lens.max()) + int(steps) > self.nmax:
+            raise ValueError(f"the caches hold {self.nmax} positions per row, the steps reach {int(self.lens.max()) + int(steps)}")
+
     def freeze(self, steps):
-        """Make the next `steps` decode steps replayable from one recorded step: the lengths then advance on the device."""
+        """Make the next `steps` decode steps replayable from one recorded step: the lengths then advance on the device, where nothing
+        looks at the caches' room, so that it is looked at here."""
+        self.provide(steps)
         self.lens_dev = self.lens.to(self.dev)
 
     def thaw(self):
@@ -375,8 +382,8 @@ class PagedAttention8:
 
     def begin_step(self):
         """Metadata of the next decode step (every row appends one token): the new tokens' positions (R,) int64."""
-        if int(self.lens.max()) >= self.nmax:
-            raise ValueError(f"the caches hold {self.nmax} positions per row")
+        if not (self.one.is_cuda and torch.cuda.is_current_stream_capturing()):   # recording a step takes no position
+            self.provide(1)
         self.lens += 1
         if self.lens_dev is None:
             lens = vc.step_lens(self.lens, self.dev)
@@ -414,6 +421,8 @@ class DecodeGraph:
 
     def __init__(self, model, attention, tokens, steps):
         self.attn, self.left = attention, int(steps)
+        if isinstance(attention, PagedAttention8):
+            attention.provide(1 + self.left)
         self.stream = torch.cuda.Stream(device=tokens.device)
         self.stream.wait_stream(torch.cuda.current_stream(tokens.device))
         with torch.cuda.stream(self.stream):
