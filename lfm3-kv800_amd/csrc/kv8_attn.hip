@@ -759,6 +759,22 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
 #pragma unroll
         for (int d = 0; d < NT; ++d) o[d] *= alpha;
       }
+      // A weight is 2^(s sl2 - m) in one instruction, whose product is not rounded, while m is a rounded one: their difference, up to half
+      // a step of m, is the same for all of the column's weights and goes out in o / l, but from scores of 2^31 on it passes what
+      // exponents reach. Large scores go by the rounded products.
+      float by = A.sl2, from = m;
+      if (__any(fabsf(m) >= 0x1p20f && fabsf(m) < FLT_MAX)) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float x = s[a][v] * A.sl2;
+            s[a][v] = x - m;
+          }
+        by = 1.f;
+        from = 0.f;
+      }
       const uint8_t* vd = lds[buf] + KB + (hf * D + cl) * 16;
       float sum = 0.f;
 #pragma unroll
@@ -766,7 +782,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], A.sl2, -m));
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], by, -from));
           sum += p[e];
         }
         const kv800::u4v pw = {kv800::bfpk(p[0], p[1]), kv800::bfpk(p[2], p[3]), kv800::bfpk(p[4], p[5]), kv800::bfpk(p[6], p[7])};
