@@ -10,7 +10,9 @@
 // in log2 units; parts of a row join by the same rule. All of m, l and o are fp32.
 //
 // Both products run on the bf16 matrix instruction: a code times its power of two is exact in bf16, two codes an instruction, so
-// that scores are those of the held keys in fp32 and a weight is rounded to 8 bits once. The fp8 instructions with block scales
+// that scores are those of the held keys in fp32 and a weight is rounded to 8 bits once, in the product and in l alike (count below).
+// Error against 64 bits 0.00173 on 1 x 16384, 0.00175 with a window of 256, where a 32-bit form rounded to bf16 has 0.00172 and 0.00167
+// (l of weights not rounded and whole maxima: 0.0024, 0.0024). The fp8 instructions with block scales
 // would take the codes as they are, but drop products below about 2^-13 of the largest one of a sum: next to a strong channel,
 // scores of 300 were 0.02 off.
 // Operands of 16 x 16 x 32 (lane l: row or column l % 16, g = l / 16): k = 8 g + j. Output: column l % 16, rows 4 g + i. Scores are
@@ -28,7 +30,8 @@ namespace {
 using kv800::f4;
 
 constexpr int GROUP = 16;             // query heads a KV head may have
-constexpr float LAZY = 8.f;           // log2 units by which a running maximum may lag over a long list of keys
+constexpr float LAZY = 8.f;           // log2 units by which a prompt's running maximum may lag: the top weight is then rounded, too (2
+                                      // prompts of 1,500: error 0.00184, 0.00176 without a lag; of 8,192: 558 us, 568)
 
 struct Desc {                         // of a workgroup whose last item others finish: where that item's outputs go
   int token, queries, head, last;     // first token, its queries, KV head, last workgroup; last -1: none
@@ -145,6 +148,13 @@ __device__ __forceinline__ kv800::b8 wide8(uint32_t a, uint32_t b, float f) {
   return kv800::b8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
 }
 
+// sum + the two rounded weights of w: what the values are multiplied by is what the sum counts, so that equal values come back as they
+// are and a dominant weight's rounding cancels
+__device__ __forceinline__ float count(uint32_t w, float sum) {
+  const kv800::bf2 ones = {(__bf16)1.f, (__bf16)1.f};
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(kv800::bf2, w), ones, sum, false);
+}
+
 // Zeros for the tokens behind the last row's, by all workgroups.
 template <int D>
 __device__ __forceinline__ void clear_padding(const Attend& A) {
@@ -159,8 +169,8 @@ constexpr int PART = D + 4;
 
 // LIST: one workgroup takes its share of the W entries of the list (row, query tile, head, step); else workgroup w is one
 // (query tile, head), found by the tiles' numbers: row r's begin at (qsl[r] + r (TQ - 1)) / TQ, which leaves none out for rows of one
-// token. The four waves take every fourth step of an item, each with its own maximum, sum and output, and are joined in LDS. Maxima are
-// integers, so that their changes scale by exact powers of two. Bound: HBM for large batches (32 rows of 32,768 188 us: 5.7 TB/s of
+// token. The four waves take every fourth step of an item, each with its own maximum, sum and output, and are joined in LDS.
+// Bound: HBM for large batches (32 rows of 32,768 188 us: 5.7 TB/s of
 // the cache), else the chain lengths - table - page - codes - join, 8 us, and the merge.
 // NB, NC: blocks of 64 positions a step, column tiles. A list by steps of 128 positions (1 x 32768 18.5 us, by 64 22.5; 8 x 4096 20.2,
 // 17.8); with 32 columns by 64, for the registers.
@@ -351,7 +361,7 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
 #pragma unroll
         for (int j = 1; j < 16 * NB; ++j) mt = fmaxf(mt, s[n][j]);
         mt = kv800::max4rows(mt);
-        const float Mn = fmaxf(M[n], ceilf(mt));
+        const float Mn = fmaxf(M[n], mt);
         if (__any(Mn > M[n])) {
           const float alpha = Mn > M[n] ? __builtin_amdgcn_exp2f(M[n] - Mn) : 1.f;    // M = -inf: 0
           l[n] *= alpha;
@@ -367,8 +377,8 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
 #pragma unroll
         for (int j = 0; j < 8 * NB; ++j) {
           const float p0 = __builtin_amdgcn_exp2f(s[n][2 * j] - M0), p1 = __builtin_amdgcn_exp2f(s[n][2 * j + 1] - M0);
-          sum += p0 + p1;
           pw[n][j] = kv800::bfpk(p0, p1);
+          sum = count(pw[n][j], sum);
         }
         if (__any(sum != sum)) {   // a column whose every key so far is NaN has no maximum, yet its sum counts
           if (kv800::max4rows(sum != sum ? 1.f : 0.f) > 0.f && M[n] == -INFINITY) M[n] = 0.f;
@@ -571,7 +581,7 @@ __device__ __forceinline__ float halves_max(float x) {
 // one is multiplied, one barrier a block. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 (lane l: row or column l % 32, k = 8 (l / 32) + j;
 // output column l % 32, rows 8 b + 4 (l / 32) + i), so a column's weights and sums stay in its two lanes. Row 8 b + 4 h + i of
 // key tile a is token 32 a + 16 (b / 2) + 8 h + 4 (b % 2) + i: the lane's weights are then those of 8 tokens side by side, half
-// of a piece of the values. Two prompts of 8,192 tokens, 16 heads: 550 us, 1 PFLOP/s, bound by the issue of both vector and matrix
+// of a piece of the values. Two prompts of 8,192 tokens, 16 heads: 558 us, 1 PFLOP/s, bound by the issue of both vector and matrix
 // instructions (50 and 46 % busy), of which two waves a SIMD overlap little.
 template <int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int per, int splits, float* __restrict__ part) {
@@ -781,11 +791,10 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
       for (int k = 0; k < 4; ++k) {
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], by, -from));
-          sum += p[e];
-        }
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], by, -from));
         const kv800::u4v pw = {kv800::bfpk(p[0], p[1]), kv800::bfpk(p[2], p[3]), kv800::bfpk(p[4], p[5]), kv800::bfpk(p[6], p[7])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = count(pw[e], sum);
 #pragma unroll
         for (int d = 0; d < NT; ++d) {
           const kv800::u4v x = *reinterpret_cast<const kv800::u4v*>(vd + (2 * k * D + 32 * d) * 16);

@@ -42,3 +42,22 @@ def test_large_scores(kv8, prev, new, byte, x):
     for r in range(len(prev)):
         first = vals[int(bt[r, 0]), :, 0].repeat_interleave(4, 0)
         assert (got[int(qsl[r]):int(qsl[r + 1])] == first).all(), r
+
+
+@pytest.mark.parametrize("window", [0, 1, 130])
+@pytest.mark.parametrize("prev,new", SHAPES + [([0, 63, 64], [1, 1, 1]), ([1500, 700], [70, 64]), ([30], [300])], ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_equal_values_come_back(kv8, prev, new, window, D):
+    """Weights that sum to 1 as they are multiplied: where every key holds the same value, that is the output, to the bit (32-bit sums
+    of up to 2,048 products are within 2^-12, a quarter of the least half step of bf16, 2^-9). A weight that is rounded in the
+    product and not in the sum is off by up to 2^-8 where it dominates."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 61, prev, new, 2, D, 64)
+    value = torch.randint(0x30, 0x48, (D,), generator=g).to(torch.uint8)     # 0.5 .. 3.75
+    data[:, :, :, 1, ref.tables(D)[1].reshape(-1)] = value.repeat(64)
+    exps[..., 1] = 127
+    up = lambda *a: [t.to(DEV) for t in a]
+    for spread in (0.3, 2.0, 8.0):
+        q = (torch.randn(T, 8, D, generator=g) * spread).to(torch.bfloat16)
+        got = kv8.attend(kv8.Cache8(*up(data, exps)), *up(q, bt, lens, qsl), window=window).cpu()
+        wrong = (got.float() != value.view(torch.float8_e4m3fn).float()).float().mean()
+        assert wrong == 0, (spread, float(wrong))
