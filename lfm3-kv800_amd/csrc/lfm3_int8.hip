@@ -141,9 +141,12 @@ __device__ __forceinline__ i4v quantized16(const uint16_t* src, int64_t k, int64
   return __builtin_bit_cast(i4v, codes16(u, inv));
 }
 
-// silu(g) u; the reciprocal is within an ulp, which the rounding to bf16 behind it does not show
+// silu(g) u. With e = 2^(-|g| log2(e) / 2) the sigmoid is 1 / (1 + e^2), of a negative g e^2 / (1 + e^2), whose two factors e go in one
+// by one: their product leaves the normal numbers at g = -87, where g u may yet be large. The reciprocal and the exponential are
+// within an ulp, which the rounding to bf16 behind them does not show.
 __device__ __forceinline__ float gate(float g, float u) {
-  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f)) * u;
+  const float e = __builtin_amdgcn_exp2f(fabsf(g) * -0.7213475204444817f), f = g < 0.f ? e : 1.f;
+  return g * f * u * f * __builtin_amdgcn_rcpf(__builtin_fmaf(e, e, 1.f));
 }
 __device__ __forceinline__ uint32_t bfpk(float a, float b) {   // two floats -> packed bf16 (round to nearest even)
   typedef __bf16 bf2 __attribute__((ext_vector_type(2)));

@@ -1,0 +1,31 @@
+"""Products in 8-bit integers at the ends of the scales' range."""
+import pytest
+import torch
+
+from test_gpu_int8 import DEV, i8, product
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("R", [1, 40, 8200])
+@pytest.mark.parametrize("u", [1.0, -1e20, 1e30])
+def test_gates_far_below_zero(i8, R, u):
+    """silu(g) u where the sigmoid leaves the normal numbers of 32 bits and the result does not: g from -200 to 90, u of any size. One
+    channel of a token meets one of the weight, so that g and u are the rows' scales by 127. (Bound: as test_linear8's.)"""
+    F = 2000
+    x = torch.zeros(R, 8)
+    x[:, 3] = 1.0
+    x = x.to(torch.bfloat16)
+    g = torch.linspace(-200, 90, F)
+    w = torch.zeros(2 * F, 8, dtype=torch.int8)
+    w[:F, 3] = torch.where(g < 0, -127, 127).to(torch.int8)
+    w[F:, 3] = 127 if u > 0 else -127
+    scale = torch.cat((g.abs(), torch.full((F,), abs(u)))) / 127
+    want, far = product(x[:1], w, scale, True)
+    assert (want[0, :1000].abs() > 1e-37).any() or u == 1.0
+    got = i8.linear8(x.to(DEV), i8.Weight8(w.to(DEV), scale.to(DEV), gated=True)).cpu().double()
+    y = 127 * scale.double()
+    near = (2 ** -8 + 2 ** -18 * (1 + y[:F])) * want.abs() + 2.0 ** -126
+    assert torch.equal(got, got[:1].expand(R, F))
+    worst = float(((got[:1] - want).abs() / near).max())
+    assert worst <= 1.0, worst
