@@ -141,6 +141,11 @@ __device__ __forceinline__ i4v quantized16(const uint16_t* src, int64_t k, int64
   return __builtin_bit_cast(i4v, codes16(u, inv));
 }
 
+// A sum by its token's and its row's scale, of which the token's comes last where it is above 1: sum s would leave the range of 32 bits
+// from tokens of about 2^97 on, whatever the row's scale makes of it. {before, after}: one of them is 1.
+__device__ __forceinline__ float2 scales(float s) { return s > 1.f ? make_float2(1.f, s) : make_float2(s, 1.f); }
+__device__ __forceinline__ float scaled(int sum, float2 s, float row) { return (float)sum * s.x * row * s.y; }
+
 // silu(g) u. With e = 2^(-|g| log2(e) / 2) the sigmoid is 1 / (1 + e^2), of a negative g e^2 / (1 + e^2), whose two factors e go in one
 // by one: their product leaves the normal numbers at g = -87, where g u may yet be large. The reciprocal and the exponential are
 // within an ulp, which the rounding to bf16 behind them does not show.
@@ -254,9 +259,10 @@ __global__ void __launch_bounds__(64 * 16 / NT) few_kernel(const uint16_t* __res
     const int q = wv & 3, row = 8 * q + 4 * (lane >> 5);
     const int64_t r = (m0 + b) * 32 + tok;
     if (r >= o.R || wv >= (GATED ? 4 : 4 * NT)) continue;
-    float s;
-    if (FUSED) s = tops[tok] < 0x7F80 ? fmaxf(kv800::bf2f((uint32_t)tops[tok]), LEAST) / 127.f : __uint_as_float(0x7FC00000u);
-    else s = sx[r];
+    float token;
+    if (FUSED) token = tops[tok] < 0x7F80 ? fmaxf(kv800::bf2f((uint32_t)tops[tok]), LEAST) / 127.f : __uint_as_float(0x7FC00000u);
+    else token = sx[r];
+    const float2 s = scales(token);
     auto sums = [&](int a, float (&f)[4]) {
       int4 t = part[0][a][q][lane];
 #pragma unroll
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(64 * 16 / NT) few_kernel(const uint16_t* __res
         t.x += p.x; t.y += p.y; t.z += p.z; t.w += p.w;
       }
       const float4 sc = *reinterpret_cast<const float4*>(ssh + (n0 + a) * 32 + row);
-      f[0] = (float)t.x * s * sc.x; f[1] = (float)t.y * s * sc.y; f[2] = (float)t.z * s * sc.z; f[3] = (float)t.w * s * sc.w;
+      f[0] = scaled(t.x, s, sc.x); f[1] = scaled(t.y, s, sc.y); f[2] = scaled(t.z, s, sc.z); f[3] = scaled(t.w, s, sc.w);
     };
     float f[4];
     if (GATED) {
@@ -378,9 +384,9 @@ __global__ void __launch_bounds__(64 * MANY, 2) many_kernel(const int8_t* __rest
   uint8_t* buf = reinterpret_cast<uint8_t*>(wv < 2 ? A.b : B.b) + (wv & 1) * 64 * ROW;
   static_assert(2 * 64 * ROW <= (int)sizeof(Stage), "two waves' outputs fit a stage");
   const int64_t width = GATED ? o.N / 2 : o.N, t0 = (m0 + 2 * wm) * 32;
-  float s[2];
+  float2 s[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) s[j] = sx[min(t0 + 32 * j + (lane & 31), o.R - 1)];
+  for (int j = 0; j < 2; ++j) s[j] = scales(sx[min(t0 + 32 * j + (lane & 31), o.R - 1)]);
 #pragma unroll
   for (int pass = 0; pass < (GATED ? 1 : 2); ++pass) {
     if (pass) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -397,8 +403,8 @@ __global__ void __launch_bounds__(64 * MANY, 2) many_kernel(const int8_t* __rest
           float f[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            f[e] = (float)acc[i][j][4 * q + e] * s[j] * ka[e];
-            if (GATED) f[e] = gate(f[e], (float)acc[i + (GATED ? 1 : 0)][j][4 * q + e] * s[j] * kb[e]);
+            f[e] = scaled(acc[i][j][4 * q + e], s[j], ka[e]);
+            if (GATED) f[e] = gate(f[e], scaled(acc[i + (GATED ? 1 : 0)][j][4 * q + e], s[j], kb[e]));
           }
           *reinterpret_cast<uint2*>(buf + (32 * j + (lane & 31)) * ROW + (32 * c + row) * 2) = make_uint2(bfpk(f[0], f[1]), bfpk(f[2], f[3]));
         }

@@ -29,3 +29,23 @@ def test_gates_far_below_zero(i8, R, u):
     assert torch.equal(got, got[:1].expand(R, F))
     worst = float(((got[:1] - want).abs() / near).max())
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("R,N,K", [(1, 96, 128), (4, 130, 2048), (40, 96, 264), (300, 514, 640), (1500, 9000, 264)], ids=str)
+@pytest.mark.parametrize("size,row", [(3e38, 1e-37), (1e38, 1e-41), (2.0 ** 100, 2.0 ** -100), (1e3, 1e-3), (2.0 ** -90, 2.0 ** 90), (1e-30, 1e27)])
+def test_scales_far_apart(i8, R, N, K, gated, size, row):
+    """Tokens near the largest bf16 and weights whose scales bring the product back, and the other way: the result is in range, and so
+    is every product on the way to it. (Bounds: as test_linear8's, a third product by a scale of 1 is exact.)"""
+    g = torch.Generator().manual_seed(R + K)
+    x = (torch.rand(R, K, generator=g) * 2 - 1).double() * size
+    x[:, 0] = size
+    x = x.to(torch.bfloat16)
+    assert torch.isfinite(x.float()).all()
+    w = torch.randint(-127, 128, (N, K), generator=g).to(torch.int8)
+    scale = ((torch.rand(N, generator=g) + 0.5).double() * row / 127).float()
+    want, far = product(x, w, scale, gated)
+    got = i8.linear8(x.to(DEV), i8.Weight8(w.to(DEV), scale.to(DEV), gated=gated)).cpu().double()
+    assert torch.isfinite(want.float()).all() and torch.isfinite(got).all()
+    worst = float(((got - want).abs() / far).max())
+    assert worst <= 1.0, worst
