@@ -178,7 +178,7 @@ __device__ __forceinline__ void put4(const Out& o, int64_t r, int64_t n, int64_t
 // Few tokens: one workgroup takes 32 NT rows of the weight x 32 WM tokens, its 16 / NT waves a part of K each, so that every wave has
 // blocks of 1 KB in flight from its first instruction on; their sums meet in LDS, 32 tokens at a time. Output of the instruction
 // (weight rows x tokens): lane l holds token l % 32, rows 8 b + 4 (l / 32) + i.
-// FUSED (up to 32 tokens): the tokens are rounded to 8 bits by every workgroup for itself, while its first weights are on their way.
+// FUSED (one tile of tokens; how() takes it up to 4): the tokens are rounded to 8 bits by every workgroup for itself, while its first weights are on their way.
 template <int NT, int WM, bool GATED, bool FUSED>
 __global__ void __launch_bounds__(64 * 16 / NT) few_kernel(const uint16_t* __restrict__ x, int64_t ldx, const int8_t* __restrict__ xq,
                                                        const float* __restrict__ sx, const int8_t* __restrict__ wsh,
@@ -441,8 +441,12 @@ bool sizes(int64_t R, int64_t N, int64_t K, int gated) {
 // How a product runs: in 256 x 128 tiles, or on few_kernel with nt tiles of the weight and wm of the tokens a workgroup, which rounds
 // the tokens itself or not. Times of whole calls on both sides of each rule, us (tokens x rows of the weight x K):
 //   tiles, from 112 on: 256 x 16384 x 2048 gated (128) 25.7, few 29.7; 512 x 6144 x 2048 (96) 26.9, few 21.2; 1024 x 2048 x 8192 (64) 80, few 40
-//   rounding inside: 1 x 16384 x 2048 gated 11.7, apart 12.9; 4 x 6144 x 2048 9.6, 13.1; 16 x 16384 x 2048 19.2, 12.8; 1 x 2048 x 8192
-//     18.0, 13.1; 4 x 65536 x 2048 47.5, 33.4
+//   rounding inside, one round of workgroups (256) of up to 8 steps of 32 channels a wave, on one tile of the weight up to 256 tiles
+//     and on two up to 512. Weight rows on the border and behind it, 1 / 4 tokens: x 2048, 8192 8.0 / 9.3, apart 12.5 / 12.7; 10240 on
+//     two tiles 8.9 / 11.0, on one 12.7 / 16.0, apart 12.4 / 12.5; 14336 10.6 / 12.1, apart 12.6 / 12.8; 16512 17.9 / 20.3, apart 12.8 / 13.1.
+//     Channels: 6144 on one tile, x 4096 11.3 / 13.4, apart 12.6 / 12.7, x 8192 20.5 / 21.5, apart 15.1 / 15.0; 8192 gated on two, x 2048
+//     9.3 / 10.5, apart 12.5 / 12.7, x 2560 12.2 / 13.8, apart 12.7 / 12.8, x 4096 16.1 / 17.3, apart 12.5 / 12.7. 16 x 16384 x 2048
+//     19.2, apart 12.8.
 //   16 waves on one tile of the weight: 256 x 2048 x 8192 18.6, 8 waves on two 21.8; 1024 x 2048 x 8192 50.6, 40.2
 //   32 tokens a workgroup: 64 x 2048 x 8192 13.2, 64 tokens 15.2; 256 x 2048 x 8192 19.1, 18.6
 struct How {
@@ -453,8 +457,11 @@ How how(int64_t R, int64_t N, int64_t K, int gated) {
   const int64_t nt = padded_rows(N, gated) / 32, mt = (R + 31) / 32;
   How h = {false, false, 2, mt > 1 ? 2 : 1};
   h.tiles = ((nt + TN - 1) / TN) * ((mt + TM - 1) / TM) >= 112;
-  h.fused = !h.tiles && R <= 4 && K <= 4096 && nt <= 512;
-  if (!gated && (nt / 2) * ((mt + 1) / 2) < 256) {
+  const bool one = !gated && nt <= 256;
+  if (!h.tiles && R <= 4 && nt <= 512 && K <= (one ? 4096 : 2048)) {
+    h.fused = true;
+    h.nt = one ? 1 : 2;
+  } else if (!gated && (nt / 2) * ((mt + 1) / 2) < 256) {
     h.nt = 1;
     h.wm = nt * mt <= 256 ? 1 : 2;
   }

@@ -49,3 +49,18 @@ def test_scales_far_apart(i8, R, N, K, gated, size, row):
     assert torch.isfinite(want.float()).all() and torch.isfinite(got).all()
     worst = float(((got - want).abs() / far).max())
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("R", [1, 3, 4, 5])
+@pytest.mark.parametrize("N,K", [(8192, 2048), (8200, 2048), (8200, 2056), (12290, 1000), (16384, 2048), (16386, 2048), (16384, 2056), (8192, 4096), (8192, 4104), (2050, 4096), (34, 2048)], ids=str)
+def test_borders_of_rounding_inside(i8, R, N, K, gated):
+    """Both sides of where a few tokens are rounded inside their product, on one and on two tiles of the weight a workgroup."""
+    g = torch.Generator().manual_seed(R + N + K)
+    x = torch.randn(R, K, generator=g).to(torch.bfloat16)
+    w = torch.randint(-127, 128, (N, K), generator=g).to(torch.int8)
+    scale = torch.rand(N, generator=g) * 1e-3 + 1e-4
+    want, far = product(x, w, scale, gated)
+    got = i8.linear8(x.to(DEV), i8.Weight8(w.to(DEV), scale.to(DEV), gated=gated)).cpu().double()
+    worst = float(((got - want).abs() / far).max())
+    assert worst <= 1.0, worst
