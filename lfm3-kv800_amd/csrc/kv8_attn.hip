@@ -867,11 +867,21 @@ Plan plan(const kv8_cache_t* c, int64_t heads, int64_t R, int64_t T, int64_t bt_
   p.bytes = 0;
   const int64_t positions = bt_cols * c->blocks * BLK, mean = (T + R - 1) / R;
   const int64_t seen = window > 0 && window < positions - mean ? window + mean : positions;   // of a row, or so
-  // Columns of a row and KV head, on average: the prompt kernel's tile has 128, the list's 16 or 32. Times, us, of 64 rows x 4,096 / 16 x
-  // 4,096 / 1 x 16,384 positions by tiles of 16, of 32, and as prompts: 16 columns 62, 64, 82 / 27, 27, 29 / 19, 23, 26; 32 columns 92, 66, 80 / 25, 32, 31 /
-  // 20, 25, 26; 48 columns 133, 92, 87 / 44, 30, 33 / 24, 47, 26; 64 columns 166, 92, 88 / 33, 31, 34 / 34, 48, 27.
+  // Columns of a row and KV head, on average: the prompt kernel's tile has 128, the list's 16 or 32 (`wide`). Times, us, by tiles of 16, of
+  // 32, and as prompts; 4 columns a token, 4 KV heads of 128:
+  //   every row with the same tokens  columns 24          36             48             64             80
+  //     1 x 16384                     17.3 23.2 19.7   22.7 20.4 20.7   22.7 21.5 21.5  18.1 23.6 22.5  25.6 26.1 23.2
+  //     16 x 4096                     24.5 25.1 30.4   41.0 31.2 32.0   40.8 31.6 33.0  32.0 32.0 34.5  60.5 45.6 36.3
+  //     64 x 4096                     86.3 56.1 106.6  131 90.2 107     131 90.6 108    160 92.0 108    208 137 109
+  //     48 x 12000                    200 119 203      297 213 206      297 213 208     348 215 211     440 313 217
+  //   rows with 1 to so many          up to 16            20               24               28               32
+  //     5 x 3000                      19.4 20.6 18.3   18.7 21.6 18.5   25.5 23.9 21.4  26.4 21.2 22.0  21.5 24.1 21.4
+  //     16 x 4097                     24.4 30.4 31.5   34.3 33.6 32.3   52.4 39.9 34.9  46.7 39.4 33.5  60.2 42.2 36.6
+  //     32 x 4096                     58.4 48.5 49.8   66.8 52.5 51.0   81.2 59.0 53.7  98.4 70.7 57.1  98.3 71.1 56.9
+  //     32 x 9000                     116 87.1 93.1    135 92.5 96.0    170 105 99.7    202 130 104     184 125 102
+  // Uniform rows would go by tiles of 32 up to 64 columns; in steps whose rows differ, as a server's do, prompts draw level at a mean of 40
+  // (up to 20 tokens) and are ahead behind it. Neither can be told from the other here.
   const int64_t cols = T * p.G / R, items = R * c->kv_heads;
-  // (Sixteen rows of 4,096 positions with 1 to 33 tokens each: 36 us by tiles of 32, 32 as prompts, so 40 is where prompts begin.)
   const bool wide = items * seen >= 1 << 19;
   // A workgroup an item without a list: short rows (1 x 1000 10.5 us, listed 14.9; 256 x 1000 51, 60), and of many rows with a token each
   // longer ones (40 x 1800 18, 23; 100 x 4000 76, 93; 100 x 8000 145, 164; 32 x 8000 58, 56.5). With more tokens a row some of the items'
