@@ -23,11 +23,13 @@ extern "C" {
 int lfm3_hip_int8_layout(const int8_t* w, int64_t ld, const float* scale, int64_t N, int64_t K, int gated, int8_t* wsh, float* ssh,
                          void* stream);
 
-/* A bf16 weight (N, K; row stride ld) quantized by rows: scale = max(max |w|, 2^-100) / 127, w8 = round(w 127 / that maximum) (N, K). */
+/* A bf16 weight (N, K; row stride ld) quantized by rows: with t = max(max |w|, 2^-100) of a row, scale = t / 127 and w8 (N, K) = w (127 / t)
+ * rounded to nearest even, quotient and product rounded to fp32 before. */
 int lfm3_hip_int8_quantize(const uint16_t* w, int64_t ld, int64_t N, int64_t K, int8_t* w8, float* scale, void* stream);
 
-/* y (R, N, or R, N / 2 for a gated weight; row stride ldy) bf16 = s_r s_n sum_k x8 w8, x8 = round(x 127 / t_r) to nearest even with
- * t_r = max(max |x_r|, 2^-100) and s_r = t_r / 127; the sums are exact. gated: silu(y_g) y_u in fp32, rounded once. A token with an
+/* y (R, N, or R, N / 2 for a gated weight; row stride ldy) bf16 = s_r s_n sum_k x8 w8, x8 and s_r of a token as w8 and scale of
+ * a weight's row (above); the sums are exact, and a scale above 1 of a token is multiplied behind the row's, so that what is finite stays
+ * finite. gated: silu(y_g) y_u in fp32, rounded once. A token with an
  * infinity or NaN gives NaN. x (R, K; row stride ldx, a multiple of 8, 16-byte aligned) bf16, K a multiple of 8 up to 65,536.
  * ws: lfm3_hip_linear8_workspace bytes, 16-byte aligned, of this call alone. */
 int64_t lfm3_hip_linear8_workspace(int64_t R, int64_t N, int64_t K, int gated);

@@ -63,7 +63,8 @@ __device__ __forceinline__ T scalar_load(const T* p) { return *(const __attribut
 __device__ __forceinline__ int64_t same(int64_t x) {
   return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
-// the exponent bytes of keys and values at p (an even address): the low and high byte
+// the exponent bytes of keys and values at p (an even address): the low and high byte. The load is of the aligned word around them, two
+// bytes of which may lie before the first or behind the last pair of exps (the header says so).
 __device__ __forceinline__ uint32_t exps_load(const uint8_t* p) {
   const uintptr_t a = (uintptr_t)p;
   return scalar_load((const uint32_t*)(a & ~(uintptr_t)3)) >> (8 * (a & 2));
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
     for (int st = s0 + wv; st < s1; st += 4) {
       const int64_t pos = row.b0 * BLK + (int64_t)st * STEP;
       if (pos > thi || pos + STEP <= tlo + 1) continue;
-      // ---- codes of the two blocks; a block that no query sees, or without a page, is not read
+      // ---- codes of the step's blocks; a block that no query sees, or without a page, is not read
       uint4 kk[4 * NB][D / 64], vv[NT][NB];
       float sc[NB][2];
       bool on[NB];

@@ -7,7 +7,7 @@
 //
 // Sums of up to 65,536 products of 8-bit integers fit 32 bits, so they are exact and any split of K gives the same result; the
 // scales are applied once, in fp32.
-#include "kv800_common.h"
+#include "kv800_attn.h"
 #include "../../include/kv800_hip.h"
 #include "../../include/lfm3_int8.h"
 
@@ -47,7 +47,8 @@ __global__ void __launch_bounds__(256) layout_kernel(const int8_t* __restrict__ 
   *reinterpret_cast<uint4*>(wsh + i * 16) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// 16 channels to codes
+// 16 channels to codes: the product with inv = 127 / t rounds to 32 bits first, so that a channel on the border between two codes (half
+// of t, say) may go to either
 __device__ __forceinline__ uint4 codes16(const uint4 (&u)[2], float inv) {
   const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
   uint32_t o[4];
@@ -153,12 +154,6 @@ __device__ __forceinline__ float gate(float g, float u) {
   const float e = __builtin_amdgcn_exp2f(fabsf(g) * -0.7213475204444817f), f = g < 0.f ? e : 1.f;
   return g * f * u * f * __builtin_amdgcn_rcpf(__builtin_fmaf(e, e, 1.f));
 }
-__device__ __forceinline__ uint32_t bfpk(float a, float b) {   // two floats -> packed bf16 (round to nearest even)
-  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-  const bf2 v = {(__bf16)a, (__bf16)b};
-  return __builtin_bit_cast(uint32_t, v);
-}
-
 struct Out {
   uint16_t* y;
   int64_t ldy, R, N;
@@ -168,12 +163,12 @@ struct Out {
 __device__ __forceinline__ void put4(const Out& o, int64_t r, int64_t n, int64_t width, const float (&v)[4]) {
   uint16_t* dst = o.y + r * o.ldy + n;
   if (o.wide && n + 4 <= width) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(bfpk(v[0], v[1]), bfpk(v[2], v[3]));
+    *reinterpret_cast<uint2*>(dst) = make_uint2(kv800::bfpk(v[0], v[1]), kv800::bfpk(v[2], v[3]));
     return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (n + i < width) dst[i] = (uint16_t)bfpk(v[i], 0.f);
+    if (n + i < width) dst[i] = (uint16_t)kv800::bfpk(v[i], 0.f);
 }
 // Few tokens: one workgroup takes 32 NT rows of the weight x 32 WM tokens, its 16 / NT waves a part of K each, so that every wave has
 // blocks of 1 KB in flight from its first instruction on; their sums meet in LDS, 32 tokens at a time. Output of the instruction
@@ -406,7 +401,7 @@ __global__ void __launch_bounds__(64 * MANY, 2) many_kernel(const int8_t* __rest
             f[e] = scaled(acc[i][j][4 * q + e], s[j], ka[e]);
             if (GATED) f[e] = gate(f[e], scaled(acc[i + (GATED ? 1 : 0)][j][4 * q + e], s[j], kb[e]));
           }
-          *reinterpret_cast<uint2*>(buf + (32 * j + (lane & 31)) * ROW + (32 * c + row) * 2) = make_uint2(bfpk(f[0], f[1]), bfpk(f[2], f[3]));
+          *reinterpret_cast<uint2*>(buf + (32 * j + (lane & 31)) * ROW + (32 * c + row) * 2) = make_uint2(kv800::bfpk(f[0], f[1]), kv800::bfpk(f[2], f[3]));
         }
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -41,8 +41,8 @@ def _rows16(x):
 
 
 def quantize_rows(w):
-    """(codes (N, K) int8, scale (N,) fp32) of a bf16 matrix: scale = max(max |w|, 2^-100) / 127 of a row, codes round(w / scale)
-    (lfm3_hip_int8_quantize)."""
+    """(codes (N, K) int8, scale (N,) fp32) of a bf16 matrix: with t = max(max |w|, 2^-100) of a row, scale = t / 127 and codes
+    round(w (127 / t)), all in fp32 (lfm3_hip_int8_quantize)."""
     L = _lib()
     if w.device.type != "cuda":
         raise ValueError(f"w must be on a GPU, got {w.device}")

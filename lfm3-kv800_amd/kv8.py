@@ -169,7 +169,8 @@ def attend(cache, q, bt, lens, qsl, window=0, scale=None):
     """Attention of a step's tokens over the cache, which holds them already (kv8_hip_attend): q (T, heads, D) bf16, query head h
     on KV head h / (heads / kv heads), up to 16 query heads a KV head; a query sees the positions up to its own and, with a
     window, the last `window` of them. scale: 1 / sqrt(D) if None. Returns (T, heads, D) bf16; zeros for queries without keys and
-    for the padding."""
+    for the padding. How it runs goes by T, R and the table's width: a prompt beside single tokens over long rows is quicker in a call
+    of its own (its rows of q, bt and lens, and their starts)."""
     L = _lib()
     dev = _dev(cache)
     _need(q, "q", torch.bfloat16, dev)

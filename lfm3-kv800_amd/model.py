@@ -326,8 +326,12 @@ class PagedAttention8:
     800h blocks), the 5 sliding layers over a window of 256. Keys are rotated on their way into the cache. One block table for the
     full layers, one for the sliding ones, whose rows own a ring of `ring` shuffled pages that holds a chunk of FILL tokens and the
     window before it. The same steps as PagedAttention800: begin_step / attend, begin_chunk / attend (rows with any number of
-    new tokens up to FILL: prompts, drafts), freeze / thaw for recorded steps, fill for synthetic histories. A draft that is taken back
-    may leave its block a larger exponent, so a loop with drafts can round a block's later tokens more coarsely than one without.
+    new tokens up to FILL: prompts, drafts), freeze / thaw for recorded steps, fill for synthetic histories.
+
+    A draft larger than its block's tokens raises the block's exponent, for its keys or its values, and stays in it when it is taken
+    back: the block's tokens, earlier and later ones, are then held at that exponent, of which values below 2^-6 lose a bit for each
+    power of two (those above are held as before). The chunk's own earlier queries see them so, too. So a loop with drafts can differ
+    from one without by that rounding.
 
     lens0: the rows' history lengths; steps: decode steps to provide for; bs: tokens per page."""
 
@@ -477,7 +481,8 @@ def speculative_loop(model, attention, tokens, steps, draft, most, temperature=N
     (R,) fp32, None: greedy. Lengths stay on the device, so a step does not wait for the one before; the attention must be a
     PagedAttention800 or PagedAttention8 with room for steps (most + 1) more positions, most < 128. Greedy tokens are those of the one-token loop
     up to near-ties: the short conv rounds once a sum and not every product, and a block that becomes eligible inside a chunk
-    is read exact by that chunk. Returns the rows' new tokens, a list of R
+    is read exact by that chunk; with PagedAttention8, drafts may also have left a block a larger exponent, and of 8-bit products a
+    rounding before them may move a token's code by a whole step, so that there more is near. Returns the rows' new tokens, a list of R
     tensors, and the (steps, R) counts; attention.lens follows."""
     dev, R = tokens.device, tokens.shape[0]
     if not 0 <= most < 128:
