@@ -149,6 +149,15 @@ __device__ __forceinline__ kv800::b8 wide8(uint32_t a, uint32_t b, float f) {
   return kv800::b8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
 }
 
+// two bf16 of a query, their signs flipped for a negative scale; an infinity becomes NaN, since no softmax has scores that are infinite,
+// while a maximum of minus infinity means that no key was seen
+__device__ __forceinline__ uint32_t query(uint32_t u, uint32_t flip) {
+  return (u ^ flip) | (((u & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 9;
+}
+__device__ __forceinline__ kv800::u4v query(uint4 u, uint32_t flip) {
+  return kv800::u4v{query(u.x, flip), query(u.y, flip), query(u.z, flip), query(u.w, flip)};
+}
+
 // sum + the two rounded weights of w: what the values are multiplied by is what the sum counts, so that equal values come back as they
 // are and a dominant weight's rounding cancels
 __device__ __forceinline__ float count(uint32_t w, float sum) {
@@ -270,7 +279,7 @@ __global__ void __launch_bounds__(256, NB * NC == 1 ? 3 : 2) attend_kernel(Atten
       for (int e = 0; e < NK; ++e) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (have) u = *reinterpret_cast<const uint4*>(A.q + ((row.q0 + i) * A.C.heads * A.G + hq) * D + (e >> 1) * 64 + 16 * g + 8 * (e & 1));
-        qr[n][e] = kv800::as_b8(kv800::u4v{u.x ^ A.flip, u.y ^ A.flip, u.z ^ A.flip, u.w ^ A.flip});
+        qr[n][e] = kv800::as_b8(query(u, A.flip));
       }
 #pragma unroll
       for (int d = 0; d < NT; ++d) o[n][d] = f4{0.f, 0.f, 0.f, 0.f};
@@ -629,7 +638,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
   for (int s = 0; s < NK; ++s) {
     uint4 u = make_uint4(0, 0, 0, 0);
     if (have) u = *reinterpret_cast<const uint4*>(A.q + ((row.q0 + iq) * Hq + hq) * D + 16 * s + 8 * hf);
-    qr[s] = kv800::u4v{u.x ^ A.flip, u.y ^ A.flip, u.z ^ A.flip, u.w ^ A.flip};
+    qr[s] = query(u, A.flip);
   }
   // blocks that some query sees, and positions that all of them see
   const int64_t thi = min(row.p0 + ilast, row.n - 1), tlo = A.window > 0 ? max(row.p0 + i0 - A.window + 1, (int64_t)0) : 0;

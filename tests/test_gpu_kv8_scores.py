@@ -61,3 +61,24 @@ def test_equal_values_come_back(kv8, prev, new, window, D):
         got = kv8.attend(kv8.Cache8(*up(data, exps)), *up(q, bt, lens, qsl), window=window).cpu()
         wrong = (got.float() != value.view(torch.float8_e4m3fn).float()).float().mean()
         assert wrong == 0, (spread, float(wrong))
+
+
+@pytest.mark.parametrize("prev,new", SHAPES + [([0], [1]), ([1500, 700], [70, 64])], ids=str)
+@pytest.mark.parametrize("scale", [0.125, -0.125])
+def test_scores_of_minus_infinity(kv8, prev, new, scale):
+    """A query with an infinity whose scores are all minus infinity has no softmax: NaN, as 0 / 0 is, not the zeros of a query without
+    keys; other queries and heads of its tile stay as they are, and so do tokens that are padding."""
+    data, exps, bt, lens, qsl, T, g = rows(kv8, 81, prev, new, 2, 64, 64, pad=2)
+    data[:, :, :, 0] = data[:, :, :, 0] & 0x7F                                  # no key is negative,
+    data[:, :, :, 0] = data[:, :, :, 0].clamp(min=0x10, max=0x7E)               # nor 0, nor NaN
+    q = torch.randn(T, 8, 64, generator=g).to(torch.bfloat16)
+    up = lambda *a: [t.to(DEV) for t in a]
+    c = kv8.Cache8(*up(data, exps))
+    plain = kv8.attend(c, *up(q, bt, lens, qsl), scale=scale).cpu()
+    bad = float("-inf") if scale > 0 else float("inf")
+    last = int(qsl[-1]) - 1
+    q[0, 1, 7] = q[last, 6, 0] = q[last + 1, 2, 5] = bad
+    got = kv8.attend(c, *up(q, bt, lens, qsl), scale=scale).cpu()
+    assert got[0, 1].isnan().all() and got[last, 6].isnan().all()
+    plain[0, 1], plain[last, 6] = got[0, 1], got[last, 6]
+    assert torch.equal(got.view(torch.int16), plain.view(torch.int16)) and not got[last + 1:].any()
