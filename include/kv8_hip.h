@@ -52,7 +52,8 @@ int kv8_hip_dequantize(const kv8_cache_t* cache, uint16_t* k, uint16_t* v, void*
  * 16, query head h on KV head h / G; out (T, heads, D) bf16 = softmax(scale q . k) v over positions <= the query's and, with
  * window > 0, > position - window. A query without keys and the padding [qsl[R], T) get zeros; what a query does not see does not
  * reach it, NaN included. An infinity or NaN in a query gives NaN where it sees a key. Scores are fp32 (finite ones have to stay in its
- * range), weights are rounded to bf16 and summed as rounded. ws: kv8_hip_attend_workspace(...) bytes, 16-byte aligned, of this call alone. bt_cols blocks 64 < 2^31.
+ * range), weights are rounded to bf16 and summed as rounded. ws: kv8_hip_attend_workspace(...) bytes, 16-byte aligned, of this
+ * call alone. bt_cols blocks 64 < 2^31.
  *
  * How a call runs goes by what the host knows, T tokens over R rows and the positions of bt_cols pages, not by the rows themselves.
  * A table wider than its rows costs little (one row of 1,000 positions 9.9 us, 13.8 in a table of 8,192 and of 65,536), a first chunk in one

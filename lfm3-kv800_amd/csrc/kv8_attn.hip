@@ -592,7 +592,7 @@ __device__ __forceinline__ float halves_max(float x) {
 // output column l % 32, rows 8 b + 4 (l / 32) + i), so a column's weights and sums stay in its two lanes. Row 8 b + 4 h + i of
 // key tile a is token 32 a + 16 (b / 2) + 8 h + 4 (b % 2) + i: the lane's weights are then those of 8 tokens side by side, half
 // of a piece of the values. Two prompts of 8,192 tokens, 16 heads: 558 us, 1 PFLOP/s, bound by the issue of both vector and matrix
-// instructions (50 and 46 % busy), of which two waves a SIMD overlap little.
+// instructions (46 and 44 % busy), of which two waves a SIMD overlap little.
 template <int D, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, int per, int splits, float* __restrict__ part) {
   constexpr int NT = D / 32, NK = D / 16, NP = 4 * D / (64 * NW);          // dim tiles, k-steps, pieces of K (and V) a thread stages

@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(64 * 16 / NT) few_kernel(const uint16_t* __res
 // Many tokens: one workgroup of 4 waves takes 256 rows of the weight x 128 tokens, 64 channels a stage, three stages in LDS: a stage's
 // blocks are loaded straight into LDS two stages ahead, one barrier a stage. A block lies in LDS as it does in memory, in operand
 // order, so that loads and reads go over consecutive addresses. A wave has 128 rows x 64 tokens: 6 blocks read from LDS for 8 products.
-// Two workgroups share a CU, so that one's epilogue and barriers pass under the other's products: 8192 x 16384 x 2048 gated 300 us;
-// one workgroup of 8 waves for 256 x 256 with two stages of 128 channels 336.
+// Two workgroups share a CU, so that one's epilogue and barriers pass under the other's products: 8192 x 16384 x 2048 gated 300 us
+// (310 with the gate that keeps small results); one workgroup of 8 waves for 256 x 256 with two stages of 128 channels 336.
 constexpr int TN = 8, TM = 4, STAGE = 2, MANY = 4;       // tiles of 32 of the weight and of tokens, k-steps a stage, waves
 constexpr int LOADS = (TN + TM) * STAGE / MANY;          // loads of a wave a stage
 struct alignas(16) Stage {
