@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(64 * NW, 2) prompt_kernel(Attend A, int TQ, in
 }
 
 // ---------------------------------------------------------------- host
-// How a call runs. PROMPT: rows bring half a tile of the prompt kernel or more on average. DIRECT: few steps an item. A row that is
+// How a call runs. PROMPT: rows bring a third of a tile of the prompt kernel or more on average. DIRECT: few steps an item. A row that is
 // not as the mean has it is right all the same.
 enum Kind { LISTED, DIRECT, PROMPT };
 struct Plan {

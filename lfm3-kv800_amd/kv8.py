@@ -69,7 +69,7 @@ class Cache8:
             raise ValueError("data must be 16-byte aligned, its pages a multiple of 16 bytes apart; exps 2-byte aligned, an even number apart")
         self.data, self.exps = data, exps
         self.pages, self.heads, self.blocks, self.dim = P, H, U, n // BLK
-        self.bs, self.dev = U * BLK, data.device
+        self.bs, self.dev, self.on_gpu = U * BLK, data.device, data.is_cuda
         self._c = _Cache(data.data_ptr(), exps.data_ptr(), P, H, U, self.dim, ps, es)
         self._p = ctypes.byref(self._c)
 
@@ -84,7 +84,7 @@ class Cache8:
 
 def _dev(cache):
     """The cache's GPU. (A cache of host tensors may be described, not worked on.)"""
-    if cache.dev.type != "cuda":
+    if not cache.on_gpu:
         raise ValueError(f"the cache must be on a GPU, got {cache.dev}")
     return cache.dev
 
